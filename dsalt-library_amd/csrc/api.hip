@@ -4,6 +4,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <mutex>
 
@@ -651,6 +652,143 @@ int64_t dsalt_norm_train_workspace_size(int64_t rows, int32_t d) {
     return rows <= 0 || d <= 0 ? 0 : dsalt::norm_train_workspace_bytes(rows, d);
 }
 size_t dsalt_norm_train_args_size(void) { return sizeof(dsalt_norm_train_args); }
+
+int dsalt_gated_ffn_check(const dsalt_gated_ffn_args *a, int32_t backward) {
+    if (!a) return fail(DSALT_ERR_INVALID, "args must be non-NULL");
+    if (a->rows < 0 || a->rows > ((int64_t)1 << 31))
+        return fail(DSALT_ERR_INVALID, "rows must be in [0, 2^31] (got %lld)", (long long)a->rows);
+    for (int n : {a->d, a->f, a->e})
+        if (n < 8 || n % 8 || n > (1 << 20))
+            return fail(DSALT_ERR_UNSUPPORTED, "d, f and e must be multiples of 8 in [8, 2^20] (got %d, %d, %d)", a->d, a->f, a->e);
+    if (a->dtype != DSALT_DTYPE_BF16 && a->dtype != DSALT_DTYPE_F16)
+        return fail(DSALT_ERR_UNSUPPORTED, "dtype must be DSALT_DTYPE_BF16 or DSALT_DTYPE_F16 (got %d)", a->dtype);
+    if (a->activation < DSALT_ACT_SILU || a->activation > DSALT_ACT_RELU)
+        return fail(DSALT_ERR_INVALID, "activation must be DSALT_ACT_* (got %d)", a->activation);
+    const struct { const char *name; int64_t stride, row; bool used; } strides[] = {
+        {"x", a->x_stride, a->d, true}, {"w_gate", a->w_gate_stride, a->d, true}, {"w_up", a->w_up_stride, a->d, true},
+        {"w_down", a->w_down_stride, a->f, true}, {"dy", a->dy_stride, a->e, backward != 0}};
+    for (const auto &s : strides)
+        if (s.used && (s.stride < s.row || s.stride % 8 || s.stride > dsalt::gated_ffn_max_ld()))
+            return fail(DSALT_ERR_UNSUPPORTED, "%s row stride must be a multiple of 8 in [%lld, 2^21] (got %lld)", s.name,
+                        (long long)s.row, (long long)s.stride);
+    const int64_t tiles = ((a->rows + 127) / 128 + 1) * ((std::max(std::max(a->d, a->f), a->e) + 63) / 64 + 1);
+    if (tiles >= (int64_t)1 << 30) return fail(DSALT_ERR_UNSUPPORTED, "rows * width is too large");
+    for (const void *q : {a->x, a->w_gate, a->w_up, a->w_down, (const void *)a->gate_up, (const void *)a->act, (const void *)a->y,
+                          a->dy, (const void *)a->d_gate_up, (const void *)a->dx, (const void *)a->dw_gate,
+                          (const void *)a->dw_up, (const void *)a->dw_down, (const void *)a->workspace})
+        if (!aligned(q, 16)) return fail(DSALT_ERR_INVALID, "pointers must be 16-byte aligned");
+    if (!backward) {
+        if (a->rows > 0 && (!a->x || !a->w_gate || !a->w_up || !a->w_down || !a->act || !a->y))
+            return fail(DSALT_ERR_INVALID, "x, the weights, act and y must be non-NULL");
+    } else {
+        const bool inner = a->dx || a->dw_gate || a->dw_up;
+        if (a->rows > 0 && inner && !a->d_gate_up) return fail(DSALT_ERR_INVALID, "dx, dw_gate and dw_up need d_gate_up");
+        if (a->rows > 0 && (!a->dy || (a->dw_down && !a->act) || (a->d_gate_up && (!a->gate_up || !a->w_down)) ||
+                            (a->dx && (!a->w_gate || !a->w_up)) || ((a->dw_gate || a->dw_up) && !a->x)))
+            return fail(DSALT_ERR_INVALID, "an operand of a wanted gradient is NULL");
+    }
+    const int64_t need = dsalt::gated_ffn_workspace_bytes(a->rows, a->d, a->f, a->e, backward != 0);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need))
+        return fail(DSALT_ERR_INVALID, "workspace of dsalt_gated_ffn_workspace_size (%lld) bytes needed", (long long)need);
+    return DSALT_OK;
+}
+
+int dsalt_gated_ffn(const dsalt_gated_ffn_args *args, void *stream) {
+    if (int rc = dsalt_gated_ffn_check(args, 0)) return rc;
+    hipError_t e = dsalt::launch_gated_ffn(*args, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_gated_ffn launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+
+int dsalt_gated_ffn_bwd(const dsalt_gated_ffn_args *args, void *stream) {
+    if (int rc = dsalt_gated_ffn_check(args, 1)) return rc;
+    hipError_t e = dsalt::launch_gated_ffn_bwd(*args, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_gated_ffn_bwd launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+
+int64_t dsalt_gated_ffn_workspace_size(int64_t rows, int32_t d, int32_t f, int32_t e, int32_t backward) {
+    return rows < 0 || d < 8 || f < 8 || e < 8 ? 0 : dsalt::gated_ffn_workspace_bytes(rows, d, f, e, backward != 0);
+}
+size_t dsalt_gated_ffn_args_size(void) { return sizeof(dsalt_gated_ffn_args); }
+
+int dsalt_dropout(const dsalt_dropout_args *a, void *stream) {
+    if (!a) return fail(DSALT_ERR_INVALID, "args must be non-NULL");
+    if (a->n < 0 || a->n > ((int64_t)1 << 40)) return fail(DSALT_ERR_INVALID, "n must be in [0, 2^40] (got %lld)", (long long)a->n);
+    if (!float_dtype(a->dtype)) return fail(DSALT_ERR_INVALID, "dtype %d is not a float dtype", a->dtype);
+    if (a->threshold < 0 || a->threshold > 65536)
+        return fail(DSALT_ERR_INVALID, "threshold must be in [0, 65536] (got %d)", a->threshold);
+    if (a->n == 0) return DSALT_OK;
+    if (!a->x || !a->out) return fail(DSALT_ERR_INVALID, "x and out must be non-NULL");
+    if (!aligned(a->x, 16) || !aligned(a->out, 16) || !aligned(a->seed_ptr, 8))
+        return fail(DSALT_ERR_INVALID, "x and out must be 16-byte aligned, seed_ptr 8");
+    hipError_t e = dsalt::launch_dropout(*a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_dropout launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+size_t dsalt_dropout_args_size(void) { return sizeof(dsalt_dropout_args); }
+
+int dsalt_branch_norm_check(const dsalt_branch_norm_args *a, int32_t backward) {
+    if (!a) return fail(DSALT_ERR_INVALID, "args must be non-NULL");
+    if (a->rows < 0 || a->rows > ((int64_t)1 << 31))
+        return fail(DSALT_ERR_INVALID, "rows must be in [0, 2^31] (got %lld)", (long long)a->rows);
+    if (a->d < 8 || a->d % 8 || a->d > dsalt::branch_norm_max_dim())
+        return fail(DSALT_ERR_UNSUPPORTED, "d must be a multiple of 8 in [8, %d] (got %d)", dsalt::branch_norm_max_dim(), a->d);
+    if (!float_dtype(a->x_dtype)) return fail(DSALT_ERR_INVALID, "x_dtype %d is not a float dtype", a->x_dtype);
+    const bool x32 = a->x_dtype == DSALT_DTYPE_F32;
+    const auto branch = [&](int dt) { return x32 ? float_dtype(dt) : dt == a->x_dtype; };
+    if (!branch(a->h_dtype)) return fail(DSALT_ERR_UNSUPPORTED, "h dtype %d with x dtype %d", a->h_dtype, a->x_dtype);
+    if (a->weight && !branch(a->y_dtype))
+        return fail(DSALT_ERR_UNSUPPORTED, "y dtype %d with x dtype %d", a->y_dtype, a->x_dtype);
+    const struct { const void *p; int dt; } ws[] = {{a->weight, a->w_dtype}, {a->post_weight, a->post_dtype}, {a->gate, a->gate_dtype}};
+    for (const auto &w : ws)
+        if (w.p && w.dt != DSALT_DTYPE_F32 && w.dt != a->x_dtype)
+            return fail(DSALT_ERR_UNSUPPORTED, "weight or gate dtype %d with x dtype %d", w.dt, a->x_dtype);
+    if (a->gate_kind < 0 || a->gate_kind > 2) return fail(DSALT_ERR_INVALID, "gate_kind must be 0, 1 or 2 (got %d)", a->gate_kind);
+    if (a->threshold < 0 || a->threshold > 65536)
+        return fail(DSALT_ERR_INVALID, "threshold must be in [0, 65536] (got %d)", a->threshold);
+    for (const void *q : {a->x, a->h, a->weight, a->post_weight, (const void *)a->x_out, (const void *)a->y, a->dx_out, a->dy,
+                          (const void *)a->dx, (const void *)a->dh, (const void *)a->d_weight, (const void *)a->d_post_weight,
+                          (const void *)a->workspace})
+        if (!aligned(q, 16)) return fail(DSALT_ERR_INVALID, "row tensors must be 16-byte aligned");
+    const size_t ga = a->gate_kind == 1 ? 16 : a->gate_dtype == DSALT_DTYPE_F32 ? 4 : 2;
+    if (!aligned(a->gate, ga) || !aligned(a->d_gate, ga)) return fail(DSALT_ERR_INVALID, "gate must be %d-byte aligned", (int)ga);
+    if (!aligned(a->rstd, 4) || !aligned(a->rstd_post, 4) || !aligned(a->seed_ptr, 8))
+        return fail(DSALT_ERR_INVALID, "statistics must be 4-byte, seed_ptr 8-byte aligned");
+    if (a->rows == 0) return DSALT_OK;
+    if (!a->x || !a->h || (a->gate_kind && !a->gate)) return fail(DSALT_ERR_INVALID, "x, h and a gate must be non-NULL");
+    if (!backward) {
+        if (!a->x_out || (a->weight && !a->y)) return fail(DSALT_ERR_INVALID, "x_out, and y with weight, must be non-NULL");
+    } else {
+        if (!a->dx_out && !a->dy) return fail(DSALT_ERR_INVALID, "dx_out or dy must be non-NULL");
+        if (a->dy && (!a->weight || !a->rstd)) return fail(DSALT_ERR_INVALID, "dy needs weight and rstd");
+        if (a->post_weight && !a->rstd_post) return fail(DSALT_ERR_INVALID, "post_weight needs rstd_post");
+        if (a->d_post_weight && !a->post_weight) return fail(DSALT_ERR_INVALID, "d_post_weight needs post_weight");
+        if ((a->d_weight || a->d_post_weight || (a->d_gate && a->gate_kind == 1)) &&
+            (!a->workspace || a->workspace_bytes < dsalt::branch_norm_workspace_bytes(a->rows, a->d)))
+            return fail(DSALT_ERR_INVALID, "the column sums need workspace of dsalt_branch_norm_workspace_size bytes");
+    }
+    return DSALT_OK;
+}
+
+int dsalt_branch_norm(const dsalt_branch_norm_args *args, void *stream) {
+    if (int rc = dsalt_branch_norm_check(args, 0)) return rc;
+    hipError_t e = dsalt::launch_branch_norm(*args, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_branch_norm launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+
+int dsalt_branch_norm_bwd(const dsalt_branch_norm_args *args, void *stream) {
+    if (int rc = dsalt_branch_norm_check(args, 1)) return rc;
+    hipError_t e = dsalt::launch_branch_norm_bwd(*args, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_branch_norm_bwd launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+
+int64_t dsalt_branch_norm_workspace_size(int64_t rows, int32_t d) {
+    return rows < 0 || d <= 0 ? 0 : dsalt::branch_norm_workspace_bytes(rows, d);
+}
+size_t dsalt_branch_norm_args_size(void) { return sizeof(dsalt_branch_norm_args); }
 
 int dsalt_rope_check(const dsalt_rope_args *a) {
     if (!a) return fail(DSALT_ERR_INVALID, "args is NULL");

@@ -1,0 +1,59 @@
+// Dropout whose mask is a function of (seed, offset, element index): see philox.h. Nothing but
+// x is read and nothing but out written, so the backward is the same pass over the gradient.
+//
+// Bound by memory: a read and a write per element against 14 multiplies per eight.
+#include "launch.h"
+#include "philox.h"
+#include "rows.h"
+
+#include <algorithm>
+
+namespace dsalt {
+namespace {
+
+template <typename DT>
+__device__ __forceinline__ float load1(const void *p, int64_t i) {
+    return Elem<DT>::ld(p, i);
+}
+
+// A thread takes groups of eight elements; the last, partial one goes to the thread after
+// the last full one.
+template <typename DT>
+__global__ void __launch_bounds__(256) dropout_kernel(const void *__restrict__ x, void *__restrict__ out, int64_t n,
+                                                      const DropoutParams p) {
+    const uint64_t seed = dropout_seed(p);
+    const int64_t full = n / 8, stride = (int64_t)gridDim.x * 256;
+    int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (; g < full; g += stride) {
+        Raw8<DT> raw;
+        raw.load(x, g);
+        float v[8];
+        raw.get(v);
+        apply_keep(keep8((uint64_t)g, p, seed), p.scale, v);
+        store8<DT>(out, g, v);
+    }
+    if (g == full) {
+        const uint32_t m = keep8((uint64_t)g, p, seed);
+        for (int64_t i = g * 8; i < n; ++i)
+            Elem<DT>::st(out, i, (m >> (i & 7)) & 1u ? load1<DT>(x, i) * p.scale : 0.f);
+    }
+}
+
+template <typename DT>
+void launch(const dsalt_dropout_args &a, const DropoutParams &p, hipStream_t stream) {
+    const int64_t groups = (a.n + 7) / 8, blocks = std::min<int64_t>((groups + 255) / 256, 256 * 8 * 4);
+    hipLaunchKernelGGL(dropout_kernel<DT>, dim3((unsigned)blocks), dim3(256), 0, stream, a.x, a.out, a.n, p);
+}
+
+}  // namespace
+
+hipError_t launch_dropout(const dsalt_dropout_args &a, hipStream_t stream) {
+    if (a.n == 0) return hipSuccess;
+    const DropoutParams p = dropout_params(a.threshold, a.seed, a.seed_ptr, a.offset);
+    if (a.dtype == DSALT_DTYPE_BF16) launch<BF16>(a, p, stream);
+    else if (a.dtype == DSALT_DTYPE_F16) launch<F16>(a, p, stream);
+    else launch<F32>(a, p, stream);
+    return hipGetLastError();
+}
+
+}  // namespace dsalt

@@ -73,6 +73,15 @@ hipError_t launch_swiglu_rows(const void *gate_up, const void *d_out, void *out,
 hipError_t launch_norm_train(const dsalt_norm_train_args &a, hipStream_t stream);
 hipError_t launch_norm_train_bwd(const dsalt_norm_train_args &a, hipStream_t stream);
 int64_t norm_train_workspace_bytes(int64_t rows, int d);
+hipError_t launch_gated_ffn(const dsalt_gated_ffn_args &a, hipStream_t stream);
+hipError_t launch_gated_ffn_bwd(const dsalt_gated_ffn_args &a, hipStream_t stream);
+int64_t gated_ffn_workspace_bytes(int64_t rows, int d, int f, int e, bool backward);
+int64_t gated_ffn_max_ld();
+hipError_t launch_dropout(const dsalt_dropout_args &a, hipStream_t stream);
+hipError_t launch_branch_norm(const dsalt_branch_norm_args &a, hipStream_t stream);
+hipError_t launch_branch_norm_bwd(const dsalt_branch_norm_args &a, hipStream_t stream);
+int64_t branch_norm_workspace_bytes(int64_t rows, int d);
+int branch_norm_max_dim();
 
 // Number of query blocks of `bm` tokens over a packed batch, as an upper bound that is
 // computable without reading cu_seqlens: sum_s ceil(L_s/bm) <= ceil(T/bm) + S.

@@ -12,13 +12,16 @@ from .kernels import (
     HybridEnergyLandmarkSelector,
     RMSENorm,
     apply_rotary_emb,
+    branch_norm,
     build_local_window_mask,
     build_local_window_mask_packed,
     build_rope_cache,
     compute_hybrid_scores,
     compute_window_sizes,
+    counter_dropout,
     dsalt_triton_attention,
     dsalt_triton_backward,
+    gated_ffn,
     hybrid_scores_per_head,
     select_landmarks,
     soft_landmark_weights,
@@ -38,6 +41,9 @@ __all__ = [
     "dsalt_triton_attention",
     "dsalt_triton_backward",
     "dsalt_triton_train_attention",
+    "gated_ffn",
+    "counter_dropout",
+    "branch_norm",
     "RMSENorm",
     "compute_window_sizes",
     "build_local_window_mask",

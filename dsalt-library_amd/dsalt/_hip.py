@@ -7,6 +7,7 @@ fallback: a missing library or a non-GPU tensor raises ``DsaltError``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p
@@ -190,6 +191,42 @@ class NormTrainArgs(ctypes.Structure):
     ]
 
 
+class GatedFfnArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("d", c_int32), ("f", c_int32), ("e", c_int32),
+        ("dtype", c_int32), ("activation", c_int32), ("reserved", c_int32),
+        ("x", c_void_p), ("x_stride", c_int64),
+        ("w_gate", c_void_p), ("w_up", c_void_p), ("w_down", c_void_p),
+        ("w_gate_stride", c_int64), ("w_up_stride", c_int64), ("w_down_stride", c_int64),
+        ("gate_up", c_void_p), ("act", c_void_p), ("y", c_void_p),
+        ("dy", c_void_p), ("dy_stride", c_int64),
+        ("d_gate_up", c_void_p), ("dx", c_void_p), ("dw_gate", c_void_p), ("dw_up", c_void_p), ("dw_down", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
+class DropoutArgs(ctypes.Structure):
+    _fields_ = [
+        ("n", c_int64), ("dtype", c_int32), ("threshold", c_int32), ("x", c_void_p), ("out", c_void_p),
+        ("seed", c_int64), ("offset", c_int64), ("seed_ptr", c_void_p),
+    ]
+
+
+class BranchNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("d", c_int32),
+        ("x_dtype", c_int32), ("h_dtype", c_int32), ("y_dtype", c_int32), ("w_dtype", c_int32), ("post_dtype", c_int32),
+        ("gate_dtype", c_int32), ("gate_kind", c_int32), ("threshold", c_int32),
+        ("eps", c_float), ("post_eps", c_float), ("residual_scale", c_float),
+        ("seed", c_int64), ("offset", c_int64), ("seed_ptr", c_void_p),
+        ("x", c_void_p), ("h", c_void_p), ("weight", c_void_p), ("post_weight", c_void_p), ("gate", c_void_p),
+        ("x_out", c_void_p), ("y", c_void_p), ("rstd", c_void_p), ("rstd_post", c_void_p),
+        ("dx_out", c_void_p), ("dy", c_void_p),
+        ("dx", c_void_p), ("dh", c_void_p), ("d_weight", c_void_p), ("d_post_weight", c_void_p), ("d_gate", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "dsalt_fwd", "dsalt_fwd_check", "dsalt_bwd", "dsalt_bwd_check", "dsalt_bwd_workspace_size",
     "dsalt_select_landmarks", "dsalt_select_check", "dsalt_quantize_windows",
@@ -202,6 +239,9 @@ EXPORTED_SYMBOLS = (
     "dsalt_select_hybrid_qkv", "dsalt_qkv_args_size", "dsalt_module_grads_v", "dsalt_module_grads_x",
     "dsalt_module_grads_workspace_size", "dsalt_module_grads_args_size", "dsalt_swiglu_rows", "dsalt_norm_train",
     "dsalt_group_sum", "dsalt_norm_train_bwd", "dsalt_norm_train_workspace_size", "dsalt_norm_train_args_size",
+    "dsalt_gated_ffn", "dsalt_gated_ffn_bwd", "dsalt_gated_ffn_check", "dsalt_gated_ffn_workspace_size",
+    "dsalt_gated_ffn_args_size", "dsalt_dropout", "dsalt_dropout_args_size", "dsalt_branch_norm",
+    "dsalt_branch_norm_bwd", "dsalt_branch_norm_check", "dsalt_branch_norm_workspace_size", "dsalt_branch_norm_args_size",
 )
 NOALLOC_SCRATCH_BYTES = 76 << 20  # DSALT_NOALLOC_SCRATCH_BYTES
 SELECT_SPLIT_MIN = 4096  # longer sequences can be selected chunk-wise
@@ -250,6 +290,13 @@ def lib() -> ctypes.CDLL:
         ("dsalt_group_sum", [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p]),
         ("dsalt_swiglu_rows", [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p]),
         ("dsalt_swiglu", [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
+        ("dsalt_gated_ffn", [ctypes.POINTER(GatedFfnArgs), c_void_p]),
+        ("dsalt_gated_ffn_bwd", [ctypes.POINTER(GatedFfnArgs), c_void_p]),
+        ("dsalt_gated_ffn_check", [ctypes.POINTER(GatedFfnArgs), c_int32]),
+        ("dsalt_dropout", [ctypes.POINTER(DropoutArgs), c_void_p]),
+        ("dsalt_branch_norm", [ctypes.POINTER(BranchNormArgs), c_void_p]),
+        ("dsalt_branch_norm_bwd", [ctypes.POINTER(BranchNormArgs), c_void_p]),
+        ("dsalt_branch_norm_check", [ctypes.POINTER(BranchNormArgs), c_int32]),
         ("dsalt_add_rms_norm", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int32,
                                 c_void_p]),
     ):
@@ -266,13 +313,18 @@ def lib() -> ctypes.CDLL:
     h.dsalt_module_grads_workspace_size.restype = c_int64
     h.dsalt_norm_train_workspace_size.argtypes = [c_int64, c_int32]
     h.dsalt_norm_train_workspace_size.restype = c_int64
+    h.dsalt_gated_ffn_workspace_size.argtypes = [c_int64] + [c_int32] * 4
+    h.dsalt_gated_ffn_workspace_size.restype = c_int64
+    h.dsalt_branch_norm_workspace_size.argtypes = [c_int64, c_int32]
+    h.dsalt_branch_norm_workspace_size.restype = c_int64
     h.dsalt_lmk_weights_workspace_size.argtypes = [c_int32] * 2
     h.dsalt_lmk_weights_workspace_size.restype = c_int64
     h.dsalt_abi_version.restype = ctypes.c_int
     h.dsalt_last_error.restype = ctypes.c_char_p
     for n in ("dsalt_fwd_args_size", "dsalt_bwd_args_size", "dsalt_select_args_size", "dsalt_scores_args_size",
               "dsalt_rope_args_size", "dsalt_lmk_weights_args_size", "dsalt_rope_tables_size", "dsalt_qkv_args_size",
-              "dsalt_module_grads_args_size", "dsalt_norm_train_args_size"):
+              "dsalt_module_grads_args_size", "dsalt_norm_train_args_size", "dsalt_gated_ffn_args_size",
+              "dsalt_dropout_args_size", "dsalt_branch_norm_args_size"):
         getattr(h, n).restype = c_size_t
     _lib = h
     check_abi()
@@ -288,7 +340,8 @@ def check_abi() -> None:
                        (RopeArgs, h.dsalt_rope_args_size), (LmkWeightsArgs, h.dsalt_lmk_weights_args_size),
                        (RopeTables, h.dsalt_rope_tables_size), (QkvArgs, h.dsalt_qkv_args_size),
                        (ModuleGradsArgs, h.dsalt_module_grads_args_size),
-                       (NormTrainArgs, h.dsalt_norm_train_args_size)):
+                       (NormTrainArgs, h.dsalt_norm_train_args_size), (GatedFfnArgs, h.dsalt_gated_ffn_args_size),
+                       (DropoutArgs, h.dsalt_dropout_args_size), (BranchNormArgs, h.dsalt_branch_norm_args_size)):
         if ctypes.sizeof(struct) != fn():
             raise DsaltError(f"{struct.__name__} layout mismatch: {ctypes.sizeof(struct)} vs {fn()} bytes")
 
@@ -324,6 +377,15 @@ def stream_handle(device: torch.device) -> int:
     """The raw handle of the current stream of `device` (read on every launch)."""
     index = device.index
     return _current_raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+def on_device(device: torch.device):
+    """A context whose current device is `device`, where launches on its streams (the default
+    one among them) belong."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(index)
 
 
 def compute_dtype(dtype: torch.dtype) -> torch.dtype:
@@ -1496,4 +1558,147 @@ def swiglu_rows(gate_up: torch.Tensor, d_out: torch.Tensor | None = None) -> tor
     out = torch.empty_like(gate_up) if d_out is not None else gate_up.new_empty(rows, f)
     _raise(lib().dsalt_swiglu_rows(gate_up.data_ptr(), _ptr(d_out), out.data_ptr(), rows, f,
                                    _SCORE_DTYPES[gate_up.dtype], stream_handle(dev)), "dsalt_swiglu_rows")
+    return out
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}  # DSALT_ACT_*
+
+
+def row_operand(t: torch.Tensor) -> torch.Tensor:
+    """t [n, m] as dsalt_gated_ffn reads it: unit stride along the rows, row strides that are
+    multiples of 8 and cover a row, 16-byte aligned (a copy only where it is not so)."""
+    if (t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.shape[1] <= t.stride(0) <= 1 << 21 and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _gated_ffn_args(rows, x, w_gate, w_up, w_down, activation: str) -> GatedFfnArgs:
+    f, d = w_gate.shape
+    return GatedFfnArgs(rows=rows, d=d, f=f, e=w_down.shape[0], dtype=_DTYPES[w_gate.dtype],
+                        activation=ACTIVATIONS[activation], x=_ptr(x), x_stride=d if x is None else x.stride(0),
+                        w_gate=w_gate.data_ptr(), w_up=w_up.data_ptr(), w_down=w_down.data_ptr(),
+                        w_gate_stride=w_gate.stride(0), w_up_stride=w_up.stride(0), w_down_stride=w_down.stride(0))
+
+
+def _ffn_workspace(a: GatedFfnArgs, backward: bool, dev: torch.device) -> torch.Tensor | None:
+    a.workspace_bytes = lib().dsalt_gated_ffn_workspace_size(a.rows, a.d, a.f, a.e, int(backward))
+    if a.workspace_bytes == 0:
+        return None
+    ws = torch.empty(a.workspace_bytes, device=dev, dtype=torch.uint8)
+    a.workspace = ws.data_ptr()
+    return ws
+
+
+def gated_ffn(x, w_gate, w_up, w_down, activation: str, lead, keep: bool):
+    """``(y [*lead, e], gate_up, act)`` of `row_operand` x [T, d] and weights: see dsalt_gated_ffn.
+    gate_up is None without `keep`."""
+    dev = require_gpu(x, w_gate, w_up, w_down)
+    a = _gated_ffn_args(x.shape[0], x, w_gate, w_up, w_down, activation)
+    act, y = x.new_empty(a.rows, a.f), x.new_empty(*lead, a.e)
+    gate_up = x.new_empty(a.rows, 2 * a.f) if keep else None
+    a.act, a.y, a.gate_up = act.data_ptr(), y.data_ptr(), _ptr(gate_up)
+    ws = _ffn_workspace(a, False, dev)  # noqa: F841  (held over the call)
+    with on_device(dev):
+        _raise(lib().dsalt_gated_ffn(ctypes.byref(a), stream_handle(dev)), "dsalt_gated_ffn")
+    return y, gate_up, act
+
+
+def gated_ffn_bwd(x, w_gate, w_up, w_down, activation: str, gate_up, act, dy, need):
+    """``(dx [T, d], dw_gate, dw_up, dw_down)``, None where not in `need`: see dsalt_gated_ffn_bwd.
+    x and gate_up may be None where only dw_down is needed."""
+    dev = require_gpu(x, w_gate, w_up, w_down, gate_up, act, dy)
+    a = _gated_ffn_args(dy.shape[0], x, w_gate, w_up, w_down, activation)
+    a.gate_up, a.act, a.dy, a.dy_stride = _ptr(gate_up), act.data_ptr(), dy.data_ptr(), dy.stride(0)
+    shapes = ((a.rows, a.d), w_gate.shape, w_up.shape, w_down.shape)
+    out = [dy.new_empty(s) if n else None for s, n in zip(shapes, need)]
+    a.dx, a.dw_gate, a.dw_up, a.dw_down = (_ptr(t) for t in out)
+    d_gate_up = torch.empty_like(gate_up) if any(need[:3]) else None
+    a.d_gate_up = _ptr(d_gate_up)
+    ws = _ffn_workspace(a, True, dev)  # noqa: F841
+    with on_device(dev):
+        _raise(lib().dsalt_gated_ffn_bwd(ctypes.byref(a), stream_handle(dev)), "dsalt_gated_ffn_bwd")
+    return out
+
+
+def seed_fields(seed, device: torch.device) -> tuple[int, int | None]:
+    """(seed, seed_ptr) of a Python int or of an int64 GPU tensor of one element."""
+    if isinstance(seed, torch.Tensor):
+        if require_gpu(seed) != device or seed.dtype != torch.int64 or seed.numel() != 1:
+            raise DsaltError(f"a seed tensor must be one int64 element on {device} (got {tuple(seed.shape)} {seed.dtype} "
+                             f"on {seed.device})")
+        return 0, seed.data_ptr()
+    if not -2 ** 63 <= seed < 2 ** 64:
+        raise ValueError(f"seed must fit 64 bits (got {seed})")
+    return (seed + 2 ** 63) % 2 ** 64 - 2 ** 63, None
+
+
+def keep_threshold(p: float) -> int:
+    """The probability of keeping an element, in units of 2^-16."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"the dropout probability must be in [0, 1] (got {p})")
+    return round((1.0 - p) * 65536)
+
+
+def dropout(x: torch.Tensor, p: float, seed, offset: int) -> torch.Tensor:
+    """Contiguous dropout of contiguous, 16-byte aligned x: see dsalt_dropout."""
+    dev = require_gpu(x)
+    out = torch.empty_like(x)
+    a = DropoutArgs(n=x.numel(), dtype=_SCORE_DTYPES[x.dtype], threshold=keep_threshold(p), x=x.data_ptr(),
+                    out=out.data_ptr(), offset=offset)
+    a.seed, a.seed_ptr = seed_fields(seed, dev)
+    with on_device(dev):
+        _raise(lib().dsalt_dropout(ctypes.byref(a), stream_handle(dev)), "dsalt_dropout")
+    return out
+
+
+BRANCH_NORM_MAX_DIM = 8192  # largest row length of dsalt_branch_norm
+
+
+def _branch_args(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, eps, post_eps, out_dtype):
+    d = x.shape[-1]
+    a = BranchNormArgs(rows=x.numel() // d, d=d, x_dtype=_SCORE_DTYPES[x.dtype], h_dtype=_SCORE_DTYPES[h.dtype],
+                       y_dtype=_SCORE_DTYPES[out_dtype], threshold=keep_threshold(p), eps=eps, post_eps=post_eps,
+                       residual_scale=residual_scale, offset=offset, x=x.data_ptr(), h=h.data_ptr(),
+                       weight=_ptr(weight), post_weight=_ptr(post_weight), gate=_ptr(gate))
+    for name, t in (("w_dtype", weight), ("post_dtype", post_weight), ("gate_dtype", gate)):
+        if t is not None:
+            setattr(a, name, _SCORE_DTYPES[t.dtype])
+    if gate is not None:
+        a.gate_kind = 1 if gate.dim() == 1 else 2
+    if a.threshold < 65536:
+        a.seed, a.seed_ptr = seed_fields(seed, x.device)
+    return a
+
+
+def branch_norm(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, eps, post_eps, out_dtype, keep: bool):
+    """``(x_out, y, rstd, rstd_post)`` of contiguous, aligned operands: see dsalt_branch_norm; gate
+    [d] or [..., 1]. The statistics are None without `keep`."""
+    dev = require_gpu(x, h, weight, post_weight, gate)
+    a = _branch_args(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, eps, post_eps, out_dtype)
+    x_out = torch.empty_like(x)
+    y = torch.empty_like(x, dtype=out_dtype) if weight is not None else None
+    rstd, rstd_post = (torch.empty(a.rows, device=dev, dtype=torch.float32) if keep and w is not None else None
+                       for w in (weight, post_weight))
+    a.x_out, a.y, a.rstd, a.rstd_post = x_out.data_ptr(), _ptr(y), _ptr(rstd), _ptr(rstd_post)
+    with on_device(dev):
+        _raise(lib().dsalt_branch_norm(ctypes.byref(a), stream_handle(dev)), "dsalt_branch_norm")
+    return x_out, y, rstd, rstd_post
+
+
+def branch_norm_bwd(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, out_dtype, rstd, rstd_post, dx_out, dy,
+                    need):
+    """``(dx, dh, d_weight, d_post_weight, d_gate)``, None where not in `need`: see
+    dsalt_branch_norm_bwd."""
+    dev = require_gpu(x, h, weight, post_weight, gate, dx_out, dy)
+    a = _branch_args(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, 0.0, 0.0, out_dtype)
+    a.rstd, a.rstd_post, a.dx_out, a.dy = _ptr(rstd), _ptr(rstd_post), _ptr(dx_out), _ptr(dy)
+    out = [torch.empty_like(t) if n else None for t, n in zip((x, h, weight, post_weight, gate), need)]
+    a.dx, a.dh, a.d_weight, a.d_post_weight, a.d_gate = (_ptr(t) for t in out)
+    ws = None
+    if need[2] or need[3] or (need[4] and a.gate_kind == 1):
+        a.workspace_bytes = lib().dsalt_branch_norm_workspace_size(a.rows, a.d)
+        ws = torch.empty(a.workspace_bytes, device=dev, dtype=torch.uint8)
+        a.workspace = ws.data_ptr()
+    with on_device(dev):
+        _raise(lib().dsalt_branch_norm_bwd(ctypes.byref(a), stream_handle(dev)), "dsalt_branch_norm_bwd")
     return out

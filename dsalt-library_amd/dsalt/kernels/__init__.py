@@ -15,7 +15,10 @@ is not part of this package.
 """
 from .. import _hip
 from .RMSENorm import RMSENorm
+from .branch_norm import branch_norm
+from .dropout import counter_dropout
 from .dsalt_triton_train import dsalt_triton_train_attention
+from .gated_ffn import gated_ffn
 from .landmark_tokens_ker import (
     HybridEnergyLandmarkSelector,
     compute_hybrid_scores,
@@ -54,6 +57,9 @@ __all__ = [
     "dsalt_triton_train_attention",
     "autotune_blocks",
     "get_tuned_config",
+    "gated_ffn",
+    "counter_dropout",
+    "branch_norm",
     "RMSENorm",
     "compute_window_sizes",
     "build_local_window_mask",

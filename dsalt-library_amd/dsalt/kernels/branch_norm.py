@@ -1,0 +1,105 @@
+"""A block's branch joined to its residual stream in one pass forward and one backward: dropout
+and RMSNorm of the branch's output, its gate, the scaled residual sum, and the RMSNorm that
+the next branch reads (the pre-norm block of dsalt_transformer.py:81-84 with a norm after its
+branch, a layer scale or token gate and a residual scale).
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _hip
+from ._block_train import graph_grads, without_autocast
+from ._sparse import no_graph
+from .dropout import _Dropout, check_seed
+from .dsalt_triton_attn import _dynamo_opaque
+
+
+def torch_branch_norm(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, eps, post_eps, out_dtype):
+    """``branch_norm`` in torch's ops (and the dropout pass), in fp32 or more."""
+    def wide(t):
+        return t.float() if t.dtype in (torch.bfloat16, torch.float16) else t
+
+    def norm(t, w, e):
+        return t * torch.rsqrt(t.square().mean(-1, keepdim=True) + e) * wide(w)
+
+    n = wide(h)
+    if _hip.keep_threshold(p) < 65536:
+        n = _Dropout.apply(n, p, seed, offset)
+    if post_weight is not None:
+        n = norm(n, post_weight, post_eps)
+    z = residual_scale * wide(x) + (n if gate is None else wide(gate) * n)
+    return z.to(x.dtype), None if weight is None else norm(z, weight, eps).to(out_dtype)
+
+
+class _BranchNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, h, weight, post_weight, gate, seed, opts):
+        ctx.set_materialize_grads(False)
+        residual_scale, p, offset, eps, post_eps, out_dtype = opts
+        ops = [None if t is None else _hip.aligned_rows(t.detach()) for t in (x, h, weight, post_weight, gate)]
+        x_out, y, rstd, rstd_post = _hip.branch_norm(*ops, residual_scale, p, seed, offset, eps, post_eps, out_dtype, True)
+        is_tensor = isinstance(seed, torch.Tensor)
+        ctx.save_for_backward(x, h, weight, post_weight, gate, rstd, rstd_post, seed if is_tensor else None)
+        ctx.dsalt = opts, None if is_tensor else seed
+        return x_out, y
+
+    @staticmethod
+    @without_autocast
+    def backward(ctx, dx_out, dy):
+        *inputs, rstd, rstd_post, seed = ctx.saved_tensors
+        opts, seed_value = ctx.dsalt
+        seed = seed_value if seed is None else seed
+        residual_scale, p, offset, eps, post_eps, out_dtype = opts
+        need = ctx.needs_input_grad[:5]
+        if dx_out is None and dy is None:
+            return (None,) * 7
+        if torch.is_grad_enabled():  # a graph of the backward is wanted: torch's own ops
+            grads = graph_grads(lambda *t: tuple(o for o in torch_branch_norm(*t, residual_scale, p, seed, offset, eps, post_eps,
+                                                                              out_dtype) if o is not None),
+                                inputs, (dx_out, dy) if inputs[2] is not None else (dx_out,))
+            return *grads, None, None
+        ops = [None if t is None else _hip.aligned_rows(t.detach()) for t in inputs]
+        dx_out, dy = (None if t is None else _hip.aligned_rows(t) for t in (dx_out, dy))
+        # without a gradient of y its norm's weight gets zeros
+        w_need = need[2] and dy is not None
+        grads = _hip.branch_norm_bwd(*ops, residual_scale, p, seed, offset, out_dtype, rstd, rstd_post, dx_out, dy,
+                                     (*need[:2], w_need, *need[3:]))
+        return *grads, None, None
+
+
+@_dynamo_opaque
+def branch_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor | None = None, *,
+                post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, residual_scale: float = 1.0,
+                p: float = 0.0, seed=None, offset: int = 0, eps: float = 1e-6, post_eps: float | None = None,
+                out_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``(x_out, y)`` of the residual stream x [..., d] and a branch's output h of its shape::
+
+        n     = rms_norm(dropout(h, p)) * post_weight      (without post_weight: dropout(h, p))
+        x_out = residual_scale * x + gate * n
+        y     = rms_norm(x_out) * weight                   (None without weight)
+
+    The dropout is ``counter_dropout(h, p, seed, offset)``. ``gate``: per channel [d], per token
+    [..., 1], or none. x bf16, fp16 or fp32; h and ``out_dtype`` (y's type, by default x's) x's
+    dtype, or any of the three beside an fp32 x; weights and gate in x's dtype or fp32. x_out has
+    x's dtype; y is formed from the sum before that rounding. d a multiple of 8 up to 8192.
+    Differentiable in x, h, weight, post_weight and gate. Other operands raise ``DsaltError``."""
+    dev = _hip.require_gpu(x, h, weight, post_weight, gate)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    post_eps = eps if post_eps is None else post_eps
+    check_seed(p, seed, offset)
+    _hip.seed_fields(0 if seed is None else seed, dev)
+    d = x.shape[-1] if x.dim() else 0
+    ok = (x.dtype in _hip._SCORE_DTYPES and h.shape == x.shape and 8 <= d <= _hip.BRANCH_NORM_MAX_DIM and d % 8 == 0
+          and all(t == x.dtype or (x.dtype == torch.float32 and t in _hip._SCORE_DTYPES) for t in (h.dtype, out_dtype))
+          and all(w is None or (w.shape == (d,) and w.dtype in (x.dtype, torch.float32)) for w in (weight, post_weight))
+          and (gate is None or (gate.shape in ((d,), (*x.shape[:-1], 1)) and gate.dtype in (x.dtype, torch.float32))))
+    if not ok:
+        raise _hip.DsaltError(
+            f"branch_norm needs x and h [..., d] of one shape, d a multiple of 8 up to {_hip.BRANCH_NORM_MAX_DIM}, h and the "
+            f"output in x's dtype or x fp32, weights [d] and a gate [d] or [..., 1] in x's dtype or fp32 (got "
+            f"{[None if t is None else (tuple(t.shape), t.dtype) for t in (x, h, weight, post_weight, gate)]}, {out_dtype})")
+    opts = (float(residual_scale), float(p), offset, float(eps), float(post_eps), out_dtype)
+    if no_graph(x, h, weight, post_weight, gate):
+        ops = (None if t is None else _hip.aligned_rows(t) for t in (x, h, weight, post_weight, gate))
+        return _hip.branch_norm(*ops, opts[0], opts[1], seed, *opts[2:], False)[:2]
+    return _BranchNorm.apply(x, h, weight, post_weight, gate, seed, opts)

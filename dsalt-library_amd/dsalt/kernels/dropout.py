@@ -1,0 +1,63 @@
+"""Dropout whose mask is a function of a seed and the element's index, so that it is never stored:
+the backward forms it again. ``nn.Dropout`` draws from torch's generator and keeps the mask.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _hip
+from ._sparse import no_graph
+from .dsalt_triton_attn import _dynamo_opaque
+
+
+def draw_seed(device: torch.device) -> torch.Tensor:
+    """A seed [1] (int64) on the GPU from torch's generator of that device: it follows
+    ``torch.manual_seed`` and the generator state that checkpointing restores, costs no
+    synchronisation, and a captured graph draws a new one on every replay."""
+    return torch.randint(-2 ** 63, 2 ** 63 - 1, (1,), device=device, dtype=torch.int64)
+
+
+def check_seed(p: float, seed, offset) -> None:
+    if _hip.keep_threshold(p) < 65536 and seed is None:
+        raise ValueError("a dropout probability above 0 needs a seed")
+    if not 0 <= offset < 2 ** 63:
+        raise ValueError(f"offset must be in [0, 2^63) (got {offset})")
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, offset):
+        is_tensor = isinstance(seed, torch.Tensor)
+        ctx.save_for_backward(seed if is_tensor else None)
+        ctx.dsalt = p, None if is_tensor else seed, offset
+        return _hip.dropout(_hip.aligned_rows(x.detach()), p, seed, offset)
+
+    @staticmethod
+    def backward(ctx, dy):
+        p, seed, offset = ctx.dsalt
+        saved, = ctx.saved_tensors
+        # linear: under a graph of the backward its gradient is the same function again
+        return _Dropout.apply(dy, p, seed if saved is None else saved, offset), None, None, None
+
+
+@_dynamo_opaque
+def counter_dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
+    """Dropout of x with probability p: a kept element is scaled by the inverse of the probability
+    of keeping, a dropped one is 0 whatever it holds. p is taken to the nearest multiple of
+    2^-16, and the scale is of that p.
+
+    The mask depends on ``seed`` (an int of 64 bits, or one int64 element on x's GPU, read when
+    the kernel runs: a replayed graph sees its new value), ``offset`` (0 to 2^63 - 1: tells
+    apart the places that use one seed) and the element's index in x's logical order, and
+    on nothing else. bf16, fp16 or fp32 of any shape. Differentiable in x; a seed tensor
+    changed in place before the backward is refused."""
+    dev = _hip.require_gpu(x)
+    if x.dtype not in _hip._SCORE_DTYPES:
+        raise _hip.DsaltError(f"counter_dropout needs a bf16, fp16 or fp32 tensor (got {x.dtype})")
+    check_seed(p, seed, offset)
+    if seed is None:
+        seed = 0
+    _hip.seed_fields(seed, dev)
+    if no_graph(x):
+        return _hip.dropout(_hip.aligned_rows(x), p, seed, offset)
+    return _Dropout.apply(x, p, seed, offset)

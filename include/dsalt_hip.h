@@ -615,6 +615,102 @@ int dsalt_lmk_weights(const dsalt_lmk_weights_args *args, void *stream);
 int dsalt_lmk_weights_bwd(const dsalt_lmk_weights_args *args, void *stream);
 int dsalt_lmk_weights_check(const dsalt_lmk_weights_args *args, int32_t backward);
 
+/*
+ * Gated feed-forward block of [rows, d] hidden states, forward and backward:
+ *   a = act(x w_gate^T) * (x w_up^T)   [rows, f]      y = a w_down^T   [rows, e]
+ * w_gate, w_up [f, d], w_down [e, f]; act one of DSALT_ACT_*. Products accumulate in fp32; a (and
+ * gate_up, where it is kept) is rounded once from fp32, y once.
+ * dsalt_gated_ffn writes `act` and y, and gate_up [rows, 2 f] (gate | up) unless it is NULL.
+ * dsalt_gated_ffn_bwd reads gate_up and `act` as the forward left them and dy [rows, e]; writes
+ * dw_down [e, f], and with d_gate_up [rows, 2 f] (the gradient of gate_up; scratch, dead when
+ * the launches end) dx [rows, d], dw_gate and dw_up [f, d]; each result may be NULL. Sums run in
+ * a fixed order. rows = 0 gives zero weight gradients.
+ * dtype BF16 or F16 for every tensor. d, e, f multiples of 8 in [8, 2^20]; row strides (in
+ * elements) multiples of 8 up to 2^21 and at least the row length, the other tensors contiguous;
+ * 16-byte aligned pointers; outputs alias no input. workspace: at least
+ * dsalt_gated_ffn_workspace_size bytes, 16-byte aligned, dead when the launches end (NULL where
+ * that is 0).
+ * Replaces SwiGLUFFN.forward (dsalt/modules/dsalt_transformer.py:10-21) with its autograd.
+ */
+enum { DSALT_ACT_SILU = 0, DSALT_ACT_GELU = 1 /* erf */, DSALT_ACT_GELU_TANH = 2, DSALT_ACT_RELU = 3 };
+typedef struct dsalt_gated_ffn_args {
+    int64_t rows;
+    int32_t d, f, e;
+    int32_t dtype, activation, reserved;
+    const void *x;
+    int64_t x_stride;
+    const void *w_gate, *w_up, *w_down;
+    int64_t w_gate_stride, w_up_stride, w_down_stride;
+    void *gate_up, *act, *y;
+    const void *dy;
+    int64_t dy_stride;
+    void *d_gate_up, *dx, *dw_gate, *dw_up, *dw_down;
+    void *workspace;
+    int64_t workspace_bytes;
+} dsalt_gated_ffn_args;
+int dsalt_gated_ffn(const dsalt_gated_ffn_args *args, void *stream);
+int dsalt_gated_ffn_bwd(const dsalt_gated_ffn_args *args, void *stream);
+int dsalt_gated_ffn_check(const dsalt_gated_ffn_args *args, int32_t backward);
+int64_t dsalt_gated_ffn_workspace_size(int64_t rows, int32_t d, int32_t f, int32_t e, int32_t backward);
+size_t dsalt_gated_ffn_args_size(void);
+
+/*
+ * Dropout without a stored mask: out[i] = x[i] * 65536 / threshold where the element's 16 random
+ * bits are below `threshold` (0 .. 65536: the probability of keeping, in 2^-16), else 0 whatever
+ * x[i] holds. The bits of element i are half i % 2 (low first) of word (i % 8) / 2 of Philox4x32
+ * with 7 rounds at counter (i / 8, offset) under key seed, so that the same call on the
+ * gradient is the backward. seed_ptr: the seed is read from the device (NULL: `seed`).
+ * n elements of dtype BF16, F16 or F32, contiguous, 16-byte aligned; out may be x.
+ */
+typedef struct dsalt_dropout_args {
+    int64_t n;
+    int32_t dtype, threshold;
+    const void *x;
+    void *out;
+    int64_t seed, offset;
+    const int64_t *seed_ptr;
+} dsalt_dropout_args;
+int dsalt_dropout(const dsalt_dropout_args *args, void *stream);
+size_t dsalt_dropout_args_size(void);
+
+/*
+ * A block's branch h joined to its residual stream x, rows [rows, d], contiguous:
+ *   hd = dropout(h) (as dsalt_dropout with threshold < 65536 over h's elements), else h
+ *   n  = hd * rstd_post * post_weight, rstd_post = rsqrt(mean(hd^2) + post_eps); hd without it
+ *   x_out = residual_scale * x + gate * n
+ *   y  = x_out * rstd * weight, rstd = rsqrt(mean(x_out^2) + eps); no y without weight
+ * gate_kind 0: no gate (1); 1: gate [d]; 2: gate [rows]. x_out is rounded to x's dtype, y (in
+ * y_dtype) formed from the fp32 x_out. rstd, rstd_post [rows] fp32 may be NULL in the forward
+ * and are what the backward reads. Backward: from dx_out and dy (either may be NULL, not both)
+ * dx (x's dtype), dh (h's dtype), d_gate, d_weight, d_post_weight in their tensors' dtypes, each
+ * of which may be NULL; the column sums need workspace of dsalt_branch_norm_workspace_size(rows,
+ * d) bytes, dead when the launches end. fp32 arithmetic, sums in a fixed order.
+ * dtypes: x BF16 or F16 with h and y of the same, or x F32 with h and y of any; weights and gate
+ * of x's dtype or F32. d a multiple of 8 up to 8192; 16-byte aligned pointers (statistics 4,
+ * a [rows] gate its element's); outputs alias no input.
+ */
+typedef struct dsalt_branch_norm_args {
+    int64_t rows;
+    int32_t d;
+    int32_t x_dtype, h_dtype, y_dtype, w_dtype, post_dtype, gate_dtype;
+    int32_t gate_kind, threshold;
+    float eps, post_eps, residual_scale;
+    int64_t seed, offset;
+    const int64_t *seed_ptr;
+    const void *x, *h, *weight, *post_weight, *gate;
+    void *x_out, *y;
+    float *rstd, *rstd_post;
+    const void *dx_out, *dy;
+    void *dx, *dh, *d_weight, *d_post_weight, *d_gate;
+    void *workspace;
+    int64_t workspace_bytes;
+} dsalt_branch_norm_args;
+int dsalt_branch_norm(const dsalt_branch_norm_args *args, void *stream);
+int dsalt_branch_norm_bwd(const dsalt_branch_norm_args *args, void *stream);
+int dsalt_branch_norm_check(const dsalt_branch_norm_args *args, int32_t backward);
+int64_t dsalt_branch_norm_workspace_size(int64_t rows, int32_t d);
+size_t dsalt_branch_norm_args_size(void);
+
 int dsalt_abi_version(void);
 const char *dsalt_last_error(void);
 /* sizeof of the argument structs as compiled into the library (ABI layout check). */

@@ -1,0 +1,261 @@
+"""branch_norm (dropout, norm, gate and scaled residual sum of a branch, and the next norm, one
+pass forward and one backward) against float64 autograd."""
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+from dsalt import _hip
+from dsalt.kernels import _block_train, branch_norm, counter_dropout
+from dsalt.kernels.RMSENorm import RMSENorm
+from philox_reference import keep_mask
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+NAMES = ("x", "h", "weight", "post_weight", "gate")
+
+
+def inputs(lead, d, xd, hd, od, post=True, pre=True, gate="channel", wd=None, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed + d)
+    wd = xd if wd is None else wd
+
+    def rnd(dt, *s, std=1.0, mean=0.0):
+        return (torch.randn(*s, device=DEV, generator=g) * std + mean).to(dt)
+
+    t = {"x": rnd(xd, *lead, d, std=2.0), "h": rnd(hd, *lead, d), "weight": rnd(wd, d, std=0.25, mean=1.0) if pre else None,
+         "post_weight": rnd(wd, d, std=0.25, mean=1.0) if post else None,
+         "gate": {"none": None, "channel": rnd(wd, d, std=0.5, mean=0.5), "token": rnd(wd, *lead, 1)}[gate]}
+    return t, rnd(xd, *lead, d), rnd(od, *lead, d)
+
+
+def reference(t, p, seed, offset, rs, eps, dz, dy):
+    w = {n: v.detach().double().requires_grad_() for n, v in t.items() if v is not None}
+    n = w["h"]
+    th = _hip.keep_threshold(p)
+    if th < 65536:
+        keep = torch.from_numpy(keep_mask(n.numel(), p, seed, offset)).view(n.shape).to(n.device)
+        n = torch.where(keep, n * (65536.0 / max(th, 1)), 0.0)
+    if "post_weight" in w:
+        n = n * torch.rsqrt(n.square().mean(-1, keepdim=True) + eps) * w["post_weight"]
+    z = rs * w["x"] + (w["gate"] * n if "gate" in w else n)
+    outs, ups = [z], [dz]
+    if "weight" in w:
+        outs.append(z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * w["weight"])
+        ups.append(dy)
+    pairs = [(o, u.double()) for o, u in zip(outs, ups) if u is not None]
+    grads = torch.autograd.grad([o for o, _ in pairs], list(w.values()), [u for _, u in pairs], allow_unused=True)
+    return [o.detach() for o in outs], dict(zip(w, grads))
+
+
+def close(got, want, dtype, what, rows_summed=1):
+    """One rounding to the dtype, plus fp32 arithmetic: a row's sums of d <= 8192 terms and the
+    column sums stay within 2^-18 of the largest magnitudes they are formed from (2^-24 a
+    term's rounding; sums run over at most 64 terms a lane, then in trees), which the row's
+    or column's largest value stands for."""
+    assert got.dtype == dtype and got.shape == want.shape, what
+    err = (got.double() - want).abs()
+    scale = want.abs().max() * rows_summed ** 0.5
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -18 * scale + (2.0 ** -25 if dtype == HF else 0.0)
+    assert bool((err <= tol).all()), (what, float((err / tol).max()))
+
+
+def run(t, dz, dy, **kw):
+    leaves = {n: v.detach().clone().requires_grad_() for n, v in t.items() if v is not None}
+    outs = [o for o in branch_norm(leaves["x"], leaves["h"], leaves.get("weight"), post_weight=leaves.get("post_weight"),
+                                   gate=leaves.get("gate"), **kw) if o is not None]
+    pairs = [(o, u) for o, u in zip(outs, (dz, dy)) if u is not None]
+    grads = torch.autograd.grad([o for o, _ in pairs], list(leaves.values()), [u for _, u in pairs], allow_unused=True)
+    return [o.detach() for o in outs], dict(zip(leaves, grads))
+
+
+def compare(t, dz, dy, rs=0.75, p=0.2, seed=77, offset=5, eps=1e-6, od=None):
+    kw = dict(residual_scale=rs, p=p, seed=seed, offset=offset, eps=eps, out_dtype=od)
+    outs, grads = run(t, dz, dy, **kw)
+    w_outs, w_grads = reference(t, p, seed, offset, rs, eps, dz, dy)
+    for n, a, b in zip(("x_out", "y"), outs, w_outs):
+        close(a, b, t["x"].dtype if n == "x_out" or od is None else od, n)
+    rows = t["x"].numel() // t["x"].shape[-1]
+    for n, g in grads.items():
+        if w_grads[n] is None:
+            assert g is None or not bool(g.any()), n
+            continue
+        close(g, w_grads[n], t[n].dtype, "d" + n, 1 if n in ("x", "h") else max(1, rows / 64))
+    with torch.no_grad():
+        bare = branch_norm(t["x"], t["h"], t["weight"], post_weight=t["post_weight"], gate=t["gate"], **kw)
+    assert all(torch.equal(a, b) for a, b in zip(outs, bare))
+    return outs, grads
+
+
+@pytest.mark.parametrize("xd,hd,od,wd", [(FP, BF, BF, FP), (FP, HF, FP, FP), (FP, FP, FP, FP), (FP, FP, HF, FP), (FP, BF, HF, FP),
+                                         (BF, BF, BF, BF), (BF, BF, BF, FP), (HF, HF, HF, HF), (HF, HF, HF, FP)])
+@pytest.mark.parametrize("rows,d", [(1, 8), (3, 512), (5, 520), (3101, 1024), (7, 1032), (2, 2056), (1601, 4096), (3, 4104), (513, 8192)])
+def test_types_and_sizes(rows, d, xd, hd, od, wd):
+    print(f"branch_norm {rows}x{d} {xd} {hd} {od} {wd}", flush=True)
+    t, dz, dy = inputs((rows,), d, xd, hd, od, wd=wd)
+    compare(t, dz, dy, od=od)
+
+
+@pytest.mark.parametrize("post,pre,gate,p", list(itertools.product((True, False), (True, False), ("none", "channel", "token"),
+                                                                   (0.0, 0.3))))
+def test_forms(post, pre, gate, p):
+    for rows, d in ((37, 200), (9, 1536)):
+        print(f"branch_norm form post={post} pre={pre} gate={gate} p={p} {rows}x{d}", flush=True)
+        t, dz, dy = inputs((rows,), d, FP, BF, BF, post, pre, gate)
+        compare(t, dz, dy if pre else None, p=p, od=BF)
+        compare(t, dz, None, p=p, od=BF)  # only the stream's gradient
+        if pre:
+            compare(t, None, dy, p=p, od=BF)  # only the norm's
+
+
+def test_leading_dimensions_strides_and_alignment():
+    t, dz, dy = inputs((3, 4), 136, BF, BF, BF, gate="token")
+    want = run(t, dz, dy, p=0.2, seed=3)
+    compare(t, dz, dy)
+    for n in ("x", "h"):
+        off = torch.zeros(t[n].numel() + 3, device=DEV, dtype=BF)[3:].view(3, 4, 136)
+        off.copy_(t[n])
+        wide = torch.zeros(3, 4, 272, device=DEV, dtype=BF)[..., ::2]
+        wide.copy_(t[n])
+        for v in (off, wide):
+            got = run({**t, n: v}, dz.transpose(0, 1).contiguous().transpose(0, 1), dy.expand(3, 4, 136), p=0.2, seed=3)
+            assert all(torch.equal(a, b) for a, b in zip(got[0], want[0]))
+            assert all(torch.equal(got[1][k], want[1][k]) for k in want[1])
+
+
+def test_no_rows():
+    t, dz, dy = inputs((0,), 64, FP, BF, BF)
+    outs, grads = run(t, dz, dy, out_dtype=BF)
+    assert outs[0].shape == (0, 64) and outs[1].dtype == BF
+    assert all(not bool(grads[n].any()) for n in ("weight", "post_weight", "gate"))
+
+
+def test_rows_of_zeros_and_dropped_rows():
+    """A branch that is all zero or all dropped leaves the scaled residual; its norm divides by
+    sqrt(eps), never by 0."""
+    t, dz, dy = inputs((6,), 72, FP, FP, FP)
+    t["h"][2] = 0
+    t["x"][4] = 0
+    compare(t, dz, dy, p=0.0)
+    outs, grads = run(t, dz, dy, p=1.0, seed=1, residual_scale=0.5)
+    assert torch.equal(outs[0], 0.5 * t["x"]) and not bool(grads["h"].any())
+
+
+def test_nan_stays_in_its_row():
+    t, dz, dy = inputs((9,), 1536, BF, BF, BF)
+    outs, grads = run(t, dz, dy, p=0.1, seed=2)
+    t2 = {**t, "h": t["h"].clone()}
+    t2["h"][3] = float("nan")
+    o2, g2 = run(t2, dz, dy, p=0.1, seed=2)
+    keep = [r for r in range(9) if r != 3]
+    for a, b in (*zip(o2, outs), (g2["x"], grads["x"]), (g2["h"], grads["h"])):
+        assert torch.equal(a[keep], b[keep]) and bool(a[3].isnan().any())
+
+
+def test_equals_the_parts():
+    """Dropout alone in the branch, no gate and scale 1: x_out has the bits of counter_dropout and
+    the add; without dropout either, those of the block's add + norm pass."""
+    t, _, _ = inputs((50,), 256, FP, FP, FP, post=False, gate="none")
+    x, h = t["x"], t["h"]
+    x_out, _ = branch_norm(x, h, p=0.3, seed=4, offset=2)
+    assert torch.equal(x_out, x + counter_dropout(h, 0.3, 4, 2))
+    norm = RMSENorm(256).to(DEV)
+    s, y = _block_train.add_norm(x, h, norm)
+    got = branch_norm(x, h, norm.weight, eps=norm.eps)
+    assert torch.equal(got[0], s)
+    close(got[1].detach(), y.detach().double(), FP, "y")
+
+
+def test_second_order():
+    t, dz, dy = inputs((5,), 64, FP, FP, FP)
+    leaves = [t[n].detach().clone().requires_grad_() for n in NAMES]
+    wide = [v.detach().double().requires_grad_() for v in leaves]
+    out = []
+    for ls, up in ((leaves, (dz, dy)), (wide, (dz.double(), dy.double()))):
+        if ls is leaves:
+            x_out, y = branch_norm(ls[0], ls[1], ls[2], post_weight=ls[3], gate=ls[4], residual_scale=0.5)
+        else:
+            nrm = lambda v, w: v * torch.rsqrt(v.square().mean(-1, keepdim=True) + 1e-6) * w
+            x_out = 0.5 * ls[0] + ls[4] * nrm(ls[1], ls[3])
+            y = nrm(x_out, ls[2])
+        g = torch.autograd.grad((x_out, y), ls, up, create_graph=True)
+        out.append(torch.autograd.grad(sum(v.square().sum() for v in g), ls))
+    for a, b in zip(*out):
+        # some tens of fp32 roundings in a row, over sums of at most 320 terms
+        assert float((a.double() - b).norm()) <= 2.0 ** -17 * float(b.norm())
+
+
+def test_changed_in_place_is_refused():
+    for i, n in enumerate(("x", "h", "post_weight")):
+        t, dz, dy = inputs((4,), 64, FP, FP, FP)
+        ls = {k: v.detach().clone().requires_grad_() for k, v in t.items()}
+        x_out, y = branch_norm(ls["x"], ls["h"], ls["weight"], post_weight=ls["post_weight"], gate=ls["gate"])
+        with torch.no_grad():
+            ls[n].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad((x_out, y), list(ls.values()), (dz, dy))
+    x_out.add_(1)  # the stream may be modified in place
+
+
+@pytest.mark.parametrize("rows,d", [(40, 256), (40, 2048)])
+def test_streams_and_graph(rows, d):
+    t, dz, dy = inputs((rows,), d, FP, BF, BF)
+    seed = torch.tensor([12], device=DEV)
+    leaves = {n: v.detach().clone().requires_grad_() for n, v in t.items()}
+
+    def step():
+        x_out, y = branch_norm(leaves["x"], leaves["h"], leaves["weight"], post_weight=leaves["post_weight"],
+                               gate=leaves["gate"], residual_scale=0.75, p=0.2, seed=seed, offset=5, out_dtype=BF)
+        return x_out.detach(), y.detach(), *torch.autograd.grad((x_out, y), list(leaves.values()), (dz, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    outs, grads = run(t, dz, dy, residual_scale=0.75, p=0.2, seed=12, offset=5, out_dtype=BF)
+    assert all(torch.equal(a, b) for a, b in zip(other, (*outs, *grads.values())))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for s in (5, -9, 2 ** 60):
+        new, nz, ny = inputs((rows,), d, FP, BF, BF, seed=abs(s) % 100)
+        with torch.no_grad():
+            for n in leaves:
+                leaves[n].copy_(new[n])
+            dz.copy_(nz)
+            dy.copy_(ny)
+        seed.fill_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        outs, grads = run(new, nz, ny, residual_scale=0.75, p=0.2, seed=s, offset=5, out_dtype=BF)
+        assert all(torch.equal(a, b) for a, b in zip(got, (*outs, *grads.values()))), s
+
+
+def test_partial_gradients():
+    t, dz, dy = inputs((70,), 136, FP, BF, BF)
+    _, want = run(t, dz, dy, p=0.2, seed=1, out_dtype=BF)
+    for need in range(1, 32):
+        ls = {n: t[n].detach().clone().requires_grad_(bool(need >> i & 1)) for i, n in enumerate(NAMES)}
+        x_out, y = branch_norm(ls["x"], ls["h"], ls["weight"], post_weight=ls["post_weight"], gate=ls["gate"], p=0.2, seed=1,
+                               out_dtype=BF)
+        outs = [(o, u) for o, u in ((x_out, dz), (y, dy)) if o.requires_grad]
+        live = [n for n in NAMES if ls[n].requires_grad]
+        for n, g in zip(live, torch.autograd.grad([o for o, _ in outs], [ls[n] for n in live], [u for _, u in outs])):
+            assert torch.equal(g, want[n]), (need, n)
+
+
+def test_refusals_on_gpu():
+    t, _, _ = inputs((4,), 64, BF, BF, BF)
+    x, h, w = t["x"], t["h"], t["weight"]
+    for args, kw in (((x, h[:, :56]), {}), ((x, h.half()), {}), ((x, h, w.half()), {}), ((x, h, w[:8]), {}),
+                     ((x, h, w), {"out_dtype": FP}), ((x, h), {"gate": x}), ((x, h), {"gate": w[:8]}),
+                     ((x[:, :12].contiguous(), h[:, :12].contiguous()), {}), ((x.double(), h.double()), {}),
+                     ((x, h), {"p": 0.1, "seed": torch.tensor([1])}), ((x, h.cpu()), {}),
+                     ((x.new_zeros(2, 8200), x.new_zeros(2, 8200)), {})):
+        with pytest.raises(_hip.DsaltError):
+            branch_norm(*args, **kw)
+    for kw in ({"p": 0.1}, {"p": -1.0}, {"p": 0.1, "seed": 1, "offset": -1}):
+        with pytest.raises(ValueError):
+            branch_norm(x, h, **kw)

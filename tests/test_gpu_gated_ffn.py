@@ -1,0 +1,313 @@
+"""gated_ffn (both projections, activation and product in one kernel, with its backward) against
+float64, at the edges of its tiles and variants, with error bounds that follow the roundings."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from dsalt import _hip
+from dsalt.kernels import gated_ffn
+from dsalt.kernels.gated_ffn import torch_gated_ffn
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, HF = torch.bfloat16, torch.float16
+ACTS = ("silu", "gelu", "gelu_tanh", "relu")
+
+
+def inputs(rows, d, f, e, dtype, seed=0, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed + 1000 * rows + f)
+
+    def rnd(*s, std=1.0):
+        return (torch.randn(*s, device=DEV, generator=g) * std).to(dtype)
+
+    return (rnd(rows, d, std=scale), rnd(f, d, std=d ** -0.5), rnd(f, d, std=d ** -0.5), rnd(e, f, std=f ** -0.5),
+            rnd(rows, e, std=0.25))
+
+
+def act64(name, g):
+    g = g.detach().requires_grad_()
+    v = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"), "relu": F.relu}[name](g)
+    s, = torch.autograd.grad(v.sum(), g)
+    return v.detach(), s
+
+
+def reference(x, wg, wu, wd, dy, act, dtype):
+    """Float64 results and a bound of each one's error. A rounding to the dtype is off by at most
+    half a step (u relative), an fp32 sum of K products by at most (K + 8) 2^-24 of the sum of
+    their magnitudes. Carried to first order through the formulas; |act'| <= 1.13, |act''| <= 0.81
+    (GELU's, the largest), relu's slope is open where g is within its error of 0. 1 % more
+    for the products of errors; fp16's smallest step 2^-25 absolute."""
+    u = torch.finfo(dtype).eps / 2
+    x, wg, wu, wd, dy = (t.double() for t in (x, wg, wu, wd, dy))
+    gam = lambda k: (k + 8) * 2.0 ** -24
+    tiny = 2.0 ** -25 if dtype == HF else 0.0
+    g, p = x @ wg.t(), x @ wu.t()
+    eg, ep = gam(x.shape[1]) * (x.abs() @ wg.abs().t()), gam(x.shape[1]) * (x.abs() @ wu.abs().t())
+    v, s = act64(act, g)
+    a = v * p
+    ea = u * a.abs() + 1.13 * eg * p.abs() + v.abs() * ep + 2.0 ** -20 * (a.abs() + p.abs() * g.abs()) + tiny
+    y = a @ wd.t()
+    ey = u * y.abs() + (gam(a.shape[1]) * a.abs() + ea) @ wd.abs().t()
+    eg, ep = eg + u * g.abs() + tiny, ep + u * p.abs() + tiny  # g and u as they are kept
+    da, eda = dy @ wd, gam(dy.shape[1]) * (dy.abs() @ wd.abs())
+    dg, du = da * p * s, da * v
+    open_ = (0.81 * eg if act != "relu" else (g.abs() <= eg).double()) + 2.0 ** -20 * (1 + g.abs())
+    edg = u * dg.abs() + eda * p.abs() * s.abs() + da.abs() * (ep * s.abs() + p.abs() * open_) + tiny
+    edu = u * du.abs() + eda * v.abs() + da.abs() * (1.13 * eg + 2.0 ** -20 * g.abs()) + tiny
+    f, T = wg.shape[0], x.shape[0]
+    dx = dg @ wg + du @ wu
+    edx = u * dx.abs() + (gam(2 * f) * dg.abs() + edg) @ wg.abs() + (gam(2 * f) * du.abs() + edu) @ wu.abs()
+    res = {"y": (y, ey), "dx": (dx, edx)}
+    for n, m, em, k in (("dwg", dg, edg, x), ("dwu", du, edu, x)):
+        w = m.t() @ k
+        res[n] = (w, u * w.abs() + (gam(T) * m.abs() + em).t() @ k.abs())
+    w = dy.t() @ a
+    res["dwd"] = (w, u * w.abs() + dy.abs().t() @ (gam(T) * a.abs() + ea))
+    return {n: (w, 1.01 * e + tiny) for n, (w, e) in res.items()}
+
+
+def check(got, want, dtype, what):
+    """Every element within its bound; and all of them together within four half-steps of their
+    norm (up to three roundings in a chain, whose errors do not line up)."""
+    ref, bound = want
+    assert got.shape == ref.shape and got.dtype == dtype, what
+    err = (got.double() - ref).abs()
+    assert bool((err <= bound).all()), (what, float((err / bound.clamp(min=1e-30)).max()))
+    if ref.numel() > 64:
+        tiny = 2.0 ** -25 * ref.numel() ** 0.5 if dtype == HF else 0.0
+        assert float(err.norm()) <= 4 * torch.finfo(dtype).eps / 2 * float(ref.norm()) + tiny, (what, float(err.norm() / ref.norm()))
+
+
+def run(x, wg, wu, wd, dy, act):
+    leaves = [t.detach().clone().requires_grad_() for t in (x, wg, wu, wd)]
+    y = gated_ffn(*leaves, activation=act)
+    return dict(zip(("y", "dx", "dwg", "dwu", "dwd"), (y.detach(), *torch.autograd.grad(y, leaves, dy))))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("rows,d,f,e", [
+    (1, 8, 8, 8), (1, 72, 136, 40), (2, 128, 64, 264), (7, 64, 200, 8), (16, 520, 24, 56), (17, 72, 136, 40), (31, 8, 520, 16),
+    (33, 64, 64, 64), (64, 264, 104, 128), (65, 56, 128, 72), (127, 128, 384, 120), (128, 192, 256, 128), (129, 200, 264, 136),
+    (257, 320, 72, 328), (513, 72, 520, 64), (700, 264, 712, 264)])
+def test_against_float64(rows, d, f, e, dtype):
+    act = ACTS[(rows + d) % 4]
+    print(f"gated_ffn {rows} x {d} -> {f} -> {e} {dtype} {act}", flush=True)
+    x, wg, wu, wd, dy = inputs(rows, d, f, e, dtype)
+    ref = reference(x, wg, wu, wd, dy, act, dtype)
+    got = run(x, wg, wu, wd, dy, act)
+    for n in ref:
+        check(got[n], ref[n], dtype, (n, act))
+    with torch.no_grad():
+        check(gated_ffn(x, wg, wu, wd, activation=act), ref["y"], dtype, "y without a graph")
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("rows", [3, 200])
+def test_activations(act, rows):
+    print(f"gated_ffn activation {act} {rows}", flush=True)
+    x, wg, wu, wd, dy = inputs(rows, 64, 128, 64, BF, seed=5, scale=4.0)
+    ref, got = reference(x, wg, wu, wd, dy, act, BF), run(x, wg, wu, wd, dy, act)
+    for n in ref:
+        check(got[n], ref[n], BF, (n, act))
+
+
+@pytest.mark.parametrize("rows,d,f", [(2049, 512, 1408), (1500, 1024, 2816)])
+def test_larger(rows, d, f):
+    print(f"gated_ffn {rows} x {d} x {f}", flush=True)
+    x, wg, wu, wd, dy = inputs(rows, d, f, d, BF)
+    ref, got = reference(x, wg, wu, wd, dy, "silu", BF), run(x, wg, wu, wd, dy, "silu")
+    for n in ref:
+        check(got[n], ref[n], BF, n)
+
+
+def test_against_differences():
+    """dx against central differences of the float64 function along random directions: the
+    difference is off by h^2 / 6 of its third derivative, the gradient by its roundings."""
+    x, wg, wu, wd, dy = inputs(9, 64, 72, 64, HF, seed=3)
+    got = run(x, wg, wu, wd, dy, "gelu")
+    ts = [t.double() for t in (x, wg, wu, wd)]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for i, n in enumerate(("dx", "dwg", "dwu", "dwd")):
+        v = torch.randn(ts[i].shape, generator=g, device=DEV, dtype=torch.float64)
+        step = 1e-4
+        hi, lo = (torch_gated_ffn(*[t + s * step * v if j == i else t for j, t in enumerate(ts)], "gelu") for s in (1, -1))
+        want = float(((hi - lo) / (2 * step) * dy.double()).sum())
+        have, size = float((got[n].double() * v).sum()), float((got[n].double().abs() * v.abs()).sum())
+        assert abs(have - want) <= 4 * 2.0 ** -11 * size + 1e-5, (n, have, want)
+
+
+def test_strides_views_and_alignment():
+    x, wg, wu, wd, dy = inputs(150, 72, 136, 40, BF)
+    want = run(x, wg, wu, wd, dy, "silu")
+    wide = torch.zeros(150, 3 * 72 + 8, device=DEV, dtype=BF)
+    both = torch.cat([wg, wu])  # gate and up as rows of one matrix
+    for lo in (0, 72, 144):
+        for shift in (0, 8, 3):  # 16-byte aligned columns and ones that are not
+            if lo + shift + 72 > wide.shape[1]:
+                continue
+            xv = wide[:, lo + shift:lo + shift + 72]
+            xv.copy_(x)
+            got = run_views(xv, both[:136], both[136:], wd.t().contiguous().t(), dy.t().contiguous().t())
+            for n, t in got.items():
+                assert torch.equal(t, want[n]), (n, lo, shift)
+    # leading dimensions, an expanded gradient, a transposed one
+    x3 = x.view(3, 50, 72).requires_grad_()
+    y = gated_ffn(x3, wg, wu, wd)
+    assert y.shape == (3, 50, 40) and torch.equal(y.detach().view(150, 40), want["y"])
+    dx, = torch.autograd.grad(y.sum(), x3)
+    one = run(x, wg, wu, wd, torch.ones_like(dy), "silu")
+    assert torch.equal(dx.view(150, 72), one["dx"])
+
+
+def run_views(x, wg, wu, wd, dy):
+    ts = [t.detach().requires_grad_() for t in (x, wg, wu, wd)]
+    y = gated_ffn(*ts)
+    return dict(zip(("y", "dx", "dwg", "dwu", "dwd"), (y.detach(), *torch.autograd.grad(y, ts, dy))))
+
+
+def test_no_rows():
+    x, wg, wu, wd, dy = inputs(0, 64, 72, 40, BF)
+    got = run(x, wg, wu, wd, dy, "silu")
+    assert got["y"].shape == (0, 40) and got["dx"].shape == (0, 64)
+    assert all(bool((got[n] == 0).all()) for n in ("dwg", "dwu", "dwd"))
+    assert gated_ffn(x.view(2, 0, 64), wg, wu, wd).shape == (2, 0, 40)
+
+
+@pytest.mark.parametrize("rows", [5, 140])
+def test_nan_and_infinity_stay_in_their_rows(rows):
+    x, wg, wu, wd, dy = inputs(rows, 72, 136, 40, BF)
+    clean = run(x, wg, wu, wd, dy, "silu")
+    x2 = x.clone()
+    x2[1] = float("nan")
+    x2[3, 5] = float("inf")
+    got = run(x2, wg, wu, wd, dy, "silu")
+    keep = [r for r in range(rows) if r not in (1, 3)]
+    for n in ("y", "dx"):
+        assert torch.equal(got[n][keep], clean[n][keep]), n
+        assert bool(got[n][1].isnan().all()) and not bool(got[n][3].isfinite().all())
+    # a weight's NaN row reaches its own column of the hidden activation only
+    wg2 = wg.clone()
+    wg2[7] = float("nan")
+    wd2 = wd.clone()
+    wd2[:, 7] = 0
+    got = run(x, wg2, wu, wd2, dy, "silu")
+    assert bool(got["dwu"][7].isnan().all()) and bool(got["dwu"][8].isfinite().all())
+
+
+@pytest.mark.parametrize("need", range(1, 16))
+def test_partial_gradients(need):
+    """Any set of inputs that require gradients: the same bits as all of them."""
+    x, wg, wu, wd, dy = inputs(70, 72, 136, 40, BF)
+    want = run(x, wg, wu, wd, dy, "gelu")
+    ts = [t.detach().clone().requires_grad_(bool(need >> i & 1)) for i, t in enumerate((x, wg, wu, wd))]
+    y = gated_ffn(*ts, activation="gelu")
+    live = [i for i in range(4) if need >> i & 1]
+    for i, g in zip(live, torch.autograd.grad(y, [ts[i] for i in live], dy)):
+        assert torch.equal(g, want[("dx", "dwg", "dwu", "dwd")[i]])
+
+
+def test_autocast():
+    x, wg, wu, wd, dy = (t.float() for t in inputs(70, 72, 136, 40, BF))
+    want = run(*(t.to(BF) for t in (x, wg, wu, wd, dy)), "silu")
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wu, wd)]
+    with torch.autocast("cuda", dtype=BF):
+        y = gated_ffn(*leaves)
+    assert y.dtype == BF and torch.equal(y, want["y"])
+    for n, g in zip(("dx", "dwg", "dwu", "dwd"), torch.autograd.grad(y, leaves, dy.to(BF))):
+        assert g.dtype == torch.float32 and torch.equal(g, want[n].float()), n
+    with torch.autocast("cuda", dtype=BF):  # a backward inside one of another dtype
+        y = gated_ffn(*leaves)
+        with torch.autocast("cuda", dtype=HF):
+            dx, = torch.autograd.grad(y, leaves[:1], dy.to(BF))
+    assert torch.equal(dx, want["dx"].float())
+
+
+def test_second_order():
+    """The graph of the backward is torch's: its gradients against float64 double backward, within
+    the roundings of five 16-bit ops in a row."""
+    ts = [t.detach().requires_grad_() for t in inputs(6, 64, 72, 64, HF, seed=9)[:4]]
+    dy = inputs(6, 64, 72, 64, HF, seed=9)[4]
+    got, want = [], []
+    for fn, leaves, up, out in ((gated_ffn, ts, dy, got), (None, [t.detach().double().requires_grad_() for t in ts], dy.double(), want)):
+        y = fn(*leaves, "gelu") if fn else torch_gated_ffn(*leaves, "gelu")
+        gx, = torch.autograd.grad(y, leaves[0], up, create_graph=True)
+        out += torch.autograd.grad(gx.double().square().sum(), leaves)
+    for a, b in zip(got, want):
+        assert float((a.double() - b).norm()) <= 8 * 2.0 ** -11 * float(b.norm())
+    wd_only = ts[3].detach().clone().requires_grad_()
+    up = dy.clone().requires_grad_()
+    g, = torch.autograd.grad(gated_ffn(ts[0].detach(), ts[1].detach(), ts[2].detach(), wd_only), wd_only, up, create_graph=True)
+    assert torch.autograd.grad(g.sum(), up)[0].shape == up.shape
+
+
+def test_changed_in_place_is_refused():
+    x, wg, wu, wd, dy = inputs(20, 64, 72, 40, BF)
+    for i in range(4):
+        ts = [t.detach().clone().requires_grad_() for t in (x, wg, wu, wd)]
+        y = gated_ffn(*ts)
+        with torch.no_grad():
+            ts[i].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad(y, ts, dy)
+    # a weight that no wanted gradient reads may change, as with linears
+    wd1 = wd.detach().clone().requires_grad_()
+    y = gated_ffn(x, wg, wu, wd1)
+    with torch.no_grad():
+        wd1.add_(1)
+    torch.autograd.grad(y, wd1, dy)
+    y = gated_ffn(x.clone().requires_grad_(), wg, wu, wd)
+    y.add_(1)  # the output may be modified in place
+
+
+def test_streams_and_graph():
+    """Another stream; a captured forward and backward replayed over new inputs, with eager work
+    between the replays, against eager results."""
+    x, wg, wu, wd, dy = inputs(90, 72, 136, 40, BF)
+    want = run(x, wg, wu, wd, dy, "silu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(x, wg, wu, wd, dy, "silu")
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    leaves = [t.detach().clone().requires_grad_() for t in (x, wg, wu, wd)]
+    up = dy.clone()
+
+    def step():
+        y = gated_ffn(*leaves)
+        return y.detach(), *torch.autograd.grad(y, leaves, up)
+
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in range(3):
+        new = inputs(90, 72, 136, 40, BF, seed=20 + seed)
+        with torch.no_grad():
+            for a, b in zip((*leaves, up), new):
+                a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = run(*new, "silu")
+        for a, n in zip(outs, ("y", "dx", "dwg", "dwu", "dwd")):
+            assert torch.equal(a, eager[n]), (seed, n)
+
+
+def test_runs_agree():
+    """Sums run in a fixed order: the same bits on every call."""
+    args = inputs(1030, 264, 712, 264, BF)
+    a, b = run(*args, "silu"), run(*args, "silu")
+    assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_refusals_on_gpu():
+    x, wg, wu, wd, _ = inputs(4, 64, 72, 40, BF)
+    for args in ((x.float(), wg, wu, wd), (x, wg.half(), wu, wd), (x[:, :60], wg[:, :60], wu[:, :60], wd), (x, wg, wu[:64], wd),
+                 (x, wg, wu, wd[:, :64]), (x, wg, wu, wd.cpu()), (x.float(), wg.float(), wu.float(), wd.float())):
+        with pytest.raises(_hip.DsaltError):
+            gated_ffn(*args)
+    with pytest.raises(ValueError, match="activation"):
+        gated_ffn(x, wg, wu, wd, activation="tanh")

@@ -1,0 +1,112 @@
+"""Host-side refusals of the gated feed-forward, dropout and branch-norm entry points (no GPU),
+and the plain form of their random bits against published values."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import dsalt._hip as hip
+from dsalt.kernels import branch_norm, counter_dropout, gated_ffn
+from philox_reference import keep_mask, philox4x32
+
+
+def test_philox_known_values():
+    """The generator's published known-answer values (10 rounds) pin rounds and key schedule."""
+    zero = [np.zeros(1, np.uint64)] * 4
+    assert [int(w[0]) for w in philox4x32(zero, (0, 0), 10)] == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    ones = [np.full(1, 0xFFFFFFFF, np.uint64)] * 4
+    assert [int(w[0]) for w in philox4x32(ones, (0xFFFFFFFF, 0xFFFFFFFF), 10)] == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert keep_mask(1000, 0.0, 1, 0).all() and not keep_mask(1000, 1.0, 1, 0).any()
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(64, 64, dtype=torch.bfloat16)
+    for call in (lambda: gated_ffn(x, w, w, w), lambda: counter_dropout(x, 0.1, 1), lambda: branch_norm(x, x, w[0])):
+        with pytest.raises(hip.DsaltError, match="ROCm GPU"):
+            call()
+
+
+def ffn_args(**kw):
+    a = hip.GatedFfnArgs(rows=32, d=64, f=128, e=64, x_stride=64, w_gate_stride=64, w_up_stride=64, w_down_stride=128,
+                         dy_stride=64, workspace_bytes=1 << 40)
+    for i, n in enumerate(("x", "w_gate", "w_up", "w_down", "gate_up", "act", "y", "dy", "d_gate_up", "dx", "dw_gate", "dw_up",
+                           "dw_down", "workspace")):
+        setattr(a, n, 0x10000000 + i * 0x100000)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({}, 0), ({"rows": -1}, 1), ({"rows": 1 << 40}, 1), ({"d": 60}, 2), ({"f": 0}, 2), ({"e": (1 << 20) + 8}, 2), ({"dtype": 2}, 2),
+    ({"dtype": 7}, 2), ({"activation": 4}, 1), ({"activation": -1}, 1), ({"x_stride": 56}, 2), ({"w_gate_stride": 68}, 2),
+    ({"w_up_stride": -64}, 2), ({"w_down_stride": (1 << 21) + 8}, 2), ({"x": 0x10000008}, 1), ({"act": None}, 1),
+    ({"x": None}, 1), ({"rows": 0, "x": None, "act": None, "y": None}, 0), ({"rows": 1 << 31, "f": 1 << 20, "w_down_stride": 1 << 20}, 2)])
+def test_gated_ffn_forward_check(kw, code):
+    assert hip.lib().dsalt_gated_ffn_check(ctypes.byref(ffn_args(**kw)), 0) == code, hip.lib().dsalt_last_error()
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({}, 0), ({"dy": None}, 1), ({"dy_stride": 60}, 2), ({"d_gate_up": None}, 1), ({"gate_up": None}, 1), ({"act": None}, 1),
+    ({"act": None, "dw_down": None}, 0), ({"x": None}, 1), ({"x": None, "dw_gate": None, "dw_up": None}, 0),
+    ({"d_gate_up": None, "dx": None, "dw_gate": None, "dw_up": None, "x": None, "gate_up": None, "w_gate": None}, 0),
+    ({"w_up": None}, 1), ({"w_up": None, "w_gate": None, "dx": None}, 0), ({"w_down": None}, 1)])
+def test_gated_ffn_backward_check(kw, code):
+    assert hip.lib().dsalt_gated_ffn_check(ctypes.byref(ffn_args(**kw)), 1) == code, hip.lib().dsalt_last_error()
+
+
+def test_gated_ffn_workspace_check():
+    need = hip.lib().dsalt_gated_ffn_workspace_size(32, 64, 128, 64, 1)
+    assert need >= 0 and hip.lib().dsalt_gated_ffn_workspace_size(-1, 64, 128, 64, 1) == 0
+    if need:
+        assert hip.lib().dsalt_gated_ffn_check(ctypes.byref(ffn_args(workspace_bytes=need - 1)), 1) == 1
+    assert hip.lib().dsalt_gated_ffn_check(None, 0) == 1
+
+
+@pytest.mark.parametrize("kw", [{"n": -1}, {"n": 1 << 41}, {"dtype": 3}, {"threshold": -1}, {"threshold": 65537}, {"x": None},
+                                {"out": 0x10000004}, {"seed_ptr": 0x10000004}])
+def test_dropout_refusals(kw):
+    a = hip.DropoutArgs(n=64, dtype=0, threshold=60000, x=0x10000000, out=0x10100000)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    assert hip.lib().dsalt_dropout(ctypes.byref(a), None) == 1
+    assert hip.lib().dsalt_dropout(None, None) == 1
+
+
+def branch_args(**kw):
+    a = hip.BranchNormArgs(rows=32, d=64, x_dtype=2, h_dtype=0, y_dtype=0, w_dtype=2, post_dtype=2, gate_dtype=2, gate_kind=1,
+                           threshold=60000, eps=1e-6, post_eps=1e-6, residual_scale=1.0, workspace_bytes=1 << 30)
+    for i, n in enumerate(("x", "h", "weight", "post_weight", "gate", "x_out", "y", "rstd", "rstd_post", "dx_out", "dy", "dx", "dh",
+                           "d_weight", "d_post_weight", "d_gate", "workspace")):
+        setattr(a, n, 0x10000000 + i * 0x100000)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,backward,code", [
+    ({}, 0, 0), ({}, 1, 0), ({"rows": -1}, 0, 1), ({"d": 12}, 0, 2), ({"d": 8200}, 0, 2), ({"x_dtype": 0}, 0, 0),
+    ({"x_dtype": 0, "h_dtype": 1}, 0, 2), ({"x_dtype": 0, "y_dtype": 2}, 0, 2), ({"x_dtype": 5}, 0, 1), ({"w_dtype": 1}, 0, 2),
+    ({"gate_kind": 3}, 0, 1), ({"threshold": 70000}, 0, 1), ({"h": None}, 0, 1), ({"gate": None}, 0, 1),
+    ({"gate": None, "gate_kind": 0}, 0, 0), ({"x_out": None}, 0, 1), ({"y": None}, 0, 1), ({"y": None, "weight": None}, 0, 0),
+    ({"x": 0x10000008}, 0, 1), ({"gate": 0x10000004}, 0, 1), ({"gate": 0x10000004, "gate_kind": 2}, 0, 0),
+    ({"seed_ptr": 0x10000004}, 0, 1), ({"dx_out": None}, 1, 0), ({"dx_out": None, "dy": None}, 1, 1), ({"rstd": None}, 1, 1),
+    ({"rstd_post": None}, 1, 1), ({"workspace": None}, 1, 1), ({"workspace_bytes": 16}, 1, 1), ({"post_weight": None}, 1, 1),
+    ({"workspace": None, "d_weight": None, "d_post_weight": None, "gate_kind": 2}, 1, 0)])
+def test_branch_norm_check(kw, backward, code):
+    assert hip.lib().dsalt_branch_norm_check(ctypes.byref(branch_args(**kw)), backward) == code, hip.lib().dsalt_last_error()
+
+
+def test_argument_values():
+    for p in (-0.5, 1.01, float("nan")):
+        with pytest.raises(ValueError, match="probability"):
+            hip.keep_threshold(p)
+    assert [hip.keep_threshold(p) for p in (0.0, 0.5, 1.0, 0.1)] == [65536, 32768, 0, 58982]
+    dev = torch.device("cuda", 0)
+    assert hip.seed_fields(-1, dev) == (-1, None) and hip.seed_fields(2 ** 64 - 1, dev) == (-1, None)
+    for bad in (2 ** 64, -2 ** 63 - 1):
+        with pytest.raises(ValueError, match="64 bits"):
+            hip.seed_fields(bad, dev)
+    with pytest.raises(hip.DsaltError):
+        hip.seed_fields(torch.tensor([1]), dev)
