@@ -44,232 +44,438 @@ __device__ __forceinline__ void act_grad(float g, float &v, float &slope) {
         slope = off ? 0.f : 1.f;
     }
 }
+// Eight at a time inside the choice of the activation, so that their chains of exp and
+// reciprocal overlap (erfc's long ones would take too many registers and go one by one).
 template <int ACT>
-__device__ __forceinline__ float act_value(float g) {
-    float v, s;
-    act_grad<ACT>(g, v, s);
-    return v;
+__device__ __forceinline__ void gated8(const float (&g)[8], const float (&u)[8], float (&a)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float v, s;
+        act_grad<ACT>(g[e], v, s);
+        a[e] = v * u[e];
+        if constexpr (ACT == DSALT_ACT_GELU) __builtin_amdgcn_sched_barrier(0);
+    }
+}
+__device__ __forceinline__ void gated8(int act, const float (&g)[8], const float (&u)[8], float (&a)[8]) {
+    if (act == DSALT_ACT_SILU) gated8<DSALT_ACT_SILU>(g, u, a);
+    else if (act == DSALT_ACT_GELU) gated8<DSALT_ACT_GELU>(g, u, a);
+    else if (act == DSALT_ACT_GELU_TANH) gated8<DSALT_ACT_GELU_TANH>(g, u, a);
+    else gated8<DSALT_ACT_RELU>(g, u, a);
+}
+// da becomes the gradient of g, u that of u.
+template <int ACT>
+__device__ __forceinline__ void gated_grad8(const float (&g)[8], float (&u)[8], float (&da)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float v, s;
+        act_grad<ACT>(g[e], v, s);
+        const float d = da[e];
+        da[e] = d * u[e] * s;
+        u[e] = d * v;
+        if constexpr (ACT == DSALT_ACT_GELU) __builtin_amdgcn_sched_barrier(0);
+    }
+}
+__device__ __forceinline__ void gated_grad8(int act, const float (&g)[8], float (&u)[8], float (&da)[8]) {
+    if (act == DSALT_ACT_SILU) gated_grad8<DSALT_ACT_SILU>(g, u, da);
+    else if (act == DSALT_ACT_GELU) gated_grad8<DSALT_ACT_GELU>(g, u, da);
+    else if (act == DSALT_ACT_GELU_TANH) gated_grad8<DSALT_ACT_GELU_TANH>(g, u, da);
+    else gated_grad8<DSALT_ACT_RELU>(g, u, da);
 }
 
-struct FfnParams {
+// One product of a launch: out [m, n] = sum over the segments of a[s] b[s] (pair: n columns of
+// each of b[0] and b[1]).
+struct Product {
     GemmOperand a[2], b[2];
-    int64_t m, n, k;     // of the product (PAIR: n of one matrix)
+    int64_t m, n;
     int tiles_m, tiles_n;
-    char *out[2];
-    int64_t out_ld;      // bytes
-    const char *gu;      // gate | up, row stride gu_ld bytes, up at gu + up_off
-    int64_t gu_ld, up_off;
+    char *out;
+    int64_t out_ld;  // bytes
 };
 
-// Tile of workgroup `id`: each XCD takes a contiguous range of ids, ids run over kGroup m-tiles
-// before the next n-tile, so that the workgroups that run at a time share operand rows in their L2.
+constexpr int kMaxProducts = 3;
+struct FfnParams {
+    Product prod[kMaxProducts];
+    int products;
+    int64_t k;        // of every product and segment
+    int act;
+    char *gu;         // gate | up: written (pair; NULL: not kept) or read (gradient)
+    int64_t gu_ld, up_off;  // bytes; up at gu + up_off
+    int whole;        // tiles computed by one workgroup each; the others by `split` workgroups,
+    int split;        // whose fp32 partial sums go to `part` and are joined by a second launch
+    float *part;
+};
+
+// A launch's tiles in order: product by product, in each kGroup m-tiles before the next n-tile,
+// so that the workgroups that run at a time on one XCD share operand rows in its L2.
 constexpr int kGroup = 8;
-__device__ __forceinline__ bool tile_of(int id, int tiles_m, int tiles_n, int &tm, int &tn) {
-    const int l = xcd_remap(id, gridDim.x);
-    if (l >= tiles_m * tiles_n) return false;
-    const int per = kGroup * tiles_n, g = l / per, r = l - g * per, rows = min(kGroup, tiles_m - g * kGroup);
+__device__ __forceinline__ const Product &tile_of(const FfnParams &p, int tile, int &tm, int &tn) {
+    int z = 0;
+    while (z + 1 < p.products && tile >= p.prod[z].tiles_m * p.prod[z].tiles_n) {
+        tile -= p.prod[z].tiles_m * p.prod[z].tiles_n;
+        ++z;
+    }
+    const Product &q = p.prod[z];
+    const int per = kGroup * q.tiles_n, g = tile / per, r = tile - g * per, rows = min(kGroup, q.tiles_m - g * kGroup);
     tn = r / rows;
     tm = g * kGroup + r - tn * rows;
-    return true;
+    return q;
 }
 
-enum { kEpiUp, kEpiUpSave, kEpiStore, kEpiGrad };
+enum { kEpiPair, kEpiStore, kEpiGrad };
 
-template <class DT, int BM, int BN, int WM, int WN, int ALAY, int BLAY, int SEGMENTS, int EPI, int ACT>
-__global__ void __launch_bounds__(WM *WN * 64) ffn_kernel(FfnParams p) {
-    constexpr bool PAIR = EPI == kEpiUp || EPI == kEpiUpSave;
-    typedef GemmCore<DT, BM, BN, WM, WN, ALAY, BLAY, PAIR> Core;
-    __shared__ __attribute__((aligned(16))) char lds[Core::LDS_BYTES];
-    int tm, tn;
-    if (!tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn)) return;
-    constexpr int BNO = PAIR ? BN / 2 : BN;  // columns of the output
-    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BNO;
-    const int z = blockIdx.y;  // independent products of one shape: their a operand and output
-    Core c;
-    if constexpr (SEGMENTS == 1 && !PAIR) {
-        c.template run<1>(lds, &p.a[z], &p.b[0], m0, n0, p.k, 0, (int)((p.k + kGemmBK - 1) / kGemmBK));
-    } else {
-        c.template run<SEGMENTS>(lds, p.a, p.b, m0, n0, p.k, 0, SEGMENTS * (int)((p.k + kGemmBK - 1) / kGemmBK));
-    }
+// The tile's row blocks first .. first + ROWS - 1 from their accumulators: the activation and
+// product of a pair, a plain store, or the gradients of gate and up from that of the product
+// (whose g and u are loaded kAhead turns before they are used: one after the other they would
+// cost a trip to memory for every 16 bytes of a lane).
+constexpr int kAhead = 3;
+template <class DT, class Core, int EPI, int ROWS>
+__device__ __forceinline__ void epilogue(const FfnParams &p, const Product &q, const Core &c,
+                                         const f32x16 (&acc)[ROWS][Core::FN], int first, int64_t m0, int64_t n0, char *lds) {
+    constexpr int WIDTH = EPI == kEpiPair ? Core::COLS / 2 : Core::COLS;  // output columns of a wave
+    const int64_t nb = n0 + c.wn * WIDTH;
+    const bool inside = nb + c.piece_col() < q.n;
+    const uint32_t ld = (uint32_t)q.out_ld, gu_ld = (uint32_t)p.gu_ld;
 #pragma unroll
-    for (int i = 0; i < Core::FM; ++i) {
-        const int64_t m = m0 + c.row(i);
-        if (m >= p.m) continue;
-        constexpr int FO = PAIR ? Core::FN / 2 : Core::FN;
+    for (int i = 0; i < ROWS; ++i) {
+        const int64_t mb = m0 + (c.wm * Core::FM + first + i) * 32;
+        const int rows = (int)min(q.m - mb, (int64_t)32);
+        // wave-uniform bases, 32-bit lane offsets
+        char *out = q.out + mb * q.out_ld + nb * 2, *gu = p.gu + mb * p.gu_ld + nb * 2;
+        const uint32_t off = (uint32_t)(c.lane / Core::PIECES) * ld + c.piece_col() * 2,
+                       gu_off = (uint32_t)(c.lane / Core::PIECES) * gu_ld + c.piece_col() * 2;
+        uint4 graw[kAhead], uraw[kAhead];
+        auto load = [&](int t) {
+            if (inside && c.piece_row(t) < rows) {
+                const char *at = gu + (uint32_t)(t * Core::TURN_ROWS) * gu_ld;
+                graw[t % kAhead] = *reinterpret_cast<const uint4 *>(at + gu_off);
+                uraw[t % kAhead] = *reinterpret_cast<const uint4 *>(at + p.up_off + gu_off);
+            }
+        };
+        if constexpr (EPI == kEpiGrad) {
 #pragma unroll
-        for (int j = 0; j < FO; ++j) {
+            for (int t = 0; t < kAhead && t < Core::TURNS; ++t) load(t);
+        }
+        c.put(lds, acc[i]);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int64_t n = n0 + (c.wn * FO + j) * 32 + c.col(half);
-                float v[8], u[8], w[8];
-                c.values(c.acc[i][j], half, v);
-                if constexpr (PAIR) {
-                    c.values(c.acc[i][FO + j], half, u);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = act_value<ACT>(v[e]) * u[e];
-                }
-                if (n >= p.n) continue;
-                if constexpr (PAIR) {
-                    *reinterpret_cast<uint4 *>(p.out[0] + m * p.out_ld + n * 2) = pack8<DT>(w);
-                    if constexpr (EPI == kEpiUpSave) {
-                        char *gu = p.out[1] + m * p.gu_ld + n * 2;
-                        *reinterpret_cast<uint4 *>(gu) = pack8<DT>(v);
-                        *reinterpret_cast<uint4 *>(gu + p.up_off) = pack8<DT>(u);
+        for (int t = 0; t < Core::TURNS; ++t) {
+            float v[8], u[8], w[8];
+            c.get(lds, t, 0, v);
+            if constexpr (EPI == kEpiPair) c.get(lds, t, WIDTH, u);
+            if (inside && c.piece_row(t) < rows) {
+                char *o = out + (uint32_t)(t * Core::TURN_ROWS) * ld;
+                if constexpr (EPI == kEpiPair) {
+                    if (p.gu) {
+                        char *at = gu + (uint32_t)(t * Core::TURN_ROWS) * gu_ld;
+                        *reinterpret_cast<uint4 *>(at + gu_off) = pack8<DT>(v);
+                        *reinterpret_cast<uint4 *>(at + p.up_off + gu_off) = pack8<DT>(u);
                     }
+                    gated8(p.act, v, u, w);
+                    *reinterpret_cast<uint4 *>(o + off) = pack8<DT>(w);
                 } else if constexpr (EPI == kEpiStore) {
-                    *reinterpret_cast<uint4 *>(p.out[z] + m * p.out_ld + n * 2) = pack8<DT>(v);
+                    *reinterpret_cast<uint4 *>(o + off) = pack8<DT>(v);
                 } else {
-                    const char *gu = p.gu + m * p.gu_ld + n * 2;
-                    float g[8];
-                    unpack8<DT>(*reinterpret_cast<const uint4 *>(gu), g);
-                    unpack8<DT>(*reinterpret_cast<const uint4 *>(gu + p.up_off), u);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float act, slope;
-                        act_grad<ACT>(g[e], act, slope);
-                        w[e] = v[e] * act;
-                        v[e] = v[e] * u[e] * slope;
-                    }
-                    char *o = p.out[0] + m * p.out_ld + n * 2;
-                    *reinterpret_cast<uint4 *>(o) = pack8<DT>(v);
-                    *reinterpret_cast<uint4 *>(o + p.up_off) = pack8<DT>(w);
+                    unpack8<DT>(graw[t % kAhead], w);
+                    unpack8<DT>(uraw[t % kAhead], u);
+                    gated_grad8(p.act, w, u, v);
+                    *reinterpret_cast<uint4 *>(o + off) = pack8<DT>(v);
+                    *reinterpret_cast<uint4 *>(o + p.up_off + off) = pack8<DT>(u);
                 }
+            }
+            if constexpr (EPI == kEpiGrad)
+                if (t + kAhead < Core::TURNS) load(t + kAhead);
+            __builtin_amdgcn_sched_barrier(0);  // no more turns in registers at a time than these
+        }
+        __builtin_amdgcn_wave_barrier();  // the next block overwrites this one
+    }
+}
+
+template <int BM_, int BN_, int RA_, int RB_, int WM_, int WN_>
+struct Shape {
+    static constexpr int BM = BM_, BN = BN_, RA = RA_, RB = RB_, WM = WM_, WN = WN_;
+};
+template <class DT, class S, int ALAY, int BLAY, int EPI>
+using Core = GemmCore<DT, S::BM, S::BN, 64, S::RA, S::RB, S::WM, S::WN, ALAY, BLAY, EPI == kEpiPair>;
+
+// Partial sums of piece `piece` of split tile r: [piece][r][i][j][quarter][thread] float4.
+template <class C>
+__device__ __forceinline__ float4 *partial(const FfnParams &p, int r, int piece, int tiles, int i, int j) {
+    return reinterpret_cast<float4 *>(p.part) +
+           ((((int64_t)piece * tiles + r) * C::FM + i) * C::FN + j) * 4 * C::THREADS + threadIdx.x;
+}
+
+template <class DT, class S, int ALAY, int BLAY, int SEGMENTS, int EPI>
+__global__ void __launch_bounds__(S::WM *S::WN * 64) ffn_kernel(const FfnParams p) {
+    typedef Core<DT, S, ALAY, BLAY, EPI> C;
+    __shared__ __attribute__((aligned(256))) char lds[C::LDS_BYTES];
+    constexpr int BNO = EPI == kEpiPair ? S::BN / 2 : S::BN;  // columns of the output
+    // the whole tiles come first; each XCD takes a contiguous range of them
+    int id = blockIdx.x, r = 0, piece = 0;
+    const int steps = SEGMENTS * (int)((p.k + C::BK - 1) / C::BK);
+    int first = 0, last = steps;
+    if (id < (p.whole & ~7)) id = xcd_remap(id, p.whole & ~7);
+    const bool split = id >= p.whole && p.split > 1;
+    if (split) {
+        r = (id - p.whole) / p.split;
+        piece = (id - p.whole) - r * p.split;
+        id = p.whole + r;
+        first = (int)((int64_t)steps * piece / p.split);
+        last = (int)((int64_t)steps * (piece + 1) / p.split);
+    }
+    int tm, tn;
+    const Product &q = tile_of(p, id, tm, tn);
+    const int64_t m0 = (int64_t)tm * S::BM, n0 = (int64_t)tn * BNO;
+    C c;
+    c.template run<SEGMENTS>(lds, q.a, q.b, m0, n0, p.k, first, last);
+    if (split) {
+        const int tiles = (gridDim.x - p.whole) / p.split;
+#pragma unroll
+        for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const f32x16 &v = c.acc[i][j];
+                    partial<C>(p, r, piece, tiles, i, j)[h * C::THREADS] =
+                        make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+                }
+        return;
+    }
+    epilogue<DT, C, EPI, C::FM>(p, q, c, c.acc, 0, m0, n0, lds);
+}
+
+// The split tiles' partial sums added in order, and their epilogue: one workgroup per row block i.
+template <class DT, class S, int ALAY, int BLAY, int EPI>
+__global__ void __launch_bounds__(S::WM *S::WN * 64) ffn_join_kernel(const FfnParams p) {
+    typedef Core<DT, S, ALAY, BLAY, EPI> C;
+    constexpr int BNO = EPI == kEpiPair ? S::BN / 2 : S::BN;
+    const int tiles = gridDim.x / C::FM, r = blockIdx.x / C::FM, i = blockIdx.x - r * C::FM;
+    int tm, tn;
+    const Product &q = tile_of(p, p.whole + r, tm, tn);
+    __shared__ __attribute__((aligned(256))) char lds[C::NW * 32 * C::COLS * 4];
+    C c;
+    f32x16 acc[1][C::FN];
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j) {
+        acc[0][j] = f32x16{};
+        for (int s = 0; s < p.split; ++s)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const float4 v = partial<C>(p, r, s, tiles, i, j)[h * C::THREADS];
+                acc[0][j][4 * h] += v.x;
+                acc[0][j][4 * h + 1] += v.y;
+                acc[0][j][4 * h + 2] += v.z;
+                acc[0][j][4 * h + 3] += v.w;
+            }
+    }
+    const int64_t m0 = (int64_t)tm * S::BM, n0 = (int64_t)tn * BNO;
+    epilogue<DT, C, EPI, 1>(p, q, c, acc, i, m0, n0, lds);
+}
+
+// How a launch covers its tiles: the shape, and into how many pieces the tiles past the last full
+// round of workgroups are cut along k.
+//
+// The times are fits to measurements: us of one 64-wide k-step with all slots busy and with few
+// (a CU alone has more of the caches, of the memory and of the power budget), and the share of
+// the epilogue's bytes, at kMemory, that nothing else runs under (one of two workgroups on a CU
+// computes while the other stores). Measured with each shape forced (bf16, us; largest is
+// 16384 rows, d 2048, f 5504, ragged 6473, 1024, 2816):
+//                     256 x 256   256 x 128   128 x 128
+//   largest, gate|up        754         911         917
+//   largest, down           341         409         410
+//   largest, da             528         540         561
+//   ragged,  down            73          51          55
+//   ragged,  da             104          88          78
+//   ragged,  dx              89 + 14    106         109
+struct Plan {
+    int shape, whole, split, tiles;
+    int64_t part_bytes;
+};
+struct ShapeCost {
+    int bm, bn, slots;  // workgroups that run at a time
+    double busy, alone, bare;
+};
+constexpr ShapeCost kShapes[] = {
+    {256, 256, 256, 1.85, 1.20, 1.0},
+    {256, 128, 256, 1.12, 0.65, 1.0},
+    {128, 128, 512, 1.17, 0.40, 0.5},
+};
+constexpr int kShapeCount = 3, kMaxSplit = 8;
+constexpr double kTile = 3.0, kJoin = 6.0, kMemory = 5.0e6, kPartials = 3.0e6;  // us, us, bytes per us
+
+int64_t tiles_of(int64_t m, int64_t n, int shape, bool pair) {
+    const int bn = kShapes[shape].bn / (pair ? 2 : 1);
+    return ((m + kShapes[shape].bm - 1) / kShapes[shape].bm) * ((n + bn - 1) / bn);
+}
+
+struct Extent {
+    int64_t m, n;
+};
+// io: bytes that an output element's epilogue moves.
+Plan plan(const Extent *e, int count, int64_t k, int segments, bool pair, int io) {
+    const int64_t steps = segments * ((k + 63) / 64);
+    Plan best{};
+    double least = 0;
+    for (int s = 0; s < kShapeCount; ++s) {
+        const ShapeCost &c = kShapes[s];
+        int64_t tiles = 0;
+        for (int z = 0; z < count; ++z) tiles += tiles_of(e[z].m, e[z].n, s, pair);
+        if (tiles == 0) return best;
+        const double out = (double)c.bm * c.bn / (pair ? 2 : 1) * io * c.bare / kMemory;  // us per workgroup of a round
+        const int64_t rounds = tiles / c.slots, rest = tiles - rounds * c.slots;
+        const int most = rest ? (int)std::min<int64_t>(std::min<int64_t>(c.slots / rest, kMaxSplit), steps / 4) : 1;
+        for (int split = 1; split <= std::max(most, 1); ++split) {
+            double t = rounds * (steps * c.busy + kTile + out * c.slots);
+            const double busy = (double)rest * split / c.slots, bytes = split > 1 ? (double)rest * split * c.bm * c.bn * 4 : 0;
+            if (rest) {
+                t += (steps + split - 1) / split * (c.alone + (c.busy - c.alone) * busy) + kTile;
+                t += split > 1 ? kJoin + 2 * bytes / kPartials : out * rest;
+            }
+            if (best.tiles == 0 || t < least) {
+                least = t;
+                best = {s, (int)(split > 1 ? tiles - rest : tiles), split, (int)tiles, (int64_t)bytes};
             }
         }
     }
+    return best;
 }
+// What each kind of launch moves per output element: see epilogue().
+constexpr int kIoStore = 2, kIoGrad = 8;
+int io_pair(bool keep) { return keep ? 6 : 2; }
 
-template <class DT, int ALAY, int BLAY, int SEGMENTS, int EPI, int ACT>
-void launch_product(FfnParams p, int batch, hipStream_t stream) {
-    constexpr int BM = 128, BN = 128;
-    constexpr bool PAIR = EPI == kEpiUp || EPI == kEpiUpSave;
-    p.tiles_m = (int)((p.m + BM - 1) / BM);
-    p.tiles_n = (int)((p.n + (PAIR ? BN / 2 : BN) - 1) / (PAIR ? BN / 2 : BN));
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    if (tiles == 0) return;
-    const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)batch);
-    hipLaunchKernelGGL((ffn_kernel<DT, BM, BN, 2, 2, ALAY, BLAY, SEGMENTS, EPI, ACT>), grid, dim3(256), 0, stream, p);
+template <class DT, class S, int ALAY, int BLAY, int SEGMENTS, int EPI>
+hipError_t launch_shape(const FfnParams &p, const Plan &w, hipStream_t stream) {
+    typedef Core<DT, S, ALAY, BLAY, EPI> C;
+    const int rest = w.tiles - w.whole;
+    hipLaunchKernelGGL((ffn_kernel<DT, S, ALAY, BLAY, SEGMENTS, EPI>), dim3(w.whole + rest * w.split), dim3(C::THREADS), 0,
+                       stream, p);
+    if (rest)
+        hipLaunchKernelGGL((ffn_join_kernel<DT, S, ALAY, BLAY, EPI>), dim3(rest * C::FM), dim3(C::THREADS), 0, stream, p);
+    return hipGetLastError();
 }
 
 template <class DT, int ALAY, int BLAY, int SEGMENTS, int EPI>
-void launch_act(const FfnParams &p, int act, hipStream_t stream) {
-    switch (act) {
-        case DSALT_ACT_SILU: return launch_product<DT, ALAY, BLAY, SEGMENTS, EPI, DSALT_ACT_SILU>(p, 1, stream);
-        case DSALT_ACT_GELU: return launch_product<DT, ALAY, BLAY, SEGMENTS, EPI, DSALT_ACT_GELU>(p, 1, stream);
-        case DSALT_ACT_GELU_TANH: return launch_product<DT, ALAY, BLAY, SEGMENTS, EPI, DSALT_ACT_GELU_TANH>(p, 1, stream);
-        default: return launch_product<DT, ALAY, BLAY, SEGMENTS, EPI, DSALT_ACT_RELU>(p, 1, stream);
+hipError_t launch_product(FfnParams p, void *workspace, hipStream_t stream) {
+    constexpr bool PAIR = EPI == kEpiPair;
+    Extent e[kMaxProducts];
+    for (int z = 0; z < p.products; ++z) e[z] = {p.prod[z].m, p.prod[z].n};
+    const int io = EPI == kEpiPair ? io_pair(p.gu != nullptr) : EPI == kEpiGrad ? kIoGrad : kIoStore;
+    const Plan w = plan(e, p.products, p.k, SEGMENTS, PAIR, io);
+    if (w.tiles == 0) return hipSuccess;
+    for (int z = 0; z < p.products; ++z) {
+        const int bm = kShapes[w.shape].bm, bn = kShapes[w.shape].bn / (PAIR ? 2 : 1);
+        p.prod[z].tiles_m = (int)((e[z].m + bm - 1) / bm);
+        p.prod[z].tiles_n = (int)((e[z].n + bn - 1) / bn);
+    }
+    p.whole = w.whole;
+    p.split = w.split;
+    p.part = static_cast<float *>(workspace);
+    if (getenv("FS")) w.shape = 0; // PROBE
+    switch (w.shape) {
+        case 0: return launch_shape<DT, Shape<256, 256, 3, 2, 4, 2>, ALAY, BLAY, SEGMENTS, EPI>(p, w, stream);
+        case 1: return launch_shape<DT, Shape<256, 128, 3, 3, 4, 2>, ALAY, BLAY, SEGMENTS, EPI>(p, w, stream);
+        default: return launch_shape<DT, Shape<128, 128, 2, 2, 2, 2>, ALAY, BLAY, SEGMENTS, EPI>(p, w, stream);
     }
 }
 
 GemmOperand operand(const void *p, int64_t ld, int64_t rows) { return {static_cast<const char *>(p), ld * 2, rows}; }
 
-template <class DT>
-void forward(const dsalt_gated_ffn_args &a, hipStream_t stream) {
-    FfnParams p{};
-    p.m = a.rows;
-    p.n = a.f;
-    p.k = a.d;
-    p.a[0] = operand(a.x, a.x_stride, a.rows);
-    p.b[0] = operand(a.w_gate, a.w_gate_stride, a.f);
-    p.b[1] = operand(a.w_up, a.w_up_stride, a.f);
-    p.out[0] = static_cast<char *>(a.act);
-    p.out_ld = (int64_t)a.f * 2;
-    if (a.gate_up) {
-        p.out[1] = static_cast<char *>(a.gate_up);
-        p.gu_ld = (int64_t)a.f * 4;
-        p.up_off = (int64_t)a.f * 2;
-        launch_act<DT, kKContig, kKContig, 1, kEpiUpSave>(p, a.activation, stream);
-    } else {
-        launch_act<DT, kKContig, kKContig, 1, kEpiUp>(p, a.activation, stream);
-    }
-    FfnParams q{};
-    q.m = a.rows;
-    q.n = a.e;
-    q.k = a.f;
-    q.a[0] = operand(a.act, a.f, a.rows);
-    q.b[0] = operand(a.w_down, a.w_down_stride, a.e);
-    q.out[0] = static_cast<char *>(a.y);
-    q.out_ld = (int64_t)a.e * 2;
-    launch_product<DT, kKContig, kKContig, 1, kEpiStore, 0>(q, 1, stream);
+Product product(GemmOperand a, GemmOperand b, int64_t m, int64_t n, void *out, int64_t out_ld) {
+    Product q{};
+    q.a[0] = a;
+    q.b[0] = b;
+    q.m = m;
+    q.n = n;
+    q.out = static_cast<char *>(out);
+    q.out_ld = out_ld * 2;
+    return q;
 }
 
 template <class DT>
-void backward(const dsalt_gated_ffn_args &a, hipStream_t stream) {
-    const int64_t f2 = (int64_t)a.f * 2;  // bytes of [f], elements of gate | up
-    if (a.dw_down) {
-        FfnParams p{};
-        p.m = a.e;
-        p.n = a.f;
-        p.k = a.rows;
-        p.a[0] = operand(a.dy, a.dy_stride, a.e);
-        p.b[0] = operand(a.act, a.f, a.f);
-        p.out[0] = static_cast<char *>(a.dw_down);
-        p.out_ld = f2;
-        launch_product<DT, kRContig, kRContig, 1, kEpiStore, 0>(p, 1, stream);
-    }
+hipError_t forward(const dsalt_gated_ffn_args &a, hipStream_t stream) {
+    FfnParams p{};
+    p.products = 1;
+    p.k = a.d;
+    p.act = a.activation;
+    p.prod[0] = product(operand(a.x, a.x_stride, a.rows), operand(a.w_gate, a.w_gate_stride, a.f), a.rows, a.f, a.act, a.f);
+    p.prod[0].b[1] = operand(a.w_up, a.w_up_stride, a.f);
+    p.gu = static_cast<char *>(a.gate_up);
+    p.gu_ld = (int64_t)a.f * 4;
+    p.up_off = (int64_t)a.f * 2;
+    hipError_t e = launch_product<DT, kKContig, kKContig, 1, kEpiPair>(p, a.workspace, stream);
+    if (e != hipSuccess) return e;
+    FfnParams q{};
+    q.products = 1;
+    q.k = a.f;
+    q.prod[0] = product(operand(a.act, a.f, a.rows), operand(a.w_down, a.w_down_stride, a.e), a.rows, a.e, a.y, a.e);
+    return launch_product<DT, kKContig, kKContig, 1, kEpiStore>(q, a.workspace, stream);
+}
+
+template <class DT>
+hipError_t backward(const dsalt_gated_ffn_args &a, hipStream_t stream) {
+    const int64_t up = (int64_t)a.f * 2;  // bytes from gate to up in a row of gate | up
+    const char *dgu = static_cast<const char *>(a.d_gate_up);
     if (a.d_gate_up) {
         FfnParams p{};
-        p.m = a.rows;
-        p.n = a.f;
+        p.products = 1;
         p.k = a.e;
-        p.a[0] = operand(a.dy, a.dy_stride, a.rows);
-        p.b[0] = operand(a.w_down, a.w_down_stride, a.f);
-        p.out[0] = static_cast<char *>(a.d_gate_up);
-        p.out_ld = p.gu_ld = f2 * 2;
-        p.gu = static_cast<const char *>(a.gate_up);
-        p.up_off = f2;
-        launch_act<DT, kKContig, kRContig, 1, kEpiGrad>(p, a.activation, stream);
+        p.act = a.activation;
+        p.prod[0] = product(operand(a.dy, a.dy_stride, a.rows), operand(a.w_down, a.w_down_stride, a.f), a.rows, a.f,
+                            a.d_gate_up, 2 * (int64_t)a.f);
+        p.gu = static_cast<char *>(a.gate_up);
+        p.gu_ld = 2 * up;
+        p.up_off = up;
+        hipError_t e = launch_product<DT, kKContig, kRContig, 1, kEpiGrad>(p, a.workspace, stream);
+        if (e != hipSuccess) return e;
     }
-    const GemmOperand dg = operand(a.d_gate_up, f2, 0), du = {dg.base + f2, dg.ld, 0};
     if (a.dx) {
         FfnParams p{};
-        p.m = a.rows;
-        p.n = a.d;
+        p.products = 1;
         p.k = a.f;
-        p.a[0] = {dg.base, dg.ld, a.rows};
-        p.a[1] = {du.base, du.ld, a.rows};
-        p.b[0] = operand(a.w_gate, a.w_gate_stride, a.d);
-        p.b[1] = operand(a.w_up, a.w_up_stride, a.d);
-        p.out[0] = static_cast<char *>(a.dx);
-        p.out_ld = (int64_t)a.d * 2;
-        launch_product<DT, kKContig, kRContig, 2, kEpiStore, 0>(p, 1, stream);
+        p.prod[0] = product(operand(dgu, 2 * (int64_t)a.f, a.rows), operand(a.w_gate, a.w_gate_stride, a.d), a.rows, a.d, a.dx, a.d);
+        p.prod[0].a[1] = operand(dgu + up, 2 * (int64_t)a.f, a.rows);
+        p.prod[0].b[1] = operand(a.w_up, a.w_up_stride, a.d);
+        hipError_t e = launch_product<DT, kKContig, kRContig, 2, kEpiStore>(p, a.workspace, stream);
+        if (e != hipSuccess) return e;
     }
-    if (a.dw_gate || a.dw_up) {
-        FfnParams p{};
-        p.m = a.f;
-        p.n = a.d;
-        p.k = a.rows;
-        int batch = 0;
-        if (a.dw_gate) {
-            p.a[batch] = {dg.base, dg.ld, a.f};
-            p.out[batch++] = static_cast<char *>(a.dw_gate);
-        }
-        if (a.dw_up) {
-            p.a[batch] = {du.base, du.ld, a.f};
-            p.out[batch++] = static_cast<char *>(a.dw_up);
-        }
-        p.b[0] = operand(a.x, a.x_stride, a.d);
-        p.out_ld = (int64_t)a.d * 2;
-        launch_product<DT, kRContig, kRContig, 1, kEpiStore, 0>(p, batch, stream);
-    }
+    // the weights' gradients share their k axis, the rows: one launch
+    FfnParams p{};
+    p.k = a.rows;
+    const GemmOperand x = operand(a.x, a.x_stride, a.d);
+    if (a.dw_gate) p.prod[p.products++] = product(operand(dgu, 2 * (int64_t)a.f, a.f), x, a.f, a.d, a.dw_gate, a.d);
+    if (a.dw_up) p.prod[p.products++] = product(operand(dgu + up, 2 * (int64_t)a.f, a.f), x, a.f, a.d, a.dw_up, a.d);
+    if (a.dw_down)
+        p.prod[p.products++] = product(operand(a.dy, a.dy_stride, a.e), operand(a.act, a.f, a.f), a.e, a.f, a.dw_down, a.f);
+    return launch_product<DT, kRContig, kRContig, 1, kEpiStore>(p, a.workspace, stream);
 }
 
 }  // namespace
 
 hipError_t launch_gated_ffn(const dsalt_gated_ffn_args &a, hipStream_t stream) {
     if (a.rows == 0) return hipSuccess;
-    if (a.dtype == DSALT_DTYPE_BF16) forward<BF16>(a, stream);
-    else forward<F16>(a, stream);
-    return hipGetLastError();
+    return a.dtype == DSALT_DTYPE_BF16 ? forward<BF16>(a, stream) : forward<F16>(a, stream);
 }
 
 hipError_t launch_gated_ffn_bwd(const dsalt_gated_ffn_args &a, hipStream_t stream) {
-    if (a.dtype == DSALT_DTYPE_BF16) backward<BF16>(a, stream);
-    else backward<F16>(a, stream);
-    return hipGetLastError();
+    return a.dtype == DSALT_DTYPE_BF16 ? backward<BF16>(a, stream) : backward<F16>(a, stream);
 }
 
-int64_t gated_ffn_workspace_bytes(int64_t, int, int, int, bool) { return 0; }
+int64_t gated_ffn_workspace_bytes(int64_t rows, int d, int f, int e, bool bwd) {
+    if (!bwd) {
+        const Extent up{rows, f}, down{rows, e};
+        int64_t most = plan(&down, 1, f, 1, false, kIoStore).part_bytes;
+        for (bool keep : {false, true}) most = std::max(most, plan(&up, 1, d, 1, true, io_pair(keep)).part_bytes);
+        return most;
+    }
+    const Extent da{rows, f}, dx{rows, d}, dw[3] = {{f, d}, {f, d}, {e, f}}, two[2] = {dw[0], dw[2]};
+    int64_t most = std::max(plan(&da, 1, e, 1, false, kIoGrad).part_bytes, plan(&dx, 1, f, 2, false, kIoStore).part_bytes);
+    // any of the three weight gradients may be wanted
+    most = std::max(most, plan(two, 2, rows, 1, false, kIoStore).part_bytes);
+    for (int first = 0; first < 3; ++first)
+        for (int count = 1; first + count <= 3; ++count)
+            most = std::max(most, plan(dw + first, count, rows, 1, false, kIoStore).part_bytes);
+    return most;
+}
+
 int64_t gated_ffn_max_ld() { return kGemmMaxLd; }
 
 }  // namespace dsalt

@@ -13,8 +13,7 @@
 // offsets inside a descriptor stay below 2^31 whatever the tensor's size.
 //
 // C's tile is formed transposed (first MFMA operand B, second A): a lane then holds four
-// consecutive n of one m per register group, and one lane-half swap makes them eight, 16 bytes
-// of a 16-bit row.
+// consecutive n of one m per register group, 16 bytes of an fp32 row.
 #pragma once
 
 #include "tiles.h"
@@ -22,7 +21,6 @@
 namespace dsalt {
 
 enum { kKContig = 0, kRContig = 1 };
-constexpr int kGemmBK = 64;
 constexpr uint32_t kOutOfRange = 0x80000000u;  // above every descriptor's size (kGemmMaxLd)
 constexpr int64_t kGemmMaxLd = 1 << 21;        // elements of a row stride: 256 rows stay below 2^30 bytes
 
@@ -32,35 +30,42 @@ struct GemmOperand {
     int64_t rows; // extent of r
 };
 
-// One operand's tile: ROWS rows of r, kGemmBK of k, filled by NW waves.
-template <int LAY, int ROWS, int NW>
+// One operand's tile: ROWS rows of r, BK of k, filled by NW waves.
+//
+// LDS has 64 banks of 4 bytes, and a 16-byte read serves 16 lanes at a time: the swizzle puts the
+// same chunk of 16 consecutive rows on 16 different places of 256 bytes (two rows of BK = 64, four
+// of BK = 32). With chunk ^ (row & 7), which spreads 8 rows, the reads took 2.2 times as long.
+template <int LAY, int ROWS, int BK, int NW>
 struct GemmTile {
-    static constexpr int BYTES = ROWS * kGemmBK * 2;
-    static constexpr int LPW = ROWS * 8 / (64 * NW);  // 16-byte loads per lane
-    static constexpr int CPR = LAY == kKContig ? 8 : ROWS / 8;  // chunks per LDS row
-    static constexpr int RPL = 64 / CPR;                        // LDS rows per load instruction
-    static_assert(ROWS * 8 % (64 * NW) == 0, "the waves cover the tile");
+    static constexpr int BYTES = ROWS * BK * 2;
+    static constexpr int LPW = BYTES / 16 / (64 * NW);               // 16-byte loads per lane
+    static constexpr int CPR = LAY == kKContig ? BK / 8 : ROWS / 8;  // chunks per LDS row
+    static constexpr int RPL = 64 / CPR;                             // LDS rows per load instruction
+    static_assert(BYTES % (16 * 64 * NW) == 0, "the waves cover the tile");
+
+    static __device__ __forceinline__ int swizzle(int row) {
+        if constexpr (LAY == kRContig) return (row & 3) << 2;
+        else return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+    }
 
     uint32_t off[2];  // of a wave's even and odd loads
-    int kchunk;       // kKContig: the lane's chunk of k
+    int kchunk[2];    // kKContig: their chunks of k
 
     __device__ __forceinline__ GemmTile(int wave, int lane, uint32_t ld) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int row = (wave * LPW + u) * RPL + lane / CPR, slot = lane % CPR;
-            if constexpr (LAY == kKContig) {
-                kchunk = slot ^ (row & 7);
-                off[u] = (uint32_t)row * ld + (kchunk << 4);
-            } else {
-                kchunk = 0;
-                off[u] = (uint32_t)row * ld + ((slot ^ ((row & 3) << 1)) << 4);
-            }
+            const int row = (wave * LPW + u) * RPL + lane / CPR, chunk = (lane % CPR) ^ swizzle(row);
+            kchunk[u] = chunk;
+            off[u] = (uint32_t)row * ld + (chunk << 4);
         }
     }
 
-    // Loads k0 .. k0 + 63 (k in all) of rows r0 .. r0 + ROWS - 1 to the tile at LDS byte `lds`.
-    __device__ __forceinline__ void load(uint32_t lds, int wave, const GemmOperand &o, int64_t r0, int64_t k0,
-                                         int64_t k) const {
+    // The loads of k0 .. k0 + BK - 1 (k in all) of rows r0 .. r0 + ROWS - 1.
+    struct Step {
+        i32x4 rsrc;
+        uint32_t v[2], ld;
+    };
+    __device__ __forceinline__ Step step(const GemmOperand &o, int64_t r0, int64_t k0, int64_t k) const {
         const int64_t left = k - k0;
         const char *p;
         int64_t bytes;
@@ -70,47 +75,46 @@ struct GemmTile {
             bytes = rows > 0 && left > 0 ? (rows - 1) * o.ld + left * 2 : 0;
         } else {
             p = o.base + k0 * o.ld + r0 * 2;
-            bytes = left > 0 && o.rows > r0 ? (min(left, (int64_t)kGemmBK) - 1) * o.ld + (o.rows - r0) * 2 : 0;
+            bytes = left > 0 && o.rows > r0 ? (min(left, (int64_t)BK) - 1) * o.ld + (o.rows - r0) * 2 : 0;
         }
-        const i32x4 rsrc = uniform_rsrc(buffer_rsrc(p, (uint32_t)bytes));
-        uint32_t v[2] = {off[0], off[1]};
-        if constexpr (LAY == kKContig) {
-            // a chunk past k would read the next row's first elements
-            if (kchunk * 8 >= left) v[0] = v[1] = kOutOfRange;
-        }
-        const uint32_t ld = (uint32_t)o.ld;
+        Step s{uniform_rsrc(buffer_rsrc(p, (uint32_t)bytes)), {off[0], off[1]}, (uint32_t)o.ld};
+        if constexpr (LAY == kKContig) {  // a chunk past k would read the next row's first elements
 #pragma unroll
-        for (int u = 0; u < LPW; ++u)
-            dma16(v[u & 1] + (uint32_t)((u & ~1) * RPL) * ld, rsrc,
-                  __builtin_amdgcn_readfirstlane(lds + (wave * LPW + u) * 1024));
+            for (int u = 0; u < 2; ++u)
+                if (kchunk[u] * 8 >= left) s.v[u] = kOutOfRange;
+        }
+        return s;
+    }
+    // Load `u` of LPW to the tile at LDS byte `lds`.
+    static __device__ __forceinline__ void issue(const Step &s, int u, uint32_t lds, int wave) {
+        dma16(s.v[u & 1] + (uint32_t)((u & ~1) * RPL) * s.ld, s.rsrc,
+              __builtin_amdgcn_readfirstlane(lds + (wave * LPW + u) * 1024));
     }
 };
 
-// Reads of a tile as MFMA operands: the lane's r = r0 + lane % 32, k = 16 step + 8 (lane / 32) .. + 7.
-template <int LAY, int ROWS>
+// Reads of a tile as MFMA operands: the lane's r = 32 block + lane % 32, k = 16 sub + 8 (lane / 32) .. + 7.
+template <int LAY, int ROWS, int BK>
 struct GemmFrag {
-    uint32_t a[2];  // byte of the lane's first element; kRContig: for even and odd 32-row blocks
+    uint32_t a;  // byte of the lane's first element in block 0, sub-step 0
     __device__ __forceinline__ explicit GemmFrag(int lane) {
+        typedef GemmTile<LAY, ROWS, BK, 1> Tile;
         if constexpr (LAY == kKContig) {
             const int row = lane & 31;
-            a[0] = a[1] = row * 128 + (((lane >> 5) ^ (row & 7)) << 4);
+            a = row * (BK * 2) + (((lane >> 5) ^ Tile::swizzle(row)) << 4);
         } else {
             // ds_read_b64_tr_b16 gives lane l element l % 4 of the 8-byte pieces that lanes
             // 16 (l / 16) + 4 e + (l % 16) / 4, e = 0..3, address: a lane addresses k-row
             // (l % 16) / 4 and columns 16 ((l / 16) % 2) + 4 (l % 4) of its half's block
             const int krow = ((lane >> 5) << 3) + ((lane >> 2) & 3);
             const int chunk = (((lane >> 4) & 1) << 1) + ((lane & 3) >> 1);
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-                a[p] = krow * (ROWS * 2) + (((chunk + 4 * p) ^ ((krow & 3) << 1)) << 4) + ((lane & 1) << 3);
+            a = krow * (ROWS * 2) + ((chunk ^ Tile::swizzle(krow)) << 4) + ((lane & 1) << 3);
         }
     }
-    // block: r0 / 32
-    __device__ __forceinline__ uint4 read(const char *tile, int block, int step) const {
+    __device__ __forceinline__ uint4 read(const char *tile, int block, int sub) const {
         if constexpr (LAY == kKContig) {
-            return *reinterpret_cast<const uint4 *>(tile + (a[0] ^ (step << 5)) + block * 4096);
+            return *reinterpret_cast<const uint4 *>(tile + (a ^ (sub << 5)) + block * (32 * BK * 2));
         } else {
-            const char *p = tile + a[block & 1] + (block >> 1) * 128 + step * (16 * ROWS * 2);
+            const char *p = tile + (a ^ ((block & 3) << 6)) + (block >> 2) * 256 + sub * (16 * ROWS * 2);
             const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)p);
             const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) shortx4 *)(p + 4 * ROWS * 2));
@@ -123,13 +127,19 @@ struct GemmFrag {
 // A workgroup's tile of the product: WM x WN waves over BM x BN, each FM x FN blocks of 32 x 32.
 // PAIR: the B tile's first half are rows of one matrix and its second half the same rows of
 // another (gate and up), and a wave holds the same n of both.
-template <class DT, int BM, int BN, int WM, int WN, int ALAY, int BLAY, bool PAIR>
+//
+// RA and RB = RA or RA - 1 stages of the A and B tiles: a step's loads are issued RA - 1 and
+// RB - 1 steps before it is read, into the stages that the barrier of the step before has freed.
+template <class DT, int BM, int BN, int BK_, int RA, int RB, int WM, int WN, int ALAY, int BLAY, bool PAIR>
 struct GemmCore {
-    static constexpr int NW = WM * WN, THREADS = NW * 64, FM = BM / WM / 32, FN = BN / WN / 32, BK = kGemmBK;
-    static constexpr int STAGE = (BM + BN) * BK * 2, LDS_BYTES = 2 * STAGE;
-    static constexpr int LOADS = (BM + BN) * 8 / THREADS;
-    typedef GemmTile<ALAY, BM, NW> TA;
-    typedef GemmTile<BLAY, PAIR ? BN / 2 : BN, PAIR ? NW / 2 : NW> TB;
+    static constexpr int BK = BK_, NW = WM * WN, THREADS = NW * 64, FM = BM / WM / 32, FN = BN / WN / 32, SUBS = BK / 16;
+    static constexpr int BNB = PAIR ? BN / 2 : BN, NWB = PAIR ? NW / 2 : NW;  // of one B matrix
+    typedef GemmTile<ALAY, BM, BK, NW> TA;
+    typedef GemmTile<BLAY, BNB, BK, NWB> TB;
+    static constexpr int ASTAGE = BM * BK * 2, BSTAGE = BN * BK * 2, LDS_BYTES = RA * ASTAGE + RB * BSTAGE;
+    static constexpr int LA = TA::LPW, LB = TB::LPW;
+    static_assert(SUBS % 2 == 0, "the operand registers alternate from one step to the next");
+    static_assert(RB >= 2 && (RA == RB || RA == RB + 1), "see the waits in run()");
 
     f32x16 acc[FM][FN];
     int wm, wn, lane, wave;
@@ -140,25 +150,36 @@ struct GemmCore {
         wm = wave % WM;
         wn = wave / WM;
     }
-    // `segments` products of the operands a[s], b[s] (PAIR: b[0], b[1] are the two matrices and
+
+    // `SEGMENTS` products of the operands a[s], b[s] (PAIR: b[0], b[1] are the two matrices and
     // there is one segment) over steps first .. last - 1 of their k-steps in order.
     template <int SEGMENTS>
     __device__ __forceinline__ void run(char *lds, const GemmOperand *a, const GemmOperand *b, int64_t m0, int64_t n0,
                                         int64_t k, int first, int last) {
         const uint32_t base = lds_addr(lds);
         const int per = (int)((k + BK - 1) / BK);  // steps of a segment
+        const int bwave = PAIR ? wave % NWB : wave;
+        const bool second = PAIR && wave >= NWB;
         const TA ta(wave, lane, (uint32_t)a[0].ld);
-        const int bwave = PAIR ? wave % (NW / 2) : wave;
-        const bool second = PAIR && wave >= NW / 2;
         const TB tb(bwave, lane, (uint32_t)(second ? b[1].ld : b[0].ld));
-        const uint32_t bbase = BM * BK * 2 + (second ? BN * BK : 0);
-        const GemmFrag<ALAY, BM> fa(lane);
-        const GemmFrag<BLAY, PAIR ? BN / 2 : BN> fb(lane);
-        auto load = [&](int stage, int step) {
+        const uint32_t bbase = base + RA * ASTAGE + (second ? TB::BYTES : 0);
+        const GemmFrag<ALAY, BM, BK> fa(lane);
+        const GemmFrag<BLAY, BNB, BK> fb(lane);
+        typename TA::Step sa;
+        typename TB::Step sb;
+        // past `last` the loads read nothing, so that every step counts the same number of loads
+        auto prepare_a = [&](int step) {
             const int s = SEGMENTS > 1 && step >= per ? 1 : 0;
-            const int64_t k0 = (int64_t)(step - s * per) * BK;
-            ta.load(base + stage * STAGE, wave, a[s], m0, k0, k);
-            tb.load(base + stage * STAGE + bbase, bwave, PAIR ? (second ? b[1] : b[0]) : b[s], n0, k0, k);
+            sa = ta.step(a[s], m0, step < last ? (int64_t)(step - s * per) * BK : k, k);
+        };
+        auto prepare_b = [&](int step) {
+            const int s = SEGMENTS > 1 && step >= per ? 1 : 0;
+            sb = tb.step(PAIR ? (second ? b[1] : b[0]) : b[s], n0, step < last ? (int64_t)(step - s * per) * BK : k, k);
+        };
+        // load u of a step: B's first, as its step is needed first where RA > RB
+        auto issue = [&](int sta, int stb, int u) {
+            if (u < LB) TB::issue(sb, u, bbase + stb * BSTAGE, bwave);
+            else TA::issue(sa, u - LB, base + sta * ASTAGE, wave);
         };
 #pragma unroll
         for (int i = 0; i < FM; ++i)
@@ -167,62 +188,117 @@ struct GemmCore {
         if (first >= last) return;
 
         uint4 ra[2][FM], rb[2][FN];
-        auto read = [&](int stage, int step, uint4 (&qa)[FM], uint4 (&qb)[FN]) {
-            const char *at = lds + stage * STAGE, *bt = at + BM * BK * 2;
-#pragma unroll
-            for (int i = 0; i < FM; ++i) qa[i] = fa.read(at, wm * FM + i, step);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                if constexpr (PAIR) {  // two tiles of BN / 2 rows
-                    const int blk = wn * (FN / 2) + j % (FN / 2);
-                    qb[j] = fb.read(bt + (j < FN / 2 ? 0 : BN * BK), blk, step);
-                } else {
-                    qb[j] = fb.read(bt, wn * FN + j, step);
-                }
+        // operand read r of FM + FN, in the order of the products' use: b0 a0 b1 b2 .. a1 ..
+        auto read = [&](int sta, int stb, int sub, int r, int buf) {
+            const char *at = lds + sta * ASTAGE, *bt = lds + RA * ASTAGE + stb * BSTAGE;
+            if (r == 0 || (r >= 2 && r <= FN)) {
+                const int j = r == 0 ? 0 : r - 1;
+                if constexpr (PAIR) rb[buf][j] = fb.read(bt + (j < FN / 2 ? 0 : TB::BYTES), wn * (FN / 2) + j % (FN / 2), sub);
+                else rb[buf][j] = fb.read(bt, wn * FN + j, sub);
+            } else {
+                const int i = r == 1 ? 0 : r - FN;
+                ra[buf][i] = fa.read(at, wm * FM + i, sub);
             }
         };
-        auto mul = [&](const uint4 (&qa)[FM], const uint4 (&qb)[FN]) {
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = DT::mfma(bitcast<typename DT::vec8>(qb[j]), bitcast<typename DT::vec8>(qa[i]), acc[i][j]);
+        auto mul = [&](int q, int buf) {
+            const int i = q / FN, j = q % FN;
+            acc[i][j] = DT::mfma(bitcast<typename DT::vec8>(rb[buf][j]), bitcast<typename DT::vec8>(ra[buf][i]), acc[i][j]);
         };
-        load(0, first);
-        if (first + 1 < last) {
-            load(1, first + 1);
-            tile_barrier<LOADS>();
-        } else {
-            tile_barrier<0>();
+        constexpr int NM = FM * FN, LT = LA + LB;
+        // the loads of a group are spread over the SUBS sub-steps after the barrier that frees their
+        // stages (part 0 .. SUBS - 1), one after every few products: issued in one go they fill the
+        // memory pipe's queue and hold the wave's products back
+        auto issue_after = [&](int sta, int stb, int part, int q) {
+#pragma unroll
+            for (int u = 0; u < LT; ++u)
+                if (u * SUBS / LT == part && (u * SUBS % LT * NM + LT * NM / 2 / LT) / LT == q) issue(sta, stb, u);
+        };
+        // group order: (A0 where RA > RB,) then B(t), A(t + RA - RB) for t = 0, 1, ..
+        if constexpr (RA > RB) {
+            prepare_a(first);
+#pragma unroll
+            for (int u = LB; u < LT; ++u) issue(0, 0, u);
         }
-        read(0, 0, ra[0], rb[0]);
+#pragma unroll
+        for (int t = 0; t < RB; ++t) {
+            prepare_b(first + t);
+            prepare_a(first + t + RA - RB);
+#pragma unroll
+            for (int u = 0; u < LT; ++u)
+                if (t < RB - 1 || u * SUBS / LT == 0) issue(t + RA - RB, t, u);
+        }
+        constexpr int PART0 = (LT + SUBS - 1) / SUBS;  // loads of a group's part 0
+        tile_barrier<PART0 + (RB - 2) * LT + (RA - RB) * LA>();
+#pragma unroll
+        for (int r = 0; r < FM + FN; ++r) read(0, 0, 0, r, 0);
+        int sta = 0, stb = 0, olda = RA - 1, oldb = RB - 1;
         for (int t = first; t < last; ++t) {
-            const int stage = (t - first) & 1;
+            // a read of the next sub-step's operands between one product and the next
 #pragma unroll
-            for (int s = 0; s < 3; ++s) {
-                read(stage, s + 1, ra[(s + 1) & 1], rb[(s + 1) & 1]);
-                mul(ra[s & 1], rb[s & 1]);
+            for (int s = 0; s < SUBS - 1; ++s)
+#pragma unroll
+                for (int q = 0; q < NM; ++q) {
+                    if (q < FM + FN) read(sta, stb, s + 1, q, (s + 1) & 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    mul(q, s & 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    issue_after(olda, oldb, s + 1, q);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            olda = sta;
+            oldb = stb;
+            sta = sta + 1 == RA ? 0 : sta + 1;
+            stb = stb + 1 == RB ? 0 : stb + 1;
+            prepare_b(t + RB);
+            prepare_a(t + RA);
+            __builtin_amdgcn_sched_barrier(0);
+            // every wave is done reading the old stages, and the next step's tiles have landed: of the
+            // loads issued since, only whole groups (and A's part of one) may be outstanding
+            tile_barrier<(RB - 2) * LT + (RA - RB) * LA>();
+#pragma unroll
+            for (int q = 0; q < NM; ++q) {
+                if (q < FM + FN) read(sta, stb, 0, q, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                mul(q, 1);
+                __builtin_amdgcn_sched_barrier(0);
+                issue_after(olda, oldb, 0, q);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            // every wave is done reading this stage, and the next step's tiles have landed
-            tile_barrier<0>();
-            if (t + 2 < last) load(stage, t + 2);
-            if (t + 1 < last) read(stage ^ 1, 0, ra[0], rb[0]);
-            mul(ra[1], rb[1]);
         }
+        tile_barrier<0>();  // no load may land in LDS that another workgroup has by then
     }
 
-    // The lane's 16-byte piece `half` (0, 1) of block (i, j): m = m0 + row(i), n = n0 + j * 32 + col(half)
-    __device__ __forceinline__ int row(int i) const { return (wm * FM + i) * 32 + (lane & 31); }
-    __device__ __forceinline__ int col(int half) const { return half * 16 + (lane >> 5) * 8; }
-    // eight fp32 values of consecutive n
-    __device__ __forceinline__ void values(const f32x16 &c, int half, float (&v)[8]) const {
+    // The accumulators hold one row m per lane; memory wants whole rows. Each wave turns its row
+    // blocks (32 rows of FN * 32 fp32 columns) in its own part of LDS, free after run(): it
+    // writes them with put() and reads them with get() as pieces of eight columns, piece t * 64 +
+    // lane of the block's pieces in row order, so that loads and stores of 16 bits a column cover
+    // 16-byte pieces of whole rows. XOR with the row spreads the rows over the banks.
+    static constexpr int COLS = FN * 32, PIECES = (PAIR ? COLS / 2 : COLS) / 8, TURNS = 32 * PIECES / 64;
+    __device__ __forceinline__ char *turn(char *lds) const { return lds + wave * (32 * COLS * 4); }
+    __device__ __forceinline__ void put(char *lds, const f32x16 (&row)[FN]) const {
+        const int r = lane & 31;
+        char *p = turn(lds) + r * (COLS * 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[half * 8 + e]), __float_as_uint(c[half * 8 + 4 + e]),
-                                                      false, false);
-            v[e] = __uint_as_float(r[0]);
-            v[4 + e] = __uint_as_float(r[1]);
-        }
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+                *reinterpret_cast<float4 *>(p + (((j * 8 + h * 2 + (lane >> 5)) ^ (r & 15)) << 4)) =
+                    make_float4(row[j][4 * h], row[j][4 * h + 1], row[j][4 * h + 2], row[j][4 * h + 3]);
+        __builtin_amdgcn_wave_barrier();
+    }
+    // Row and first column (of the wave's) of the lane's piece in turn t.
+    static constexpr int TURN_ROWS = 64 / PIECES;
+    static_assert(64 % PIECES == 0, "a turn covers whole rows");
+    __device__ __forceinline__ int piece_row(int t) const { return t * TURN_ROWS + lane / PIECES; }
+    __device__ __forceinline__ int piece_col() const { return lane % PIECES * 8; }
+    // offset: columns from the piece's (PAIR: COLS / 2 reaches the second matrix)
+    __device__ __forceinline__ void get(const char *lds, int t, int offset, float (&v)[8]) const {
+        const int r = piece_row(t), c = (piece_col() + offset) / 4;
+        const char *p = turn(const_cast<char *>(lds)) + r * (COLS * 4);
+        const float4 lo = *reinterpret_cast<const float4 *>(p + ((c ^ (r & 15)) << 4));
+        const float4 hi = *reinterpret_cast<const float4 *>(p + (((c + 1) ^ (r & 15)) << 4));
+        v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+        v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
     }
 };
 
