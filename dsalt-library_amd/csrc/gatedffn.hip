@@ -13,9 +13,12 @@
 #include "launch.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace dsalt {
 namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
 
@@ -35,9 +38,15 @@ __device__ __forceinline__ void act_grad(float g, float &v, float &slope) {
         v = g * s;
         slope = s + g * s * (1.f - s) * (2.f * kGeluTanhC) * (1.f + 3.f * 0.044715f * c2);
     } else if constexpr (ACT == DSALT_ACT_GELU) {
-        const float phi = 0.5f * erfcf(-0.7071067811865476f * g);
+        // 0.5 erfc(|g| / sqrt 2) by Abramowitz and Stegun 7.1.26 (error below 1.5e-7, a quarter of
+        // a thousandth of a 16-bit rounding), whose exp(-g^2 / 2) the slope takes too
+        const float x = 0.7071067811865476f * fabsf(g), t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+        const float ex = fast_exp2(-0.5f * kLog2e * g * g);
+        const float tail = 0.5f * ex * t *
+            (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        const float phi = g < 0.f ? tail : 1.f - tail;
         v = g * phi;
-        slope = phi + g * 0.3989422804014327f * fast_exp2(-0.5f * kLog2e * g * g);
+        slope = phi + g * 0.3989422804014327f * ex;
     } else {
         const bool off = g <= 0.f;  // NaN stays NaN
         v = off ? 0.f : g;
@@ -45,7 +54,7 @@ __device__ __forceinline__ void act_grad(float g, float &v, float &slope) {
     }
 }
 // Eight at a time inside the choice of the activation, so that their chains of exp and
-// reciprocal overlap (erfc's long ones would take too many registers and go one by one).
+// reciprocal overlap.
 template <int ACT>
 __device__ __forceinline__ void gated8(const float (&g)[8], const float (&u)[8], float (&a)[8]) {
 #pragma unroll
@@ -53,7 +62,6 @@ __device__ __forceinline__ void gated8(const float (&g)[8], const float (&u)[8],
         float v, s;
         act_grad<ACT>(g[e], v, s);
         a[e] = v * u[e];
-        if constexpr (ACT == DSALT_ACT_GELU) __builtin_amdgcn_sched_barrier(0);
     }
 }
 __device__ __forceinline__ void gated8(int act, const float (&g)[8], const float (&u)[8], float (&a)[8]) {
@@ -72,7 +80,6 @@ __device__ __forceinline__ void gated_grad8(const float (&g)[8], float (&u)[8], 
         const float d = da[e];
         da[e] = d * u[e] * s;
         u[e] = d * v;
-        if constexpr (ACT == DSALT_ACT_GELU) __builtin_amdgcn_sched_barrier(0);
     }
 }
 __device__ __forceinline__ void gated_grad8(int act, const float (&g)[8], float (&u)[8], float (&da)[8]) {
@@ -271,6 +278,106 @@ __global__ void __launch_bounds__(S::WM *S::WN * 64) ffn_join_kernel(const FfnPa
     epilogue<DT, C, EPI, 1>(p, q, c, acc, i, m0, n0, lds);
 }
 
+// Few rows (up to 16 TT): bound by the weights' bytes, and by the latency of a call this short.
+// A workgroup takes 16 weight rows (pair: the same 8 of both weights) and all rows of x; its waves
+// take every NW-th 32 of k straight from memory into the operands of v_mfma_f32_16x16x32, so that
+// nothing waits on LDS until their sums are added there, in order.
+template <class DT>
+__device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (std::is_same<DT, BF16>::value)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bitcast<bf16x8>(a), bitcast<bf16x8>(b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
+}
+
+constexpr int kFewRows = 64, kFewUnroll = 4;
+template <class DT, int TT, int NW, int EPI>
+__global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const FfnParams p) {
+    constexpr bool PAIR = EPI == kEpiPair;
+    __shared__ float4 part[NW][TT][64];
+    const Product &q = p.prod[0];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15;
+    const int n0 = blockIdx.x * (PAIR ? 8 : 16);
+    // the lane's weight row: gate or up row n0 + l16 % 8 of a pair
+    const GemmOperand &b = PAIR && l16 >= 8 ? q.b[1] : q.b[0];
+    const int n = n0 + (PAIR ? l16 & 7 : l16), kl = (lane >> 4) * 8;
+    const char *w = b.base + (int64_t)n * b.ld + kl * 2, *x[TT];
+    bool xin[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        xin[t] = t * 16 + l16 < q.m;
+        x[t] = q.a[0].base + (int64_t)(t * 16 + l16) * q.a[0].ld + kl * 2;
+    }
+    const bool win = n < q.n;
+    const int k = (int)p.k;
+    f32x4 acc[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = wave * 32; k0 < k; k0 += NW * 32 * kFewUnroll) {
+        uint4 wv[kFewUnroll], xv[kFewUnroll][TT];
+#pragma unroll
+        for (int s = 0; s < kFewUnroll; ++s) {
+            const int at = k0 + s * NW * 32;
+            const bool in = at + kl < k;
+            wv[s] = in && win ? *reinterpret_cast<const uint4 *>(w + at * 2) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+                xv[s][t] = in && xin[t] ? *reinterpret_cast<const uint4 *>(x[t] + at * 2) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int s = 0; s < kFewUnroll; ++s)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[t] = mfma16<DT>(wv[s], xv[s][t], acc[t]);
+    }
+    // lane l holds rows 4 (l / 16) .. + 3 of the 16 weight rows for x row t * 16 + l % 16
+#pragma unroll
+    for (int t = 0; t < TT; ++t) part[wave][t][lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+    __syncthreads();
+    // a thread forms eight columns of one row: the gates and ups of a pair, or one half of 16
+    const int id = threadIdx.x, half = PAIR ? 0 : id / (16 * TT), r = id % (16 * TT);
+    if (id >= 16 * TT * (PAIR ? 1 : 2) || r >= q.m) return;
+    auto sum = [&](int group, float (&v)[8]) {  // of weight rows 4 group .. + 7
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float4 s = part[0][r >> 4][(group + h) * 16 + (r & 15)];
+            for (int wv = 1; wv < NW; ++wv) {
+                const float4 o = part[wv][r >> 4][(group + h) * 16 + (r & 15)];
+                s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
+            }
+            v[4 * h] = s.x; v[4 * h + 1] = s.y; v[4 * h + 2] = s.z; v[4 * h + 3] = s.w;
+        }
+    };
+    float v[8], u[8], a[8];
+    const int64_t col = n0 + half * 8;
+    if (col >= q.n) return;
+    sum(half * 2, v);
+    char *o = q.out + (int64_t)r * q.out_ld + col * 2;
+    if constexpr (PAIR) {
+        sum(2, u);
+        if (p.gu) {
+            char *gu = p.gu + (int64_t)r * p.gu_ld + col * 2;
+            *reinterpret_cast<uint4 *>(gu) = pack8<DT>(v);
+            *reinterpret_cast<uint4 *>(gu + p.up_off) = pack8<DT>(u);
+        }
+        gated8(p.act, v, u, a);
+        *reinterpret_cast<uint4 *>(o) = pack8<DT>(a);
+    } else {
+        *reinterpret_cast<uint4 *>(o) = pack8<DT>(v);
+    }
+}
+
+template <class DT, int EPI>
+hipError_t launch_few(const FfnParams &p, hipStream_t stream) {
+    // the second product's k is the longer one, and its grid the smaller
+    constexpr int NW = EPI == kEpiPair ? 8 : 16;
+    const Product &q = p.prod[0];
+    const dim3 grid((unsigned)((q.n + (EPI == kEpiPair ? 7 : 15)) / (EPI == kEpiPair ? 8 : 16))), block(NW * 64);
+    if (q.m <= 16) hipLaunchKernelGGL((ffn_few_kernel<DT, 1, NW, EPI>), grid, block, 0, stream, p);
+    else if (q.m <= 32) hipLaunchKernelGGL((ffn_few_kernel<DT, 2, NW, EPI>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((ffn_few_kernel<DT, 4, NW, EPI>), grid, block, 0, stream, p);
+    return hipGetLastError();
+}
+
 // How a launch covers its tiles: the shape, and into how many pieces the tiles past the last full
 // round of workgroups are cut along k.
 //
@@ -298,8 +405,9 @@ constexpr ShapeCost kShapes[] = {
     {256, 256, 256, 1.85, 1.20, 1.0},
     {256, 128, 256, 1.12, 0.65, 1.0},
     {128, 128, 512, 1.17, 0.40, 0.5},
+    {64, 128, 768, 0.95, 0.30, 0.4},
 };
-constexpr int kShapeCount = 3, kMaxSplit = 8;
+constexpr int kShapeCount = 4, kMaxSplit = 8;
 constexpr double kTile = 3.0, kJoin = 6.0, kMemory = 5.0e6, kPartials = 3.0e6;  // us, us, bytes per us
 
 int64_t tiles_of(int64_t m, int64_t n, int shape, bool pair) {
@@ -369,11 +477,11 @@ hipError_t launch_product(FfnParams p, void *workspace, hipStream_t stream) {
     p.whole = w.whole;
     p.split = w.split;
     p.part = static_cast<float *>(workspace);
-    if (getenv("FS")) w.shape = 0; // PROBE
     switch (w.shape) {
         case 0: return launch_shape<DT, Shape<256, 256, 3, 2, 4, 2>, ALAY, BLAY, SEGMENTS, EPI>(p, w, stream);
         case 1: return launch_shape<DT, Shape<256, 128, 3, 3, 4, 2>, ALAY, BLAY, SEGMENTS, EPI>(p, w, stream);
-        default: return launch_shape<DT, Shape<128, 128, 2, 2, 2, 2>, ALAY, BLAY, SEGMENTS, EPI>(p, w, stream);
+        case 2: return launch_shape<DT, Shape<128, 128, 2, 2, 2, 2>, ALAY, BLAY, SEGMENTS, EPI>(p, w, stream);
+        default: return launch_shape<DT, Shape<64, 128, 2, 2, 2, 2>, ALAY, BLAY, SEGMENTS, EPI>(p, w, stream);
     }
 }
 
@@ -401,13 +509,16 @@ hipError_t forward(const dsalt_gated_ffn_args &a, hipStream_t stream) {
     p.gu = static_cast<char *>(a.gate_up);
     p.gu_ld = (int64_t)a.f * 4;
     p.up_off = (int64_t)a.f * 2;
-    hipError_t e = launch_product<DT, kKContig, kKContig, 1, kEpiPair>(p, a.workspace, stream);
+    const bool few = a.rows <= kFewRows;
+    hipError_t e = few ? launch_few<DT, kEpiPair>(p, stream)
+                       : launch_product<DT, kKContig, kKContig, 1, kEpiPair>(p, a.workspace, stream);
     if (e != hipSuccess) return e;
     FfnParams q{};
     q.products = 1;
     q.k = a.f;
     q.prod[0] = product(operand(a.act, a.f, a.rows), operand(a.w_down, a.w_down_stride, a.e), a.rows, a.e, a.y, a.e);
-    return launch_product<DT, kKContig, kKContig, 1, kEpiStore>(q, a.workspace, stream);
+    return few ? launch_few<DT, kEpiStore>(q, stream)
+               : launch_product<DT, kKContig, kKContig, 1, kEpiStore>(q, a.workspace, stream);
 }
 
 template <class DT>
@@ -461,6 +572,7 @@ hipError_t launch_gated_ffn_bwd(const dsalt_gated_ffn_args &a, hipStream_t strea
 
 int64_t gated_ffn_workspace_bytes(int64_t rows, int d, int f, int e, bool bwd) {
     if (!bwd) {
+        if (rows <= kFewRows) return 0;
         const Extent up{rows, f}, down{rows, e};
         int64_t most = plan(&down, 1, f, 1, false, kIoStore).part_bytes;
         for (bool keep : {false, true}) most = std::max(most, plan(&up, 1, d, 1, true, io_pair(keep)).part_bytes);

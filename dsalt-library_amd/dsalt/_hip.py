@@ -7,9 +7,9 @@ fallback: a missing library or a non-GPU tensor raises ``DsaltError``.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
@@ -335,15 +335,18 @@ def check_abi() -> None:
     h = lib()
     if h.dsalt_abi_version() != ABI_VERSION:
         raise DsaltError(f"ABI version mismatch: library {h.dsalt_abi_version()} vs binding {ABI_VERSION}")
-    for struct, fn in ((FwdArgs, h.dsalt_fwd_args_size), (BwdArgs, h.dsalt_bwd_args_size),
+    for args, fn in ((FwdArgs, h.dsalt_fwd_args_size), (BwdArgs, h.dsalt_bwd_args_size),
                        (SelectArgs, h.dsalt_select_args_size), (ScoresArgs, h.dsalt_scores_args_size),
                        (RopeArgs, h.dsalt_rope_args_size), (LmkWeightsArgs, h.dsalt_lmk_weights_args_size),
                        (RopeTables, h.dsalt_rope_tables_size), (QkvArgs, h.dsalt_qkv_args_size),
                        (ModuleGradsArgs, h.dsalt_module_grads_args_size),
                        (NormTrainArgs, h.dsalt_norm_train_args_size), (GatedFfnArgs, h.dsalt_gated_ffn_args_size),
                        (DropoutArgs, h.dsalt_dropout_args_size), (BranchNormArgs, h.dsalt_branch_norm_args_size)):
-        if ctypes.sizeof(struct) != fn():
-            raise DsaltError(f"{struct.__name__} layout mismatch: {ctypes.sizeof(struct)} vs {fn()} bytes")
+        if ctypes.sizeof(args) != fn():
+            raise DsaltError(f"{args.__name__} layout mismatch: {ctypes.sizeof(args)} vs {fn()} bytes")
+    for pack, args in ((_FFN_PACK, GatedFfnArgs), (_DROPOUT_PACK, DropoutArgs), (_BRANCH_PACK, BranchNormArgs)):
+        if pack.size != ctypes.sizeof(args):
+            raise DsaltError(f"{args.__name__} packs to {pack.size} of {ctypes.sizeof(args)} bytes")
 
 
 def _raise(rc: int, what: str) -> None:
@@ -377,15 +380,6 @@ def stream_handle(device: torch.device) -> int:
     """The raw handle of the current stream of `device` (read on every launch)."""
     index = device.index
     return _current_raw_stream(torch.cuda.current_device() if index is None else index)
-
-
-def on_device(device: torch.device):
-    """A context whose current device is `device`, where launches on its streams (the default
-    one among them) belong."""
-    index = device.index
-    if index is None or index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(index)
 
 
 def compute_dtype(dtype: torch.dtype) -> torch.dtype:
@@ -1563,73 +1557,96 @@ def swiglu_rows(gate_up: torch.Tensor, d_out: torch.Tensor | None = None) -> tor
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}  # DSALT_ACT_*
 
+# The argument structs of the calls below as struct.pack formats: a call packs its values in one
+# go, which costs a tenth of filling a ctypes.Structure field by field.
+_FFN_PACK = struct.Struct("@q6iPq3P3q3PPq5PPq")
+_DROPOUT_PACK = struct.Struct("@q2iPP2qP")
+_BRANCH_PACK = struct.Struct("@q9i3f2qP5P2P2P2P5PPq")
+_packed_calls: dict = {}
+
+
+def _call(name: str, args: bytes, device: torch.device) -> None:
+    """The library's `name`(args, stream) on the current stream of `device`."""
+    fn = _packed_calls.get(name)
+    if fn is None:
+        fn = lib()[name]  # a function object of its own: lib()'s keeps its typed arguments
+        fn.argtypes, fn.restype = [ctypes.c_char_p, c_void_p], ctypes.c_int
+        _packed_calls[name] = fn
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(args, _current_raw_stream(index))
+    else:  # launches on a device's streams (the default one among them) belong to it
+        with torch.cuda.device(device):
+            rc = fn(args, stream_handle(device))
+    if rc:
+        _raise(rc, name)
+
 
 def row_operand(t: torch.Tensor) -> torch.Tensor:
     """t [n, m] as dsalt_gated_ffn reads it: unit stride along the rows, row strides that are
     multiples of 8 and cover a row, 16-byte aligned (a copy only where it is not so)."""
-    if (t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.shape[1] <= t.stride(0) <= 1 << 21 and t.data_ptr() % 16 == 0):
+    rs, cs = t.stride()
+    if cs == 1 and rs % 8 == 0 and t.shape[1] <= rs <= 1 << 21 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _gated_ffn_args(rows, x, w_gate, w_up, w_down, activation: str) -> GatedFfnArgs:
-    f, d = w_gate.shape
-    return GatedFfnArgs(rows=rows, d=d, f=f, e=w_down.shape[0], dtype=_DTYPES[w_gate.dtype],
-                        activation=ACTIVATIONS[activation], x=_ptr(x), x_stride=d if x is None else x.stride(0),
-                        w_gate=w_gate.data_ptr(), w_up=w_up.data_ptr(), w_down=w_down.data_ptr(),
-                        w_gate_stride=w_gate.stride(0), w_up_stride=w_up.stride(0), w_down_stride=w_down.stride(0))
-
-
-def _ffn_workspace(a: GatedFfnArgs, backward: bool, dev: torch.device) -> torch.Tensor | None:
-    a.workspace_bytes = lib().dsalt_gated_ffn_workspace_size(a.rows, a.d, a.f, a.e, int(backward))
-    if a.workspace_bytes == 0:
-        return None
-    ws = torch.empty(a.workspace_bytes, device=dev, dtype=torch.uint8)
-    a.workspace = ws.data_ptr()
-    return ws
-
-
 def gated_ffn(x, w_gate, w_up, w_down, activation: str, lead, keep: bool):
-    """``(y [*lead, e], gate_up, act)`` of `row_operand` x [T, d] and weights: see dsalt_gated_ffn.
-    gate_up is None without `keep`."""
-    dev = require_gpu(x, w_gate, w_up, w_down)
-    a = _gated_ffn_args(x.shape[0], x, w_gate, w_up, w_down, activation)
-    act, y = x.new_empty(a.rows, a.f), x.new_empty(*lead, a.e)
-    gate_up = x.new_empty(a.rows, 2 * a.f) if keep else None
-    a.act, a.y, a.gate_up = act.data_ptr(), y.data_ptr(), _ptr(gate_up)
-    ws = _ffn_workspace(a, False, dev)  # noqa: F841  (held over the call)
-    with on_device(dev):
-        _raise(lib().dsalt_gated_ffn(ctypes.byref(a), stream_handle(dev)), "dsalt_gated_ffn")
-    return y, gate_up, act
+    """``(y [*lead, e], kept)`` of `row_operand` x [T, d] and weights: see dsalt_gated_ffn. kept is
+    one buffer for the backward: act [T, f], and gate | up [T, 2 f] behind it with `keep`."""
+    dev = x.device
+    rows, d = x.shape
+    f, e = w_gate.shape[0], w_down.shape[0]
+    kept = x.new_empty(rows * f * (3 if keep else 1))
+    y = x.new_empty(*lead, e)
+    act = kept.data_ptr()
+    need = lib().dsalt_gated_ffn_workspace_size(rows, d, f, e, 0)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None  # held over the call
+    _call("dsalt_gated_ffn",
+          _FFN_PACK.pack(rows, d, f, e, _DTYPES[x.dtype], ACTIVATIONS[activation], 0, x.data_ptr(), x.stride(0),
+                         w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), w_gate.stride(0), w_up.stride(0),
+                         w_down.stride(0), act + rows * f * 2 if keep else 0, act, y.data_ptr(), 0, 0, 0, 0, 0, 0, 0,
+                         ws.data_ptr() if need else 0, need), dev)
+    return y, kept
 
 
-def gated_ffn_bwd(x, w_gate, w_up, w_down, activation: str, gate_up, act, dy, need):
+def gated_ffn_bwd(x, w_gate, w_up, w_down, activation: str, kept, dy, need):
     """``(dx [T, d], dw_gate, dw_up, dw_down)``, None where not in `need`: see dsalt_gated_ffn_bwd.
-    x and gate_up may be None where only dw_down is needed."""
-    dev = require_gpu(x, w_gate, w_up, w_down, gate_up, act, dy)
-    a = _gated_ffn_args(dy.shape[0], x, w_gate, w_up, w_down, activation)
-    a.gate_up, a.act, a.dy, a.dy_stride = _ptr(gate_up), act.data_ptr(), dy.data_ptr(), dy.stride(0)
-    shapes = ((a.rows, a.d), w_gate.shape, w_up.shape, w_down.shape)
-    out = [dy.new_empty(s) if n else None for s, n in zip(shapes, need)]
-    a.dx, a.dw_gate, a.dw_up, a.dw_down = (_ptr(t) for t in out)
-    d_gate_up = torch.empty_like(gate_up) if any(need[:3]) else None
-    a.d_gate_up = _ptr(d_gate_up)
-    ws = _ffn_workspace(a, True, dev)  # noqa: F841
-    with on_device(dev):
-        _raise(lib().dsalt_gated_ffn_bwd(ctypes.byref(a), stream_handle(dev)), "dsalt_gated_ffn_bwd")
-    return out
+    x may be None, and `kept` without gate | up, where only dw_down is needed."""
+    dev = dy.device
+    rows, e = dy.shape
+    f, d = w_gate.shape
+    inner = need[0] or need[1] or need[2]
+    dx = dy.new_empty(rows, d) if need[0] else None
+    dwg, dwu, dwd = (torch.empty(w.shape, device=dev, dtype=dy.dtype) if n else None
+                     for w, n in ((w_gate, need[1]), (w_up, need[2]), (w_down, need[3])))
+    # one scratch buffer: the gradient of gate | up, then the workspace
+    part = rows * f * 4 if inner else 0
+    size = lib().dsalt_gated_ffn_workspace_size(rows, d, f, e, 1)
+    scratch = torch.empty(part + size, device=dev, dtype=torch.uint8) if part + size else None
+    base = scratch.data_ptr() if part + size else 0
+    act = kept.data_ptr()
+    _call("dsalt_gated_ffn_bwd",
+          _FFN_PACK.pack(rows, d, f, e, _DTYPES[dy.dtype], ACTIVATIONS[activation], 0,
+                         *((0, d) if x is None else (x.data_ptr(), x.stride(0))),
+                         w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), w_gate.stride(0), w_up.stride(0),
+                         w_down.stride(0), act + rows * f * 2 if inner else 0, act, 0, dy.data_ptr(), dy.stride(0),
+                         base if inner else 0, dx.data_ptr() if need[0] else 0, dwg.data_ptr() if need[1] else 0,
+                         dwu.data_ptr() if need[2] else 0, dwd.data_ptr() if need[3] else 0, base + part if size else 0, size),
+          dev)
+    return dx, dwg, dwu, dwd
 
 
-def seed_fields(seed, device: torch.device) -> tuple[int, int | None]:
+def seed_fields(seed, device: torch.device) -> tuple[int, int]:
     """(seed, seed_ptr) of a Python int or of an int64 GPU tensor of one element."""
     if isinstance(seed, torch.Tensor):
-        if require_gpu(seed) != device or seed.dtype != torch.int64 or seed.numel() != 1:
+        if seed.device != device or seed.dtype != torch.int64 or seed.numel() != 1:
             raise DsaltError(f"a seed tensor must be one int64 element on {device} (got {tuple(seed.shape)} {seed.dtype} "
                              f"on {seed.device})")
         return 0, seed.data_ptr()
     if not -2 ** 63 <= seed < 2 ** 64:
         raise ValueError(f"seed must fit 64 bits (got {seed})")
-    return (seed + 2 ** 63) % 2 ** 64 - 2 ** 63, None
+    return (seed + 2 ** 63) % 2 ** 64 - 2 ** 63, 0
 
 
 def keep_threshold(p: float) -> int:
@@ -1641,64 +1658,71 @@ def keep_threshold(p: float) -> int:
 
 def dropout(x: torch.Tensor, p: float, seed, offset: int) -> torch.Tensor:
     """Contiguous dropout of contiguous, 16-byte aligned x: see dsalt_dropout."""
-    dev = require_gpu(x)
+    dev = x.device
     out = torch.empty_like(x)
-    a = DropoutArgs(n=x.numel(), dtype=_SCORE_DTYPES[x.dtype], threshold=keep_threshold(p), x=x.data_ptr(),
-                    out=out.data_ptr(), offset=offset)
-    a.seed, a.seed_ptr = seed_fields(seed, dev)
-    with on_device(dev):
-        _raise(lib().dsalt_dropout(ctypes.byref(a), stream_handle(dev)), "dsalt_dropout")
+    _call("dsalt_dropout", _DROPOUT_PACK.pack(x.numel(), _SCORE_DTYPES[x.dtype], keep_threshold(p), x.data_ptr(),
+                                              out.data_ptr(), *((seed, offset, 0) if type(seed) is int and -2 ** 63 <= seed < 2 ** 63
+                                                                else _seed_offset(seed, offset, dev))), dev)
     return out
+
+
+def _seed_offset(seed, offset: int, device: torch.device) -> tuple[int, int, int]:
+    """(seed, offset, seed_ptr) as the argument structs hold them."""
+    value, ptr = seed_fields(seed, device)
+    return value, offset, ptr
 
 
 BRANCH_NORM_MAX_DIM = 8192  # largest row length of dsalt_branch_norm
 
 
-def _branch_args(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, eps, post_eps, out_dtype):
+def _code(t: torch.Tensor | None) -> int:
+    return 0 if t is None else _SCORE_DTYPES[t.dtype]
+
+
+def _addr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _branch_pack(x, h, weight, post_weight, gate, opts, seed, *, x_out=0, y=0, rstd=0, rstd_post=0, dx_out=0, dy=0,
+                 grads=(0, 0, 0, 0, 0), ws=(0, 0)) -> bytes:
+    residual_scale, p, offset, eps, post_eps, out_dtype = opts
     d = x.shape[-1]
-    a = BranchNormArgs(rows=x.numel() // d, d=d, x_dtype=_SCORE_DTYPES[x.dtype], h_dtype=_SCORE_DTYPES[h.dtype],
-                       y_dtype=_SCORE_DTYPES[out_dtype], threshold=keep_threshold(p), eps=eps, post_eps=post_eps,
-                       residual_scale=residual_scale, offset=offset, x=x.data_ptr(), h=h.data_ptr(),
-                       weight=_ptr(weight), post_weight=_ptr(post_weight), gate=_ptr(gate))
-    for name, t in (("w_dtype", weight), ("post_dtype", post_weight), ("gate_dtype", gate)):
-        if t is not None:
-            setattr(a, name, _SCORE_DTYPES[t.dtype])
-    if gate is not None:
-        a.gate_kind = 1 if gate.dim() == 1 else 2
-    if a.threshold < 65536:
-        a.seed, a.seed_ptr = seed_fields(seed, x.device)
-    return a
+    threshold = keep_threshold(p)
+    return _BRANCH_PACK.pack(
+        x.numel() // d, d, _SCORE_DTYPES[x.dtype], _SCORE_DTYPES[h.dtype], _SCORE_DTYPES[out_dtype], _code(weight),
+        _code(post_weight), _code(gate), 0 if gate is None else 1 if gate.dim() == 1 else 2, threshold, eps, post_eps,
+        residual_scale, *(_seed_offset(seed, offset, x.device) if threshold < 65536 else (0, 0, 0)), x.data_ptr(), h.data_ptr(),
+        _addr(weight), _addr(post_weight), _addr(gate), x_out, y, rstd, rstd_post, dx_out, dy, *grads, *ws)
 
 
-def branch_norm(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, eps, post_eps, out_dtype, keep: bool):
-    """``(x_out, y, rstd, rstd_post)`` of contiguous, aligned operands: see dsalt_branch_norm; gate
-    [d] or [..., 1]. The statistics are None without `keep`."""
-    dev = require_gpu(x, h, weight, post_weight, gate)
-    a = _branch_args(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, eps, post_eps, out_dtype)
+def branch_norm(x, h, weight, post_weight, gate, opts, seed, keep: bool):
+    """``(x_out, y, stats)`` of contiguous, aligned operands: see dsalt_branch_norm; gate [d] or
+    [..., 1]; opts = (residual_scale, p, offset, eps, post_eps, out_dtype). stats: rstd and
+    rstd_post [2, rows] for the backward, None without `keep`."""
+    dev = x.device
     x_out = torch.empty_like(x)
-    y = torch.empty_like(x, dtype=out_dtype) if weight is not None else None
-    rstd, rstd_post = (torch.empty(a.rows, device=dev, dtype=torch.float32) if keep and w is not None else None
-                       for w in (weight, post_weight))
-    a.x_out, a.y, a.rstd, a.rstd_post = x_out.data_ptr(), _ptr(y), _ptr(rstd), _ptr(rstd_post)
-    with on_device(dev):
-        _raise(lib().dsalt_branch_norm(ctypes.byref(a), stream_handle(dev)), "dsalt_branch_norm")
-    return x_out, y, rstd, rstd_post
+    y = torch.empty_like(x, dtype=opts[5]) if weight is not None else None
+    rows = x.numel() // x.shape[-1]
+    stats = torch.empty((2, rows), device=dev, dtype=torch.float32) if keep else None
+    at = stats.data_ptr() if keep else 0
+    _call("dsalt_branch_norm", _branch_pack(x, h, weight, post_weight, gate, opts, seed, x_out=x_out.data_ptr(), y=_addr(y),
+                                            rstd=at, rstd_post=at + 4 * rows if keep else 0), dev)
+    return x_out, y, stats
 
 
-def branch_norm_bwd(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, out_dtype, rstd, rstd_post, dx_out, dy,
-                    need):
+def branch_norm_bwd(x, h, weight, post_weight, gate, opts, seed, stats, dx_out, dy, need):
     """``(dx, dh, d_weight, d_post_weight, d_gate)``, None where not in `need`: see
     dsalt_branch_norm_bwd."""
-    dev = require_gpu(x, h, weight, post_weight, gate, dx_out, dy)
-    a = _branch_args(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, 0.0, 0.0, out_dtype)
-    a.rstd, a.rstd_post, a.dx_out, a.dy = _ptr(rstd), _ptr(rstd_post), _ptr(dx_out), _ptr(dy)
+    dev = x.device
+    rows, d = x.numel() // x.shape[-1], x.shape[-1]
     out = [torch.empty_like(t) if n else None for t, n in zip((x, h, weight, post_weight, gate), need)]
-    a.dx, a.dh, a.d_weight, a.d_post_weight, a.d_gate = (_ptr(t) for t in out)
-    ws = None
-    if need[2] or need[3] or (need[4] and a.gate_kind == 1):
-        a.workspace_bytes = lib().dsalt_branch_norm_workspace_size(a.rows, a.d)
-        ws = torch.empty(a.workspace_bytes, device=dev, dtype=torch.uint8)
-        a.workspace = ws.data_ptr()
-    with on_device(dev):
-        _raise(lib().dsalt_branch_norm_bwd(ctypes.byref(a), stream_handle(dev)), "dsalt_branch_norm_bwd")
+    ws = (0, 0)
+    if need[2] or need[3] or (need[4] and gate.dim() == 1):
+        size = lib().dsalt_branch_norm_workspace_size(rows, d)
+        scratch = torch.empty(size, device=dev, dtype=torch.uint8)
+        ws = (scratch.data_ptr(), size)
+    at = stats.data_ptr()
+    _call("dsalt_branch_norm_bwd",
+          _branch_pack(x, h, weight, post_weight, gate, opts, seed, rstd=at, rstd_post=at + 4 * rows, dx_out=_addr(dx_out),
+                       dy=_addr(dy), grads=[_addr(t) for t in out], ws=ws), dev)
     return out

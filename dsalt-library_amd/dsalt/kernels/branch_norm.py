@@ -14,8 +14,10 @@ from .dropout import _Dropout, check_seed
 from .dsalt_triton_attn import _dynamo_opaque
 
 
-def torch_branch_norm(x, h, weight, post_weight, gate, residual_scale, p, seed, offset, eps, post_eps, out_dtype):
+def torch_branch_norm(x, h, weight, post_weight, gate, opts, seed):
     """``branch_norm`` in torch's ops (and the dropout pass), in fp32 or more."""
+    residual_scale, p, offset, eps, post_eps, out_dtype = opts
+
     def wide(t):
         return t.float() if t.dtype in (torch.bfloat16, torch.float16) else t
 
@@ -35,36 +37,41 @@ class _BranchNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h, weight, post_weight, gate, seed, opts):
         ctx.set_materialize_grads(False)
-        residual_scale, p, offset, eps, post_eps, out_dtype = opts
-        ops = [None if t is None else _hip.aligned_rows(t.detach()) for t in (x, h, weight, post_weight, gate)]
-        x_out, y, rstd, rstd_post = _hip.branch_norm(*ops, residual_scale, p, seed, offset, eps, post_eps, out_dtype, True)
+        x_out, y, stats = _hip.branch_norm(*_operands(x, h, weight, post_weight, gate), opts, seed, True)
         is_tensor = isinstance(seed, torch.Tensor)
-        ctx.save_for_backward(x, h, weight, post_weight, gate, rstd, rstd_post, seed if is_tensor else None)
+        ctx.save_for_backward(x, h, weight, post_weight, gate, stats, seed if is_tensor else None)
         ctx.dsalt = opts, None if is_tensor else seed
         return x_out, y
 
     @staticmethod
     @without_autocast
     def backward(ctx, dx_out, dy):
-        *inputs, rstd, rstd_post, seed = ctx.saved_tensors
+        x, h, weight, post_weight, gate, stats, seed = ctx.saved_tensors
         opts, seed_value = ctx.dsalt
         seed = seed_value if seed is None else seed
-        residual_scale, p, offset, eps, post_eps, out_dtype = opts
         need = ctx.needs_input_grad[:5]
         if dx_out is None and dy is None:
             return (None,) * 7
         if torch.is_grad_enabled():  # a graph of the backward is wanted: torch's own ops
-            grads = graph_grads(lambda *t: tuple(o for o in torch_branch_norm(*t, residual_scale, p, seed, offset, eps, post_eps,
-                                                                              out_dtype) if o is not None),
-                                inputs, (dx_out, dy) if inputs[2] is not None else (dx_out,))
+            grads = graph_grads(lambda *t: tuple(o for o in torch_branch_norm(*t, opts, seed) if o is not None),
+                                (x, h, weight, post_weight, gate), (dx_out, dy) if weight is not None else (dx_out,))
             return *grads, None, None
-        ops = [None if t is None else _hip.aligned_rows(t.detach()) for t in inputs]
-        dx_out, dy = (None if t is None else _hip.aligned_rows(t) for t in (dx_out, dy))
-        # without a gradient of y its norm's weight gets zeros
-        w_need = need[2] and dy is not None
-        grads = _hip.branch_norm_bwd(*ops, residual_scale, p, seed, offset, out_dtype, rstd, rstd_post, dx_out, dy,
-                                     (*need[:2], w_need, *need[3:]))
+        if dy is None and need[2]:  # without a gradient of y, none of its norm's weight
+            need = (*need[:2], False, *need[3:])
+        grads = _hip.branch_norm_bwd(*_operands(x, h, weight, post_weight, gate), opts, seed, stats,
+                                     None if dx_out is None else _hip.aligned_rows(dx_out),
+                                     None if dy is None else _hip.aligned_rows(dy), need)
         return *grads, None, None
+
+
+def _operands(x, h, weight, post_weight, gate):
+    rows = _hip.aligned_rows
+    return (rows(x.detach()), rows(h.detach()), None if weight is None else rows(weight.detach()),
+            None if post_weight is None else rows(post_weight.detach()), None if gate is None else rows(gate.detach()))
+
+
+def _weight_ok(w, d: int, dtype: torch.dtype, dev: torch.device) -> bool:
+    return w is None or (w.shape == (d,) and (w.dtype is dtype or w.dtype is torch.float32) and w.device == dev)
 
 
 @_dynamo_opaque
@@ -83,23 +90,25 @@ def branch_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor | None = 
     dtype, or any of the three beside an fp32 x; weights and gate in x's dtype or fp32. x_out has
     x's dtype; y is formed from the sum before that rounding. d a multiple of 8 up to 8192.
     Differentiable in x, h, weight, post_weight and gate. Other operands raise ``DsaltError``."""
-    dev = _hip.require_gpu(x, h, weight, post_weight, gate)
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    post_eps = eps if post_eps is None else post_eps
-    check_seed(p, seed, offset)
-    _hip.seed_fields(0 if seed is None else seed, dev)
+    dev, dtype = x.device, x.dtype
+    out_dtype = dtype if out_dtype is None else out_dtype
+    check_seed(p, seed, offset, dev)
     d = x.shape[-1] if x.dim() else 0
-    ok = (x.dtype in _hip._SCORE_DTYPES and h.shape == x.shape and 8 <= d <= _hip.BRANCH_NORM_MAX_DIM and d % 8 == 0
-          and all(t == x.dtype or (x.dtype == torch.float32 and t in _hip._SCORE_DTYPES) for t in (h.dtype, out_dtype))
-          and all(w is None or (w.shape == (d,) and w.dtype in (x.dtype, torch.float32)) for w in (weight, post_weight))
-          and (gate is None or (gate.shape in ((d,), (*x.shape[:-1], 1)) and gate.dtype in (x.dtype, torch.float32))))
+    wide = dtype is torch.float32
+    ok = (dev.type == "cuda" and h.device == dev and dtype in _hip._SCORE_DTYPES and h.shape == x.shape
+          and 8 <= d <= _hip.BRANCH_NORM_MAX_DIM and d % 8 == 0
+          and (h.dtype is dtype or (wide and h.dtype in _hip._SCORE_DTYPES))
+          and (out_dtype is dtype or (wide and out_dtype in _hip._SCORE_DTYPES))
+          and _weight_ok(weight, d, dtype, dev) and _weight_ok(post_weight, d, dtype, dev)
+          and (gate is None or ((gate.shape == (d,) or gate.shape == (*x.shape[:-1], 1)) and gate.device == dev
+                                and (gate.dtype is dtype or gate.dtype is torch.float32))))
     if not ok:
+        _hip.require_gpu(x, h, weight, post_weight, gate)
         raise _hip.DsaltError(
             f"branch_norm needs x and h [..., d] of one shape, d a multiple of 8 up to {_hip.BRANCH_NORM_MAX_DIM}, h and the "
             f"output in x's dtype or x fp32, weights [d] and a gate [d] or [..., 1] in x's dtype or fp32 (got "
             f"{[None if t is None else (tuple(t.shape), t.dtype) for t in (x, h, weight, post_weight, gate)]}, {out_dtype})")
-    opts = (float(residual_scale), float(p), offset, float(eps), float(post_eps), out_dtype)
+    opts = (float(residual_scale), p, offset, float(eps), float(eps if post_eps is None else post_eps), out_dtype)
     if no_graph(x, h, weight, post_weight, gate):
-        ops = (None if t is None else _hip.aligned_rows(t) for t in (x, h, weight, post_weight, gate))
-        return _hip.branch_norm(*ops, opts[0], opts[1], seed, *opts[2:], False)[:2]
+        return _hip.branch_norm(*_operands(x, h, weight, post_weight, gate), opts, seed, False)[:2]
     return _BranchNorm.apply(x, h, weight, post_weight, gate, seed, opts)

@@ -17,9 +17,13 @@ def draw_seed(device: torch.device) -> torch.Tensor:
     return torch.randint(-2 ** 63, 2 ** 63 - 1, (1,), device=device, dtype=torch.int64)
 
 
-def check_seed(p: float, seed, offset) -> None:
-    if _hip.keep_threshold(p) < 65536 and seed is None:
-        raise ValueError("a dropout probability above 0 needs a seed")
+def check_seed(p: float, seed, offset: int, device: torch.device) -> None:
+    threshold = _hip.keep_threshold(p)
+    if seed is None:
+        if threshold < 65536:
+            raise ValueError("a dropout probability above 0 needs a seed")
+    else:
+        _hip.seed_fields(seed, device)
     if not 0 <= offset < 2 ** 63:
         raise ValueError(f"offset must be in [0, 2^63) (got {offset})")
 
@@ -36,8 +40,11 @@ class _Dropout(torch.autograd.Function):
     def backward(ctx, dy):
         p, seed, offset = ctx.dsalt
         saved, = ctx.saved_tensors
-        # linear: under a graph of the backward its gradient is the same function again
-        return _Dropout.apply(dy, p, seed if saved is None else saved, offset), None, None, None
+        seed = seed if saved is None else saved
+        if not torch.is_grad_enabled():
+            return _hip.dropout(_hip.aligned_rows(dy), p, seed, offset), None, None, None
+        # a graph of the backward is wanted: linear, its gradient is the same function again
+        return _Dropout.apply(dy, p, seed, offset), None, None, None
 
 
 @_dynamo_opaque
@@ -54,10 +61,8 @@ def counter_dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.T
     dev = _hip.require_gpu(x)
     if x.dtype not in _hip._SCORE_DTYPES:
         raise _hip.DsaltError(f"counter_dropout needs a bf16, fp16 or fp32 tensor (got {x.dtype})")
-    check_seed(p, seed, offset)
-    if seed is None:
-        seed = 0
-    _hip.seed_fields(seed, dev)
+    check_seed(p, seed, offset, dev)
+    seed = 0 if seed is None else seed
     if no_graph(x):
         return _hip.dropout(_hip.aligned_rows(x), p, seed, offset)
     return _Dropout.apply(x, p, seed, offset)

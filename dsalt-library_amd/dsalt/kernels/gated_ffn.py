@@ -31,49 +31,58 @@ class _GatedFFN(torch.autograd.Function):
         # the backward is refused where a gradient reads it
         need = ctx.needs_input_grad[:4]
         inner = any(need[:3])
-        y, gate_up, act = _hip.gated_ffn(_hip.row_operand(x.detach().reshape(-1, x.shape[-1])),
-                                         *(_hip.row_operand(w.detach()) for w in (w_gate, w_up, w_down)), activation,
-                                         x.shape[:-1], inner)
+        y, kept = _run(x, w_gate, w_up, w_down, activation, inner)
         ctx.save_for_backward(x if inner else None, *((w_gate, w_up) if need[0] else (None, None)),
-                              w_down if inner else None, gate_up, act)
-        ws = w_gate, w_up, w_down
-        ctx.dsalt = x.shape, ws, tuple(w._version for w in ws), activation
+                              w_down if inner else None, kept)
+        ctx.dsalt = x.shape, (w_gate, w_up, w_down), (w_gate._version, w_up._version, w_down._version), activation
         return y
 
     @staticmethod
     @without_autocast
     def backward(ctx, dy):
-        x, _, _, _, gate_up, act = ctx.saved_tensors
+        x, _, _, _, kept = ctx.saved_tensors
         shape, ws, versions, activation = ctx.dsalt
         need = ctx.needs_input_grad[:4]
         if torch.is_grad_enabled():  # a graph of the backward is wanted: torch's own ops
             if tuple(w._version for w in ws) != versions:
                 raise RuntimeError("a weight of gated_ffn was changed in place before a backward that records a graph")
             if x is None:  # only w_down has a gradient
-                dw, = graph_grads(lambda w: (F.linear(act.view(*shape[:-1], -1), w),), ws[2:], (dy,))
+                dw, = graph_grads(lambda w: (F.linear(kept.view(*shape[:-1], w.shape[1]), w),), ws[2:], (dy,))
                 return None, None, None, dw, None
             return *graph_grads(lambda *t: (torch_gated_ffn(*t, activation),), (x, *ws), (dy,)), None
-        dy = _hip.row_operand(dy.reshape(-1, dy.shape[-1]))
-        xr = None if x is None else _hip.row_operand(x.detach().reshape(-1, shape[-1]))
-        dx, *dw = _hip.gated_ffn_bwd(xr, *(_hip.row_operand(w.detach()) for w in ws), activation, gate_up, act, dy, need)
-        return None if dx is None else dx.view(shape), *dw, None
+        row = _hip.row_operand
+        dy = row(dy.reshape(-1, dy.shape[-1]))
+        dx, dwg, dwu, dwd = _hip.gated_ffn_bwd(None if x is None else row(x.reshape(-1, shape[-1])), row(ws[0]), row(ws[1]),
+                                               row(ws[2]), activation, kept, dy, need)
+        return None if dx is None else dx.view(shape), dwg, dwu, dwd, None
+
+
+def _run(x, w_gate, w_up, w_down, activation, keep):
+    row = _hip.row_operand
+    return _hip.gated_ffn(row(x.detach() if x.dim() == 2 else x.detach().reshape(-1, x.shape[-1])), row(w_gate.detach()),
+                          row(w_up.detach()), row(w_down.detach()), activation, x.shape[:-1], keep)
 
 
 def gated_ffn_supported(x, w_gate, w_up, w_down) -> bool:
     """Whether `gated_ffn` takes these tensors: bf16 or fp16 on one GPU (fp32 ones under a 16-bit
     autocast are cast), x [..., d], w_gate and w_up [f, d], w_down [e, f] with d, e and f
     multiples of 8."""
-    ts = (x, w_gate, w_up, w_down)
-    if any(t.device.type != "cuda" or t.device != x.device for t in ts) or x.dim() < 1 or any(w.dim() != 2 for w in ts[1:]):
+    dev = x.device
+    if dev.type != "cuda" or w_gate.device != dev or w_up.device != dev or w_down.device != dev:
         return False
     dt = autocast_dtype(x)
-    if dt not in (torch.bfloat16, torch.float16):
+    if dt is not torch.bfloat16 and dt is not torch.float16:
         return False
-    if any(t.dtype != dt and not (t.dtype == torch.float32 and torch.is_autocast_enabled("cuda")) for t in ts):
+    if not (x.dtype is w_gate.dtype is w_up.dtype is w_down.dtype is dt):
+        ok = (dt, torch.float32) if torch.is_autocast_enabled("cuda") else (dt,)
+        if x.dtype not in ok or w_gate.dtype not in ok or w_up.dtype not in ok or w_down.dtype not in ok:
+            return False
+    if x.dim() < 1 or w_gate.dim() != 2 or w_down.dim() != 2 or w_up.shape != w_gate.shape:
         return False
     f, d = w_gate.shape
-    return (w_up.shape == (f, d) and w_down.shape[1] == f and x.shape[-1] == d
-            and all(n >= 8 and n % 8 == 0 and n <= 1 << 20 for n in (d, f, w_down.shape[0])))
+    e = w_down.shape[0]
+    return (x.shape[-1] == d and w_down.shape[1] == f and d % 8 == f % 8 == e % 8 == 0 and 8 <= d <= 1 << 20
+            and 8 <= f <= 1 << 20 and 8 <= e <= 1 << 20)
 
 
 @_dynamo_opaque
@@ -87,14 +96,14 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     taken. Differentiable in every tensor. Other operands raise ``DsaltError``."""
     if activation not in _hip.ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(_hip.ACTIVATIONS)}, got {activation!r}")
-    _hip.require_gpu(x, w_gate, w_up, w_down)
     if not gated_ffn_supported(x, w_gate, w_up, w_down):
+        _hip.require_gpu(x, w_gate, w_up, w_down)
         raise _hip.DsaltError(
             f"gated_ffn needs bf16 or fp16 x [..., d], w_gate and w_up [f, d], w_down [e, f] of one dtype with d, e and f "
             f"multiples of 8 (got {[(tuple(t.shape), t.dtype) for t in (x, w_gate, w_up, w_down)]})")
-    dt = autocast_dtype(x)
-    x, w_gate, w_up, w_down = (t if t.dtype == dt else t.to(dt) for t in (x, w_gate, w_up, w_down))
+    if torch.is_autocast_enabled("cuda"):
+        dt = autocast_dtype(x)
+        x, w_gate, w_up, w_down = x.to(dt), w_gate.to(dt), w_up.to(dt), w_down.to(dt)
     if no_graph(x, w_gate, w_up, w_down):
-        return _hip.gated_ffn(_hip.row_operand(x.reshape(-1, x.shape[-1])),
-                              *(_hip.row_operand(w) for w in (w_gate, w_up, w_down)), activation, x.shape[:-1], False)[0]
+        return _run(x, w_gate, w_up, w_down, activation, False)[0]
     return _GatedFFN.apply(x, w_gate, w_up, w_down, activation)

@@ -104,7 +104,7 @@ def test_argument_values():
             hip.keep_threshold(p)
     assert [hip.keep_threshold(p) for p in (0.0, 0.5, 1.0, 0.1)] == [65536, 32768, 0, 58982]
     dev = torch.device("cuda", 0)
-    assert hip.seed_fields(-1, dev) == (-1, None) and hip.seed_fields(2 ** 64 - 1, dev) == (-1, None)
+    assert hip.seed_fields(-1, dev) == (-1, 0) and hip.seed_fields(2 ** 64 - 1, dev) == (-1, 0)
     for bad in (2 ** 64, -2 ** 63 - 1):
         with pytest.raises(ValueError, match="64 bits"):
             hip.seed_fields(bad, dev)
