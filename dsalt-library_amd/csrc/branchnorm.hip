@@ -13,8 +13,12 @@
 // Sums are fp32 in a fixed order: per lane over the rows of a workgroup, over its waves in LDS,
 // then over the workgroups.
 //
-// Bound by HBM bytes: a row stays in the registers of one wave (d <= 1024), four (d <= 4096) or
-// eight, so that every tensor is read and written once.
+// Bound by HBM bytes: a row stays in registers, eight columns a lane, so that every tensor is read
+// and written once. Rows of up to 512 columns take one wave, longer ones 2, 4, 8 or 16 whose
+// sums are joined in LDS. With 16 columns a lane and half the waves the backward's registers
+// leave two waves on a SIMD instead of four, and too few loads in flight: 16384 x 4096 bf16
+// backward 178 us (805 MB, 4.5 TB/s) against 212, 6473 x 1024 with an fp32 stream 23.8 us (119 MB,
+// 5.0 TB/s) against 29.6. Forward 102 us (537 MB, 5.3 TB/s) and 16.3 us (80 MB, 4.9 TB/s).
 #include "launch.h"
 #include "lanes.h"
 #include "philox.h"
@@ -83,260 +87,185 @@ struct RowSums {
         if constexpr (WPR > 1) {
             float *s = lds + phase * WPR * N;
             phase ^= 1;
-            const int wave = threadIdx.x >> 6;
+            const int wave = (threadIdx.x >> 6) % WPR;
             if ((threadIdx.x & 63) == 0)
 #pragma unroll
                 for (int i = 0; i < N; ++i) s[wave * N + i] = v[i];
             __syncthreads();
+            const int lane = threadIdx.x & (WPR - 1);  // each lane takes one wave's sum, in every group of WPR lanes
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                float t = 0.f;
-#pragma unroll
-                for (int w = 0; w < WPR; ++w) t += s[w * N + i];
-                v[i] = t;
-            }
+            for (int i = 0; i < N; ++i) v[i] = group_sum_lanes(s[lane * N + i], WPR);
         }
     }
 };
 
-constexpr int branch_waves(int wpr) { return wpr > 4 ? wpr : 4; }
+// WPR waves a row, ROWS rows a workgroup at a time: every wave keeps the barriers of the row
+// sums, also where its row is past the last.
+template <int WPR>
+struct RowShape {
+    static constexpr int WAVES = WPR > 8 ? WPR : 8, ROWS = WAVES / WPR, THREADS = 64 * WAVES;
+};
 
-// A wave's share of its rows: chunk c of lane l is chunk c * 64 WPR + l of the row. All rows of a
-// workgroup with WPR > 1 are the same row, so its barriers are met by every wave.
-template <typename DX, typename DH, int NCH, int WPR>
-__global__ void __launch_bounds__(64 * branch_waves(WPR)) branch_fwd_kernel(const BranchParams p) {
-    constexpr int NW = branch_waves(WPR), ROWS = NW / WPR;
-    __shared__ float lds[2 * WPR];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l = (wave % WPR) * 64 + (threadIdx.x & 63);
-    RowSums<WPR, 1> row_sum{lds};
+template <typename DX, typename DH, int WPR>
+__global__ void __launch_bounds__(RowShape<WPR>::THREADS) branch_fwd_kernel(const BranchParams p) {
+    constexpr int ROWS = RowShape<WPR>::ROWS;
+    __shared__ float lds[ROWS][2 * WPR];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slot = wave / WPR;
+    const int ch = (wave % WPR) * 64 + (threadIdx.x & 63);  // the lane's chunk of a row
+    const bool in = ch < p.nch;
+    RowSums<WPR, 1> row_sum{lds[slot]};
     const uint64_t seed = p.dropout ? dropout_seed(p.drop) : 0;
-    float wp[NCH][8], wf[NCH][8], gc[NCH][8];
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const int ch = c * 64 * WPR + l;
-        if (ch < p.nch) {
-            if (p.w_post) load8_dt(p.w_post, ch, p.post_dtype, wp[c]);
-            if (p.w) load8_dt(p.w, ch, p.w_dtype, wf[c]);
-            if (p.gate_kind == kGateChannel) load8_dt(p.gate, ch, p.gate_dtype, gc[c]);
-        }
+    float wp[8] = {}, wf[8] = {}, gc[8] = {};
+    if (in) {
+        if (p.w_post) load8_dt(p.w_post, ch, p.post_dtype, wp);
+        if (p.w) load8_dt(p.w, ch, p.w_dtype, wf);
+        if (p.gate_kind == kGateChannel) load8_dt(p.gate, ch, p.gate_dtype, gc);
     }
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + wave / WPR; row < p.rows; row += (int64_t)gridDim.x * ROWS) {
-        const int64_t base = row * p.nch;
-        Raw8<DX> xv[NCH];
-        Raw8<DH> hv[NCH];
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = c * 64 * WPR + l;
-            if (ch < p.nch) {
-                xv[c].load(p.x, base + ch);
-                hv[c].load(p.h, base + ch);
-            }
-        }
-        float n[NCH][8], g = 1.f, ss[1] = {0.f};
-        if (p.gate_kind == kGateRow) g = load1_dt(p.gate, row, p.gate_dtype);
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = c * 64 * WPR + l;
-            if (ch < p.nch) {
-                hv[c].get(n[c]);
-                if (p.dropout) apply_keep(keep8<true>((uint64_t)(base + ch), p.drop, seed), p.drop.scale, n[c]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ss[0] = fmaf(n[c][e], n[c][e], ss[0]);
-            }
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < p.rows; r0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = r0 + slot, at = row * p.nch + ch;
+        const bool live = in && row < p.rows;
+        float n[8] = {}, z[8] = {}, g = 1.f, ss[1] = {0.f};
+        if (live) {
+            Raw8<DX> xv;
+            Raw8<DH> hv;
+            xv.load(p.x, at);
+            hv.load(p.h, at);
+            if (p.gate_kind == kGateRow) g = load1_dt(p.gate, row, p.gate_dtype);
+            hv.get(n);
+            if (p.dropout) apply_keep(keep8<true>((uint64_t)at, p.drop, seed), p.drop.scale, n);
+            xv.get(z);
         }
         if (p.w_post) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss[0] = fmaf(n[e], n[e], ss[0]);
             row_sum(ss, 1);
             const float rh = rsqrtf(ss[0] * p.inv_d + p.post_eps);
-            if (l == 0 && p.rstd_post) p.rstd_post[row] = rh;
+            if (live && ch == 0 && p.rstd_post) p.rstd_post[row] = rh;
 #pragma unroll
-            for (int c = 0; c < NCH; ++c)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) n[c][e] = n[c][e] * rh * wp[c][e];
+            for (int e = 0; e < 8; ++e) n[e] = n[e] * rh * wp[e];
         }
         ss[0] = 0.f;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = c * 64 * WPR + l;
-            if (ch < p.nch) {
-                float z[8];
-                xv[c].get(z);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float gn = p.gate_kind == kGateChannel ? gc[c][e] * n[c][e] : g * n[c][e];
-                    z[e] = fmaf(p.rs, z[e], gn);
-                    n[c][e] = z[e];
-                    ss[0] = fmaf(z[e], z[e], ss[0]);
-                }
-                store8<DX>(p.x_out, base + ch, z);
-            }
+        for (int e = 0; e < 8; ++e) {
+            z[e] = fmaf(p.rs, z[e], p.gate_kind == kGateChannel ? gc[e] * n[e] : g * n[e]);
+            ss[0] = fmaf(z[e], z[e], ss[0]);
         }
+        if (live) store8<DX>(p.x_out, at, z);
         if (!p.w) continue;
         row_sum(ss, 1);
         const float r = rsqrtf(ss[0] * p.inv_d + p.eps);
-        if (l == 0 && p.rstd) p.rstd[row] = r;
+        if (live) {
+            if (ch == 0 && p.rstd) p.rstd[row] = r;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = c * 64 * WPR + l;
-            if (ch < p.nch) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) n[c][e] = n[c][e] * r * wf[c][e];
-                store8_dt(p.y, base + ch, n[c], p.y_dtype);
-            }
+            for (int e = 0; e < 8; ++e) z[e] = z[e] * r * wf[e];
+            store8_dt(p.y, at, z, p.y_dtype);
         }
     }
 }
 
-template <typename DX, typename DH, int NCH, int WPR>
-__global__ void __launch_bounds__(64 * branch_waves(WPR)) branch_bwd_kernel(const BranchParams p) {
-    constexpr int NW = branch_waves(WPR), ROWS = NW / WPR;
-    __shared__ float lds[2 * 2 * WPR];
-    __shared__ float4 acc[WPR == 1 ? NW : 1][NCH * 2][64];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int l = (wave % WPR) * 64 + lane;
-    RowSums<WPR, 2> row_sum{lds};
+template <typename DX, typename DH, int WPR>
+__global__ void __launch_bounds__(RowShape<WPR>::THREADS) branch_bwd_kernel(const BranchParams p) {
+    constexpr int ROWS = RowShape<WPR>::ROWS;
+    __shared__ float lds[ROWS][2 * 2 * WPR];
+    __shared__ float4 acc[ROWS > 1 ? ROWS : 1][2][ROWS > 1 ? 64 * WPR : 1];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slot = wave / WPR;
+    const int ch = (wave % WPR) * 64 + (threadIdx.x & 63);
+    const bool in = ch < p.nch;
+    RowSums<WPR, 2> row_sum{lds[slot]};
     const uint64_t seed = p.dropout ? dropout_seed(p.drop) : 0;
-    float wp[NCH][8], wf[NCH][8], gc[NCH][8], sum[3][NCH][8];
+    float wp[8], wf[8], gc[8], sum[3][8];
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const int ch = c * 64 * WPR + l;
+    for (int e = 0; e < 8; ++e) {
+        wp[e] = gc[e] = 1.f;
+        wf[e] = sum[0][e] = sum[1][e] = sum[2][e] = 0.f;
+    }
+    if (in) {
+        if (p.w_post) load8_dt(p.w_post, ch, p.post_dtype, wp);
+        if (p.w) load8_dt(p.w, ch, p.w_dtype, wf);
+        if (p.gate_kind == kGateChannel) load8_dt(p.gate, ch, p.gate_dtype, gc);
+    }
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < p.rows; r0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = r0 + slot, at = row * p.nch + ch;
+        const bool live = in && row < p.rows;
+        float a[8] = {}, hh[8] = {}, t[8] = {}, dz[8] = {}, r = 0.f, rh = 1.f, g = 1.f;
+        uint32_t keep = 0xffu;
+        if (live) {
+            Raw8<DX> xv, zv = {};
+            Raw8<DH> hv;
+            xv.load(p.x, at);
+            hv.load(p.h, at);
+            if (p.dx_out) zv.load(p.dx_out, at);
+            if (p.dy) {
+                load8_dt(p.dy, at, p.y_dtype, a);
+                r = p.rstd[row];
+            }
+            if (p.w_post) rh = p.rstd_post[row];
+            if (p.gate_kind == kGateRow) g = load1_dt(p.gate, row, p.gate_dtype);
+            hv.get(hh);
+            if (p.dropout) {
+                keep = keep8<true>((uint64_t)at, p.drop, seed);
+                apply_keep(keep, p.drop.scale, hh);
+            }
+            xv.get(t);
+            zv.get(dz);
+        }
+        float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            wp[c][e] = gc[c][e] = 1.f;
-            wf[c][e] = 0.f;
-            sum[0][c][e] = sum[1][c][e] = sum[2][c][e] = 0.f;
+            hh[e] *= rh;
+            t[e] = fmaf(p.rs, t[e], g * gc[e] * (hh[e] * wp[e])) * r;  // xh
+            sum[kSumW][e] = fmaf(a[e], t[e], sum[kSumW][e]);
+            a[e] *= wf[e];
+            s[0] = fmaf(a[e], t[e], s[0]);
         }
-        if (ch < p.nch) {
-            if (p.w_post) load8_dt(p.w_post, ch, p.post_dtype, wp[c]);
-            if (p.w) load8_dt(p.w, ch, p.w_dtype, wf[c]);
-            if (p.gate_kind == kGateChannel) load8_dt(p.gate, ch, p.gate_dtype, gc[c]);
-        }
-    }
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + wave / WPR; row < p.rows; row += (int64_t)gridDim.x * ROWS) {
-        const int64_t base = row * p.nch;
-        Raw8<DX> xv[NCH], zv[NCH];
-        Raw8<DH> hv[NCH];
-        float a[NCH][8];
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = c * 64 * WPR + l;
-            if (ch < p.nch) {
-                xv[c].load(p.x, base + ch);
-                hv[c].load(p.h, base + ch);
-                if (p.dx_out) zv[c].load(p.dx_out, base + ch);
-                if (p.dy) load8_dt(p.dy, base + ch, p.y_dtype, a[c]);
-            }
-        }
-        const float r = p.dy ? p.rstd[row] : 0.f, rh = p.w_post ? p.rstd_post[row] : 1.f;
-        const float g = p.gate_kind == kGateRow ? load1_dt(p.gate, row, p.gate_dtype) : 1.f;
-        uint32_t keep[NCH];
-        float hh[NCH][8], t[NCH][8], s[2] = {0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = c * 64 * WPR + l;
-            keep[c] = 0xffu;
-            if (ch < p.nch) {
-                hv[c].get(hh[c]);
-                if (p.dropout) {
-                    keep[c] = keep8<true>((uint64_t)(base + ch), p.drop, seed);
-                    apply_keep(keep[c], p.drop.scale, hh[c]);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) hh[c][e] *= rh;
-                if (p.dy) {
-                    xv[c].get(t[c]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float xh = fmaf(p.rs, t[c][e], g * gc[c][e] * (hh[c][e] * wp[c][e])) * r;
-                        sum[kSumW][c][e] = fmaf(a[c][e], xh, sum[kSumW][c][e]);
-                        a[c][e] *= wf[c][e];
-                        t[c][e] = xh;
-                        s[0] = fmaf(a[c][e], xh, s[0]);
-                    }
-                }
-            }
-        }
-        float c1 = 0.f;
-        if (p.dy) {
-            row_sum(s, 1);
-            c1 = s[0] * p.inv_d;
-        }
+        if (p.dy) row_sum(s, 1);
+        const float c1 = s[0] * p.inv_d;
         s[0] = s[1] = 0.f;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = c * 64 * WPR + l;
-            if (ch < p.nch) {
-                float o[8];
-                if (p.dx_out) zv[c].get(o);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float dn = p.dy ? r * fmaf(-t[c][e], c1, a[c][e]) : 0.f;
-                    t[c][e] = p.dx_out ? o[e] + dn : dn;
-                    o[e] = p.rs * t[c][e];
-                }
-                if (p.dx) store8<DX>(p.dx, base + ch, o);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float tn = t[c][e] * hh[c][e];
-                    sum[kSumGate][c][e] = fmaf(tn, wp[c][e], sum[kSumGate][c][e]);
-                    sum[kSumPost][c][e] = fmaf(tn, g * gc[c][e], sum[kSumPost][c][e]);
-                    s[1] = fmaf(tn, wp[c][e], s[1]);
-                    t[c][e] *= g * gc[c][e] * wp[c][e];
-                    s[0] = fmaf(t[c][e], hh[c][e], s[0]);
-                }
-            }
+        for (int e = 0; e < 8; ++e) {
+            t[e] = p.dy ? fmaf(r, fmaf(-t[e], c1, a[e]), dz[e]) : dz[e];
+            dz[e] = p.rs * t[e];
+            const float tn = t[e] * hh[e];
+            sum[kSumGate][e] = fmaf(tn, wp[e], sum[kSumGate][e]);
+            sum[kSumPost][e] = fmaf(tn, g * gc[e], sum[kSumPost][e]);
+            s[1] = fmaf(tn, wp[e], s[1]);
+            t[e] *= g * gc[e] * wp[e];
+            s[0] = fmaf(t[e], hh[e], s[0]);
         }
+        if (live && p.dx) store8<DX>(p.dx, at, dz);
         if (p.w_post || p.d_gate_row) row_sum(s, 2);
-        if (p.d_gate_row && l == 0) store1_dt(p.d_gate_row, row, p.gate_dtype, s[1]);
+        if (!live) continue;
+        if (p.d_gate_row && ch == 0) store1_dt(p.d_gate_row, row, p.gate_dtype, s[1]);
         if (p.dh) {
             const float c2 = p.w_post ? s[0] * p.inv_d : 0.f;
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                const int ch = c * 64 * WPR + l;
-                if (ch < p.nch) {
-                    float o[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] = rh * fmaf(-hh[c][e], c2, t[c][e]);
-                    if (p.dropout) apply_keep(keep[c], p.drop.scale, o);
-                    store8<DH>(p.dh, base + ch, o);
-                }
-            }
+            for (int e = 0; e < 8; ++e) t[e] = rh * fmaf(-hh[e], c2, t[e]);
+            if (p.dropout) apply_keep(keep, p.drop.scale, t);
+            store8<DH>(p.dh, at, t);
         }
     }
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
         if (!((p.sums >> q) & 1)) continue;
-        float4 *out = reinterpret_cast<float4 *>(p.part) + ((int64_t)blockIdx.x * 3 + q) * p.nch * 2;
-        if constexpr (WPR > 1) {
-#pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                const int ch = c * 64 * WPR + l;
-                if (ch < p.nch) {
-                    const float *v = sum[q][c];
-                    out[2 * ch] = make_float4(v[0], v[1], v[2], v[3]);
-                    out[2 * ch + 1] = make_float4(v[4], v[5], v[6], v[7]);
-                }
-            }
-        } else {
+        float4 lo = make_float4(sum[q][0], sum[q][1], sum[q][2], sum[q][3]);
+        float4 hi = make_float4(sum[q][4], sum[q][5], sum[q][6], sum[q][7]);
+        if constexpr (ROWS > 1) {
             __syncthreads();  // the previous sums have been read
-#pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                const float *v = sum[q][c];
-                acc[wave][2 * c][lane] = make_float4(v[0], v[1], v[2], v[3]);
-                acc[wave][2 * c + 1][lane] = make_float4(v[4], v[5], v[6], v[7]);
-            }
+            acc[slot][0][ch] = lo;
+            acc[slot][1][ch] = hi;
             __syncthreads();
-            for (int i = threadIdx.x; i < NCH * 2 * 64; i += 64 * NW) {
-                const int ln = i & 63, hc = i >> 6;
-                float4 s = acc[0][hc][ln];
+            if (slot) continue;
 #pragma unroll
-                for (int w = 1; w < NW; ++w) {
-                    const float4 b = acc[w][hc][ln];
-                    s.x += b.x; s.y += b.y; s.z += b.z; s.w += b.w;
-                }
-                const int ch = (hc >> 1) * 64 + ln;
-                if (ch < p.nch) out[2 * ch + (hc & 1)] = s;
+            for (int w = 1; w < ROWS; ++w) {
+                const float4 b = acc[w][0][ch], c = acc[w][1][ch];
+                lo.x += b.x; lo.y += b.y; lo.z += b.z; lo.w += b.w;
+                hi.x += c.x; hi.y += c.y; hi.z += c.z; hi.w += c.w;
             }
+        }
+        if (in) {
+            float4 *out = reinterpret_cast<float4 *>(p.part) + (((int64_t)blockIdx.x * 3 + q) * p.nch + ch) * 2;
+            out[0] = lo;
+            out[1] = hi;
         }
     }
 }
@@ -371,32 +300,35 @@ __global__ void __launch_bounds__(1024) branch_sums_kernel(const float *__restri
     }
 }
 
-constexpr int kBranchMaxGroups = 512;
+constexpr int kBranchMaxGroups = 512;  // workgroups of the backward: what its registers allow, two per CU
 
+int row_waves(int d) { return d <= 512 ? 1 : d <= 1024 ? 2 : d <= 2048 ? 4 : d <= 4096 ? 8 : 16; }
 int64_t row_groups(int64_t rows, int d) {
-    const int per = d <= 1024 ? 4 : 1;
+    const int per = std::max(8 / row_waves(d), 1);
     return (rows + per - 1) / per;
 }
 int branch_bwd_groups(int64_t rows, int d) { return (int)std::min<int64_t>(row_groups(rows, d), kBranchMaxGroups); }
 
-template <typename DX, typename DH, int NCH, int WPR>
+template <typename DX, typename DH, int WPR>
 void launch_shape(const BranchParams &p, bool bwd, hipStream_t stream) {
-    const dim3 block(64 * branch_waves(WPR));
+    const dim3 block(RowShape<WPR>::THREADS);
+    const int64_t groups = row_groups(p.rows, p.nch * 8);
     if (bwd)
-        hipLaunchKernelGGL((branch_bwd_kernel<DX, DH, NCH, WPR>), dim3(branch_bwd_groups(p.rows, p.nch * 8)), block, 0,
-                           stream, p);
+        hipLaunchKernelGGL((branch_bwd_kernel<DX, DH, WPR>), dim3(branch_bwd_groups(p.rows, p.nch * 8)), block, 0, stream, p);
     else
-        hipLaunchKernelGGL((branch_fwd_kernel<DX, DH, NCH, WPR>),
-                           dim3((unsigned)std::min<int64_t>(row_groups(p.rows, p.nch * 8), 2048)), block, 0, stream, p);
+        hipLaunchKernelGGL((branch_fwd_kernel<DX, DH, WPR>), dim3((unsigned)std::min<int64_t>(groups, 2048)), block, 0,
+                           stream, p);
 }
 
 template <typename DX, typename DH>
 void launch_types(const BranchParams &p, bool bwd, hipStream_t stream) {
-    if (p.nch <= 64) launch_shape<DX, DH, 1, 1>(p, bwd, stream);
-    else if (p.nch <= 128) launch_shape<DX, DH, 2, 1>(p, bwd, stream);
-    else if (p.nch <= 256) launch_shape<DX, DH, 1, 4>(p, bwd, stream);
-    else if (p.nch <= 512) launch_shape<DX, DH, 2, 4>(p, bwd, stream);
-    else launch_shape<DX, DH, 2, 8>(p, bwd, stream);
+    switch (row_waves(p.nch * 8)) {
+        case 1: return launch_shape<DX, DH, 1>(p, bwd, stream);
+        case 2: return launch_shape<DX, DH, 2>(p, bwd, stream);
+        case 4: return launch_shape<DX, DH, 4>(p, bwd, stream);
+        case 8: return launch_shape<DX, DH, 8>(p, bwd, stream);
+        default: return launch_shape<DX, DH, 16>(p, bwd, stream);
+    }
 }
 
 hipError_t launch_branch(const dsalt_branch_norm_args &a, bool bwd, hipStream_t stream) {

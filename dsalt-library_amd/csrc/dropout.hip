@@ -1,7 +1,8 @@
 // Dropout whose mask is a function of (seed, offset, element index): see philox.h. Nothing but
 // x is read and nothing but out written, so the backward is the same pass over the gradient.
 //
-// Bound by memory: a read and a write per element against 14 multiplies per eight.
+// Bound by memory: a read and a write per element against 14 multiplies per eight. 33.6 M bf16
+// elements 20.9 us (134 MB, 6.4 TB/s; a copy of as much takes 18.6 us).
 #include "launch.h"
 #include "philox.h"
 #include "rows.h"

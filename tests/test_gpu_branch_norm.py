@@ -153,6 +153,15 @@ def test_nan_stays_in_its_row():
         assert torch.equal(a[keep], b[keep]) and bool(a[3].isnan().any())
 
 
+def test_nan_without_a_norm_gradient():
+    """Only x_out's gradient: it passes whatever the stream holds."""
+    t, dz, dy = inputs((5,), 200, FP, FP, FP, post=False, gate="none")
+    t["x"][1] = float("nan")
+    t["x"][2, 3] = float("inf")
+    _, grads = run(t, dz, None, residual_scale=0.5)
+    assert torch.equal(grads["x"], 0.5 * dz) and torch.equal(grads["h"], dz)
+
+
 def test_equals_the_parts():
     """Dropout alone in the branch, no gate and scale 1: x_out has the bits of counter_dropout and
     the add; without dropout either, those of the block's add + norm pass."""
