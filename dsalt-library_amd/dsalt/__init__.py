@@ -30,12 +30,13 @@ from .kernels import (
 )
 from .kernels.dsalt_triton_train import dsalt_triton_train_attention
 from .model import DSALTLMHeadModel
-from .modules import DSALTAttention, DSALTTransformerBlock, SwiGLUFFN
+from .modules import CounterDropout, DSALTAttention, DSALTTransformerBlock, SwiGLUFFN
 
 __all__ = [
     "DSALTAttention",
     "DSALTTransformerBlock",
     "SwiGLUFFN",
+    "CounterDropout",
     "DSALTLMHeadModel",
     "DsaltError",
     "dsalt_triton_attention",

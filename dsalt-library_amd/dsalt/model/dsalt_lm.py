@@ -20,6 +20,11 @@ Inference without autograd in bf16/fp16 runs every residual add in the pass of t
 RMSNorm after it (dsalt_add_rms_norm: each block hands its FFN output to the next
 block's norm, the last one to the final norm); the FFN's gated product and the window
 gate run as HIP passes too (SwiGLUFFN, DSALTAttention).
+
+The options of DSALTTransformerBlock beyond the reference (post_norm, layer_scale,
+residual_scale, fused_ffn, activation, counter_dropout) apply to every layer; with
+counter_dropout the embedding's dropout is a CounterDropout too, and one seed drawn a forward
+serves all places, told apart by their offsets.
 """
 from __future__ import annotations
 
@@ -30,8 +35,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import _hip
+from ..kernels import _block_train
 from ..kernels.RMSENorm import RMSENorm
-from ..modules.dsalt_transformer import DSALTTransformerBlock
+from ..kernels.dropout import draw_seed
+from ..modules.dsalt_transformer import CounterDropout, DSALTTransformerBlock
 
 _LOSS_FNS = ("auto", "liger", "chunked")
 
@@ -53,7 +60,9 @@ class DSALTLMHeadModel(nn.Module):
                  k_lmk: int, max_seq_len: int, d_ff: int | None = None, dropout: float = 0.0,
                  yarn_scale: float = 1.0, tie_weights: bool = True, padding_idx: int | None = None,
                  lm_head_chunk_size: int = 2048, loss_fn: str = "chunked", aux_loss_weight: float = 0.0,
-                 n_kv_heads: int | None = None, qkv_bias: bool = False, rope_base: float = 10000.0):
+                 n_kv_heads: int | None = None, qkv_bias: bool = False, rope_base: float = 10000.0,
+                 post_norm: bool = False, layer_scale: float | None = None, residual_scale: float = 1.0,
+                 fused_ffn: bool = False, activation: str = "silu", counter_dropout: bool = False):
         super().__init__()
         if loss_fn not in _LOSS_FNS:
             raise ValueError(f"loss_fn must be one of {list(_LOSS_FNS)}, got {loss_fn!r}")
@@ -70,11 +79,13 @@ class DSALTLMHeadModel(nn.Module):
             d_ff = -(-int(8 / 3 * d_model) // 128) * 128
 
         self.embed_tokens = nn.Embedding(vocab_size, d_model, padding_idx=padding_idx)
-        self.embed_dropout = nn.Dropout(dropout)
+        self.embed_dropout = CounterDropout(dropout) if counter_dropout else nn.Dropout(dropout)
         self.layers = nn.ModuleList(
             DSALTTransformerBlock(d_model=d_model, n_heads=n_heads, n_min=n_min, n_max=n_max, k_lmk=k_lmk,
                                   max_seq_len=max_seq_len, d_ff=d_ff, dropout=dropout, yarn_scale=yarn_scale,
-                                  layer_idx=i, n_kv_heads=n_kv_heads, qkv_bias=qkv_bias, rope_base=rope_base)
+                                  layer_idx=i, n_kv_heads=n_kv_heads, qkv_bias=qkv_bias, rope_base=rope_base,
+                                  post_norm=post_norm, layer_scale=layer_scale, residual_scale=residual_scale,
+                                  fused_ffn=fused_ffn, activation=activation, counter_dropout=counter_dropout)
             for i in range(n_layers))
         self.final_norm = RMSENorm(d_model)
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)
@@ -116,7 +127,12 @@ class DSALTLMHeadModel(nn.Module):
                 gradient_checkpointing: bool = False, padding_mask: torch.Tensor | None = None) -> dict:
         if max_seqlen is None:
             max_seqlen = input_ids.shape[-1]
-        x = self._to_autocast_dtype(self.embed_dropout(self.embed_tokens(input_ids)))
+        seed = None
+        if type(self.embed_dropout) is CounterDropout and self.training and self.embed_dropout.p > 0:
+            seed = draw_seed(input_ids.device)
+            x = self._to_autocast_dtype(self.embed_dropout(self.embed_tokens(input_ids), seed))
+        else:
+            x = self._to_autocast_dtype(self.embed_dropout(self.embed_tokens(input_ids)))
         cu_list = None
         if cu_seqlens is not None and not self._device_packing(cu_seqlens, x):
             cu_list = cu_seqlens.detach().cpu().tolist()
@@ -129,12 +145,20 @@ class DSALTLMHeadModel(nn.Module):
             _, x = _hip.add_rms_norm(x, delta, self.final_norm.weight, self.final_norm.eps)
             return {"loss": None, "logits": self.lm_head(x), "aux_loss": None}
         aux = torch.zeros((), device=input_ids.device, dtype=x.dtype)
-        for layer in self.layers:
-            x, a = layer(x, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
-                         gradient_checkpointing=gradient_checkpointing, cu_list=cu_list)
+        joins = bool(self.layers) and all(type(layer) is DSALTTransformerBlock and layer.joins_branches
+                                          and _block_train.plain(layer) for layer in self.layers)
+        h = self.layers[0].attn_norm(x) if joins else None
+        for i, layer in enumerate(self.layers):
+            if joins:  # each block's last pass also forms the norm that the next block reads
+                after = self.layers[i + 1].attn_norm if i + 1 < len(self.layers) else self.final_norm
+                x, h, a = layer.join_branches(x, h, after, seed, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
+                                              gradient_checkpointing=gradient_checkpointing, cu_list=cu_list)
+            else:
+                x, a = layer(x, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
+                             gradient_checkpointing=gradient_checkpointing, cu_list=cu_list)
             if labels is not None:  # the layers' auxiliary losses are only returned with a loss
                 aux = aux + a
-        x = self.final_norm(x)
+        x = h if joins else self.final_norm(x)
         if labels is None:
             return {"loss": None, "logits": self.lm_head(x), "aux_loss": None}
         loss = _chunked_cross_entropy(x.reshape(-1, self.d_model), self.lm_head.weight,
@@ -152,6 +176,8 @@ class DSALTLMHeadModel(nn.Module):
         """Whether every residual add and norm of the forward can run as dsalt_add_rms_norm
         passes (inference without autograd, 16-bit rows, norm weights of x's dtype)."""
         if not self.layers or not _hip.add_rms_norm_supported(x, self.final_norm.weight):
+            return False
+        if any(getattr(layer, "joins_branches", False) for layer in self.layers):
             return False
         return all(layer._norms_fusable(x, None, layer.attn_norm) and layer._norms_fusable(x, None, layer.ffn_norm)
                    for layer in self.layers)

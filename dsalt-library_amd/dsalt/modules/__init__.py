@@ -1,4 +1,4 @@
 from .dsalt_attention import DSALTAttention
-from .dsalt_transformer import DSALTTransformerBlock, SwiGLUFFN
+from .dsalt_transformer import CounterDropout, DSALTTransformerBlock, SwiGLUFFN
 
-__all__ = ["DSALTAttention", "DSALTTransformerBlock", "SwiGLUFFN"]
+__all__ = ["CounterDropout", "DSALTAttention", "DSALTTransformerBlock", "SwiGLUFFN"]

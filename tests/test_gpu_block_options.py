@@ -1,0 +1,204 @@
+"""The transformer block's and the LM's options (fused feed-forward, counter-based dropout, post
+norms, layer scale, residual scale): all of them in one run, against the same modules composed
+from torch's ops, and what they leave as it was."""
+import copy
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from dsalt import _hip
+from dsalt.kernels import counter_dropout
+from dsalt.kernels.gated_ffn import torch_gated_ffn
+from dsalt.model import DSALTLMHeadModel
+from dsalt.modules import CounterDropout, DSALTTransformerBlock, SwiGLUFFN
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+OPTIONS = dict(post_norm=True, layer_scale=0.2, residual_scale=0.9, fused_ffn=True, counter_dropout=True)
+LENS = [200, 57, 131]
+CU = [0, 200, 257, 388]
+
+
+def block(dtype=FP, dropout=0.1, **kw):
+    torch.manual_seed(5)
+    b = DSALTTransformerBlock(128, 2, 4, 40, 4, 256, 264, dropout=dropout, layer_idx=2, **{**OPTIONS, **kw}).to(DEV, dtype).train()
+    with torch.no_grad():
+        for n, p in b.named_parameters():
+            if "norm" in n or n.endswith("gate"):
+                p.add_(0.2 * torch.randn(p.shape, device=DEV).to(dtype))
+    return b
+
+
+def composed(b, x, cu, seed, autocast=None):
+    """The block's formulas in torch's ops, around the same attention module."""
+    def rms(t, norm):
+        return F.rms_norm(t.float(), (t.shape[-1],), norm.weight.float(), norm.eps)
+
+    def join(x, o, post, gate):
+        n = rms(o, post) if post is not None else o.float()
+        n = n if gate is None else gate.float() * n
+        return (b.residual_scale * x.float() + n).to(x.dtype)
+
+    o, aux = b.attn(rms(x, b.attn_norm).to(x.dtype), cu_seqlens=cu, max_seqlen=256)
+    x = join(x, o, b.attn_post_norm, b.attn_gate)
+    h = rms(x, b.ffn_norm).to(x.dtype)
+    f = torch_gated_ffn(h, b.ffn.gate_proj.weight, b.ffn.up_proj.weight, b.ffn.down_proj.weight, b.ffn.activation)
+    if b.training and b.ffn.drop.p > 0:
+        f = counter_dropout(f, b.ffn.drop.p, seed, b.layer_idx + 1)
+    return join(x, f, b.ffn_post_norm, b.ffn_gate), aux
+
+
+@pytest.mark.parametrize("dtype,autocast", [(FP, None), (BF, None), (HF, None), (FP, BF)])
+@pytest.mark.parametrize("activation,extra", [("silu", {}), ("gelu_tanh", {}), ("relu", {"post_norm": False}),
+                                              ("gelu", {"layer_scale": None, "residual_scale": 1.0})])
+def test_block(dtype, autocast, activation, extra):
+    print(f"block options {dtype} autocast={autocast} {activation} {extra}", flush=True)
+    b = block(dtype, activation=activation, **extra)
+    cu = torch.tensor(CU, dtype=torch.int32, device=DEV)
+    x = torch.randn(CU[-1], 128, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(dtype)
+    dy = torch.randn(CU[-1], 128, device=DEV, generator=torch.Generator(DEV).manual_seed(2)).to(dtype)
+    seed = torch.tensor([9], device=DEV)
+    got, want = [], []
+    for out in (got, want):
+        xi = x.clone().requires_grad_()
+        b.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", dtype=autocast or BF, enabled=autocast is not None):
+            if out is got:
+                y, _, _ = b.join_branches(xi, b.attn_norm(xi), None, seed, cu_seqlens=cu, max_seqlen=256)
+            else:
+                y, _ = composed(b, xi, cu, seed)
+        y.backward(dy)
+        out += [("y", y.detach()), ("x", xi.grad)] + [(n, p.grad) for n, p in b.named_parameters() if p.grad is not None]
+    assert [n for n, _ in got] == [n for n, _ in want]
+    # both sides round at every op's output in the compute dtype: some ten roundings in a chain
+    # of up to half a step each, which add up like a random walk; windows and landmarks are
+    # whole-number decisions on roundings that the two sides' norms may take differently, in
+    # a few rows
+    u = torch.finfo(autocast or dtype).eps / 2 if (autocast or dtype) != FP else 2.0 ** -11  # fp32 attention computes in fp16
+    # relu's slope jumps: the two sides' h differ by a rounding, g = h Wg^T then by about u of its
+    # scale s, and of gates with density 1 / (s sqrt(2 pi)) at 0 a share of 2 u / sqrt(2 pi) < u lies
+    # within u s of it. Where the slopes differ the whole gradient of that gate does, in u of all
+    # gates against the half that pass: sqrt(2 u) of its norm
+    tol = 24 * u + ((2 * u) ** 0.5 if activation == "relu" else 0.0)
+    for (n, a), (_, c) in zip(got, want):
+        assert a.dtype == c.dtype and a.shape == c.shape, n
+        err, size = float((a.float() - c.float()).norm()), float(c.float().norm())
+        assert err <= tol * size + 1e-6, (n, err / max(size, 1e-12), u)
+
+
+def test_ffn_fused_against_separate():
+    for dtype in (BF, HF):
+        torch.manual_seed(1)
+        ffn = SwiGLUFFN(128, 264, fused=True, activation="gelu").to(DEV, dtype)
+        x = torch.randn(3, 41, 128, device=DEV).to(dtype).requires_grad_()
+        y = ffn(x)
+        want = torch_gated_ffn(x.double(), *(m.weight.double() for m in (ffn.gate_proj, ffn.up_proj, ffn.down_proj)), "gelu")
+        assert float((y.double() - want).norm()) <= 4 * torch.finfo(dtype).eps / 2 * float(want.norm())
+        hooked = copy.deepcopy(ffn)
+        calls = []
+        hooked.up_proj.register_forward_hook(lambda *a: calls.append(1))
+        assert float((hooked(x).double() - want).norm()) <= 8 * torch.finfo(dtype).eps / 2 * float(want.norm()) and calls
+    ffn = SwiGLUFFN(128, 264, fused=True).to(DEV)  # fp32 projections run as without the option
+    x = torch.randn(9, 128, device=DEV)
+    other = SwiGLUFFN(128, 264).to(DEV)
+    other.load_state_dict(ffn.state_dict())
+    assert torch.equal(ffn(x), other(x))
+
+
+def test_defaults_have_no_new_parameters():
+    a = DSALTTransformerBlock(128, 2, 4, 40, 4, 256, 264)
+    assert not a.joins_branches and not any("post_norm" in n or n.endswith("_gate") for n, _ in a.named_parameters())
+    names = {n for n, _ in DSALTTransformerBlock(128, 2, 4, 40, 4, 256, 264, **OPTIONS).named_parameters()}
+    assert names - {n for n, _ in a.named_parameters()} == {"attn_post_norm.weight", "ffn_post_norm.weight", "attn_gate", "ffn_gate"}
+    with pytest.raises(ValueError, match="activation"):
+        SwiGLUFFN(64, 64, activation="tanh")
+    with pytest.raises(ValueError, match="probability"):
+        CounterDropout(1.5)
+
+
+def test_counter_dropout_module():
+    m = CounterDropout(0.25).to(DEV)
+    x = torch.randn(1000, device=DEV)
+    assert m.eval()(x) is x
+    m.train()
+    torch.manual_seed(3)
+    a = m(x)
+    b = m(x)
+    torch.manual_seed(3)
+    assert torch.equal(m(x), a) and not torch.equal(a, b)
+    assert torch.equal(m(x, 7, 2), counter_dropout(x, 0.25, 7, 2))
+    with pytest.raises(_hip.DsaltError):
+        m(x.cpu(), 1)
+
+
+def test_replaced_and_hooked_norms_are_called():
+    b = block(dropout=0.0, fused_ffn=False)
+    cu = torch.tensor(CU, dtype=torch.int32, device=DEV)
+    x = torch.randn(CU[-1], 128, device=DEV)
+    with torch.no_grad():
+        want, _ = b(x, cu_seqlens=cu, max_seqlen=256)
+        calls = []
+        for n in (b.attn_post_norm, b.ffn_norm, b.ffn_post_norm):
+            n.register_forward_hook(lambda m, i, o: calls.append(m))
+        got, _ = b(x, cu_seqlens=cu, max_seqlen=256)
+    assert [id(c) for c in calls] == [id(n) for n in (b.attn_post_norm, b.ffn_norm, b.ffn_post_norm)]
+    assert float((got - want).norm()) <= 16 * 2.0 ** -11 * float(want.norm())
+
+
+def lm(**kw):
+    torch.manual_seed(2)
+    return DSALTLMHeadModel(vocab_size=500, d_model=128, n_layers=3, n_heads=2, n_min=4, n_max=40, k_lmk=4, max_seq_len=256,
+                            **{**OPTIONS, "dropout": 0.1, **kw}).to(DEV)
+
+
+def test_lm_training_step():
+    """Loss and gradients of a step: the same with the same torch seed, with checkpointing, and not
+    with another seed; every parameter gets a finite gradient."""
+    m = lm().train()
+    ids = torch.randint(0, 500, (CU[-1],), device=DEV)
+    cu = torch.tensor(CU, dtype=torch.int32, device=DEV)
+
+    def step(seed, **kw):
+        torch.manual_seed(seed)
+        m.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", dtype=BF):
+            loss = m(ids, cu_seqlens=cu, max_seqlen=256, labels=ids, **kw)["loss"]
+        loss.backward()
+        return loss.detach(), {n: p.grad for n, p in m.named_parameters() if p.grad is not None}
+
+    a, b, c, d = step(1), step(1), step(2), step(1, gradient_checkpointing=True)
+    assert torch.equal(a[0], b[0]) and not torch.equal(a[0], c[0]) and torch.equal(a[0], d[0])
+    for n in a[1]:
+        assert torch.isfinite(a[1][n]).all(), n
+        assert torch.equal(a[1][n], b[1][n]) and torch.equal(a[1][n], d[1][n]), n
+    missing = [n for n, p in m.named_parameters() if n not in a[1]]
+    assert not missing, missing
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_lm_inference_takes_the_next_norms_along(dtype):
+    """The LM's loop is join_branches of every layer with the norm that follows it, to the bit; and each
+    layer by itself gives the same stream, whose norm differs by the stream's rounding alone.
+    (Compared layer by layer on the same input: behind a norm that differs in its last bit a
+    landmark near a tie may be another one, and every later query of the sequence sees it.)"""
+    m = lm().to(dtype).eval()
+    m.set_collect_last_P(False)
+    ids = torch.randint(0, 500, (CU[-1],), device=DEV)
+    cu = torch.tensor(CU, dtype=torch.int32, device=DEV)
+    with torch.no_grad():
+        got = m(ids, cu_seqlens=cu, max_seqlen=256)["logits"]
+        x = m.embed_tokens(ids)
+        h = m.layers[0].attn_norm(x)
+        for i, layer in enumerate(m.layers):
+            after = m.layers[i + 1].attn_norm if i + 1 < len(m.layers) else m.final_norm
+            alone, none, _ = layer.join_branches(x, h, None, cu_seqlens=cu, max_seqlen=256)
+            x, h, _ = layer.join_branches(x, h, after, cu_seqlens=cu, max_seqlen=256)
+            assert none is None and torch.equal(alone, x)
+            want = after(x).double()
+            u = torch.finfo(dtype).eps / 2
+            # y's own rounding and that of the stream on the other side, whose rms moves less
+            assert bool(((h.double() - want).abs() <= (4 * u + 2.0 ** -20) * want.abs() + 2.0 ** -18).all())
+        assert torch.equal(got, m.lm_head(h))
+        assert torch.equal(got, m(ids, cu_seqlens=cu, max_seqlen=256)["logits"])
