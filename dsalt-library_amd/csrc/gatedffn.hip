@@ -19,6 +19,7 @@ namespace dsalt {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
 
@@ -130,11 +131,35 @@ __device__ __forceinline__ const Product &tile_of(const FfnParams &p, int tile, 
 
 enum { kEpiPair, kEpiStore, kEpiGrad };
 
-// The tile's row blocks first .. first + ROWS - 1 from their accumulators: the activation and
-// product of a pair, a plain store, or the gradients of gate and up from that of the product
-// (whose g and u are loaded kAhead turns before they are used: one after the other they would
-// cost a trip to memory for every 16 bytes of a lane).
+// g and u of a tile's elements, in the epilogue's pieces, loaded kAhead turns before they are used:
+// one after the other they would cost a trip to memory for every 16 bytes of a lane. (All of
+// them loaded as the product starts, where the registers hold them, measured no faster.)
+// Bounds by descriptor: the largest size's da took 528 us with addresses and bounds per lane, 497 so.
 constexpr int kAhead = 3;
+template <class Core>
+struct GateUp {
+    u32x4 g[kAhead], u[kAhead];
+    // piece t of the wave's row block `block`
+    __device__ __forceinline__ void load(const FfnParams &p, const Product &q, const Core &c, int block, int t, int64_t m0,
+                                         int64_t n0) {
+        const int64_t mb = m0 + (c.wm * Core::FM + block) * 32, nb = n0 + c.wn * Core::COLS;
+        const int64_t rows = min(q.m - mb, (int64_t)32);
+        // past the last row, and past the row's end, nothing is read
+        const int64_t bytes = rows > 0 && nb < q.n ? (rows - 1) * p.gu_ld + (q.n - nb) * 2 : 0;
+        const char *base = p.gu + mb * p.gu_ld + nb * 2;
+        const uint32_t off = nb + c.piece_col() < q.n
+                                 ? (uint32_t)c.piece_row(t) * (uint32_t)p.gu_ld + c.piece_col() * 2 : kOutOfRange;
+        g[t % kAhead] = __builtin_amdgcn_raw_buffer_load_b128(
+            __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, (int)bytes, 0x00020000), (int)off, 0, 0);
+        u[t % kAhead] = __builtin_amdgcn_raw_buffer_load_b128(
+            __builtin_amdgcn_make_buffer_rsrc((void *)(base + p.up_off), (short)0, (int)bytes, 0x00020000), (int)off, 0, 0);
+    }
+    __device__ __forceinline__ uint4 gate(int t) const { return bitcast<uint4>(g[t % kAhead]); }
+    __device__ __forceinline__ uint4 up(int t) const { return bitcast<uint4>(u[t % kAhead]); }
+};
+
+// The tile's row blocks first .. first + ROWS - 1 from their accumulators: the activation and
+// product of a pair, a plain store, or the gradients of gate and up from that of the product.
 template <class DT, class Core, int EPI, int ROWS>
 __device__ __forceinline__ void epilogue(const FfnParams &p, const Product &q, const Core &c,
                                          const f32x16 (&acc)[ROWS][Core::FN], int first, int64_t m0, int64_t n0, char *lds) {
@@ -147,20 +172,13 @@ __device__ __forceinline__ void epilogue(const FfnParams &p, const Product &q, c
         const int64_t mb = m0 + (c.wm * Core::FM + first + i) * 32;
         const int rows = (int)min(q.m - mb, (int64_t)32);
         // wave-uniform bases, 32-bit lane offsets
-        char *out = q.out + mb * q.out_ld + nb * 2, *gu = p.gu + mb * p.gu_ld + nb * 2;
+        char *out = q.out + mb * q.out_ld + nb * 2, *gu_out = p.gu + mb * p.gu_ld + nb * 2;
         const uint32_t off = (uint32_t)(c.lane / Core::PIECES) * ld + c.piece_col() * 2,
                        gu_off = (uint32_t)(c.lane / Core::PIECES) * gu_ld + c.piece_col() * 2;
-        uint4 graw[kAhead], uraw[kAhead];
-        auto load = [&](int t) {
-            if (inside && c.piece_row(t) < rows) {
-                const char *at = gu + (uint32_t)(t * Core::TURN_ROWS) * gu_ld;
-                graw[t % kAhead] = *reinterpret_cast<const uint4 *>(at + gu_off);
-                uraw[t % kAhead] = *reinterpret_cast<const uint4 *>(at + p.up_off + gu_off);
-            }
-        };
+        GateUp<Core> gu;
         if constexpr (EPI == kEpiGrad) {
 #pragma unroll
-            for (int t = 0; t < kAhead && t < Core::TURNS; ++t) load(t);
+            for (int t = 0; t < kAhead && t < Core::TURNS; ++t) gu.load(p, q, c, first + i, t, m0, n0);
         }
         c.put(lds, acc[i]);
 #pragma unroll
@@ -172,7 +190,7 @@ __device__ __forceinline__ void epilogue(const FfnParams &p, const Product &q, c
                 char *o = out + (uint32_t)(t * Core::TURN_ROWS) * ld;
                 if constexpr (EPI == kEpiPair) {
                     if (p.gu) {
-                        char *at = gu + (uint32_t)(t * Core::TURN_ROWS) * gu_ld;
+                        char *at = gu_out + (uint32_t)(t * Core::TURN_ROWS) * gu_ld;
                         *reinterpret_cast<uint4 *>(at + gu_off) = pack8<DT>(v);
                         *reinterpret_cast<uint4 *>(at + p.up_off + gu_off) = pack8<DT>(u);
                     }
@@ -181,15 +199,15 @@ __device__ __forceinline__ void epilogue(const FfnParams &p, const Product &q, c
                 } else if constexpr (EPI == kEpiStore) {
                     *reinterpret_cast<uint4 *>(o + off) = pack8<DT>(v);
                 } else {
-                    unpack8<DT>(graw[t % kAhead], w);
-                    unpack8<DT>(uraw[t % kAhead], u);
+                    unpack8<DT>(gu.gate(t), w);
+                    unpack8<DT>(gu.up(t), u);
                     gated_grad8(p.act, w, u, v);
                     *reinterpret_cast<uint4 *>(o + off) = pack8<DT>(v);
                     *reinterpret_cast<uint4 *>(o + p.up_off + off) = pack8<DT>(u);
                 }
             }
             if constexpr (EPI == kEpiGrad)
-                if (t + kAhead < Core::TURNS) load(t + kAhead);
+                if (t + kAhead < Core::TURNS) gu.load(p, q, c, first + i, t + kAhead, m0, n0);
             __builtin_amdgcn_sched_barrier(0);  // no more turns in registers at a time than these
         }
         __builtin_amdgcn_wave_barrier();  // the next block overwrites this one
@@ -403,9 +421,9 @@ struct ShapeCost {
 };
 constexpr ShapeCost kShapes[] = {
     {256, 256, 256, 1.85, 1.20, 1.0},
-    {256, 128, 256, 1.12, 0.65, 1.0},
-    {128, 128, 512, 1.17, 0.40, 0.5},
-    {64, 128, 768, 0.95, 0.30, 0.4},
+    {256, 128, 256, 1.05, 0.65, 1.0},
+    {128, 128, 512, 1.17, 0.50, 0.5},
+    {64, 128, 768, 1.00, 0.38, 0.4},
 };
 constexpr int kShapeCount = 4, kMaxSplit = 8;
 constexpr double kTile = 3.0, kJoin = 6.0, kMemory = 5.0e6, kPartials = 3.0e6;  // us, us, bytes per us
