@@ -223,9 +223,9 @@ using Core = GemmCore<DT, S::BM, S::BN, 64, S::RA, S::RB, S::WM, S::WN, ALAY, BL
 
 // Partial sums of piece `piece` of split tile r: [piece][r][i][j][quarter][thread] float4.
 template <class C>
-__device__ __forceinline__ float4 *partial(const FfnParams &p, int r, int piece, int tiles, int i, int j) {
+__device__ __forceinline__ float4 *partial(const FfnParams &p, int r, int piece, int tiles, int i, int j, int thread) {
     return reinterpret_cast<float4 *>(p.part) +
-           ((((int64_t)piece * tiles + r) * C::FM + i) * C::FN + j) * 4 * C::THREADS + threadIdx.x;
+           ((((int64_t)piece * tiles + r) * C::FM + i) * C::FN + j) * 4 * C::THREADS + thread;
 }
 
 template <class DT, class S, int ALAY, int BLAY, int SEGMENTS, int EPI>
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(S::WM *S::WN * 64) ffn_kernel(const FfnParams 
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     const f32x16 &v = c.acc[i][j];
-                    partial<C>(p, r, piece, tiles, i, j)[h * C::THREADS] =
+                    partial<C>(p, r, piece, tiles, i, j, threadIdx.x)[h * C::THREADS] =
                         make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
                 }
         return;
@@ -268,29 +268,44 @@ __global__ void __launch_bounds__(S::WM *S::WN * 64) ffn_kernel(const FfnParams 
     epilogue<DT, C, EPI, C::FM>(p, q, c, c.acc, 0, m0, n0, lds);
 }
 
-// The split tiles' partial sums added in order, and their epilogue: one workgroup per row block i.
+// The split tiles' partial sums added in order, and their epilogue: a workgroup of one wave for
+// each row block of each of the tile's waves (a CU alone reads too slowly for more).
 template <class DT, class S, int ALAY, int BLAY, int EPI>
-__global__ void __launch_bounds__(S::WM *S::WN * 64) ffn_join_kernel(const FfnParams p) {
+__global__ void __launch_bounds__(64) ffn_join_kernel(const FfnParams p) {
     typedef Core<DT, S, ALAY, BLAY, EPI> C;
     constexpr int BNO = EPI == kEpiPair ? S::BN / 2 : S::BN;
-    const int tiles = gridDim.x / C::FM, r = blockIdx.x / C::FM, i = blockIdx.x - r * C::FM;
+    const int tiles = gridDim.x / (C::FM * C::NW), r = blockIdx.x / (C::FM * C::NW);
+    const int i = blockIdx.x / C::NW % C::FM, wave = blockIdx.x % C::NW;
     int tm, tn;
     const Product &q = tile_of(p, p.whole + r, tm, tn);
-    __shared__ __attribute__((aligned(256))) char lds[C::NW * 32 * C::COLS * 4];
-    C c;
+    __shared__ __attribute__((aligned(256))) char lds[32 * C::COLS * 4];
+    C c;  // the only wave of its workgroup, in the place of one of the tile's
+    c.wm = wave % S::WM;
+    c.wn = wave / S::WM;
     f32x16 acc[1][C::FN];
+    const int64_t stride = (int64_t)tiles * C::FM * C::FN * 4 * C::THREADS;
+    constexpr int kPieces = 8;  // partial sums in flight: one after the other each is a trip to memory
 #pragma unroll
     for (int j = 0; j < C::FN; ++j) {
         acc[0][j] = f32x16{};
-        for (int s = 0; s < p.split; ++s)
+        const float4 *first = partial<C>(p, r, 0, tiles, i, j, wave * 64 + threadIdx.x);
+        for (int s0 = 0; s0 < p.split; s0 += kPieces) {
+            float4 v[kPieces][4];
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                const float4 v = partial<C>(p, r, s, tiles, i, j)[h * C::THREADS];
-                acc[0][j][4 * h] += v.x;
-                acc[0][j][4 * h + 1] += v.y;
-                acc[0][j][4 * h + 2] += v.z;
-                acc[0][j][4 * h + 3] += v.w;
-            }
+            for (int s = 0; s < kPieces; ++s)
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    v[s][h] = first[min(s0 + s, p.split - 1) * stride + h * C::THREADS];
+#pragma unroll
+            for (int s = 0; s < kPieces; ++s)
+#pragma unroll
+                for (int h = 0; s0 + s < p.split && h < 4; ++h) {
+                    acc[0][j][4 * h] += v[s][h].x;
+                    acc[0][j][4 * h + 1] += v[s][h].y;
+                    acc[0][j][4 * h + 2] += v[s][h].z;
+                    acc[0][j][4 * h + 3] += v[s][h].w;
+                }
+        }
     }
     const int64_t m0 = (int64_t)tm * S::BM, n0 = (int64_t)tn * BNO;
     epilogue<DT, C, EPI, 1>(p, q, c, acc, i, m0, n0, lds);
@@ -475,7 +490,8 @@ hipError_t launch_shape(const FfnParams &p, const Plan &w, hipStream_t stream) {
     hipLaunchKernelGGL((ffn_kernel<DT, S, ALAY, BLAY, SEGMENTS, EPI>), dim3(w.whole + rest * w.split), dim3(C::THREADS), 0,
                        stream, p);
     if (rest)
-        hipLaunchKernelGGL((ffn_join_kernel<DT, S, ALAY, BLAY, EPI>), dim3(rest * C::FM), dim3(C::THREADS), 0, stream, p);
+        hipLaunchKernelGGL((ffn_join_kernel<DT, S, ALAY, BLAY, EPI>), dim3(rest * C::FM * C::NW), dim3(64), 0, stream,
+                           p);
     return hipGetLastError();
 }
 
