@@ -111,13 +111,21 @@ def test_activations(act, rows):
         check(got[n], ref[n], BF, (n, act))
 
 
-@pytest.mark.parametrize("rows,d,f", [(2049, 512, 1408), (1500, 1024, 2816)])
+# sizes that between them take every tile shape, with whole tiles only, with tiles split along k
+# besides whole ones and with split ones only, in each of the five products
+@pytest.mark.parametrize("rows,d,f", [
+    (2049, 512, 1408), (1500, 1024, 2816), (74, 64, 64), (3062, 2344, 64), (8579, 904, 712), (3298, 1952, 2496),
+    (846, 520, 3504), (9414, 888, 2672), (3684, 2200, 2440), (7748, 2216, 1504), (2629, 784, 3176), (9228, 472, 848),
+    (2378, 1560, 1712), (1383, 1480, 3120), (7376, 1776, 536), (7355, 2264, 1848)])
 def test_larger(rows, d, f):
-    print(f"gated_ffn {rows} x {d} x {f}", flush=True)
-    x, wg, wu, wd, dy = inputs(rows, d, f, d, BF)
-    ref, got = reference(x, wg, wu, wd, dy, "silu", BF), run(x, wg, wu, wd, dy, "silu")
+    dtype = (BF, HF)[rows % 2]
+    print(f"gated_ffn {rows} x {d} x {f} {dtype}", flush=True)
+    x, wg, wu, wd, dy = inputs(rows, d, f, d, dtype)
+    ref, got = reference(x, wg, wu, wd, dy, "silu", dtype), run(x, wg, wu, wd, dy, "silu")
     for n in ref:
-        check(got[n], ref[n], BF, n)
+        check(got[n], ref[n], dtype, n)
+    with torch.no_grad():
+        check(gated_ffn(x, wg, wu, wd), ref["y"], dtype, "y without a graph")
 
 
 def test_against_differences():
