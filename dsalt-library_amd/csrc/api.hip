@@ -710,6 +710,9 @@ int dsalt_gated_ffn_bwd(const dsalt_gated_ffn_args *args, void *stream) {
 int64_t dsalt_gated_ffn_workspace_size(int64_t rows, int32_t d, int32_t f, int32_t e, int32_t backward) {
     return rows < 0 || d < 8 || f < 8 || e < 8 ? 0 : dsalt::gated_ffn_workspace_bytes(rows, d, f, e, backward != 0);
 }
+int64_t dsalt_gated_ffn_kept_size(int64_t rows, int32_t f, int32_t dtype) {
+    return rows < 0 || f < 8 ? 0 : dsalt::gated_ffn_kept_bytes(rows, f, dtype);
+}
 size_t dsalt_gated_ffn_args_size(void) { return sizeof(dsalt_gated_ffn_args); }
 
 int dsalt_dropout(const dsalt_dropout_args *a, void *stream) {

@@ -6,9 +6,9 @@
 //
 // Gate and up projection, activation and product are one kernel: a workgroup's B tile holds
 // the same columns of both weights, so that a lane ends with g and u of the same elements
-// in its fp32 accumulators and rounds only a (and g, u where a backward will read them). The
-// backward's first kernel ends da = dy Wd in the gradients of g and u the same way: da is
-// never written.
+// in its fp32 accumulators and rounds only a. Where a backward will read g and u they are
+// kept in more bits than the element type's (see Kept). The backward's first kernel ends
+// da = dy Wd in the gradients of g and u the same way: da is never written.
 #include "gemm.h"
 #include "launch.h"
 
@@ -20,6 +20,7 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
 
@@ -90,6 +91,59 @@ __device__ __forceinline__ void gated_grad8(int act, const float (&g)[8], float 
     else gated_grad8<DSALT_ACT_RELU>(g, u, da);
 }
 
+// g and u kept for the backward. Their gradients are rounded to the element type once, as operands
+// of the matrix units have to be, and so is every result; g and u rounded to it too would put
+// a third rounding into dx and the weights' gradients (1.8 times the error of the last rounding
+// alone, against 1.4 so; the extra byte costs under 1 % of a training pass of 16384 rows). So they keep the upper 20 bits of their fp32 value beside bf16 (four bits
+// more than it has), and the upper 24 beside fp16 (five more): the upper 16 bits in a plane of
+// gate | up rows, the rest in a plane behind it, a byte for both (low half g) or a byte each.
+template <class DT>
+struct Kept {
+    static constexpr bool NIBBLE = std::is_same<DT, BF16>::value;
+    static constexpr int LOW = NIBBLE ? 4 : 8;                // bits in the second plane
+    static constexpr int LOW_BYTES = NIBBLE ? 1 : 2;          // of a (g, u) pair there
+    static __device__ __forceinline__ uint32_t round(float x) {
+        const uint32_t b = __float_as_uint(x), r = b + (1u << (15 - LOW));  // to nearest
+        return (b & 0x7fffffffu) > 0x7f800000u ? b : r;                    // a NaN stays one
+    }
+    // eight columns: the planes' words
+    static __device__ __forceinline__ void pack(const float (&v)[8], uint4 &high, uint32_t (&low)[2]) {
+        uint32_t h[4];
+        low[0] = low[1] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t x = round(v[2 * e]), y = round(v[2 * e + 1]);
+            h[e] = (x >> 16) | (y & 0xffff0000u);
+            low[e >> 1] |= (((x & 0xffffu) >> (16 - LOW)) | (((y & 0xffffu) >> (16 - LOW)) << 8)) << (16 * (e & 1));
+        }
+        high = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+    static __device__ __forceinline__ void store(const float (&g)[8], const float (&u)[8], char *high, char *low, int64_t up_off) {
+        uint4 gh, uh;
+        uint32_t gl[2], ul[2];
+        pack(g, gh, gl);
+        pack(u, uh, ul);
+        *reinterpret_cast<uint4 *>(high) = gh;
+        *reinterpret_cast<uint4 *>(high + up_off) = uh;
+        if constexpr (NIBBLE) {
+            *reinterpret_cast<uint2 *>(low) = make_uint2(gl[0] | (ul[0] << 4), gl[1] | (ul[1] << 4));
+        } else {
+            *reinterpret_cast<uint2 *>(low) = make_uint2(gl[0], gl[1]);
+            *reinterpret_cast<uint2 *>(low + up_off / 2) = make_uint2(ul[0], ul[1]);
+        }
+    }
+    // low: the bytes of one matrix, shift: where its nibble is in them
+    static __device__ __forceinline__ void unpack(uint4 high, uint2 low, int shift, float (&v)[8]) {
+        const uint32_t h[4] = {high.x, high.y, high.z, high.w}, l[2] = {low.x >> shift, low.y >> shift};
+        constexpr uint32_t MASK = (1u << LOW) - 1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t top = e & 1 ? h[e >> 1] & 0xffff0000u : h[e >> 1] << 16;
+            v[e] = __uint_as_float(top | (((l[e >> 2] >> (8 * (e & 3))) & MASK) << (16 - LOW)));
+        }
+    }
+};
+
 // One product of a launch: out [m, n] = sum over the segments of a[s] b[s] (pair: n columns of
 // each of b[0] and b[1]).
 struct Product {
@@ -106,8 +160,8 @@ struct FfnParams {
     int products;
     int64_t k;        // of every product and segment
     int act;
-    char *gu;         // gate | up: written (pair; NULL: not kept) or read (gradient)
-    int64_t gu_ld, up_off;  // bytes; up at gu + up_off
+    char *gu, *low;   // the planes of gate | up (Kept): written (pair; gu NULL: not kept) or read (gradient)
+    int64_t gu_ld, up_off, low_ld;  // bytes; up at gu + up_off and, with a byte of its own, low + up_off / 2
     int whole;        // tiles computed by one workgroup each; the others by `split` workgroups,
     int split;        // whose fp32 partial sums go to `part` and are joined by a second launch
     float *part;
@@ -136,26 +190,36 @@ enum { kEpiPair, kEpiStore, kEpiGrad };
 // them loaded as the product starts, where the registers hold them, measured no faster.)
 // Bounds by descriptor: the largest size's da took 528 us with addresses and bounds per lane, 497 so.
 constexpr int kAhead = 3;
-template <class Core>
+template <class DT, class Core>
 struct GateUp {
     u32x4 g[kAhead], u[kAhead];
+    u32x2 gl[kAhead], ul[kAhead];
     // piece t of the wave's row block `block`
     __device__ __forceinline__ void load(const FfnParams &p, const Product &q, const Core &c, int block, int t, int64_t m0,
                                          int64_t n0) {
         const int64_t mb = m0 + (c.wm * Core::FM + block) * 32, nb = n0 + c.wn * Core::COLS;
-        const int64_t rows = min(q.m - mb, (int64_t)32);
+        const int64_t rows = min(q.m - mb, (int64_t)32), cols = q.n - nb;
+        const bool some = rows > 0 && cols > 0, in = c.piece_col() < cols;
+        const int at = t % kAhead;
         // past the last row, and past the row's end, nothing is read
-        const int64_t bytes = rows > 0 && nb < q.n ? (rows - 1) * p.gu_ld + (q.n - nb) * 2 : 0;
-        const char *base = p.gu + mb * p.gu_ld + nb * 2;
-        const uint32_t off = nb + c.piece_col() < q.n
-                                 ? (uint32_t)c.piece_row(t) * (uint32_t)p.gu_ld + c.piece_col() * 2 : kOutOfRange;
-        g[t % kAhead] = __builtin_amdgcn_raw_buffer_load_b128(
-            __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, (int)bytes, 0x00020000), (int)off, 0, 0);
-        u[t % kAhead] = __builtin_amdgcn_raw_buffer_load_b128(
-            __builtin_amdgcn_make_buffer_rsrc((void *)(base + p.up_off), (short)0, (int)bytes, 0x00020000), (int)off, 0, 0);
+        auto rsrc = [&](const char *plane, int64_t ld, int64_t off, int size) {
+            return __builtin_amdgcn_make_buffer_rsrc((void *)(plane + mb * ld + nb * size + off), (short)0,
+                                                     (int)(some ? (rows - 1) * ld + cols * size : 0), 0x00020000);
+        };
+        const int off = in ? (int)((uint32_t)c.piece_row(t) * (uint32_t)p.gu_ld) + c.piece_col() * 2 : (int)kOutOfRange;
+        g[at] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(p.gu, p.gu_ld, 0, 2), off, 0, 0);
+        u[at] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(p.gu, p.gu_ld, p.up_off, 2), off, 0, 0);
+        const int low = in ? (int)((uint32_t)c.piece_row(t) * (uint32_t)p.low_ld) + c.piece_col() : (int)kOutOfRange;
+        gl[at] = __builtin_amdgcn_raw_buffer_load_b64(rsrc(p.low, p.low_ld, 0, 1), low, 0, 0);
+        if constexpr (!Kept<DT>::NIBBLE)
+            ul[at] = __builtin_amdgcn_raw_buffer_load_b64(rsrc(p.low, p.low_ld, p.up_off / 2, 1), low, 0, 0);
     }
-    __device__ __forceinline__ uint4 gate(int t) const { return bitcast<uint4>(g[t % kAhead]); }
-    __device__ __forceinline__ uint4 up(int t) const { return bitcast<uint4>(u[t % kAhead]); }
+    __device__ __forceinline__ void get(int t, float (&gate)[8], float (&up)[8]) const {
+        const int at = t % kAhead;
+        Kept<DT>::unpack(bitcast<uint4>(g[at]), bitcast<uint2>(gl[at]), 0, gate);
+        if constexpr (Kept<DT>::NIBBLE) Kept<DT>::unpack(bitcast<uint4>(u[at]), bitcast<uint2>(gl[at]), 4, up);
+        else Kept<DT>::unpack(bitcast<uint4>(u[at]), bitcast<uint2>(ul[at]), 0, up);
+    }
 };
 
 // The tile's row blocks first .. first + ROWS - 1 from their accumulators: the activation and
@@ -166,16 +230,17 @@ __device__ __forceinline__ void epilogue(const FfnParams &p, const Product &q, c
     constexpr int WIDTH = EPI == kEpiPair ? Core::COLS / 2 : Core::COLS;  // output columns of a wave
     const int64_t nb = n0 + c.wn * WIDTH;
     const bool inside = nb + c.piece_col() < q.n;
-    const uint32_t ld = (uint32_t)q.out_ld, gu_ld = (uint32_t)p.gu_ld;
+    const uint32_t ld = (uint32_t)q.out_ld, gu_ld = (uint32_t)p.gu_ld, low_ld = (uint32_t)p.low_ld;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int64_t mb = m0 + (c.wm * Core::FM + first + i) * 32;
         const int rows = (int)min(q.m - mb, (int64_t)32);
         // wave-uniform bases, 32-bit lane offsets
-        char *out = q.out + mb * q.out_ld + nb * 2, *gu_out = p.gu + mb * p.gu_ld + nb * 2;
+        char *out = q.out + mb * q.out_ld + nb * 2, *gu_out = p.gu + mb * p.gu_ld + nb * 2, *low_out = p.low + mb * p.low_ld + nb;
         const uint32_t off = (uint32_t)(c.lane / Core::PIECES) * ld + c.piece_col() * 2,
-                       gu_off = (uint32_t)(c.lane / Core::PIECES) * gu_ld + c.piece_col() * 2;
-        GateUp<Core> gu;
+                       gu_off = (uint32_t)(c.lane / Core::PIECES) * gu_ld + c.piece_col() * 2,
+                       low_off = (uint32_t)(c.lane / Core::PIECES) * low_ld + c.piece_col();
+        GateUp<DT, Core> gu;
         if constexpr (EPI == kEpiGrad) {
 #pragma unroll
             for (int t = 0; t < kAhead && t < Core::TURNS; ++t) gu.load(p, q, c, first + i, t, m0, n0);
@@ -189,18 +254,15 @@ __device__ __forceinline__ void epilogue(const FfnParams &p, const Product &q, c
             if (inside && c.piece_row(t) < rows) {
                 char *o = out + (uint32_t)(t * Core::TURN_ROWS) * ld;
                 if constexpr (EPI == kEpiPair) {
-                    if (p.gu) {
-                        char *at = gu_out + (uint32_t)(t * Core::TURN_ROWS) * gu_ld;
-                        *reinterpret_cast<uint4 *>(at + gu_off) = pack8<DT>(v);
-                        *reinterpret_cast<uint4 *>(at + p.up_off + gu_off) = pack8<DT>(u);
-                    }
+                    if (p.gu)
+                        Kept<DT>::store(v, u, gu_out + (uint32_t)(t * Core::TURN_ROWS) * gu_ld + gu_off,
+                                        low_out + (uint32_t)(t * Core::TURN_ROWS) * low_ld + low_off, p.up_off);
                     gated8(p.act, v, u, w);
                     *reinterpret_cast<uint4 *>(o + off) = pack8<DT>(w);
                 } else if constexpr (EPI == kEpiStore) {
                     *reinterpret_cast<uint4 *>(o + off) = pack8<DT>(v);
                 } else {
-                    unpack8<DT>(gu.gate(t), w);
-                    unpack8<DT>(gu.up(t), u);
+                    gu.get(t, w, u);
                     gated_grad8(p.act, w, u, v);
                     *reinterpret_cast<uint4 *>(o + off) = pack8<DT>(v);
                     *reinterpret_cast<uint4 *>(o + p.up_off + off) = pack8<DT>(u);
@@ -387,11 +449,7 @@ __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const FfnParams p) {
     char *o = q.out + (int64_t)r * q.out_ld + col * 2;
     if constexpr (PAIR) {
         sum(2, u);
-        if (p.gu) {
-            char *gu = p.gu + (int64_t)r * p.gu_ld + col * 2;
-            *reinterpret_cast<uint4 *>(gu) = pack8<DT>(v);
-            *reinterpret_cast<uint4 *>(gu + p.up_off) = pack8<DT>(u);
-        }
+        if (p.gu) Kept<DT>::store(v, u, p.gu + (int64_t)r * p.gu_ld + col * 2, p.low + (int64_t)r * p.low_ld + col, p.up_off);
         gated8(p.act, v, u, a);
         *reinterpret_cast<uint4 *>(o) = pack8<DT>(a);
     } else {
@@ -480,8 +538,8 @@ Plan plan(const Extent *e, int count, int64_t k, int segments, bool pair, int io
     return best;
 }
 // What each kind of launch moves per output element: see epilogue().
-constexpr int kIoStore = 2, kIoGrad = 8;
-int io_pair(bool keep) { return keep ? 6 : 2; }
+constexpr int kIoStore = 2, kIoGrad = 9;
+int io_pair(bool keep) { return keep ? 7 : 2; }
 
 template <class DT, class S, int ALAY, int BLAY, int SEGMENTS, int EPI>
 hipError_t launch_shape(const FfnParams &p, const Plan &w, hipStream_t stream) {
@@ -519,6 +577,16 @@ hipError_t launch_product(FfnParams p, void *workspace, hipStream_t stream) {
     }
 }
 
+// The planes of the kept gate | up of `rows` rows.
+template <class DT>
+void set_kept(FfnParams &p, void *gate_up, int64_t rows, int64_t f) {
+    p.gu = static_cast<char *>(gate_up);
+    p.gu_ld = f * 4;
+    p.up_off = f * 2;
+    p.low = p.gu + rows * p.gu_ld;
+    p.low_ld = f * Kept<DT>::LOW_BYTES;
+}
+
 GemmOperand operand(const void *p, int64_t ld, int64_t rows) { return {static_cast<const char *>(p), ld * 2, rows}; }
 
 Product product(GemmOperand a, GemmOperand b, int64_t m, int64_t n, void *out, int64_t out_ld) {
@@ -540,9 +608,7 @@ hipError_t forward(const dsalt_gated_ffn_args &a, hipStream_t stream) {
     p.act = a.activation;
     p.prod[0] = product(operand(a.x, a.x_stride, a.rows), operand(a.w_gate, a.w_gate_stride, a.f), a.rows, a.f, a.act, a.f);
     p.prod[0].b[1] = operand(a.w_up, a.w_up_stride, a.f);
-    p.gu = static_cast<char *>(a.gate_up);
-    p.gu_ld = (int64_t)a.f * 4;
-    p.up_off = (int64_t)a.f * 2;
+    if (a.gate_up) set_kept<DT>(p, a.gate_up, a.rows, a.f);
     const bool few = a.rows <= kFewRows;
     hipError_t e = few ? launch_few<DT, kEpiPair>(p, stream)
                        : launch_product<DT, kKContig, kKContig, 1, kEpiPair>(p, a.workspace, stream);
@@ -566,9 +632,7 @@ hipError_t backward(const dsalt_gated_ffn_args &a, hipStream_t stream) {
         p.act = a.activation;
         p.prod[0] = product(operand(a.dy, a.dy_stride, a.rows), operand(a.w_down, a.w_down_stride, a.f), a.rows, a.f,
                             a.d_gate_up, 2 * (int64_t)a.f);
-        p.gu = static_cast<char *>(a.gate_up);
-        p.gu_ld = 2 * up;
-        p.up_off = up;
+        set_kept<DT>(p, a.gate_up, a.rows, a.f);
         hipError_t e = launch_product<DT, kKContig, kRContig, 1, kEpiGrad>(p, a.workspace, stream);
         if (e != hipSuccess) return e;
     }
@@ -622,6 +686,9 @@ int64_t gated_ffn_workspace_bytes(int64_t rows, int d, int f, int e, bool bwd) {
     return most;
 }
 
+int64_t gated_ffn_kept_bytes(int64_t rows, int f, int dtype) {
+    return rows * f * (4 + (dtype == DSALT_DTYPE_BF16 ? Kept<BF16>::LOW_BYTES : Kept<F16>::LOW_BYTES));
+}
 int64_t gated_ffn_max_ld() { return kGemmMaxLd; }
 
 }  // namespace dsalt

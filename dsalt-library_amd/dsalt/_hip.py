@@ -239,7 +239,7 @@ EXPORTED_SYMBOLS = (
     "dsalt_select_hybrid_qkv", "dsalt_qkv_args_size", "dsalt_module_grads_v", "dsalt_module_grads_x",
     "dsalt_module_grads_workspace_size", "dsalt_module_grads_args_size", "dsalt_swiglu_rows", "dsalt_norm_train",
     "dsalt_group_sum", "dsalt_norm_train_bwd", "dsalt_norm_train_workspace_size", "dsalt_norm_train_args_size",
-    "dsalt_gated_ffn", "dsalt_gated_ffn_bwd", "dsalt_gated_ffn_check", "dsalt_gated_ffn_workspace_size",
+    "dsalt_gated_ffn", "dsalt_gated_ffn_bwd", "dsalt_gated_ffn_check", "dsalt_gated_ffn_workspace_size", "dsalt_gated_ffn_kept_size",
     "dsalt_gated_ffn_args_size", "dsalt_dropout", "dsalt_dropout_args_size", "dsalt_branch_norm",
     "dsalt_branch_norm_bwd", "dsalt_branch_norm_check", "dsalt_branch_norm_workspace_size", "dsalt_branch_norm_args_size",
 )
@@ -315,6 +315,8 @@ def lib() -> ctypes.CDLL:
     h.dsalt_norm_train_workspace_size.restype = c_int64
     h.dsalt_gated_ffn_workspace_size.argtypes = [c_int64] + [c_int32] * 4
     h.dsalt_gated_ffn_workspace_size.restype = c_int64
+    h.dsalt_gated_ffn_kept_size.argtypes = [c_int64, c_int32, c_int32]
+    h.dsalt_gated_ffn_kept_size.restype = c_int64
     h.dsalt_branch_norm_workspace_size.argtypes = [c_int64, c_int32]
     h.dsalt_branch_norm_workspace_size.restype = c_int64
     h.dsalt_lmk_weights_workspace_size.argtypes = [c_int32] * 2
@@ -1593,17 +1595,19 @@ def row_operand(t: torch.Tensor) -> torch.Tensor:
 
 def gated_ffn(x, w_gate, w_up, w_down, activation: str, lead, keep: bool):
     """``(y [*lead, e], kept)`` of `row_operand` x [T, d] and weights: see dsalt_gated_ffn. kept is
-    one buffer for the backward: act [T, f], and gate | up [T, 2 f] behind it with `keep`."""
+    one buffer (bytes) for the backward: act [T, f], and behind it, with `keep`, gate and up."""
     dev = x.device
     rows, d = x.shape
     f, e = w_gate.shape[0], w_down.shape[0]
-    kept = x.new_empty(rows * f * (3 if keep else 1))
+    code = _DTYPES[x.dtype]
+    kept = torch.empty(rows * f * 2 + (lib().dsalt_gated_ffn_kept_size(rows, f, code) if keep else 0), device=dev,
+                       dtype=torch.uint8)
     y = x.new_empty(*lead, e)
     act = kept.data_ptr()
     need = lib().dsalt_gated_ffn_workspace_size(rows, d, f, e, 0)
     ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None  # held over the call
     _call("dsalt_gated_ffn",
-          _FFN_PACK.pack(rows, d, f, e, _DTYPES[x.dtype], ACTIVATIONS[activation], 0, x.data_ptr(), x.stride(0),
+          _FFN_PACK.pack(rows, d, f, e, code, ACTIVATIONS[activation], 0, x.data_ptr(), x.stride(0),
                          w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), w_gate.stride(0), w_up.stride(0),
                          w_down.stride(0), act + rows * f * 2 if keep else 0, act, y.data_ptr(), 0, 0, 0, 0, 0, 0, 0,
                          ws.data_ptr() if need else 0, need), dev)

@@ -4,7 +4,8 @@ its GELU and ReLU relatives).
 
 Both projections, the activation and the product are one kernel, and so are the gradient of
 the product and the activation's gradient. Products accumulate in fp32; the hidden activation
-and its gradients are rounded once, from fp32.
+and the gradients of gate and up are rounded once, from fp32, and gate and up are kept for the
+backward in four or five bits more than the element type has.
 """
 from __future__ import annotations
 
@@ -47,7 +48,8 @@ class _GatedFFN(torch.autograd.Function):
             if tuple(w._version for w in ws) != versions:
                 raise RuntimeError("a weight of gated_ffn was changed in place before a backward that records a graph")
             if x is None:  # only w_down has a gradient
-                dw, = graph_grads(lambda w: (F.linear(kept.view(*shape[:-1], w.shape[1]), w),), ws[2:], (dy,))
+                act = kept.view(dy.dtype).view(*shape[:-1], ws[2].shape[1])
+                dw, = graph_grads(lambda w: (F.linear(act, w),), ws[2:], (dy,))
                 return None, None, None, dw, None
             return *graph_grads(lambda *t: (torch_gated_ffn(*t, activation),), (x, *ws), (dy,)), None
         row = _hip.row_operand

@@ -618,13 +618,15 @@ int dsalt_lmk_weights_check(const dsalt_lmk_weights_args *args, int32_t backward
 /*
  * Gated feed-forward block of [rows, d] hidden states, forward and backward:
  *   a = act(x w_gate^T) * (x w_up^T)   [rows, f]      y = a w_down^T   [rows, e]
- * w_gate, w_up [f, d], w_down [e, f]; act one of DSALT_ACT_*. Products accumulate in fp32; a (and
- * gate_up, where it is kept) is rounded once from fp32, y once.
- * dsalt_gated_ffn writes `act` and y, and gate_up [rows, 2 f] (gate | up) unless it is NULL.
- * dsalt_gated_ffn_bwd reads gate_up and `act` as the forward left them and dy [rows, e]; writes
- * dw_down [e, f], and with d_gate_up [rows, 2 f] (the gradient of gate_up; scratch, dead when
- * the launches end) dx [rows, d], dw_gate and dw_up [f, d]; each result may be NULL. Sums run in
- * a fixed order. rows = 0 gives zero weight gradients.
+ * w_gate, w_up [f, d], w_down [e, f]; act one of DSALT_ACT_*. Products accumulate in fp32; a is
+ * rounded once from fp32, y once, and so are the gradients of gate and up and each result of the
+ * backward.
+ * dsalt_gated_ffn writes `act` and y, and what the backward needs of gate and up to gate_up
+ * (dsalt_gated_ffn_kept_size bytes, a layout of its own) unless it is NULL. dsalt_gated_ffn_bwd
+ * reads gate_up and `act` as the forward left them and dy [rows, e]; writes dw_down [e, f], and
+ * with d_gate_up [rows, 2 f] (the gradients of gate | up; scratch, dead when the launches end)
+ * dx [rows, d], dw_gate and dw_up [f, d]; each result may be NULL. Sums run in a fixed order.
+ * rows = 0 gives zero weight gradients.
  * dtype BF16 or F16 for every tensor. d, e, f multiples of 8 in [8, 2^20]; row strides (in
  * elements) multiples of 8 up to 2^21 and at least the row length, the other tensors contiguous;
  * 16-byte aligned pointers; outputs alias no input. workspace: at least
@@ -652,6 +654,7 @@ int dsalt_gated_ffn(const dsalt_gated_ffn_args *args, void *stream);
 int dsalt_gated_ffn_bwd(const dsalt_gated_ffn_args *args, void *stream);
 int dsalt_gated_ffn_check(const dsalt_gated_ffn_args *args, int32_t backward);
 int64_t dsalt_gated_ffn_workspace_size(int64_t rows, int32_t d, int32_t f, int32_t e, int32_t backward);
+int64_t dsalt_gated_ffn_kept_size(int64_t rows, int32_t f, int32_t dtype);
 size_t dsalt_gated_ffn_args_size(void);
 
 /*
