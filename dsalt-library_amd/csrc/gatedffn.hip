@@ -376,7 +376,14 @@ __global__ void __launch_bounds__(64) ffn_join_kernel(const FfnParams p) {
 // Few rows (up to 16 TT): bound by the weights' bytes, and by the latency of a call this short.
 // A workgroup takes 16 weight rows (pair: the same 8 of both weights) and all rows of x; its waves
 // take every NW-th 32 of k straight from memory into the operands of v_mfma_f32_16x16x32, so that
-// nothing waits on LDS until their sums are added there, in order.
+// nothing waits on LDS until their sums are added there, in order. Every workgroup reads all of x,
+// so that its time grows with the rows while the tiles' stays; the two products took (bf16, us,
+// weights from memory; tiles with the join of their split)
+//     d, f            1 row   16 rows   32 rows   64 rows   tiles, 1 to 64 rows
+//     1024, 2816       12.0      14.8      19.9      28.5   25
+//     2048, 5504                           40.4      61.1   49
+//     4096, 11008                86.3               179.7   91
+// 1 row: 17.3 MB of weights, 1.4 TB/s; a launch of nothing takes 2 us of each 6.
 template <class DT>
 __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
     if constexpr (std::is_same<DT, BF16>::value)
@@ -385,7 +392,7 @@ __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
 }
 
-constexpr int kFewRows = 64, kFewUnroll = 4;
+constexpr int kFewRows = 32, kFewUnroll = 4;
 template <class DT, int TT, int NW, int EPI>
 __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const FfnParams p) {
     constexpr bool PAIR = EPI == kEpiPair;
@@ -464,8 +471,7 @@ hipError_t launch_few(const FfnParams &p, hipStream_t stream) {
     const Product &q = p.prod[0];
     const dim3 grid((unsigned)((q.n + (EPI == kEpiPair ? 7 : 15)) / (EPI == kEpiPair ? 8 : 16))), block(NW * 64);
     if (q.m <= 16) hipLaunchKernelGGL((ffn_few_kernel<DT, 1, NW, EPI>), grid, block, 0, stream, p);
-    else if (q.m <= 32) hipLaunchKernelGGL((ffn_few_kernel<DT, 2, NW, EPI>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((ffn_few_kernel<DT, 4, NW, EPI>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((ffn_few_kernel<DT, 2, NW, EPI>), grid, block, 0, stream, p);
     return hipGetLastError();
 }
 
@@ -476,14 +482,20 @@ hipError_t launch_few(const FfnParams &p, hipStream_t stream) {
 // (a CU alone has more of the caches, of the memory and of the power budget), and the share of
 // the epilogue's bytes, at kMemory, that nothing else runs under (one of two workgroups on a CU
 // computes while the other stores). Measured with each shape forced (bf16, us; largest is
-// 16384 rows, d 2048, f 5504, ragged 6473, 1024, 2816):
-//                     256 x 256   256 x 128   128 x 128
-//   largest, gate|up        754         911         917
-//   largest, down           341         409         410
-//   largest, da             528         540         561
-//   ragged,  down            73          51          55
-//   ragged,  da             104          88          78
-//   ragged,  dx              89 + 14    106         109
+// 16384 rows, d 2048, f 5504, ragged 6473, 1024, 2816, small 300, 512, 1408; + the join):
+//                     256 x 256   256 x 128   128 x 128    64 x 128
+//   largest, gate|up        822        1016        1003        1061
+//   largest, down           371         424         424         493
+//   largest, da             534         546         561         570
+//   largest, dx             688         807         820        1045
+//   ragged,  gate|up        122         127         116         130
+//   ragged,  down            74          53          57          61 + 6
+//   ragged,  da             107          93          83          80
+//   ragged,  dx              92 + 17    109         114         124 + 6
+//   ragged,  weights        162         140 + 7     135 + 7     176 + 9
+//   small,   gate|up         24          16          14          11
+//   small,   da              33          19          18          12
+//   small,   dx              16 + 9      14 + 5      11 + 5      10 + 6
 struct Plan {
     int shape, whole, split, tiles;
     int64_t part_bytes;
