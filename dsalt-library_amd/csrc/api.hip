@@ -671,8 +671,9 @@ int dsalt_gated_ffn_check(const dsalt_gated_ffn_args *a, int32_t backward) {
         if (s.used && (s.stride < s.row || s.stride % 8 || s.stride > dsalt::gated_ffn_max_ld()))
             return fail(DSALT_ERR_UNSUPPORTED, "%s row stride must be a multiple of 8 in [%lld, 2^21] (got %lld)", s.name,
                         (long long)s.row, (long long)s.stride);
-    const int64_t tiles = ((a->rows + 127) / 128 + 1) * ((std::max(std::max(a->d, a->f), a->e) + 63) / 64 + 1);
-    if (tiles >= (int64_t)1 << 30) return fail(DSALT_ERR_UNSUPPORTED, "rows * width is too large");
+    if (!dsalt::gated_ffn_fits(a->rows, a->d, a->f, a->e, backward != 0))
+        return fail(DSALT_ERR_UNSUPPORTED, "a product of more than 2^22 tiles of 256 x 128 (rows %lld, d, f, e %d, %d, %d)",
+                    (long long)a->rows, a->d, a->f, a->e);
     for (const void *q : {a->x, a->w_gate, a->w_up, a->w_down, (const void *)a->gate_up, (const void *)a->act, (const void *)a->y,
                           a->dy, (const void *)a->d_gate_up, (const void *)a->dx, (const void *)a->dw_gate,
                           (const void *)a->dw_up, (const void *)a->dw_down, (const void *)a->workspace})

@@ -511,6 +511,7 @@ constexpr ShapeCost kShapes[] = {
     {64, 128, 768, 1.00, 0.38, 0.4},
 };
 constexpr int kShapeCount = 4, kMaxSplit = 8;
+constexpr int64_t kMaxTiles = 1 << 22;  // of one launch: with up to 512 threads each, half of what a grid may hold
 constexpr double kTile = 3.0, kJoin = 6.0, kMemory = 5.0e6, kPartials = 3.0e6;  // us, us, bytes per us
 
 int64_t tiles_of(int64_t m, int64_t n, int shape, bool pair) {
@@ -531,6 +532,7 @@ Plan plan(const Extent *e, int count, int64_t k, int segments, bool pair, int io
         int64_t tiles = 0;
         for (int z = 0; z < count; ++z) tiles += tiles_of(e[z].m, e[z].n, s, pair);
         if (tiles == 0) return best;
+        if (tiles > kMaxTiles) continue;  // not of the largest tile: gated_ffn_fits()
         const double out = (double)c.bm * c.bn / (pair ? 2 : 1) * io * c.bare / kMemory;  // us per workgroup of a round
         const int64_t rounds = tiles / c.slots, rest = tiles - rounds * c.slots;
         const int most = rest ? (int)std::min<int64_t>(std::min<int64_t>(c.slots / rest, kMaxSplit), steps / 4) : 1;
@@ -696,6 +698,13 @@ int64_t gated_ffn_workspace_bytes(int64_t rows, int d, int f, int e, bool bwd) {
         for (int count = 1; first + count <= 3; ++count)
             most = std::max(most, plan(dw + first, count, rows, 1, false, kIoStore).part_bytes);
     return most;
+}
+
+bool gated_ffn_fits(int64_t rows, int d, int f, int e, bool bwd) {
+    const auto tiles = [](int64_t m, int64_t n, bool pair) { return tiles_of(m, n, 0, pair); };
+    if (!bwd) return tiles(rows, f, true) <= kMaxTiles && tiles(rows, e, false) <= kMaxTiles;
+    return tiles(rows, f, false) <= kMaxTiles && tiles(rows, d, false) <= kMaxTiles &&
+           2 * tiles(f, d, false) + tiles(e, f, false) <= kMaxTiles;
 }
 
 int64_t gated_ffn_kept_bytes(int64_t rows, int f, int dtype) {

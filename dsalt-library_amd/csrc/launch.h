@@ -76,6 +76,7 @@ int64_t norm_train_workspace_bytes(int64_t rows, int d);
 hipError_t launch_gated_ffn(const dsalt_gated_ffn_args &a, hipStream_t stream);
 hipError_t launch_gated_ffn_bwd(const dsalt_gated_ffn_args &a, hipStream_t stream);
 int64_t gated_ffn_workspace_bytes(int64_t rows, int d, int f, int e, bool backward);
+bool gated_ffn_fits(int64_t rows, int d, int f, int e, bool bwd);
 int64_t gated_ffn_kept_bytes(int64_t rows, int f, int dtype);
 int64_t gated_ffn_max_ld();
 hipError_t launch_dropout(const dsalt_dropout_args &a, hipStream_t stream);

@@ -629,7 +629,8 @@ int dsalt_lmk_weights_check(const dsalt_lmk_weights_args *args, int32_t backward
  * rows = 0 gives zero weight gradients.
  * dtype BF16 or F16 for every tensor. d, e, f multiples of 8 in [8, 2^20]; row strides (in
  * elements) multiples of 8 up to 2^21 and at least the row length, the other tensors contiguous;
- * 16-byte aligned pointers; outputs alias no input. workspace: at least
+ * 16-byte aligned pointers; outputs alias no input; products of up to 2^22 tiles of 256 x 128
+ * (rows up to 2^30, rows * f up to 2^37). workspace: at least
  * dsalt_gated_ffn_workspace_size bytes, 16-byte aligned, dead when the launches end (NULL where
  * that is 0).
  * Replaces SwiGLUFFN.forward (dsalt/modules/dsalt_transformer.py:10-21) with its autograd.

@@ -14,9 +14,10 @@ def philox4x32(counter, key, rounds):
     return c
 
 
-def keep_mask(n, p, seed, offset):
-    """Whether each of n elements is kept: 16 bits of the stream below round((1 - p) 65536)."""
-    j = np.arange(-(-n // 8), dtype=np.uint64)
+def keep_mask(n, p, seed, offset, first=0):
+    """Whether each of n elements from element 8 first on is kept: 16 bits of the stream below
+    round((1 - p) 65536)."""
+    j = np.arange(first, first - (-n // 8), dtype=np.uint64)
     lo = np.uint64(0xFFFFFFFF)
     words = philox4x32((j & lo, j >> np.uint64(32), np.full_like(j, offset & 0xFFFFFFFF), np.full_like(j, offset >> 32)),
                        (seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF), 7)

@@ -124,6 +124,26 @@ def test_leading_dimensions_strides_and_alignment():
             assert all(torch.equal(got[1][k], want[1][k]) for k in want[1])
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 elements and 2^32 bytes a tensor: rows at both ends equal those of a call of
+    their own."""
+    rows, d = 262207, 8192
+    print(f"branch_norm {rows}x{d}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x, h, dz, dy = (torch.randn(rows, d, device=DEV, generator=g, dtype=BF) for _ in range(4))
+    w, post, gate = (torch.rand(s, device=DEV, generator=g) for s in ((d,), (d,), (rows, 1)))
+
+    def call(at):
+        t = {"x": x[at], "h": h[at], "weight": w, "post_weight": post, "gate": gate[at]}
+        outs, grads = run(t, dz[at], dy[at], residual_scale=0.75)
+        return [*outs, grads["x"], grads["h"], grads["gate"]]
+
+    whole = call(slice(None))
+    for at in (slice(0, 5), slice(rows - 70, rows)):
+        for n, a, b in zip(("x_out", "y", "dx", "dh", "dgate"), whole, call(at)):
+            assert torch.equal(a[at], b), (n, at)
+
+
 def test_no_rows():
     t, dz, dy = inputs((0,), 64, FP, BF, BF)
     outs, grads = run(t, dz, dy, out_dtype=BF)

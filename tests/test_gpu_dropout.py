@@ -30,6 +30,19 @@ def test_values(n, dtype):
         assert torch.equal(counter_dropout(x, p, seed, offset), want(x, p, seed, offset)), (p, seed, offset)
 
 
+def test_offsets_past_32_bits():
+    """More than 2^32 elements: pieces on both sides of 2^31 and 2^32, and the odd end."""
+    n = 2 ** 32 + 2 ** 20 + 5
+    print(f"dropout {n}", flush=True)
+    y = counter_dropout(torch.ones(n, device=DEV, dtype=BF), 0.25, 11, 3)
+    for at, size in ((0, 4096), (2 ** 31 - 2048, 4096), (2 ** 32 - 2048, 4096), (2 ** 32 + 2 ** 20 - 2043, 2048)):
+        first = at // 8 * 8
+        keep = keep_mask(at + size - first, 0.25, 11, 3, first // 8)[at - first:]
+        want = torch.from_numpy(keep).to(DEV).to(BF) * (1 / 0.75)
+        assert torch.equal(y[at:at + size], want.to(BF)), at
+    assert y[at + size:].numel() == 0
+
+
 def test_gradient_is_the_same_mask():
     x = torch.randn(33, 77, device=DEV, requires_grad=True)
     dy = torch.randn(33, 77, device=DEV)

@@ -130,6 +130,24 @@ def test_larger(rows, d, f):
         check(gated_ffn(x, wg, wu, wd), ref["y"], dtype, "y without a graph")
 
 
+def test_offsets_past_32_bits():
+    """Every buffer of rows and hidden columns is larger than 2^32 bytes: the last rows against
+    float64, and the weights' gradients, by their norm, against float64 sums over pieces."""
+    rows, d, f, piece = 270001, 64, 8192, 4096
+    print(f"gated_ffn {rows} x {d} x {f}", flush=True)
+    x, wg, wu, wd, dy = inputs(rows, d, f, d, BF)
+    got = run(x, wg, wu, wd, dy, "silu")
+    last = reference(x[-257:], wg, wu, wd, dy[-257:], "silu", BF)
+    check(got["y"][-257:], last["y"], BF, "y")
+    check(got["dx"][-257:], last["dx"], BF, "dx")
+    want = {n: 0 for n in ("dwg", "dwu", "dwd")}
+    for i in range(0, rows, piece):
+        ref = reference(x[i:i + piece], wg, wu, wd, dy[i:i + piece], "silu", BF)
+        want = {n: w + ref[n][0] for n, w in want.items()}
+    for n, w in want.items():
+        assert float((got[n].double() - w).norm()) <= torch.finfo(BF).eps * float(w.norm()), n
+
+
 def test_against_differences():
     """dx against central differences of the float64 function along random directions: the
     difference is off by h^2 / 6 of its third derivative, the gradient by its roundings."""

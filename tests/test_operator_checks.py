@@ -56,6 +56,17 @@ def test_gated_ffn_backward_check(kw, code):
     assert hip.lib().dsalt_gated_ffn_check(ctypes.byref(ffn_args(**kw)), 1) == code, hip.lib().dsalt_last_error()
 
 
+@pytest.mark.parametrize("kw,backward,code", [
+    ({"rows": 1 << 30, "f": 8, "w_down_stride": 8}, 0, 0), ({"rows": (1 << 30) + 1, "f": 8, "w_down_stride": 8}, 0, 2),
+    ({"rows": (1 << 30) + 1, "f": 8, "w_down_stride": 8}, 1, 2), ({"rows": 1 << 23, "f": 1 << 14, "w_down_stride": 1 << 14}, 0, 0),
+    ({"rows": (1 << 23) + 1, "f": 1 << 14, "w_down_stride": 1 << 14}, 0, 2), ({"rows": 8, "f": 1 << 20, "w_down_stride": 1 << 20}, 1, 0),
+    ({"rows": 8, "f": 1 << 20, "d": 1 << 17, "x_stride": 1 << 17, "w_gate_stride": 1 << 17, "w_up_stride": 1 << 17,
+      "w_down_stride": 1 << 20}, 1, 2)])
+def test_gated_ffn_grids_that_a_launch_cannot_hold(kw, backward, code):
+    """A launch holds fewer than 2^32 threads: what would need more is refused."""
+    assert hip.lib().dsalt_gated_ffn_check(ctypes.byref(ffn_args(**kw)), backward) == code, hip.lib().dsalt_last_error()
+
+
 def test_gated_ffn_workspace_check():
     need = hip.lib().dsalt_gated_ffn_workspace_size(32, 64, 128, 64, 1)
     assert need >= 0 and hip.lib().dsalt_gated_ffn_workspace_size(-1, 64, 128, 64, 1) == 0
