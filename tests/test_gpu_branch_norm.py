@@ -288,3 +288,35 @@ def test_refusals_on_gpu():
     for kw in ({"p": 0.1}, {"p": -1.0}, {"p": 0.1, "seed": 1, "offset": -1}):
         with pytest.raises(ValueError):
             branch_norm(x, h, **kw)
+
+
+@pytest.mark.parametrize("only", ["x_out", "y"])
+def test_second_order_of_one_output(only):
+    """A graph of the backward where one output has no gradient: float64's double backward, through
+    fp32 operations (2^-18 of the largest value, as close() counts them, twice over)."""
+    t, dz, dy = inputs((6,), 64, FP, FP, FP)
+    up = dz if only == "x_out" else dy
+    res = []
+    for dt in (FP, torch.float64):
+        w = {n: v.detach().to(dt).requires_grad_() for n, v in t.items()}
+        if dt is FP:
+            x_out, y = branch_norm(w["x"], w["h"], w["weight"], post_weight=w["post_weight"], gate=w["gate"], residual_scale=0.5)
+        else:
+            n = w["h"] * torch.rsqrt(w["h"].square().mean(-1, keepdim=True) + 1e-6) * w["post_weight"]
+            x_out = 0.5 * w["x"] + w["gate"] * n
+            y = x_out * torch.rsqrt(x_out.square().mean(-1, keepdim=True) + 1e-6) * w["weight"]
+        first, = torch.autograd.grad(x_out if only == "x_out" else y, w["h"], up.to(dt), create_graph=True)
+        res.append(torch.autograd.grad(first.square().sum(), (w["h"], w["post_weight"])))
+    for a, b in zip(*res):
+        assert bool(((a.double() - b).abs() <= 2.0 ** -17 * b.abs().max()).all())
+
+
+def test_stream_and_branch_one_tensor():
+    """x given as h too: its gradient is the sum of both."""
+    t, dz, dy = inputs((5,), 72, BF, BF, BF)
+    x = t["x"].clone().requires_grad_()
+    outs = branch_norm(x, x, t["weight"], gate=t["gate"])
+    got, = torch.autograd.grad(outs, x, (dz, dy))
+    two = {n: t["x"].clone().requires_grad_() for n in ("x", "h")}
+    parts = torch.autograd.grad(branch_norm(two["x"], two["h"], t["weight"], gate=t["gate"]), (two["x"], two["h"]), (dz, dy))
+    assert torch.equal(got, parts[0] + parts[1])

@@ -133,3 +133,12 @@ def test_refusals_on_gpu():
     for seed, offset in ((None, 0), (2 ** 64, 0), (-2 ** 63 - 1, 0), (1, -1), (1, 2 ** 63)):
         with pytest.raises(ValueError):
             counter_dropout(x, 0.1, seed, offset)
+
+
+def test_scalars_and_no_elements():
+    x = torch.full((), 2.0, device=DEV)
+    assert torch.equal(counter_dropout(x, 0.5, 3), want(x, 0.5, 3, 0)) and counter_dropout(x, 0.5, 3).shape == ()
+    empty = torch.zeros(4, 0, 8, device=DEV, dtype=BF, requires_grad=True)
+    y = counter_dropout(empty, 0.5, 3)
+    g, = torch.autograd.grad(y, empty, torch.zeros_like(y))
+    assert y.shape == g.shape == (4, 0, 8)

@@ -339,3 +339,47 @@ def test_refusals_on_gpu():
             gated_ffn(*args)
     with pytest.raises(ValueError, match="activation"):
         gated_ffn(x, wg, wu, wd, activation="tanh")
+
+
+@pytest.mark.parametrize("rows", [5, 150])
+def test_one_tensor_in_several_places_and_two_backwards(rows):
+    """x a row, w_gate used as w_up and w_down too: the gradients add up; a graph kept for a second
+    backward gives the same."""
+    x, wg, _, _, dy = inputs(rows, 64, 64, 64, HF, seed=2)
+    print(f"gated_ffn one weight three times {rows}", flush=True)
+    apart = run(x, wg, wg, wg, dy, "silu")
+    a, w = x.clone().requires_grad_(), wg.clone().requires_grad_()
+    y = gated_ffn(a, w, w, w)
+    first = torch.autograd.grad(y, (a, w), dy, retain_graph=True)
+    second = torch.autograd.grad(y, (a, w), dy)
+    assert torch.equal(y, apart["y"]) and torch.equal(first[0], apart["dx"])
+    assert all(torch.equal(p, q) for p, q in zip(first, second))
+    total = apart["dwg"].double() + apart["dwu"].double() + apart["dwd"].double()
+    # autograd's two additions in fp16: a half-step each, of sums within the magnitudes' sum
+    bound = 2 * 2.0 ** -11 * 1.01 * sum(apart[n].double().abs() for n in ("dwg", "dwu", "dwd")) + 2.0 ** -24
+    assert bool(((first[1].double() - total).abs() <= bound).all())
+    one = gated_ffn(x[0], wg, wg, wg)
+    assert one.shape == (64,) and torch.equal(one, gated_ffn(x[:1], wg, wg, wg)[0])
+
+
+def test_two_graphs_and_eager_calls_in_turn():
+    """Two captured forward passes of unlike sizes (split products, so that each has a workspace),
+    replayed in turn with eager calls between."""
+    cases = [inputs(300, 512, 1408, 512, BF), inputs(90, 1024, 2816, 1024, BF)]
+    graphs, outs = [], []
+    with torch.no_grad():
+        want = [gated_ffn(x, wg, wu, wd) for x, wg, wu, wd, _ in cases]
+        for x, wg, wu, wd, _ in cases:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                outs.append(gated_ffn(x, wg, wu, wd))
+            graphs.append(g)
+        for turn in range(4):
+            print(f"gated_ffn replay {turn}", flush=True)
+            for i in (0, 1) if turn % 2 else (1, 0):
+                outs[i].zero_()
+                graphs[i].replay()
+                x, wg, wu, wd, _ = cases[1 - i]
+                assert torch.equal(gated_ffn(x, wg, wu, wd), want[1 - i])
+            for got, ref in zip(outs, want):
+                assert torch.equal(got, ref)
