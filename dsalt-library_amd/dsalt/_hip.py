@@ -1475,7 +1475,7 @@ def _rows_aligned(*ts: torch.Tensor | None) -> bool:
 
 def aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """t itself when it is contiguous and 16-byte aligned, otherwise a copy that is."""
-    return t if _rows_aligned(t) else t.clone(memory_format=torch.contiguous_format)
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def norm_train_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:

@@ -66,8 +66,8 @@ class _BranchNorm(torch.autograd.Function):
 
 def _operands(x, h, weight, post_weight, gate):
     rows = _hip.aligned_rows
-    return (rows(x.detach()), rows(h.detach()), None if weight is None else rows(weight.detach()),
-            None if post_weight is None else rows(post_weight.detach()), None if gate is None else rows(gate.detach()))
+    return (rows(x), rows(h), None if weight is None else rows(weight), None if post_weight is None else rows(post_weight),
+            None if gate is None else rows(gate))
 
 
 def _weight_ok(w, d: int, dtype: torch.dtype, dev: torch.device) -> bool:

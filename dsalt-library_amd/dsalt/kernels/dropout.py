@@ -34,7 +34,7 @@ class _Dropout(torch.autograd.Function):
         is_tensor = isinstance(seed, torch.Tensor)
         ctx.save_for_backward(seed if is_tensor else None)
         ctx.dsalt = p, None if is_tensor else seed, offset
-        return _hip.dropout(_hip.aligned_rows(x.detach()), p, seed, offset)
+        return _hip.dropout(_hip.aligned_rows(x), p, seed, offset)
 
     @staticmethod
     def backward(ctx, dy):

@@ -61,8 +61,8 @@ class _GatedFFN(torch.autograd.Function):
 
 def _run(x, w_gate, w_up, w_down, activation, keep):
     row = _hip.row_operand
-    return _hip.gated_ffn(row(x.detach() if x.dim() == 2 else x.detach().reshape(-1, x.shape[-1])), row(w_gate.detach()),
-                          row(w_up.detach()), row(w_down.detach()), activation, x.shape[:-1], keep)
+    return _hip.gated_ffn(row(x if x.dim() == 2 else x.reshape(-1, x.shape[-1])), row(w_gate), row(w_up), row(w_down),
+                          activation, x.shape[:-1], keep)
 
 
 def gated_ffn_supported(x, w_gate, w_up, w_down) -> bool:
