@@ -392,10 +392,13 @@ __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
 }
 
-constexpr int kFewRows = 32, kFewUnroll = 4;
+constexpr int kFewRows = 32;
 template <class DT, int TT, int NW, int EPI>
 __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const FfnParams p) {
     constexpr bool PAIR = EPI == kEpiPair;
+    // weight loads in flight a lane: gate and up of d 4096, f 11008 took 36.0 us with 8, 40.8 with 4 (5.0
+    // TB/s); 32 rows' registers hold 4, and gained nothing from more
+    constexpr int UNROLL = TT == 1 ? 8 : 4;
     __shared__ float4 part[NW][TT][64];
     const Product &q = p.prod[0];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15;
@@ -415,10 +418,10 @@ __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const FfnParams p) {
     f32x4 acc[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = wave * 32; k0 < k; k0 += NW * 32 * kFewUnroll) {
-        uint4 wv[kFewUnroll], xv[kFewUnroll][TT];
+    for (int k0 = wave * 32; k0 < k; k0 += NW * 32 * UNROLL) {
+        uint4 wv[UNROLL], xv[UNROLL][TT];
 #pragma unroll
-        for (int s = 0; s < kFewUnroll; ++s) {
+        for (int s = 0; s < UNROLL; ++s) {
             const int at = k0 + s * NW * 32;
             const bool in = at + kl < k;
             wv[s] = in && win ? *reinterpret_cast<const uint4 *>(w + at * 2) : make_uint4(0, 0, 0, 0);
@@ -427,7 +430,7 @@ __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const FfnParams p) {
                 xv[s][t] = in && xin[t] ? *reinterpret_cast<const uint4 *>(x[t] + at * 2) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int s = 0; s < kFewUnroll; ++s)
+        for (int s = 0; s < UNROLL; ++s)
 #pragma unroll
             for (int t = 0; t < TT; ++t) acc[t] = mfma16<DT>(wv[s], xv[s][t], acc[t]);
     }
