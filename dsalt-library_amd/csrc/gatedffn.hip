@@ -499,6 +499,8 @@ hipError_t launch_few(const FfnParams &p, hipStream_t stream) {
 //   small,   gate|up         24          16          14          11
 //   small,   da              33          19          18          12
 //   small,   dx              16 + 9      14 + 5      11 + 5      10 + 6
+// A split costs a join of 5 to 6 us, less what it saves: dx of 575, 264, 712 takes 17.2 us whole and 13.6 in
+// pieces, of 3000, 768, 2048 50.4 and 37.5, down of 1500, 1024, 2816 27.9 and 24.6.
 struct Plan {
     int shape, whole, split, tiles;
     int64_t part_bytes;
@@ -509,13 +511,13 @@ struct ShapeCost {
 };
 constexpr ShapeCost kShapes[] = {
     {256, 256, 256, 1.85, 1.20, 1.0},
-    {256, 128, 256, 1.05, 0.65, 1.0},
-    {128, 128, 512, 1.17, 0.50, 0.5},
-    {64, 128, 768, 1.00, 0.38, 0.4},
+    {256, 128, 256, 1.05, 0.80, 1.0},
+    {128, 128, 512, 1.17, 0.60, 0.5},
+    {64, 128, 768, 1.00, 0.50, 0.4},
 };
 constexpr int kShapeCount = 4, kMaxSplit = 8;
 constexpr int64_t kMaxTiles = 1 << 22;  // of one launch: with up to 512 threads each, half of what a grid may hold
-constexpr double kTile = 3.0, kJoin = 6.0, kMemory = 5.0e6, kPartials = 3.0e6;  // us, us, bytes per us
+constexpr double kTile = 3.0, kJoin = 4.0, kMemory = 5.0e6, kPartials = 4.0e6;  // us, us, bytes per us
 
 int64_t tiles_of(int64_t m, int64_t n, int shape, bool pair) {
     const int bn = kShapes[shape].bn / (pair ? 2 : 1);

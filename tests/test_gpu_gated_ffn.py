@@ -130,6 +130,14 @@ def test_larger(rows, d, f):
         check(gated_ffn(x, wg, wu, wd), ref["y"], dtype, "y without a graph")
 
 
+# and those that the plan's constants, refitted, moved to other shapes or splits
+@pytest.mark.parametrize("rows,d,f", [
+    (9680, 2024, 400), (8080, 152, 3256), (9408, 200, 3840), (8361, 424, 3576), (1627, 1192, 3728), (3415, 2376, 608),
+    (1500, 512, 1408), (3000, 768, 2048)])
+def test_larger_splits(rows, d, f):
+    test_larger(rows, d, f)
+
+
 def test_offsets_past_32_bits():
     """Every buffer of rows and hidden columns is larger than 2^32 bytes: the last rows against
     float64, and the weights' gradients, by their norm, against float64 sums over pieces."""
