@@ -188,7 +188,8 @@ enum { kEpiPair, kEpiStore, kEpiGrad };
 // g and u of a tile's elements, in the epilogue's pieces, loaded kAhead turns before they are used:
 // one after the other they would cost a trip to memory for every 16 bytes of a lane. (All of
 // them loaded as the product starts, where the registers hold them, measured no faster.)
-// Bounds by descriptor: the largest size's da took 528 us with addresses and bounds per lane, 497 so.
+// Bounds by descriptor: the largest size's da took 528 us with addresses and bounds per lane, 497 so
+// (g and u of 16 bits; 534 as they are kept).
 constexpr int kAhead = 3;
 template <class DT, class Core>
 struct GateUp {
