@@ -33,10 +33,10 @@ struct GemmOperand {
 // One operand's tile: ROWS rows of r, BK of k, filled by NW waves.
 //
 // LDS has 64 banks of 4 bytes, and a 16-byte read serves 16 lanes at a time: the swizzle puts the
-// same chunk of 16 consecutive rows on 16 different places of 256 bytes (two rows of BK = 64, four
-// of BK = 32): 4.2 clocks a read, against 8.3 with chunk ^ (row & 7), which spreads 8 rows. A
-// transposing read takes 32 bytes of each of four rows, which go to four different 64-byte places
-// (32-byte places where a row has only 128 bytes): 2.9 clocks, 4.2 with 32-byte places, 8 without.
+// same chunk of 16 consecutive rows on 16 different places of 256 bytes (two rows of 64): 4.2
+// clocks a read, against 8.3 with chunk ^ (row & 7), which spreads 8 rows. A transposing read
+// takes 32 bytes of each of four rows, which go to four different 64-byte places (32-byte
+// places where a row has only 128 bytes): 2.9 clocks, 4.2 with 32-byte places, 8 without.
 template <int LAY, int ROWS, int BK, int NW>
 struct GemmTile {
     static constexpr int BYTES = ROWS * BK * 2;
@@ -44,11 +44,11 @@ struct GemmTile {
     static constexpr int CPR = LAY == kKContig ? BK / 8 : ROWS / 8;  // chunks per LDS row
     static constexpr int RPL = 64 / CPR;                             // LDS rows per load instruction
     static_assert(BYTES % (16 * 64 * NW) == 0, "the waves cover the tile");
-    static_assert(CPR >= (LAY == kKContig ? BK / 8 : 8), "a swizzle stays inside its row");
+    static_assert(CPR == 8 || (LAY == kRContig && CPR > 8), "a swizzle stays inside its row");
 
     static __device__ __forceinline__ int swizzle(int row) {
         if constexpr (LAY == kRContig) return (row & 3) << (CPR >= 16 ? 2 : 1);
-        else return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+        else return (row >> 1) & 7;
     }
 
     uint32_t off[2];  // of a wave's even and odd loads
@@ -313,15 +313,6 @@ struct GemmCore {
 template <class DT>
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
     return make_uint4(DT::pack2(v[0], v[1]), DT::pack2(v[2], v[3]), DT::pack2(v[4], v[5]), DT::pack2(v[6], v[7]));
-}
-template <class DT>
-__device__ __forceinline__ void unpack8(uint4 w, float (&v)[8]) {
-    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[2 * e] = DT::lo_f32(q[e]);
-        v[2 * e + 1] = DT::hi_f32(q[e]);
-    }
 }
 
 }  // namespace dsalt
