@@ -202,3 +202,66 @@ def test_lm_inference_takes_the_next_norms_along(dtype):
             assert bool(((h.double() - want).abs() <= (4 * u + 2.0 ** -20) * want.abs() + 2.0 ** -18).all())
         assert torch.equal(got, m.lm_head(h))
         assert torch.equal(got, m(ids, cu_seqlens=cu, max_seqlen=256)["logits"])
+
+
+def test_lm_inference_in_a_graph():
+    """The LM with every option, captured and replayed over new tokens, with eager calls between."""
+    m = lm().to(BF).eval()
+    m.set_collect_last_P(False)
+    cu = torch.tensor(CU, dtype=torch.int32, device=DEV)
+    batches = [torch.randint(0, 500, (CU[-1],), device=DEV) for _ in range(4)]
+    ids = batches[0].clone()
+    with torch.no_grad():
+        want = [m(b, cu_seqlens=cu, max_seqlen=256)["logits"] for b in batches]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            m(ids, cu_seqlens=cu, max_seqlen=256)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(ids, cu_seqlens=cu, max_seqlen=256)["logits"]
+        for i, b in enumerate(batches):
+            print(f"lm graph replay {i}", flush=True)
+            ids.copy_(b)
+            graph.replay()
+            assert torch.equal(out, want[i])
+            assert torch.equal(m(batches[i - 1], cu_seqlens=cu, max_seqlen=256)["logits"], want[i - 1])
+
+
+def test_counter_dropout_draws_anew_on_every_replay():
+    m = CounterDropout(0.25).train()
+    x = torch.ones(4096, device=DEV)
+    m(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m(x)
+    seen = []
+    for i in range(4):
+        print(f"dropout replay {i}", flush=True)
+        graph.replay()
+        seen.append(out.clone())
+        m(x)  # an eager draw between
+        # 4096 draws of a share of 3/4: five standard deviations of sqrt(3 / 16 / 4096)
+        assert abs(float((out != 0).float().mean()) - 0.75) <= 5 * (3 / 16 / 4096) ** 0.5
+    assert all(not torch.equal(a, b) for i, a in enumerate(seen) for b in seen[:i])
+
+
+def test_unpacked_input_and_odd_widths():
+    """[1, T, d] input (whose attention takes no dropout of its own); a hidden width that the fused
+    feed-forward does not take runs as separate projections."""
+    for d_ff in (264, 260):
+        torch.manual_seed(5)
+        b = DSALTTransformerBlock(128, 2, 4, 40, 4, 256, d_ff, dropout=0.0, layer_idx=1, **OPTIONS).to(DEV, BF).train()
+        b.ffn.drop.p = 0.1
+        x = torch.randn(1, 150, 128, device=DEV, dtype=BF, requires_grad=True)
+        res = []
+        for checkpoint in (False, True):
+            torch.manual_seed(9)
+            y, _ = b(x, gradient_checkpointing=checkpoint)
+            res.append((y, *torch.autograd.grad(y.float().square().sum(), [x, *b.parameters()], allow_unused=True)))
+        assert y.shape == x.shape
+        for p, q in zip(*res):
+            assert (p is None and q is None) or (torch.isfinite(p).all() and torch.equal(p, q))
+        missing = [n for (n, _), g in zip(b.named_parameters(), res[0][2:]) if g is None]
+        assert not [n for n in missing if "ffn" in n or "gate" in n and "win" not in n or "norm" in n], missing
