@@ -508,17 +508,17 @@ struct Plan {
 };
 struct ShapeCost {
     int bm, bn, slots;  // workgroups that run at a time
-    double busy, alone, bare;
+    double busy, alone, bare, tile;  // tile: us of a tile besides its k-steps and bytes
 };
 constexpr ShapeCost kShapes[] = {
-    {256, 256, 256, 1.85, 1.20, 1.0},
-    {256, 128, 256, 1.05, 0.80, 1.0},
-    {128, 128, 512, 1.17, 0.60, 0.5},
-    {64, 128, 768, 1.00, 0.50, 0.4},
+    {256, 256, 256, 1.85, 1.20, 1.0, 4.0},
+    {256, 128, 256, 1.05, 0.80, 1.0, 3.0},
+    {128, 128, 512, 1.17, 0.60, 0.6, 3.0},
+    {64, 128, 768, 1.00, 0.50, 0.4, 3.0},
 };
 constexpr int kShapeCount = 4, kMaxSplit = 8;
 constexpr int64_t kMaxTiles = 1 << 22;  // of one launch: with up to 512 threads each, half of what a grid may hold
-constexpr double kTile = 3.0, kJoin = 4.0, kMemory = 5.0e6, kPartials = 4.0e6;  // us, us, bytes per us
+constexpr double kJoin = 4.0, kMemory = 5.0e6, kPartials = 4.0e6;  // us, bytes per us twice
 
 int64_t tiles_of(int64_t m, int64_t n, int shape, bool pair) {
     const int bn = kShapes[shape].bn / (pair ? 2 : 1);
@@ -543,10 +543,10 @@ Plan plan(const Extent *e, int count, int64_t k, int segments, bool pair, int io
         const int64_t rounds = tiles / c.slots, rest = tiles - rounds * c.slots;
         const int most = rest ? (int)std::min<int64_t>(std::min<int64_t>(c.slots / rest, kMaxSplit), steps / 4) : 1;
         for (int split = 1; split <= std::max(most, 1); ++split) {
-            double t = rounds * (steps * c.busy + kTile + out * c.slots);
+            double t = rounds * (steps * c.busy + c.tile + out * c.slots);
             const double busy = (double)rest * split / c.slots, bytes = split > 1 ? (double)rest * split * c.bm * c.bn * 4 : 0;
             if (rest) {
-                t += (steps + split - 1) / split * (c.alone + (c.busy - c.alone) * busy) + kTile;
+                t += (steps + split - 1) / split * (c.alone + (c.busy - c.alone) * busy) + c.tile;
                 t += split > 1 ? kJoin + 2 * bytes / kPartials : out * rest;
             }
             if (best.tiles == 0 || t < least) {
