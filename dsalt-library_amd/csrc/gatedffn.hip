@@ -18,7 +18,6 @@
 namespace dsalt {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
@@ -189,7 +188,7 @@ enum { kEpiPair, kEpiStore, kEpiGrad };
 // one after the other they would cost a trip to memory for every 16 bytes of a lane. (All of
 // them loaded as the product starts, where the registers hold them, measured no faster.)
 // Bounds by descriptor: the largest size's da took 528 us with addresses and bounds per lane, 497 so
-// (g and u of 16 bits; 534 as they are kept).
+// (g and u of 16 bits; 512 as they are kept now).
 constexpr int kAhead = 3;
 template <class DT, class Core>
 struct GateUp {
@@ -227,7 +226,7 @@ struct GateUp {
 // product of a pair, a plain store, or the gradients of gate and up from that of the product.
 template <class DT, class Core, int EPI, int ROWS>
 __device__ __forceinline__ void epilogue(const FfnParams &p, const Product &q, const Core &c,
-                                         const f32x16 (&acc)[ROWS][Core::FN], int first, int64_t m0, int64_t n0, char *lds) {
+                                         const f32x4 (&acc)[ROWS][Core::FN][4], int first, int64_t m0, int64_t n0, char *lds) {
     constexpr int WIDTH = EPI == kEpiPair ? Core::COLS / 2 : Core::COLS;  // output columns of a wave
     const int64_t nb = n0 + c.wn * WIDTH;
     const bool inside = nb + c.piece_col() < q.n;
@@ -321,11 +320,8 @@ __global__ void __launch_bounds__(S::WM *S::WN * 64) ffn_kernel(const FfnParams 
 #pragma unroll
             for (int j = 0; j < C::FN; ++j)
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const f32x16 &v = c.acc[i][j];
-                    partial<C>(p, r, piece, tiles, i, j, threadIdx.x)[h * C::THREADS] =
-                        make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-                }
+                for (int h = 0; h < 4; ++h)
+                    partial<C>(p, r, piece, tiles, i, j, threadIdx.x)[h * C::THREADS] = bitcast<float4>(c.acc[i][j][h]);
         return;
     }
     epilogue<DT, C, EPI, C::FM>(p, q, c, c.acc, 0, m0, n0, lds);
@@ -345,12 +341,13 @@ __global__ void __launch_bounds__(64) ffn_join_kernel(const FfnParams p) {
     C c;  // the only wave of its workgroup, in the place of one of the tile's
     c.wm = wave % S::WM;
     c.wn = wave / S::WM;
-    f32x16 acc[1][C::FN];
+    f32x4 acc[1][C::FN][4];
     const int64_t stride = (int64_t)tiles * C::FM * C::FN * 4 * C::THREADS;
     constexpr int kPieces = 8;  // partial sums in flight: one after the other each is a trip to memory
 #pragma unroll
     for (int j = 0; j < C::FN; ++j) {
-        acc[0][j] = f32x16{};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) acc[0][j][h] = f32x4{0.f, 0.f, 0.f, 0.f};
         const float4 *first = partial<C>(p, r, 0, tiles, i, j, wave * 64 + threadIdx.x);
         for (int s0 = 0; s0 < p.split; s0 += kPieces) {
             float4 v[kPieces][4];
@@ -362,12 +359,7 @@ __global__ void __launch_bounds__(64) ffn_join_kernel(const FfnParams p) {
 #pragma unroll
             for (int s = 0; s < kPieces; ++s)
 #pragma unroll
-                for (int h = 0; s0 + s < p.split && h < 4; ++h) {
-                    acc[0][j][4 * h] += v[s][h].x;
-                    acc[0][j][4 * h + 1] += v[s][h].y;
-                    acc[0][j][4 * h + 2] += v[s][h].z;
-                    acc[0][j][4 * h + 3] += v[s][h].w;
-                }
+                for (int h = 0; s0 + s < p.split && h < 4; ++h) acc[0][j][h] += bitcast<f32x4>(v[s][h]);
         }
     }
     const int64_t m0 = (int64_t)tm * S::BM, n0 = (int64_t)tn * BNO;
@@ -385,14 +377,6 @@ __global__ void __launch_bounds__(64) ffn_join_kernel(const FfnParams p) {
 //     2048, 5504                           40.4      61.1   49
 //     4096, 11008                86.3               179.7   91
 // 1 row: 17.3 MB of weights, 1.4 TB/s; a launch of nothing takes 2 us of each 6.
-template <class DT>
-__device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
-    if constexpr (std::is_same<DT, BF16>::value)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bitcast<bf16x8>(a), bitcast<bf16x8>(b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
-}
-
 constexpr int kFewRows = 32;
 template <class DT, int TT, int NW, int EPI>
 __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const FfnParams p) {
@@ -486,20 +470,21 @@ hipError_t launch_few(const FfnParams &p, hipStream_t stream) {
 // (a CU alone has more of the caches, of the memory and of the power budget), and the share of
 // the epilogue's bytes, at kMemory, that nothing else runs under (one of two workgroups on a CU
 // computes while the other stores). Measured with each shape forced (bf16, us; largest is
-// 16384 rows, d 2048, f 5504, ragged 6473, 1024, 2816, small 300, 512, 1408; + the join):
+// 16384 rows, d 2048, f 5504, ragged 6473, 1024, 2816, small 1500, 512, 1408; + the join):
 //                     256 x 256   256 x 128   128 x 128    64 x 128
-//   largest, gate|up        822        1016        1003        1061
-//   largest, down           371         424         424         493
-//   largest, da             534         546         561         570
-//   largest, dx             688         807         820        1045
-//   ragged,  gate|up        122         127         116         130
-//   ragged,  down            74          53          57          61 + 6
-//   ragged,  da             107          93          83          80
-//   ragged,  dx              92 + 17    109         114         124 + 6
-//   ragged,  weights        162         140 + 7     135 + 7     176 + 9
-//   small,   gate|up         24          16          14          11
-//   small,   da              33          19          18          12
-//   small,   dx              16 + 9      14 + 5      11 + 5      10 + 6
+//   largest, gate|up        794         975         940        1023
+//   largest, down           359         418         397         480 + 8
+//   largest, da             512         530         540         567
+//   largest, dx             646         787         774         990 + 8
+//   largest, weights        963 + 12   1189 + 8    1200 + 6    1767 + 9
+//   ragged,  gate|up        118         122         105         127
+//   ragged,  down            73          52          52          58 + 6
+//   ragged,  da              84 + 17     90          79          79
+//   ragged,  dx              87 + 16    105         104         117 + 6
+//   ragged,  weights        158         137 + 6     126 + 6     173 + 8
+//   small,   gate|up         26          18          18          17
+//   small,   da              34          21          17          16
+//   small,   dx              21 + 9      16 + 6      14 + 6      14 + 5
 // A split costs a join of 5 to 6 us, less what it saves: dx of 575, 264, 712 takes 17.2 us whole and 13.6 in
 // pieces, of 3000, 768, 2048 50.4 and 37.5, down of 1500, 1024, 2816 27.9 and 24.6.
 struct Plan {
@@ -511,9 +496,9 @@ struct ShapeCost {
     double busy, alone, bare, tile;  // tile: us of a tile besides its k-steps and bytes
 };
 constexpr ShapeCost kShapes[] = {
-    {256, 256, 256, 1.85, 1.20, 1.0, 4.0},
-    {256, 128, 256, 1.05, 0.80, 1.0, 3.0},
-    {128, 128, 512, 1.17, 0.60, 0.6, 3.0},
+    {256, 256, 256, 1.80, 1.20, 1.0, 4.0},
+    {256, 128, 256, 1.10, 0.80, 1.0, 3.0},
+    {128, 128, 512, 1.12, 0.60, 0.65, 3.0},
     {64, 128, 768, 1.00, 0.50, 0.4, 3.0},
 };
 constexpr int kShapeCount = 4, kMaxSplit = 8;

@@ -1,5 +1,10 @@
-// Tile products C[m, n] = sum_k A(m, k) B(n, k) of 16-bit matrices on v_mfma_f32_32x32x16 with
+// Tile products C[m, n] = sum_k A(m, k) B(n, k) of 16-bit matrices on v_mfma_f32_16x16x32 with
 // fp32 accumulators, for the kernels that end a product in an epilogue of their own.
+//
+// Large products run at the card's power limit, and there the smaller blocks are the cheaper ones (a
+// result element is read and written once per 32 of k instead of 16): operands held in registers,
+// random bf16, 2077 TFLOP/s against 1301 with v_mfma_f32_32x32x16 in the same loop. Of whole
+// products, where loads and LDS reads take their share, 2 to 8 % came of it.
 //
 // An operand's element (r, k) lies at base[r * ld + k] (kKContig: weights and hidden states of a
 // forward product) or at base[k * ld + r] (kRContig: the same tensors in their gradients'
@@ -18,7 +23,11 @@
 
 #include "tiles.h"
 
+#include <type_traits>
+
 namespace dsalt {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 enum { kKContig = 0, kRContig = 1 };
 constexpr uint32_t kOutOfRange = 0x80000000u;  // above every descriptor's size (kGemmMaxLd)
@@ -30,13 +39,23 @@ struct GemmOperand {
     int64_t rows; // extent of r
 };
 
+// What a chunk's place in a row of `CPR` chunks is XORed with.
+template <int LAY, int CPR>
+__device__ __forceinline__ int gemm_swizzle(int row) {
+    static_assert(CPR == 8 || (LAY == kRContig && CPR >= 16), "a swizzle stays inside its row");
+    if constexpr (LAY == kKContig) return (row >> 1) & 7;
+    else if constexpr (CPR >= 16) return ((row & 3) << 2) | ((row >> 2) & 2);
+    else return (row & 2) | ((row >> 1) & 4);
+}
+
 // One operand's tile: ROWS rows of r, BK of k, filled by NW waves.
 //
 // LDS has 64 banks of 4 bytes, and a 16-byte read serves 16 lanes at a time: the swizzle puts the
 // same chunk of 16 consecutive rows on 16 different places of 256 bytes (two rows of 64): 4.2
-// clocks a read, against 8.3 with chunk ^ (row & 7), which spreads 8 rows. A transposing read
-// takes 32 bytes of each of four rows, which go to four different 64-byte places (32-byte
-// places where a row has only 128 bytes): 2.9 clocks, 4.2 with 32-byte places, 8 without.
+// clocks a read, against 8.3 with chunk ^ (row & 7), which spreads 8 rows. A transposing read's 32
+// lanes take 32 bytes of each of eight rows, r .. r + 3 and r + 8 .. r + 11: the first four go to
+// different 64-byte places, the others to those places' other halves (of 128-byte rows, two to
+// a 256 bytes, to four 32-byte places each).
 template <int LAY, int ROWS, int BK, int NW>
 struct GemmTile {
     static constexpr int BYTES = ROWS * BK * 2;
@@ -44,20 +63,16 @@ struct GemmTile {
     static constexpr int CPR = LAY == kKContig ? BK / 8 : ROWS / 8;  // chunks per LDS row
     static constexpr int RPL = 64 / CPR;                             // LDS rows per load instruction
     static_assert(BYTES % (16 * 64 * NW) == 0, "the waves cover the tile");
-    static_assert(CPR == 8 || (LAY == kRContig && CPR > 8), "a swizzle stays inside its row");
-
-    static __device__ __forceinline__ int swizzle(int row) {
-        if constexpr (LAY == kRContig) return (row & 3) << (CPR >= 16 ? 2 : 1);
-        else return (row >> 1) & 7;
-    }
-
-    uint32_t off[2];  // of a wave's even and odd loads
-    int kchunk[2];    // kKContig: their chunks of k
+    // loads of a wave after which the swizzle is that of the first again
+    static constexpr int OFFS = LAY == kRContig && CPR == 16 && LPW == 4 ? 4 : 2;
+    static_assert(LAY == kKContig || OFFS * RPL % 16 == 0 || (LPW * RPL == 8 && OFFS * RPL % 4 == 0), "swizzle's period");
+    uint32_t off[OFFS];
+    int kchunk[OFFS];  // kKContig: their chunks of k
 
     __device__ __forceinline__ GemmTile(int wave, int lane, uint32_t ld) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = (wave * LPW + u) * RPL + lane / CPR, chunk = (lane % CPR) ^ swizzle(row);
+        for (int u = 0; u < OFFS; ++u) {
+            const int row = (wave * LPW + u) * RPL + lane / CPR, chunk = (lane % CPR) ^ gemm_swizzle<LAY, CPR>(row);
             kchunk[u] = chunk;
             off[u] = (uint32_t)row * ld + (chunk << 4);
         }
@@ -66,7 +81,7 @@ struct GemmTile {
     // The loads of k0 .. k0 + BK - 1 (k in all) of rows r0 .. r0 + ROWS - 1.
     struct Step {
         i32x4 rsrc;
-        uint32_t v[2], ld;
+        uint32_t v[OFFS], ld;
     };
     __device__ __forceinline__ Step step(const GemmOperand &o, int64_t r0, int64_t k0, int64_t k) const {
         const int64_t left = k - k0;
@@ -80,44 +95,47 @@ struct GemmTile {
             p = o.base + k0 * o.ld + r0 * 2;
             bytes = left > 0 && o.rows > r0 ? (min(left, (int64_t)BK) - 1) * o.ld + (o.rows - r0) * 2 : 0;
         }
-        Step s{uniform_rsrc(buffer_rsrc(p, (uint32_t)bytes)), {off[0], off[1]}, (uint32_t)o.ld};
+        Step s;
+        s.rsrc = uniform_rsrc(buffer_rsrc(p, (uint32_t)bytes));
+        s.ld = (uint32_t)o.ld;
+#pragma unroll
+        for (int u = 0; u < OFFS; ++u) s.v[u] = off[u];
         if constexpr (LAY == kKContig) {  // a chunk past k would read the next row's first elements
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < OFFS; ++u)
                 if (kchunk[u] * 8 >= left) s.v[u] = kOutOfRange;
         }
         return s;
     }
     // Load `u` of LPW to the tile at LDS byte `lds`.
     static __device__ __forceinline__ void issue(const Step &s, int u, uint32_t lds, int wave) {
-        dma16(s.v[u & 1] + (uint32_t)((u & ~1) * RPL) * s.ld, s.rsrc,
+        dma16(s.v[u % OFFS] + (uint32_t)(u / OFFS * OFFS * RPL) * s.ld, s.rsrc,
               __builtin_amdgcn_readfirstlane(lds + (wave * LPW + u) * 1024));
     }
 };
 
-// Reads of a tile as MFMA operands: the lane's r = 32 block + lane % 32, k = 16 sub + 8 (lane / 32) .. + 7.
+// Reads of a tile as MFMA operands: the lane's r = 16 block + lane % 16, k = 32 sub + 8 (lane / 16) .. + 7.
 template <int LAY, int ROWS, int BK>
 struct GemmFrag {
     uint32_t a;  // byte of the lane's first element in block 0, sub-step 0
     __device__ __forceinline__ explicit GemmFrag(int lane) {
-        typedef GemmTile<LAY, ROWS, BK, 1> Tile;
+        constexpr int CPR = LAY == kKContig ? BK / 8 : ROWS / 8;
         if constexpr (LAY == kKContig) {
-            const int row = lane & 31;
-            a = row * (BK * 2) + (((lane >> 5) ^ Tile::swizzle(row)) << 4);
+            const int row = lane & 15;
+            a = row * (BK * 2) + (((lane >> 4) ^ gemm_swizzle<LAY, CPR>(row)) << 4);
         } else {
             // ds_read_b64_tr_b16 gives lane l element l % 4 of the 8-byte pieces that lanes
             // 16 (l / 16) + 4 e + (l % 16) / 4, e = 0..3, address: a lane addresses k-row
-            // (l % 16) / 4 and columns 16 ((l / 16) % 2) + 4 (l % 4) of its half's block
-            const int krow = ((lane >> 5) << 3) + ((lane >> 2) & 3);
-            const int chunk = (((lane >> 4) & 1) << 1) + ((lane & 3) >> 1);
-            a = krow * (ROWS * 2) + ((chunk ^ Tile::swizzle(krow)) << 4) + ((lane & 1) << 3);
+            // (l % 16) / 4 and columns 4 (l % 4) of its 16 lanes' block
+            const int krow = ((lane >> 4) << 3) + ((lane >> 2) & 3);
+            a = krow * (ROWS * 2) + ((((lane & 3) >> 1) ^ gemm_swizzle<LAY, CPR>(krow)) << 4) + ((lane & 1) << 3);
         }
     }
     __device__ __forceinline__ uint4 read(const char *tile, int block, int sub) const {
         if constexpr (LAY == kKContig) {
-            return *reinterpret_cast<const uint4 *>(tile + (a ^ (sub << 5)) + block * (32 * BK * 2));
+            return *reinterpret_cast<const uint4 *>(tile + (a ^ (sub << 6)) + block * (16 * BK * 2));
         } else {
-            const char *p = tile + (a ^ ((block & 3) << 6)) + (block >> 2) * 256 + sub * (16 * ROWS * 2);
+            const char *p = tile + (a ^ ((block & 7) << 5)) + (block >> 3) * 256 + sub * (32 * ROWS * 2);
             const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)p);
             const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) shortx4 *)(p + 4 * ROWS * 2));
@@ -127,6 +145,14 @@ struct GemmFrag {
     }
 };
 
+template <class DT>
+__device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (std::is_same<DT, BF16>::value)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bitcast<bf16x8>(a), bitcast<bf16x8>(b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
+}
+
 // A workgroup's tile of the product: WM x WN waves over BM x BN, each FM x FN blocks of 32 x 32.
 // PAIR: the B tile's first half are rows of one matrix and its second half the same rows of
 // another (gate and up), and a wave holds the same n of both.
@@ -135,7 +161,7 @@ struct GemmFrag {
 // RB - 1 steps before it is read, into the stages that the barrier of the step before has freed.
 template <class DT, int BM, int BN, int BK_, int RA, int RB, int WM, int WN, int ALAY, int BLAY, bool PAIR>
 struct GemmCore {
-    static constexpr int BK = BK_, NW = WM * WN, THREADS = NW * 64, FM = BM / WM / 32, FN = BN / WN / 32, SUBS = BK / 16;
+    static constexpr int BK = BK_, NW = WM * WN, THREADS = NW * 64, FM = BM / WM / 32, FN = BN / WN / 32, SUBS = BK / 32;
     static constexpr int BNB = PAIR ? BN / 2 : BN, NWB = PAIR ? NW / 2 : NW;  // of one B matrix
     typedef GemmTile<ALAY, BM, BK, NW> TA;
     typedef GemmTile<BLAY, BNB, BK, NWB> TB;
@@ -144,7 +170,7 @@ struct GemmCore {
     static_assert(SUBS % 2 == 0, "the operand registers alternate from one step to the next");
     static_assert(RB >= 2 && (RA == RB || RA == RB + 1), "see the waits in run()");
 
-    f32x16 acc[FM][FN];
+    f32x4 acc[FM][FN][4];  // of a block's quarters: 16 rows each, then 16 columns
     int wm, wn, lane, wave;
 
     __device__ __forceinline__ GemmCore() {
@@ -187,31 +213,35 @@ struct GemmCore {
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = f32x16{};
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) acc[i][j][h] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (first >= last) return;
 
-        uint4 ra[2][FM], rb[2][FN];
-        // operand read r of FM + FN, in the order of the products' use: b0 a0 b1 b2 .. a1 ..
+        constexpr int M16 = 2 * FM, N16 = 2 * FN, READS = M16 + N16;
+        uint4 ra[2][M16], rb[2][N16];
+        // operand read r of READS, in the order of the products' use: b0 a0 b1 b2 .. a1 ..
         auto read = [&](int sta, int stb, int sub, int r, int buf) {
             const char *at = lds + sta * ASTAGE, *bt = lds + RA * ASTAGE + stb * BSTAGE;
-            if (r == 0 || (r >= 2 && r <= FN)) {
+            if (r == 0 || (r >= 2 && r <= N16)) {
                 const int j = r == 0 ? 0 : r - 1;
-                if constexpr (PAIR) rb[buf][j] = fb.read(bt + (j < FN / 2 ? 0 : TB::BYTES), wn * (FN / 2) + j % (FN / 2), sub);
-                else rb[buf][j] = fb.read(bt, wn * FN + j, sub);
+                if constexpr (PAIR) rb[buf][j] = fb.read(bt + (j < FN ? 0 : TB::BYTES), wn * FN + j % FN, sub);
+                else rb[buf][j] = fb.read(bt, wn * N16 + j, sub);
             } else {
-                const int i = r == 1 ? 0 : r - FN;
-                ra[buf][i] = fa.read(at, wm * FM + i, sub);
+                const int i = r == 1 ? 0 : r - N16;
+                ra[buf][i] = fa.read(at, wm * M16 + i, sub);
             }
         };
         auto mul = [&](int q, int buf) {
-            const int i = q / FN, j = q % FN;
-            acc[i][j] = DT::mfma(bitcast<typename DT::vec8>(rb[buf][j]), bitcast<typename DT::vec8>(ra[buf][i]), acc[i][j]);
+            const int i = q / N16, j = q % N16;
+            f32x4 &c = acc[i >> 1][j >> 1][(i & 1) * 2 + (j & 1)];
+            c = mfma16<DT>(rb[buf][j], ra[buf][i], c);
         };
-        constexpr int NM = FM * FN, LT = LA + LB;
-        constexpr int RPP = (FM + FN + NM - 1) / NM;  // operand reads before each product
+        constexpr int NM = M16 * N16, LT = LA + LB;
         auto read_before = [&](int sta, int stb, int sub, int q, int buf) {
 #pragma unroll
-            for (int r = q * RPP; r < (q + 1) * RPP && r < FM + FN; ++r) read(sta, stb, sub, r, buf);
+            for (int r = 0; r < READS; ++r)  // spread over three quarters of the products
+                if (r * (NM * 3 / 4) / READS == q) read(sta, stb, sub, r, buf);
         };
         // the loads of a group are spread over the SUBS sub-steps after the barrier that frees their
         // stages (part 0 .. SUBS - 1), one after every few products: issued in one go they fill the
@@ -238,7 +268,7 @@ struct GemmCore {
         constexpr int PART0 = (LT + SUBS - 1) / SUBS;  // loads of a group's part 0
         tile_barrier<PART0 + (RB - 2) * LT + (RA - RB) * LA>();
 #pragma unroll
-        for (int r = 0; r < FM + FN; ++r) read(0, 0, 0, r, 0);
+        for (int r = 0; r < READS; ++r) read(0, 0, 0, r, 0);
         int sta = 0, stb = 0, olda = RA - 1, oldb = RB - 1;
         for (int t = first; t < last; ++t) {
             // a read of the next sub-step's operands between one product and the next
@@ -283,15 +313,14 @@ struct GemmCore {
     // 16-byte pieces of whole rows. XOR with the row spreads the rows over the banks.
     static constexpr int COLS = FN * 32, PIECES = (PAIR ? COLS / 2 : COLS) / 8, TURNS = 32 * PIECES / 64;
     __device__ __forceinline__ char *turn(char *lds) const { return lds + wave * (32 * COLS * 4); }
-    __device__ __forceinline__ void put(char *lds, const f32x16 (&row)[FN]) const {
-        const int r = lane & 31;
-        char *p = turn(lds) + r * (COLS * 4);
+    __device__ __forceinline__ void put(char *lds, const f32x4 (&row)[FN][4]) const {
+        char *p = turn(lds) + (lane & 15) * (COLS * 4);
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int h = 0; h < 4; ++h)
-                *reinterpret_cast<float4 *>(p + (((j * 8 + h * 2 + (lane >> 5)) ^ (r & 15)) << 4)) =
-                    make_float4(row[j][4 * h], row[j][4 * h + 1], row[j][4 * h + 2], row[j][4 * h + 3]);
+                *reinterpret_cast<f32x4 *>(p + (h >> 1) * (16 * COLS * 4) +
+                                           (((j * 8 + (h & 1) * 4 + (lane >> 4)) ^ (lane & 15)) << 4)) = row[j][h];
         __builtin_amdgcn_wave_barrier();
     }
     // Row and first column (of the wave's) of the lane's piece in turn t.

@@ -133,7 +133,8 @@ def test_larger(rows, d, f):
 # and those that the plan's constants, refitted, moved to other shapes or splits
 @pytest.mark.parametrize("rows,d,f", [
     (9680, 2024, 400), (8080, 152, 3256), (9408, 200, 3840), (8361, 424, 3576), (1627, 1192, 3728), (3415, 2376, 608),
-    (1500, 512, 1408), (3000, 768, 2048), (5452, 656, 3632), (7836, 880, 3168)])
+    (1500, 512, 1408), (3000, 768, 2048), (5452, 656, 3632), (7836, 880, 3168),
+    (5407, 1224, 2440), (6843, 280, 3904), (8368, 1040, 2848), (4510, 680, 3544), (4022, 1952, 1864)])
 def test_larger_splits(rows, d, f):
     test_larger(rows, d, f)
 
