@@ -244,8 +244,9 @@ struct GemmCore {
                 if (r * (NM * 3 / 4) / READS == q) read(sta, stb, sub, r, buf);
         };
         // the loads of a group are spread over the SUBS sub-steps after the barrier that frees their
-        // stages (part 0 .. SUBS - 1), one after every few products: issued in one go they fill the
-        // memory pipe's queue and hold the wave's products back
+        // stages (part 0 .. SUBS - 1), one after every few products, so that they do not fill the memory
+        // pipe's queue and hold the wave's products back (in the first half of each sub-step: up to 4 %
+        // slower dx, 2 % faster down)
         auto issue_after = [&](int sta, int stb, int part, int q) {
 #pragma unroll
             for (int u = 0; u < LT; ++u)
