@@ -1687,6 +1687,12 @@ def _addr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def gate_kind(gate: torch.Tensor | None, d: int) -> int:
+    """dsalt_branch_norm_args.gate_kind: 0 none, 1 per channel [d], 2 per token [..., 1]. By the shape: a
+    token's gate beside x [d] has one dimension too, and one element, fewer than any d."""
+    return 0 if gate is None else 1 if gate.shape == (d,) else 2
+
+
 def _branch_pack(x, h, weight, post_weight, gate, opts, seed, *, x_out=0, y=0, rstd=0, rstd_post=0, dx_out=0, dy=0,
                  grads=(0, 0, 0, 0, 0), ws=(0, 0)) -> bytes:
     residual_scale, p, offset, eps, post_eps, out_dtype = opts
@@ -1694,7 +1700,7 @@ def _branch_pack(x, h, weight, post_weight, gate, opts, seed, *, x_out=0, y=0, r
     threshold = keep_threshold(p)
     return _BRANCH_PACK.pack(
         x.numel() // d, d, _SCORE_DTYPES[x.dtype], _SCORE_DTYPES[h.dtype], _SCORE_DTYPES[out_dtype], _code(weight),
-        _code(post_weight), _code(gate), 0 if gate is None else 1 if gate.dim() == 1 else 2, threshold, eps, post_eps,
+        _code(post_weight), _code(gate), gate_kind(gate, d), threshold, eps, post_eps,
         residual_scale, *(_seed_offset(seed, offset, x.device) if threshold < 65536 else (0, 0, 0)), x.data_ptr(), h.data_ptr(),
         _addr(weight), _addr(post_weight), _addr(gate), x_out, y, rstd, rstd_post, dx_out, dy, *grads, *ws)
 
@@ -1721,7 +1727,7 @@ def branch_norm_bwd(x, h, weight, post_weight, gate, opts, seed, stats, dx_out, 
     rows, d = x.numel() // x.shape[-1], x.shape[-1]
     out = [torch.empty_like(t) if n else None for t, n in zip((x, h, weight, post_weight, gate), need)]
     ws = (0, 0)
-    if need[2] or need[3] or (need[4] and gate.dim() == 1):
+    if need[2] or need[3] or (need[4] and gate_kind(gate, d) == 1):
         size = lib().dsalt_branch_norm_workspace_size(rows, d)
         scratch = torch.empty(size, device=dev, dtype=torch.uint8)
         ws = (scratch.data_ptr(), size)

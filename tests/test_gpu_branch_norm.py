@@ -320,3 +320,19 @@ def test_stream_and_branch_one_tensor():
     two = {n: t["x"].clone().requires_grad_() for n in ("x", "h")}
     parts = torch.autograd.grad(branch_norm(two["x"], two["h"], t["weight"], gate=t["gate"]), (two["x"], two["h"]), (dz, dy))
     assert torch.equal(got, parts[0] + parts[1])
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token"])
+@pytest.mark.parametrize("d", [8, 1032, 8192])
+def test_one_dimensional_stream(gate, d):
+    """x [d]: one row, whose token gate is [1]."""
+    for xd, hd in ((FP, BF), (HF, HF)):
+        print(f"branch_norm [{d}] gate={gate} {xd}", flush=True)
+        t, dz, dy = inputs((), d, xd, hd, hd, gate=gate)
+        outs, grads = compare(t, dz, dy, od=hd)
+        assert outs[0].shape == outs[1].shape == (d,)
+        assert gate == "none" or grads["gate"].shape == ((1,) if gate == "token" else (d,))
+        two = run({n: v if v is None or n in ("weight", "post_weight") or gate == "channel" and n == "gate" else v[None]
+                   for n, v in t.items()}, dz[None], dy[None], residual_scale=0.75, p=0.2, seed=77, offset=5, out_dtype=hd)
+        assert all(torch.equal(a, b[0]) for a, b in zip(outs, two[0]))
+        assert all(torch.equal(grads[n], two[1][n].view(grads[n].shape)) for n in grads)

@@ -121,3 +121,16 @@ def test_argument_values():
             hip.seed_fields(bad, dev)
     with pytest.raises(hip.DsaltError):
         hip.seed_fields(torch.tensor([1]), dev)
+
+
+@pytest.mark.parametrize("lead", [(), (1,), (64,), (3, 5), (64, 1)])
+def test_branch_norm_gate_kinds(lead):
+    """A channel's gate is [d] and a token's [..., 1] beside x [..., d], x [d] and its gate [1] among
+    them: the kind in the argument struct says how many elements the kernels read and write."""
+    d = 64
+    x = torch.zeros(*lead, d)
+    opts = (1.0, 0.0, 0, 1e-6, 1e-6, x.dtype)
+    for gate, kind in ((None, 0), (torch.zeros(d), 1), (torch.zeros(*lead, 1), 2)):
+        a = hip.BranchNormArgs.from_buffer_copy(hip._branch_pack(x, x, None, None, gate, opts, None))
+        assert a.gate_kind == kind and a.d == d and a.rows * d == x.numel()
+        assert gate is None or gate.numel() == (a.d if kind == 1 else a.rows)
