@@ -190,20 +190,26 @@ struct GemmCore {
         const int per = (int)((k + BK - 1) / BK);  // steps of a segment
         const int bwave = PAIR ? wave % NWB : wave;
         const bool second = PAIR && wave >= NWB;
-        const TA ta(wave, lane, (uint32_t)a[0].ld);
-        const TB tb(bwave, lane, (uint32_t)(second ? b[1].ld : b[0].ld));
+        const int from = SEGMENTS > 1 && first >= per ? 1 : 0;  // the first step's segment
+        TA ta(wave, lane, (uint32_t)a[from].ld);
+        TB tb(bwave, lane, (uint32_t)(second ? b[1].ld : b[from].ld));
         const uint32_t bbase = base + RA * ASTAGE + (second ? TB::BYTES : 0);
         const GemmFrag<ALAY, BM, BK> fa(lane);
         const GemmFrag<BLAY, BNB, BK> fb(lane);
         typename TA::Step sa;
         typename TB::Step sb;
-        // past `last` the loads read nothing, so that every step counts the same number of loads
+        // past `last` the loads read nothing, so that every step counts the same number of loads; steps are
+        // prepared in order, and where the second segment starts the lanes take its row strides
         auto prepare_a = [&](int step) {
             const int s = SEGMENTS > 1 && step >= per ? 1 : 0;
+            if constexpr (SEGMENTS > 1)
+                if (step == per) ta = TA(wave, lane, (uint32_t)a[1].ld);
             sa = ta.step(a[s], m0, step < last ? (int64_t)(step - s * per) * BK : k, k);
         };
         auto prepare_b = [&](int step) {
             const int s = SEGMENTS > 1 && step >= per ? 1 : 0;
+            if constexpr (SEGMENTS > 1)
+                if (step == per) tb = TB(bwave, lane, (uint32_t)b[1].ld);
             sb = tb.step(PAIR ? (second ? b[1] : b[0]) : b[s], n0, step < last ? (int64_t)(step - s * per) * BK : k, k);
         };
         // load u of a step: B's first, as its step is needed first where RA > RB

@@ -392,3 +392,25 @@ def test_two_graphs_and_eager_calls_in_turn():
                 assert torch.equal(gated_ffn(x, wg, wu, wd), want[1 - i])
             for got, ref in zip(outs, want):
                 assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("rows,d,f", [(20, 72, 136), (150, 72, 136), (575, 264, 712), (1500, 512, 1408), (8579, 904, 712), (2049, 2048, 1408)])
+def test_weights_of_different_row_strides(rows, d, f, dtype):
+    """Each weight a column slice of a wider matrix of its own: the bits of contiguous weights, with w_up's
+    stride above and below w_gate's. Sizes with whole and with split tiles of every shape."""
+    x, wg, wu, wd, dy = inputs(rows, d, f, d, dtype)
+    want = run(x, wg, wu, wd, dy, "silu")
+
+    def wider(t, more):  # NaN beside it: what is read of it shows
+        w = torch.full((t.shape[0], t.shape[1] + more), float("nan"), device=DEV, dtype=dtype)
+        w[:, 8:8 + t.shape[1]] = t
+        return w[:, 8:8 + t.shape[1]]
+
+    for more in ((0, 16, 8), (64, 8, 24), (8, 1024, 16)):
+        print(f"gated_ffn strides {rows} x {d} x {f} + {more} {dtype}", flush=True)
+        ws = [wider(w, m) if m else w for w, m in zip((wg, wu, wd), more)]
+        assert [w.stride(0) for w in ws] == [d + more[0], d + more[1], f + more[2]]
+        got = run_views(x, *ws, dy)
+        for n in want:
+            assert torch.equal(got[n], want[n]), (more, n)
