@@ -414,3 +414,30 @@ def test_weights_of_different_row_strides(rows, d, f, dtype):
         got = run_views(x, *ws, dy)
         for n in want:
             assert torch.equal(got[n], want[n]), (more, n)
+
+
+@pytest.mark.parametrize("rows", [25, 97])
+@pytest.mark.parametrize("dtype,lowest,up,scale", [(BF, -10.0, 1.0, 1.0), (HF, -5.5, 2.0 ** 14, 2.0 ** 10)], ids=["bf16", "fp16"])
+def test_gelu_of_far_negative_gates(dtype, lowest, up, scale, rows):
+    """GELU and its slope where phi(g) is small, each element by itself: g and u are single products, y, dx
+    and the inner gradients single ones of what was rounded, so that a relative bound holds: half a
+    step, plus 2^-15 for an exp of exponents up to 72, rounded to 2^-24 of that three times, and the
+    sum of slope's two terms, of which the smaller is at most a sixteenth. fp16's u and dy keep the
+    values above its smallest normal one."""
+    print(f"gated_ffn gelu tail {rows} {dtype}", flush=True)
+    g = torch.linspace(lowest, -4.0, rows, device=DEV).to(dtype)
+    x = torch.zeros(rows, 8, device=DEV, dtype=dtype)
+    x[:, 0], x[:, 1] = g, up
+    wg, wu, wd = (torch.zeros(8, 8, device=DEV, dtype=dtype) for _ in range(3))
+    wg[0, 0] = wu[0, 1] = wd[0, 0] = 1
+    dy = torch.zeros_like(x)
+    dy[:, 0] = scale
+    got = run(x, wg, wu, wd, dy, "gelu")
+    z = g.double()
+    phi = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5)
+    slope = phi + z * torch.exp(-0.5 * z * z) * (2 * torch.pi) ** -0.5
+    bound = torch.finfo(dtype).eps / 2 + 2.0 ** -15
+    for n, have, want in (("y", got["y"][:, 0], z * phi * up), ("dg", got["dx"][:, 0], scale * up * slope),
+                          ("du", got["dx"][:, 1], scale * z * phi)):
+        assert float(want.abs().min()) > torch.finfo(dtype).tiny and float(want.abs().max()) < torch.finfo(dtype).max
+        assert bool(((have.double() - want).abs() <= bound * want.abs()).all()), (n, float((have.double() / want - 1).abs().max()))
