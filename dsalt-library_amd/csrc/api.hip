@@ -767,7 +767,8 @@ int dsalt_branch_norm_check(const dsalt_branch_norm_args *a, int32_t backward) {
         if (!a->dx_out && !a->dy) return fail(DSALT_ERR_INVALID, "dx_out or dy must be non-NULL");
         if (a->dy && (!a->weight || !a->rstd)) return fail(DSALT_ERR_INVALID, "dy needs weight and rstd");
         if (a->post_weight && !a->rstd_post) return fail(DSALT_ERR_INVALID, "post_weight needs rstd_post");
-        if (a->d_post_weight && !a->post_weight) return fail(DSALT_ERR_INVALID, "d_post_weight needs post_weight");
+        if ((a->d_weight && !a->weight) || (a->d_post_weight && !a->post_weight) || (a->d_gate && !a->gate_kind))
+            return fail(DSALT_ERR_INVALID, "d_weight needs weight, d_post_weight post_weight, d_gate a gate");
         if ((a->d_weight || a->d_post_weight || (a->d_gate && a->gate_kind == 1)) &&
             (!a->workspace || a->workspace_bytes < dsalt::branch_norm_workspace_bytes(a->rows, a->d)))
             return fail(DSALT_ERR_INVALID, "the column sums need workspace of dsalt_branch_norm_workspace_size bytes");

@@ -275,11 +275,13 @@ __global__ void __launch_bounds__(RowShape<WPR>::THREADS) branch_bwd_kernel(cons
 struct SumOut {
     void *out[3];
     int dtype[3];
+    int groups[3];  // workgroups with partials: none of a sum that is zero
 };
-__global__ void __launch_bounds__(1024) branch_sums_kernel(const float *__restrict__ part, const SumOut o, int groups, int d) {
+__global__ void __launch_bounds__(1024) branch_sums_kernel(const float *__restrict__ part, const SumOut o, int d) {
     __shared__ float lds[32][33];
     const int q = blockIdx.y;
     if (!o.out[q]) return;
+    const int groups = o.groups[q];
     const int col = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
     float t = 0.f;
     if (col < d) {
@@ -361,10 +363,16 @@ hipError_t launch_branch(const dsalt_branch_norm_args &a, bool bwd, hipStream_t 
     p.rs = a.residual_scale;
     p.dropout = a.threshold < 65536;
     p.drop = dropout_params(a.threshold, a.seed, a.seed_ptr, a.offset);
-    SumOut o = {{a.dy || a.rows == 0 ? a.d_weight : nullptr, a.d_post_weight, a.gate_kind == kGateChannel ? a.d_gate : nullptr},
-                {a.w_dtype, a.post_dtype, a.gate_dtype}};
-    if (bwd)
-        for (int q = 0; q < 3; ++q) p.sums |= o.out[q] ? 1 << q : 0;
+    const int groups = branch_bwd_groups(a.rows, a.d);
+    // without a gradient of y that of its norm's weight is zero
+    SumOut o = {{a.d_weight, a.d_post_weight, a.gate_kind == kGateChannel ? a.d_gate : nullptr},
+                {a.w_dtype, a.post_dtype, a.gate_dtype},
+                {a.dy ? groups : 0, groups, groups}};
+    bool sums = false;
+    for (int q = 0; bwd && q < 3; ++q) {
+        p.sums |= o.out[q] && o.groups[q] ? 1 << q : 0;
+        sums |= o.out[q] != nullptr;
+    }
     if (a.rows > 0) {
         if (a.x_dtype == DSALT_DTYPE_BF16) launch_types<BF16, BF16>(p, bwd, stream);
         else if (a.x_dtype == DSALT_DTYPE_F16) launch_types<F16, F16>(p, bwd, stream);
@@ -372,9 +380,8 @@ hipError_t launch_branch(const dsalt_branch_norm_args &a, bool bwd, hipStream_t 
         else if (a.h_dtype == DSALT_DTYPE_F16) launch_types<F32, F16>(p, bwd, stream);
         else launch_types<F32, F32>(p, bwd, stream);
     }
-    if (p.sums)
-        hipLaunchKernelGGL(branch_sums_kernel, dim3((a.d + 31) / 32, 3), dim3(1024), 0, stream, p.part, o,
-                           branch_bwd_groups(a.rows, a.d), a.d);
+    if (sums)
+        hipLaunchKernelGGL(branch_sums_kernel, dim3((a.d + 31) / 32, 3), dim3(1024), 0, stream, p.part, o, a.d);
     return hipGetLastError();
 }
 

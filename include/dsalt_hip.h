@@ -687,8 +687,9 @@ size_t dsalt_dropout_args_size(void);
  * y_dtype) formed from the fp32 x_out. rstd, rstd_post [rows] fp32 may be NULL in the forward
  * and are what the backward reads. Backward: from dx_out and dy (either may be NULL, not both)
  * dx (x's dtype), dh (h's dtype), d_gate, d_weight, d_post_weight in their tensors' dtypes, each
- * of which may be NULL; the column sums need workspace of dsalt_branch_norm_workspace_size(rows,
- * d) bytes, dead when the launches end. fp32 arithmetic, sums in a fixed order.
+ * of which may be NULL and is refused where its tensor is missing (without dy d_weight is zero);
+ * the column sums need workspace of dsalt_branch_norm_workspace_size(rows, d) bytes, dead when the
+ * launches end. fp32 arithmetic, sums in a fixed order.
  * dtypes: x BF16 or F16 with h and y of the same, or x F32 with h and y of any; weights and gate
  * of x's dtype or F32. d a multiple of 8 up to 8192; 16-byte aligned pointers (statistics 4,
  * a [rows] gate its element's); outputs alias no input.

@@ -336,3 +336,24 @@ def test_one_dimensional_stream(gate, d):
                    for n, v in t.items()}, dz[None], dy[None], residual_scale=0.75, p=0.2, seed=77, offset=5, out_dtype=hd)
         assert all(torch.equal(a, b[0]) for a, b in zip(outs, two[0]))
         assert all(torch.equal(grads[n], two[1][n].view(grads[n].shape)) for n in grads)
+
+
+@pytest.mark.parametrize("rows", [0, 1, 700])
+def test_backward_entry_without_dy(rows):
+    """The C entry with d_weight wanted and no gradient of y: zeros, whatever the stream and the buffer
+    held; the other results as without d_weight."""
+    print(f"branch_norm backward without dy {rows}", flush=True)
+    t, dz, _ = inputs((rows,), 136, FP, BF, BF)
+    if rows:
+        t["x"][0, 3] = float("inf")
+    opts = (0.5, 0.0, 0, 1e-6, 1e-6, BF)
+    _, _, stats = _hip.branch_norm(*t.values(), opts, None, True)
+    want = _hip.branch_norm_bwd(*t.values(), opts, None, stats, dz, None, (True, True, False, True, True))
+    ws = torch.empty(max(16, _hip.lib().dsalt_branch_norm_workspace_size(rows, 136)), device=DEV, dtype=torch.uint8)
+    got = [torch.full_like(v, 7.0) for v in t.values()]
+    _hip._call("dsalt_branch_norm_bwd", _hip._branch_pack(
+        *t.values(), opts, None, rstd=stats.data_ptr(), rstd_post=stats.data_ptr() + 4 * rows, dx_out=dz.data_ptr(), dy=0,
+        grads=[g.data_ptr() for g in got], ws=(ws.data_ptr(), ws.numel())), dz.device)
+    assert not bool(got[2].any())
+    for i in (0, 1, 3, 4):
+        assert torch.equal(got[i], want[i]), i

@@ -134,3 +134,11 @@ def test_branch_norm_gate_kinds(lead):
         a = hip.BranchNormArgs.from_buffer_copy(hip._branch_pack(x, x, None, None, gate, opts, None))
         assert a.gate_kind == kind and a.d == d and a.rows * d == x.numel()
         assert gate is None or gate.numel() == (a.d if kind == 1 else a.rows)
+
+
+@pytest.mark.parametrize("kw", [{"weight": None, "dy": None}, {"gate": None, "gate_kind": 0}])
+def test_branch_norm_gradients_without_their_tensor(kw):
+    """The gradient of a weight or a gate that the call does not have would be left as it was."""
+    assert hip.lib().dsalt_branch_norm_check(ctypes.byref(branch_args(**kw)), 1) == 1
+    grads = {"d_weight": None} if "weight" in kw else {"d_gate": None}
+    assert hip.lib().dsalt_branch_norm_check(ctypes.byref(branch_args(**kw, **grads)), 1) == 0, hip.lib().dsalt_last_error()
