@@ -142,3 +142,14 @@ def test_branch_norm_gradients_without_their_tensor(kw):
     assert hip.lib().dsalt_branch_norm_check(ctypes.byref(branch_args(**kw)), 1) == 1
     grads = {"d_weight": None} if "weight" in kw else {"d_gate": None}
     assert hip.lib().dsalt_branch_norm_check(ctypes.byref(branch_args(**kw, **grads)), 1) == 0, hip.lib().dsalt_last_error()
+
+
+@pytest.mark.parametrize("rows,d,f,e,backward", [(1500, 1024, 2816, 1024, 0), (575, 264, 712, 264, 1), (700, 264, 712, 264, 1)])
+def test_gated_ffn_workspace_of_split_products(rows, d, f, e, backward):
+    """Sizes whose products are split along k keep partial sums: less workspace, or none, is refused."""
+    need = hip.lib().dsalt_gated_ffn_workspace_size(rows, d, f, e, backward)
+    assert need > 0
+    size = dict(rows=rows, d=d, f=f, e=e, x_stride=d, w_gate_stride=d, w_up_stride=d, w_down_stride=f, dy_stride=e)
+    for more, code in (({"workspace_bytes": need}, 0), ({"workspace_bytes": need - 1}, 1), ({"workspace_bytes": 0}, 1),
+                       ({"workspace": None}, 1), ({"workspace": 0x10000008}, 1)):
+        assert hip.lib().dsalt_gated_ffn_check(ctypes.byref(ffn_args(**size, **more)), backward) == code, more
