@@ -8,6 +8,7 @@ fallback: a missing library or a non-GPU tensor raises ``DsaltError``.
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 import struct
 from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p
@@ -1642,12 +1643,13 @@ def gated_ffn_bwd(x, w_gate, w_up, w_down, activation: str, kept, dy, need):
 
 
 def seed_fields(seed, device: torch.device) -> tuple[int, int]:
-    """(seed, seed_ptr) of a Python int or of an int64 GPU tensor of one element."""
+    """(seed, seed_ptr) of an int (numpy's too) or of an int64 GPU tensor of one element."""
     if isinstance(seed, torch.Tensor):
         if seed.device != device or seed.dtype != torch.int64 or seed.numel() != 1:
             raise DsaltError(f"a seed tensor must be one int64 element on {device} (got {tuple(seed.shape)} {seed.dtype} "
                              f"on {seed.device})")
         return 0, seed.data_ptr()
+    seed = operator.index(seed)
     if not -2 ** 63 <= seed < 2 ** 64:
         raise ValueError(f"seed must fit 64 bits (got {seed})")
     return (seed + 2 ** 63) % 2 ** 64 - 2 ** 63, 0

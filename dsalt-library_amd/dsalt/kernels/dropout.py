@@ -3,6 +3,8 @@ the backward forms it again. ``nn.Dropout`` draws from torch's generator and kee
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from .. import _hip
@@ -24,7 +26,7 @@ def check_seed(p: float, seed, offset: int, device: torch.device) -> None:
             raise ValueError("a dropout probability above 0 needs a seed")
     else:
         _hip.seed_fields(seed, device)
-    if not 0 <= offset < 2 ** 63:
+    if not 0 <= operator.index(offset) < 2 ** 63:
         raise ValueError(f"offset must be in [0, 2^63) (got {offset})")
 
 

@@ -142,3 +142,10 @@ def test_scalars_and_no_elements():
     y = counter_dropout(empty, 0.5, 3)
     g, = torch.autograd.grad(y, empty, torch.zeros_like(y))
     assert y.shape == g.shape == (4, 0, 8)
+
+
+def test_numpy_seeds_and_offsets():
+    x = torch.randn(100, device=DEV, requires_grad=True)
+    for seed, offset in ((np.int64(-7), np.int32(3)), (np.uint64(2 ** 64 - 7), np.int64(3))):
+        y = counter_dropout(x, 0.4, seed, offset)
+        assert torch.equal(y, want(x, 0.4, -7, 3)) and torch.equal(torch.autograd.grad(y, x, x)[0], y)

@@ -8,6 +8,7 @@ import torch
 
 import dsalt._hip as hip
 from dsalt.kernels import branch_norm, counter_dropout, gated_ffn
+from dsalt.kernels.dropout import check_seed
 from philox_reference import keep_mask, philox4x32
 
 
@@ -153,3 +154,18 @@ def test_gated_ffn_workspace_of_split_products(rows, d, f, e, backward):
     for more, code in (({"workspace_bytes": need}, 0), ({"workspace_bytes": need - 1}, 1), ({"workspace_bytes": 0}, 1),
                        ({"workspace": None}, 1), ({"workspace": 0x10000008}, 1)):
         assert hip.lib().dsalt_gated_ffn_check(ctypes.byref(ffn_args(**size, **more)), backward) == code, more
+
+
+@pytest.mark.parametrize("integer", [np.int64, np.int32, np.uint64, np.uint8, int])
+def test_seeds_and_offsets_of_any_integer_type(integer):
+    """A seed or offset that a program drew with numpy is its value; one that is no integer is refused by
+    type, before anything is packed."""
+    dev = torch.device("cuda", 0)
+    info = None if integer is int else np.iinfo(integer)
+    for v in (0, 5, int(info.max) if info else 2 ** 64 - 1, int(info.min) if info else -2 ** 63):
+        assert hip.seed_fields(integer(v), dev) == hip.seed_fields(v, dev)
+        check_seed(0.1, integer(v), integer(abs(v) % 100), dev)
+    for bad in (1.0, "1", np.float64(2)):
+        for seed, offset in ((bad, 0), (1, bad)):
+            with pytest.raises(TypeError):
+                check_seed(0.1, seed, offset, dev)
