@@ -201,22 +201,31 @@ class DSALTTransformerBlock(nn.Module):
             p = drop.p if drop.training else 0.0
             if p > 0 and seed is None:
                 seed = draw_seed(x.device)
-            x, h = self._join(x, f, self.ffn_post_norm, self.ffn_gate, next_norm, x.dtype, p, seed)
+            x, h = self._join(x, f, self.ffn_post_norm, self.ffn_gate, next_norm, None, p, seed)
         else:
-            x, h = self._join(x, run(self.ffn, h), self.ffn_post_norm, self.ffn_gate, next_norm, x.dtype)
+            x, h = self._join(x, run(self.ffn, h), self.ffn_post_norm, self.ffn_gate, next_norm, None)
         return x, h, aux
 
     def _join(self, x, o, post, gate, norm, out_dtype, p: float = 0.0, seed=None):
-        """x joined with the branch's output o, and its norm: norms that are replaced or hooked are
-        called as they are."""
+        """x joined with the branch's output o, and its norm (in out_dtype; None: the sum's): norms that
+        are replaced or hooked are called as they are. The sum has the type that x + o has: a
+        16-bit stream beside an fp32 o (a replaced norm's, under autocast) goes on in fp32."""
         def inside(m):
             return m is None or (type(m) is RMSENorm and _block_train.plain(m))
 
         offset = self.layer_idx + 1
         if not inside(post):
             o, p, post = post(counter_dropout(o, p, seed, offset) if p > 0 else o), 0.0, None
+        wide = torch.promote_types(x.dtype, o.dtype)
+        if wide is not x.dtype:
+            x = x.to(wide)
+
+        def taken(w):
+            return w if w is None or w.dtype is wide or w.dtype is torch.float32 else w.to(wide)
+
         n = norm if inside(norm) else None
-        x, h = branch_norm(x, o, None if n is None else n.weight, post_weight=None if post is None else post.weight, gate=gate,
+        x, h = branch_norm(x, o, None if n is None else taken(n.weight),
+                           post_weight=None if post is None else taken(post.weight), gate=taken(gate),
                            residual_scale=self.residual_scale, p=p, seed=seed, offset=offset,
                            eps=1e-6 if n is None else n.eps, post_eps=1e-6 if post is None else post.eps,
                            out_dtype=out_dtype if n is not None else None)

@@ -265,3 +265,78 @@ def test_unpacked_input_and_odd_widths():
             assert (p is None and q is None) or (torch.isfinite(p).all() and torch.equal(p, q))
         missing = [n for (n, _), g in zip(b.named_parameters(), res[0][2:]) if g is None]
         assert not [n for n in missing if "ffn" in n or "gate" in n and "win" not in n or "norm" in n], missing
+
+
+class Widened(torch.nn.Module):
+    """A module's result in fp32, as torch's normalisations give it under autocast."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, x):
+        return self.inner(x).float()
+
+
+REPLACED = {"attn_post_norm": lambda b: torch.nn.LayerNorm(128), "ffn_post_norm": lambda b: torch.nn.LayerNorm(128),
+            "ffn": lambda b: Widened(copy.deepcopy(b.ffn))}
+
+
+@pytest.mark.parametrize("which", list(REPLACED))
+@pytest.mark.parametrize("stream,weights,autocast", [(BF, FP, BF), (HF, FP, HF), (BF, BF, None), (FP, FP, BF)])
+def test_replaced_modules_that_return_fp32(which, stream, weights, autocast):
+    """A replaced norm or feed-forward that returns fp32 beside a 16-bit stream: the sum is fp32, as
+    torch's addition promotes it. Values and gradients against the composition in torch's ops."""
+    print(f"replaced {which} {stream} {weights} {autocast}", flush=True)
+    b = block(weights, dropout=0.0)
+    setattr(b, which, REPLACED[which](b).to(DEV))
+    cu = torch.tensor(CU, dtype=torch.int32, device=DEV)
+    x, dy = (torch.randn(CU[-1], 128, device=DEV, generator=torch.Generator(DEV).manual_seed(s)).to(stream) for s in (1, 2))
+
+    def norm(m, t):  # LayerNorm in fp32 where the run is without autocast
+        if type(m) is not torch.nn.LayerNorm:
+            return F.rms_norm(t.float(), (128,), m.weight.float(), m.eps)
+        return F.layer_norm(t.float(), (128,), m.weight.float(), m.bias.float(), m.eps)
+
+    def composed_run(xi):
+        o, _ = b.attn(norm(b.attn_norm, xi).to(xi.dtype), cu_seqlens=cu, max_seqlen=256)
+        z = b.residual_scale * xi.float() + b.attn_gate.float() * norm(b.attn_post_norm, o)
+        if which != "attn_post_norm":
+            z = z.to(xi.dtype)
+        f = b.ffn(norm(b.ffn_norm, z).to(autocast or weights))
+        return b.residual_scale * z.float() + b.ffn_gate.float() * norm(b.ffn_post_norm, f)
+
+    if weights != FP:  # without autocast LayerNorm's input has its weight's type
+        for n in ("attn_post_norm", "ffn_post_norm"):
+            m = getattr(b, n)
+            if type(m) is torch.nn.LayerNorm:
+                m.forward = lambda t, m=m: F.layer_norm(t.float(), (128,), m.weight, m.bias, m.eps)
+    res = []
+    for fn in (lambda xi: b(xi, cu_seqlens=cu, max_seqlen=256)[0], composed_run):
+        xi = x.clone().requires_grad_()
+        b.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", dtype=autocast or BF, enabled=autocast is not None):
+            y = fn(xi)
+        y.backward(dy.to(y.dtype))
+        res.append([("y", y.detach()), ("x", xi.grad)] + [(n, p.grad) for n, p in b.named_parameters() if p.grad is not None])
+    assert res[0][0][1].dtype == FP and [n for n, _ in res[0]] == [n for n, _ in res[1]]
+    u = torch.finfo(autocast or weights).eps / 2  # test_block's count of roundings
+    for (n, a), (_, c) in zip(*res):
+        assert a.dtype == c.dtype, n
+        err, size = float((a.float() - c.float()).norm()), float(c.float().norm())
+        assert err <= 24 * u * size + 1e-6, (n, err / max(size, 1e-12), u)
+
+
+@pytest.mark.parametrize("which", ["attn_post_norm", "ffn_post_norm"])
+def test_lm_with_replaced_norms_under_autocast(which):
+    m = lm().train()
+    for layer in m.layers:
+        setattr(layer, which, torch.nn.LayerNorm(128).to(DEV))
+    ids = torch.randint(0, 500, (CU[-1],), device=DEV)
+    cu = torch.tensor(CU, dtype=torch.int32, device=DEV)
+    with torch.autocast("cuda", dtype=BF):
+        loss = m(ids, cu_seqlens=cu, max_seqlen=256, labels=ids)["loss"]
+    loss.backward()
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in m.parameters())
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF):
+        assert bool(torch.isfinite(m.eval()(ids, cu_seqlens=cu, max_seqlen=256)["logits"]).all())
