@@ -214,7 +214,8 @@ def swiglu_supported(ffn, x: torch.Tensor) -> bool:
     without bias, of one dtype that is x's own, or fp32 under a 16-bit autocast (x fp32 or
     already rounded)."""
     lin = (ffn.gate_proj, ffn.up_proj, ffn.down_proj)
-    if not (eager(x, *(m.weight for m in lin)) and x.is_cuda and x.dim() >= 2 and x.numel() and all(type(m) is nn.Linear for m in lin) and plain(*lin)):
+    if not (x.is_cuda and x.dim() >= 2 and x.numel() and all(type(m) is nn.Linear for m in lin) and plain(*lin)
+            and eager(x, *(m.weight for m in lin))):
         return False
     wg, wu, wd = (m.weight for m in lin)
     if any(m.bias is not None for m in lin) or any(w.dtype != wg.dtype or w.device != x.device for w in (wg, wu, wd)):

@@ -340,3 +340,16 @@ def test_lm_with_replaced_norms_under_autocast(which):
     assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in m.parameters())
     with torch.no_grad(), torch.autocast("cuda", dtype=BF):
         assert bool(torch.isfinite(m.eval()(ids, cu_seqlens=cu, max_seqlen=256)["logits"]).all())
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_projections_without_a_weight(fused):
+    """A projection replaced by a module that has no weight of its own is called as it is, in training too."""
+    torch.manual_seed(1)
+    ffn = SwiGLUFFN(64, 128, fused=fused).to(DEV)
+    x = torch.randn(5, 64, device=DEV, requires_grad=True)
+    want, = torch.autograd.grad(ffn(x).sum(), x)
+    ffn.up_proj = Widened(ffn.up_proj)
+    got, = torch.autograd.grad(ffn(x).sum(), x)
+    # fp32 sums of 64 and 128 terms in another order on either side
+    assert float((got - want).norm()) <= 2.0 ** -17 * float(want.norm())
