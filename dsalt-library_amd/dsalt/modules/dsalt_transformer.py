@@ -192,8 +192,8 @@ class DSALTTransformerBlock(nn.Module):
             return torch.utils.checkpoint.checkpoint(fn, t, use_reentrant=False) if recompute else fn(t)
 
         o, aux = run(lambda t: self.attn(t, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, rope_cs=rope_cs, cu_list=cu_list), h)
-        # the feed-forward's operand in the type that its projections compute in
-        low = _block_train.autocast_dtype(x) if x.is_cuda and x.dtype == torch.float32 else x.dtype
+        # the norm in the type that the feed-forward's projections compute in, where only they read it
+        low = None if not self._plain_ffn() else _block_train.autocast_dtype(x) if x.dtype == torch.float32 else x.dtype
         x, h = self._join(x, o, self.attn_post_norm, self.attn_gate, self.ffn_norm, low)
         drop = self.ffn.drop if type(self.ffn) is SwiGLUFFN else None
         if type(drop) is CounterDropout and _block_train.plain(self.ffn, drop):
@@ -205,6 +205,13 @@ class DSALTTransformerBlock(nn.Module):
         else:
             x, h = self._join(x, run(self.ffn, h), self.ffn_post_norm, self.ffn_gate, next_norm, None)
         return x, h, aux
+
+    def _plain_ffn(self) -> bool:
+        """Whether nothing but plain projections reads the feed-forward's operand."""
+        if type(self.ffn) is not SwiGLUFFN:
+            return False
+        lin = (self.ffn.gate_proj, self.ffn.up_proj)
+        return all(type(m) is nn.Linear for m in lin) and _block_train.plain(self.ffn, *lin)
 
     def _join(self, x, o, post, gate, norm, out_dtype, p: float = 0.0, seed=None):
         """x joined with the branch's output o, and its norm (in out_dtype; None: the sum's): norms that

@@ -353,3 +353,25 @@ def test_projections_without_a_weight(fused):
     got, = torch.autograd.grad(ffn(x).sum(), x)
     # fp32 sums of 64 and 128 terms in another order on either side
     assert float((got - want).norm()) <= 2.0 ** -17 * float(want.norm())
+
+
+@pytest.mark.parametrize("how", ["replaced", "hooked", "projection replaced", "projection hooked"])
+def test_feed_forward_sees_the_stream_type(how):
+    """Under autocast an fp32 stream's norm is rounded for the feed-forward only where plain projections,
+    which round it themselves, are all that reads it."""
+    b = block(FP, dropout=0.0, fused_ffn=False)
+    seen = []
+    if how == "replaced":
+        b.ffn = Widened(b.ffn)
+        target = b.ffn
+    else:
+        target = b.ffn if how == "hooked" else b.ffn.up_proj
+        if how == "projection replaced":
+            target = b.ffn.up_proj = Widened(b.ffn.up_proj)
+    target.register_forward_pre_hook(lambda m, i: seen.append(i[0].dtype))
+    cu = torch.tensor(CU, dtype=torch.int32, device=DEV)
+    x = torch.randn(CU[-1], 128, device=DEV)
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), torch.autocast("cuda", dtype=BF):
+            b(x, cu_seqlens=cu, max_seqlen=256)
+    assert seen == [FP, FP]
