@@ -1642,16 +1642,24 @@ def gated_ffn_bwd(x, w_gate, w_up, w_down, activation: str, kept, dy, need):
     return dx, dwg, dwu, dwd
 
 
-def seed_fields(seed, device: torch.device) -> tuple[int, int]:
-    """(seed, seed_ptr) of an int (numpy's too) or of an int64 GPU tensor of one element."""
+def check_seed(seed, device: torch.device):
+    """seed as an int of 64 bits (from numpy's too), or the int64 GPU tensor of one element that it is."""
     if isinstance(seed, torch.Tensor):
         if seed.device != device or seed.dtype != torch.int64 or seed.numel() != 1:
             raise DsaltError(f"a seed tensor must be one int64 element on {device} (got {tuple(seed.shape)} {seed.dtype} "
                              f"on {seed.device})")
-        return 0, seed.data_ptr()
+        return seed
     seed = operator.index(seed)
     if not -2 ** 63 <= seed < 2 ** 64:
         raise ValueError(f"seed must fit 64 bits (got {seed})")
+    return seed
+
+
+def seed_fields(seed, device: torch.device) -> tuple[int, int]:
+    """(seed, seed_ptr) of a seed that check_seed takes."""
+    seed = check_seed(seed, device)
+    if isinstance(seed, torch.Tensor):
+        return 0, seed.data_ptr()
     return (seed + 2 ** 63) % 2 ** 64 - 2 ** 63, 0
 
 

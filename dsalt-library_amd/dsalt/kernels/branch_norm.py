@@ -8,14 +8,13 @@ from __future__ import annotations
 import torch
 
 from .. import _hip
-from ._block_train import graph_grads, without_autocast
-from ._sparse import no_graph
-from .dropout import _Dropout, check_seed
+from ._block_train import eager, graph_grads, without_autocast
+from .dropout import check_seed, counter_dropout
 from .dsalt_triton_attn import _dynamo_opaque
 
 
 def torch_branch_norm(x, h, weight, post_weight, gate, opts, seed):
-    """``branch_norm`` in torch's ops (and the dropout pass), in fp32 or more."""
+    """``branch_norm`` in torch's ops and ``counter_dropout``, in fp32 or more."""
     residual_scale, p, offset, eps, post_eps, out_dtype = opts
 
     def wide(t):
@@ -26,7 +25,7 @@ def torch_branch_norm(x, h, weight, post_weight, gate, opts, seed):
 
     n = wide(h)
     if _hip.keep_threshold(p) < 65536:
-        n = _Dropout.apply(n, p, seed, offset)
+        n = counter_dropout(n, p, seed, offset)
     if post_weight is not None:
         n = norm(n, post_weight, post_eps)
     z = residual_scale * wide(x) + (n if gate is None else wide(gate) * n)
@@ -89,7 +88,9 @@ def branch_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor | None = 
     [..., 1], or none. x bf16, fp16 or fp32; h and ``out_dtype`` (y's type, by default x's) x's
     dtype, or any of the three beside an fp32 x; weights and gate in x's dtype or fp32. x_out has
     x's dtype; y is formed from the sum before that rounding. d a multiple of 8 up to 8192.
-    Differentiable in x, h, weight, post_weight and gate. Other operands raise ``DsaltError``."""
+    Differentiable in x, h, weight, post_weight and gate; functorch's transforms, forward-mode
+    differentiation, tracing and tensor subclasses take torch's ops instead. Other operands raise
+    ``DsaltError``."""
     dev, dtype = x.device, x.dtype
     out_dtype = dtype if out_dtype is None else out_dtype
     check_seed(p, seed, offset, dev)
@@ -109,6 +110,9 @@ def branch_norm(x: torch.Tensor, h: torch.Tensor, weight: torch.Tensor | None = 
             f"output in x's dtype or x fp32, weights [d] and a gate [d] or [..., 1] in x's dtype or fp32 (got "
             f"{[None if t is None else (tuple(t.shape), t.dtype) for t in (x, h, weight, post_weight, gate)]}, {out_dtype})")
     opts = (float(residual_scale), p, offset, float(eps), float(eps if post_eps is None else post_eps), out_dtype)
-    if no_graph(x, h, weight, post_weight, gate):
+    tensors = (x, h, weight, post_weight, gate, seed if isinstance(seed, torch.Tensor) else None)
+    if not eager(*(t for t in tensors if t is not None)):
+        return torch_branch_norm(x, h, weight, post_weight, gate, opts, seed)
+    if not torch.is_grad_enabled():
         return _hip.branch_norm(*_operands(x, h, weight, post_weight, gate), opts, seed, False)[:2]
     return _BranchNorm.apply(x, h, weight, post_weight, gate, seed, opts)

@@ -8,7 +8,7 @@ import operator
 import torch
 
 from .. import _hip
-from ._sparse import no_graph
+from ._block_train import eager
 from .dsalt_triton_attn import _dynamo_opaque
 
 
@@ -25,9 +25,27 @@ def check_seed(p: float, seed, offset: int, device: torch.device) -> None:
         if threshold < 65536:
             raise ValueError("a dropout probability above 0 needs a seed")
     else:
-        _hip.seed_fields(seed, device)
+        _hip.check_seed(seed, device)
     if not 0 <= operator.index(offset) < 2 ** 63:
         raise ValueError(f"offset must be in [0, 2^63) (got {offset})")
+
+
+def torch_counter_dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
+    """``counter_dropout`` in torch's ops, the same bits: Philox4x32 with 7 rounds at counter (i / 8, offset)
+    under key seed in int64 arithmetic, 16 bits for each of eight consecutive elements."""
+    threshold, low, n = _hip.keep_threshold(p), 0xFFFFFFFF, x.numel()
+    seed, offset = seed if isinstance(seed, torch.Tensor) else operator.index(seed), operator.index(offset)
+    ctr = torch.arange(-(-n // 8), device=x.device)
+    c0, c1, c2, c3 = ctr & low, ctr >> 32, torch.full_like(ctr, offset & low), torch.full_like(ctr, offset >> 32)
+    k0, k1 = seed & low, (seed >> 32) & low
+    for _ in range(7):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57  # the low 64 bits of the products
+        c0, c1, c2, c3 = ((b >> 32) & low) ^ c1 ^ k0, b & low, ((a >> 32) & low) ^ c3 ^ k1, a & low
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    words = torch.stack((c0, c1, c2, c3), -1)
+    keep = (torch.stack((words & 0xFFFF, words >> 16), -1).reshape(-1)[:n] < threshold).view(x.shape)
+    scale = torch.tensor(65536 / threshold if threshold else 0.0, dtype=torch.float32).item()  # as the kernels hold it
+    return torch.where(keep, x.float() * scale, 0.0).to(x.dtype)
 
 
 class _Dropout(torch.autograd.Function):
@@ -59,12 +77,16 @@ def counter_dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.T
     the kernel runs: a replayed graph sees its new value), ``offset`` (0 to 2^63 - 1: tells
     apart the places that use one seed) and the element's index in x's logical order, and
     on nothing else. bf16, fp16 or fp32 of any shape. Differentiable in x; a seed tensor
-    changed in place before the backward is refused."""
+    changed in place before the backward is refused. Under functorch's transforms, forward-mode
+    differentiation and tracing, and for tensor subclasses, torch's ops run instead, with the
+    same bits (under vmap an example's element has its index in the example)."""
     dev = _hip.require_gpu(x)
     if x.dtype not in _hip._SCORE_DTYPES:
         raise _hip.DsaltError(f"counter_dropout needs a bf16, fp16 or fp32 tensor (got {x.dtype})")
     check_seed(p, seed, offset, dev)
     seed = 0 if seed is None else seed
-    if no_graph(x):
+    if not eager(x, *((seed,) if isinstance(seed, torch.Tensor) else ())):
+        return torch_counter_dropout(x, p, seed, offset)
+    if not torch.is_grad_enabled():
         return _hip.dropout(_hip.aligned_rows(x), p, seed, offset)
     return _Dropout.apply(x, p, seed, offset)

@@ -13,8 +13,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _hip
-from ._block_train import autocast_dtype, graph_grads, without_autocast
-from ._sparse import no_graph
+from ._block_train import autocast_dtype, eager, graph_grads, without_autocast
 from .dsalt_triton_attn import _dynamo_opaque
 
 _TORCH_ACT = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"), "relu": F.relu}
@@ -95,7 +94,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     bf16 or fp16, all of one dtype; under a 16-bit autocast fp32 tensors are cast to its dtype
     first. d, e and f multiples of 8. Row strides and any number of rows, none included, are
-    taken. Differentiable in every tensor. Other operands raise ``DsaltError``."""
+    taken. Differentiable in every tensor; functorch's transforms, forward-mode differentiation,
+    tracing and tensor subclasses take torch's ops instead. Other operands raise ``DsaltError``."""
     if activation not in _hip.ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(_hip.ACTIVATIONS)}, got {activation!r}")
     if not gated_ffn_supported(x, w_gate, w_up, w_down):
@@ -106,6 +106,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if torch.is_autocast_enabled("cuda"):
         dt = autocast_dtype(x)
         x, w_gate, w_up, w_down = x.to(dt), w_gate.to(dt), w_up.to(dt), w_down.to(dt)
-    if no_graph(x, w_gate, w_up, w_down):
+    if not eager(x, w_gate, w_up, w_down):
+        return torch_gated_ffn(x, w_gate, w_up, w_down, activation)
+    if not torch.is_grad_enabled():
         return _run(x, w_gate, w_up, w_down, activation, False)[0]
     return _GatedFFN.apply(x, w_gate, w_up, w_down, activation)

@@ -357,3 +357,42 @@ def test_backward_entry_without_dy(rows):
     assert not bool(got[2].any())
     for i in (0, 1, 3, 4):
         assert torch.equal(got[i], want[i]), i
+
+
+class Tagged(torch.Tensor):
+    """A tensor subclass with nothing of its own."""
+
+
+@pytest.mark.parametrize("p", [0.0, 0.2])
+def test_transforms_tracing_and_subclasses(p):
+    """What an autograd function with a HIP kernel does not know runs as torch's ops: the kernels' values
+    within their fp32 roundings."""
+    t, dz, dy = inputs((6,), 64, FP, FP, FP, gate="token")
+    ts = tuple(t.values())
+
+    def call(x, h, w, post, gate):
+        return branch_norm(x, h, w, post_weight=post, gate=gate, residual_scale=0.75, p=p, seed=5, offset=2)
+
+    with torch.no_grad():
+        want = call(*ts)
+    _, grads = run(t, dz, dy, residual_scale=0.75, p=p, seed=5, offset=2)
+    got = torch.func.grad(lambda ts: sum((o * u).sum() for o, u in zip(call(*ts), (dz, dy))))(ts)
+    for n, g in zip(NAMES, got):
+        close(g, grads[n].double(), FP, n, 6)
+    vs = tuple(torch.randn_like(v) for v in ts)
+    _, tangents = torch.func.jvp(call, ts, vs)
+    # sum of outputs' tangents against the upstream gradients = sum of the gradients against the tangents
+    a = sum(float((o.double() * u.double()).sum()) for o, u in zip(tangents, (dz, dy)))
+    parts = [(grads[n].double() * v.double()) for n, v in zip(NAMES, vs)]
+    assert abs(a - sum(float(q.sum()) for q in parts)) <= 2.0 ** -18 * sum(float(q.abs().sum()) for q in parts)
+    for o, w in zip(torch.jit.trace(call, ts)(*ts), want):
+        close(o, w.double(), FP, "traced")
+    for o, w in zip(call(ts[0].as_subclass(Tagged), *ts[1:]), want):
+        assert type(o) is Tagged
+        close(o.as_subclass(torch.Tensor), w.double(), FP, "subclass")
+    # each example a row [d] with a gate [1]: the mask of one row for all of them
+    rows = torch.func.vmap(call, in_dims=(0, 0, None, None, 0))(*ts)
+    with torch.no_grad():
+        for i in range(6):
+            for o, w in zip(rows, call(ts[0][i], ts[1][i], ts[2], ts[3], ts[4][i])):
+                close(o[i], w.double(), FP, "vmap")

@@ -149,3 +149,28 @@ def test_numpy_seeds_and_offsets():
     for seed, offset in ((np.int64(-7), np.int32(3)), (np.uint64(2 ** 64 - 7), np.int64(3))):
         y = counter_dropout(x, 0.4, seed, offset)
         assert torch.equal(y, want(x, 0.4, -7, 3)) and torch.equal(torch.autograd.grad(y, x, x)[0], y)
+
+
+class Tagged(torch.Tensor):
+    """A tensor subclass with nothing of its own."""
+
+
+def test_transforms_tracing_and_subclasses():
+    """What an autograd function with a HIP kernel does not know runs as torch's ops, with the same bits."""
+    x, up = torch.randn(6, 50, device=DEV), torch.randn(6, 50, device=DEV)
+    seed = torch.tensor([21], device=DEV)
+    for s in (21, seed):
+        drop = lambda t: counter_dropout(t, 0.3, s, 4)
+        mask, each = want(torch.ones_like(x), 0.3, 21, 4), want(torch.ones(50, device=DEV), 0.3, 21, 4)
+        assert torch.equal(torch.func.grad(lambda t: (drop(t) * up).sum())(x), want(up, 0.3, 21, 4))
+        assert torch.equal(torch.func.jvp(drop, (x,), (up,))[1], mask * up)
+        assert torch.equal(torch.func.vmap(drop)(x), x * each)
+        with torch.no_grad():
+            assert torch.equal(torch.func.vmap(drop)(x), x * each)
+        traced = torch.jit.trace(drop, (x,))
+        assert torch.equal(traced(up), up * mask)
+        got = drop(x.as_subclass(Tagged))
+        assert type(got) is Tagged and torch.equal(got.as_subclass(torch.Tensor), x * mask)
+    seeds = torch.arange(6, device=DEV)[:, None]
+    got = torch.func.vmap(lambda t, s: counter_dropout(t, 0.3, s, 4))(x, seeds)
+    assert torch.equal(got, torch.stack([want(x[i], 0.3, i, 4) for i in range(6)]))

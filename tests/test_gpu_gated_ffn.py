@@ -441,3 +441,20 @@ def test_gelu_of_far_negative_gates(dtype, lowest, up, scale, rows):
                           ("du", got["dx"][:, 1], scale * z * phi)):
         assert float(want.abs().min()) > torch.finfo(dtype).tiny and float(want.abs().max()) < torch.finfo(dtype).max
         assert bool(((have.double() - want).abs() <= bound * want.abs()).all()), (n, float((have.double() / want - 1).abs().max()))
+
+
+def test_transforms_and_tracing():
+    """What an autograd function with a HIP kernel does not know runs as torch's ops."""
+    x, wg, wu, wd, dy = inputs(12, 64, 72, 40, HF)
+    ref = reference(x, wg, wu, wd, dy, "silu", HF)
+    got = torch.func.grad(lambda t: (gated_ffn(t, wg, wu, wd).float() * dy.float()).sum())(x)
+    want = run(x, wg, wu, wd, dy, "silu")
+    # some five fp16 roundings in a chain on torch's side, two on the kernels', each half a step at most
+    near = lambda a, b: float((a.double() - b.double()).norm()) <= 7 * 2.0 ** -11 * float(b.double().norm())
+    assert near(got, want["dx"])
+    assert near(torch.jit.trace(lambda t: gated_ffn(t, wg, wu, wd), (x,), check_trace=False)(x), ref["y"][0])
+    assert near(torch.func.vmap(lambda t: gated_ffn(t, wg, wu, wd))(x.view(3, 4, 64)).view(12, 40), ref["y"][0])
+    v = torch.randn(12, 64, device=DEV).to(HF)
+    _, tangent = torch.func.jvp(lambda t: gated_ffn(t, wg, wu, wd), (x,), (v,))
+    size = float((want["dx"].double() * v.double()).abs().sum())
+    assert abs(float((tangent.double() * dy.double()).sum() - (want["dx"].double() * v.double()).sum())) <= 7 * 2.0 ** -11 * size

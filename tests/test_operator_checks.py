@@ -8,7 +8,7 @@ import torch
 
 import dsalt._hip as hip
 from dsalt.kernels import branch_norm, counter_dropout, gated_ffn
-from dsalt.kernels.dropout import check_seed
+from dsalt.kernels.dropout import check_seed, torch_counter_dropout
 from philox_reference import keep_mask, philox4x32
 
 
@@ -169,3 +169,15 @@ def test_seeds_and_offsets_of_any_integer_type(integer):
         for seed, offset in ((bad, 0), (1, bad)):
             with pytest.raises(TypeError):
                 check_seed(0.1, seed, offset, dev)
+
+
+@pytest.mark.parametrize("n", [0, 1, 7, 8, 1003])
+@pytest.mark.parametrize("p,seed,offset", [(0.25, 11, 3), (0.5, -2 ** 63, 2 ** 63 - 1), (0.97, 2 ** 64 - 1, 2 ** 32), (1.0, 0, 0), (0.0, 5, 1)])
+def test_dropout_in_torch_ops_has_the_same_mask(n, p, seed, offset):
+    x = torch.randn(n, generator=torch.Generator().manual_seed(n))
+    keep = torch.from_numpy(keep_mask(n, p, seed, offset))
+    scale = np.float32(65536 / max(hip.keep_threshold(p), 1)).item()
+    want = torch.where(keep, x * scale, 0.0)
+    assert torch.equal(torch_counter_dropout(x, p, seed, offset), want)
+    tensor = torch.tensor([(seed + 2 ** 63) % 2 ** 64 - 2 ** 63])
+    assert torch.equal(torch_counter_dropout(x.bfloat16(), p, tensor, offset), torch.where(keep, x.bfloat16().float() * scale, 0.0).bfloat16())
