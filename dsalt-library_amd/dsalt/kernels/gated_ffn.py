@@ -24,6 +24,11 @@ def torch_gated_ffn(x, w_gate, w_up, w_down, activation: str):
     return F.linear(_TORCH_ACT[activation](F.linear(x, w_gate)) * F.linear(x, w_up), w_down)
 
 
+def _versions(*ws):
+    """What tells whether a tensor was changed in place (inference tensors count no versions)."""
+    return tuple(None if w.is_inference() else w._version for w in ws)
+
+
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
@@ -34,7 +39,7 @@ class _GatedFFN(torch.autograd.Function):
         y, kept = _run(x, w_gate, w_up, w_down, activation, inner)
         ctx.save_for_backward(x if inner else None, *((w_gate, w_up) if need[0] else (None, None)),
                               w_down if inner else None, kept)
-        ctx.dsalt = x.shape, (w_gate, w_up, w_down), (w_gate._version, w_up._version, w_down._version), activation
+        ctx.dsalt = x.shape, (w_gate, w_up, w_down), _versions(w_gate, w_up, w_down), activation
         return y
 
     @staticmethod
@@ -44,7 +49,7 @@ class _GatedFFN(torch.autograd.Function):
         shape, ws, versions, activation = ctx.dsalt
         need = ctx.needs_input_grad[:4]
         if torch.is_grad_enabled():  # a graph of the backward is wanted: torch's own ops
-            if tuple(w._version for w in ws) != versions:
+            if _versions(*ws) != versions:
                 raise RuntimeError("a weight of gated_ffn was changed in place before a backward that records a graph")
             if x is None:  # only w_down has a gradient
                 act = kept.view(dy.dtype).view(*shape[:-1], ws[2].shape[1])

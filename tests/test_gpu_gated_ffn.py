@@ -458,3 +458,29 @@ def test_transforms_and_tracing():
     _, tangent = torch.func.jvp(lambda t: gated_ffn(t, wg, wu, wd), (x,), (v,))
     size = float((want["dx"].double() * v.double()).abs().sum())
     assert abs(float((tangent.double() * dy.double()).sum() - (want["dx"].double() * v.double()).sum())) <= 7 * 2.0 ** -11 * size
+
+
+@pytest.mark.parametrize("rows", [5, 140])
+def test_frozen_inference_tensors(rows):
+    """Weights and rows loaded under inference_mode, which count no versions, beside a trainable down
+    projection: as linears, which save neither."""
+    x, wg, wu, wd, dy = inputs(rows, 64, 72, 40, BF)
+    want = run(x, wg, wu, wd, dy, "silu")
+    with torch.inference_mode():
+        frozen = [t.clone() for t in (x, wg, wu)]
+    w = wd.clone().requires_grad_()
+    y = gated_ffn(*frozen, w)
+    assert torch.equal(y, want["y"]) and torch.equal(torch.autograd.grad(y, w, dy)[0], want["dwd"])
+    y = gated_ffn(*frozen, w)
+    up = dy.clone().requires_grad_()
+    g, = torch.autograd.grad(y, w, up, create_graph=True)
+    assert torch.autograd.grad(g.sum(), up)[0].shape == up.shape
+    gate = wg.clone().requires_grad_()
+    for graph in (False, True):
+        g, = torch.autograd.grad(gated_ffn(x, gate, frozen[2], wd), gate, dy, create_graph=graph)
+        # with a graph the backward is torch's, with some five roundings to bf16 in a chain
+        assert torch.equal(g, want["dwg"]) if not graph else float((g - want["dwg"]).norm()) <= 7 * 2.0 ** -8 * float(g.norm())
+    with pytest.raises(RuntimeError, match="[Ii]nference"):  # a gradient that reads them is refused by torch
+        gated_ffn(x.clone().requires_grad_(), *frozen[1:], wd)
+    with torch.inference_mode():
+        assert torch.equal(gated_ffn(*frozen, wd), want["y"])
