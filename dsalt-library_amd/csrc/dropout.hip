@@ -12,16 +12,10 @@
 namespace dsalt {
 namespace {
 
-template <typename DT>
-__device__ __forceinline__ float load1(const void *p, int64_t i) {
-    return Elem<DT>::ld(p, i);
-}
-
 // A thread takes groups of eight elements; the last, partial one goes to the thread after
-// the last full one.
+// the last full one. out may be x: a thread reads its elements before it writes them.
 template <typename DT>
-__global__ void __launch_bounds__(256) dropout_kernel(const void *__restrict__ x, void *__restrict__ out, int64_t n,
-                                                      const DropoutParams p) {
+__global__ void __launch_bounds__(256) dropout_kernel(const void *x, void *out, int64_t n, const DropoutParams p) {
     const uint64_t seed = dropout_seed(p);
     const int64_t full = n / 8, stride = (int64_t)gridDim.x * 256;
     int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -36,7 +30,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const void *__restrict__ x
     if (g == full) {
         const uint32_t m = keep8((uint64_t)g, p, seed);
         for (int64_t i = g * 8; i < n; ++i)
-            Elem<DT>::st(out, i, (m >> (i & 7)) & 1u ? load1<DT>(x, i) * p.scale : 0.f);
+            Elem<DT>::st(out, i, (m >> (i & 7)) & 1u ? Elem<DT>::ld(x, i) * p.scale : 0.f);
     }
 }
 

@@ -174,3 +174,14 @@ def test_transforms_tracing_and_subclasses():
     seeds = torch.arange(6, device=DEV)[:, None]
     got = torch.func.vmap(lambda t, s: counter_dropout(t, 0.3, s, 4))(x, seeds)
     assert torch.equal(got, torch.stack([want(x[i], 0.3, i, 4) for i in range(6)]))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n", [5, 8, 4099, 5000011])
+def test_entry_in_place(n, dtype):
+    """The C entry takes out = x."""
+    x = torch.randn(n, device=DEV).to(dtype)
+    ref = want(x, 0.3, 9, 1)
+    _hip._call("dsalt_dropout", _hip._DROPOUT_PACK.pack(n, _hip._SCORE_DTYPES[dtype], _hip.keep_threshold(0.3), x.data_ptr(),
+                                                        x.data_ptr(), 9, 1, 0), x.device)
+    assert torch.equal(x, ref)
