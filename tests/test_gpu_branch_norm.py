@@ -396,3 +396,26 @@ def test_transforms_tracing_and_subclasses(p):
         for i in range(6):
             for o, w in zip(rows, call(ts[0][i], ts[1][i], ts[2], ts[3], ts[4][i])):
                 close(o[i], w.double(), FP, "vmap")
+
+
+@pytest.mark.parametrize("gate", ["channel", "token"])
+def test_against_differences(gate):
+    """The kernels' gradients along random directions against central differences of the float64
+    function, which are off by h^2 / 6 of its third derivative (h = 1e-5: below 1e-8 of the size)."""
+    t, dz, dy = inputs((7,), 72, FP, FP, FP, gate=gate)
+    _, grads = run(t, dz, dy, residual_scale=0.75, p=0.2, seed=3, offset=1)
+    keep = torch.from_numpy(keep_mask(7 * 72, 0.2, 3, 1)).view(7, 72).to(DEV).double() * (65536 / _hip.keep_threshold(0.2))
+
+    def value(ts):
+        nrm = lambda v, w: v * torch.rsqrt(v.square().mean(-1, keepdim=True) + 1e-6) * w
+        x_out = 0.75 * ts["x"] + ts["gate"] * nrm(ts["h"] * keep, ts["post_weight"])
+        return float((x_out * dz.double()).sum() + (nrm(x_out, ts["weight"]) * dy.double()).sum())
+
+    g = torch.Generator(device=DEV).manual_seed(1)
+    base = {n: v.double() for n, v in t.items()}
+    for n in NAMES:
+        v = torch.randn(t[n].shape, generator=g, device=DEV, dtype=torch.float64)
+        hi, lo = (value({**base, n: base[n] + s * 1e-5 * v}) for s in (1, -1))
+        parts = grads[n].double() * v
+        # fp32 gradients: a few 2^-24 of each, over sums of up to 504 terms
+        assert abs(float(parts.sum()) - (hi - lo) / 2e-5) <= 2.0 ** -18 * float(parts.abs().sum()) + 1e-6, n
