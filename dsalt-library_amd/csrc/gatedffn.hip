@@ -39,11 +39,12 @@ __device__ __forceinline__ void act_grad(float g, float &v, float &slope) {
         v = g * s;
         slope = s + g * s * (1.f - s) * (2.f * kGeluTanhC) * (1.f + 3.f * 0.044715f * c2);
     } else if constexpr (ACT == DSALT_ACT_GELU) {
-        // The tail 0.5 erfc(|g| / sqrt 2) is exp(-g^2 / 2), which the slope takes too, times t P(t) with t = 1 /
-        // (1 + 0.375 x), x = |g| / sqrt 2: as erfc(x) exp(x^2) falls like 1 / x, seven terms hold its relative
-        // error below 2^-20 for every x of a normal result (fitted in float64, largest relative error least). The
-        // exponent's fp32 rounding leaves 2^-16 of the tail at |g| = 13, 2^-19 below 4. Abramowitz and Stegun's
-        // 7.1.26, of two terms less, holds the absolute error instead, and is 2 % off at -10.
+        // The tail 0.5 erfc(|g| / sqrt 2) is exp(-g^2 / 2), which the slope takes too, times t P(t) with
+        // t = 1 / (1 + 0.375 x), x = |g| / sqrt 2: as erfc(x) exp(x^2) falls like 1 / x, seven terms hold
+        // its relative error below 2^-20 for every x of a normal result (fitted in float64, the largest
+        // relative error least). The exponent's fp32 rounding adds 2^-16 of the tail at |g| = 13, 2^-19
+        // below 4. Abramowitz and Stegun's 7.1.26, two terms less, holds the absolute error instead
+        // and is 2 % off at -10; 8192 x 1024 x 2816 took 1 % less with it.
         const float x = 0.7071067811865476f * fabsf(g), t = __builtin_amdgcn_rcpf(1.f + 0.375f * x);
         const float ex = fast_exp2(-0.5f * kLog2e * g * g);
         const float tail = 0.5f * ex * t *
@@ -97,9 +98,10 @@ __device__ __forceinline__ void gated_grad8(int act, const float (&g)[8], float 
 // g and u kept for the backward. Their gradients are rounded to the element type once, as operands
 // of the matrix units have to be, and so is every result; g and u rounded to it too would put
 // a third rounding into dx and the weights' gradients (1.8 times the error of the last rounding
-// alone, against 1.4 so; the extra byte costs under 1 % of a training pass of 16384 rows). So they keep the upper 20 bits of their fp32 value beside bf16 (four bits
-// more than it has), and the upper 24 beside fp16 (five more): the upper 16 bits in a plane of
-// gate | up rows, the rest in a plane behind it, a byte for both (low half g) or a byte each.
+// alone, against 1.4 so; the extra byte costs under 1 % of a training pass of 16384 rows). So they
+// keep the upper 20 bits of their fp32 value beside bf16 (four bits more than it has), and the upper
+// 24 beside fp16 (five more): the upper 16 bits in a plane of gate | up rows, the rest in a plane
+// behind it, a byte for both (low half g) or a byte each.
 template <class DT>
 struct Kept {
     static constexpr bool NIBBLE = std::is_same<DT, BF16>::value;
@@ -192,7 +194,7 @@ enum { kEpiPair, kEpiStore, kEpiGrad };
 // one after the other they would cost a trip to memory for every 16 bytes of a lane. (All of
 // them loaded as the product starts, where the registers hold them, measured no faster.)
 // Bounds by descriptor: the largest size's da took 528 us with addresses and bounds per lane, 497 so
-// (g and u of 16 bits; 512 as they are kept now).
+// (both with g and u of 16 bits, on the core's earlier matrix instructions).
 constexpr int kAhead = 3;
 template <class DT, class Core>
 struct GateUp {
@@ -374,13 +376,15 @@ __global__ void __launch_bounds__(64) ffn_join_kernel(const FfnParams p) {
 // A workgroup takes 16 weight rows (pair: the same 8 of both weights) and all rows of x; its waves
 // take every NW-th 32 of k straight from memory into the operands of v_mfma_f32_16x16x32, so that
 // nothing waits on LDS until their sums are added there, in order. Every workgroup reads all of x,
-// so that its time grows with the rows while the tiles' stays; the two products took (bf16, us,
-// weights from memory; tiles with the join of their split)
-//     d, f            1 row   16 rows   32 rows   64 rows   tiles, 1 to 64 rows
-//     1024, 2816       12.0      14.8      19.9      28.5   25
-//     2048, 5504                           40.4      61.1   49
-//     4096, 11008                86.3               179.7   91
-// 1 row: 17.3 MB of weights, 1.4 TB/s; a launch of nothing takes 2 us of each 6.
+// so that its time grows with the rows while the tiles' stays; the two products took (bf16, us under
+// the profiler, weights from memory; tiles with the join of their split)
+//     d, f            1 row   16 rows   32 rows   tiles, 1 to 64 rows
+//     1024, 2816       12.9      15.8      20.6   30.4 to 31.2
+//     2048, 5504       21.2      27.8      39.1   38.7 to 40.3
+//     4096, 11008      58.8      80.4     112.2   74.7 to 77.1
+// The limit is that of the block's widths; at 4096 x 11008 tiles are ahead from 16 rows on.
+// 1 row of 1024: 17.3 MB of weights, 1.4 TB/s; a launch of nothing takes 2 us of each 6, and the
+// second product's 64 workgroups leave three quarters of the CUs without one.
 constexpr int kFewRows = 32;
 template <class DT, int TT, int NW, int EPI>
 __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const FfnParams p) {
@@ -473,24 +477,27 @@ hipError_t launch_few(const FfnParams &p, hipStream_t stream) {
 // The times are fits to measurements: us of one 64-wide k-step with all slots busy and with few
 // (a CU alone has more of the caches, of the memory and of the power budget), and the share of
 // the epilogue's bytes, at kMemory, that nothing else runs under (one of two workgroups on a CU
-// computes while the other stores). Measured with each shape forced (bf16, us; largest is
+// computes while the other stores). With each shape forced (bf16, us under the profiler; largest is
 // 16384 rows, d 2048, f 5504, ragged 6473, 1024, 2816, small 1500, 512, 1408; + the join):
 //                     256 x 256   256 x 128   128 x 128    64 x 128
-//   largest, gate|up        794         975         940        1023
-//   largest, down           359         418         397         480 + 8
-//   largest, da             512         530         540         567
-//   largest, dx             646         787         774         990 + 8
-//   largest, weights        963 + 12   1189 + 8    1200 + 6    1767 + 9
-//   ragged,  gate|up        118         122         105         127
-//   ragged,  down            73          52          52          58 + 6
-//   ragged,  da              84 + 17     90          79          79
-//   ragged,  dx              87 + 16    105         104         117 + 6
-//   ragged,  weights        158         137 + 6     126 + 6     173 + 8
-//   small,   gate|up         26          18          18          17
-//   small,   da              34          21          17          16
-//   small,   dx              21 + 9      16 + 6      14 + 6      14 + 5
-// A split costs a join of 5 to 6 us, less what it saves: dx of 575, 264, 712 takes 17.2 us whole and 13.6 in
-// pieces, of 3000, 768, 2048 50.4 and 37.5, down of 1500, 1024, 2816 27.9 and 24.6.
+//   largest, gate|up        722         917         887         972
+//   largest, down           325         388         369         470 + 7
+//   largest, da             477         508         516         541
+//   largest, dx             589         762         724         955 + 8
+//   largest, weights        864 + 11   1064 + 8    1086 + 7    1758 + 9
+//   ragged,  gate|up        104         109          89         103
+//   ragged,  down            65          44          43          48 + 5
+//   ragged,  da              68 + 15     80          68          67
+//   ragged,  dx              76 + 14     95          91         102 + 6
+//   ragged,  weights        139         118 + 6     106 + 6     144 + 8
+//   small,   gate|up         24          16          16          14
+//   small,   down            15 + 8      12 + 5      17          14
+//   small,   da              32          20          17          13
+//   small,   dx              21 + 9      18 + 5      14 + 5      14 + 5
+//   small,   weights         20 + 9      27          21          19
+// The constants below were fitted to such a table of an earlier build, 8 % slower throughout, in which
+// the same shapes led, row by row. A split costs a join of 5 to 6 us, less what it saves: dx of 575, 264, 712 took
+// 17.2 us whole and 13.6 in pieces, of 3000, 768, 2048 50.4 and 37.5, down of 1500, 1024, 2816 27.9 and 24.6.
 struct Plan {
     int shape, whole, split, tiles;
     int64_t part_bytes;
