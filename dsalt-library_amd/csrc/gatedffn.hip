@@ -495,7 +495,7 @@ hipError_t launch_few(const FfnParams &p, hipStream_t stream) {
 //   small,   da              32          20          17          13
 //   small,   dx              21 + 9      18 + 5      14 + 5      14 + 5
 //   small,   weights         20 + 9      27          21          19
-// The constants below were fitted to such a table of an earlier build, 8 % slower throughout, in which
+// The constants below were fitted to such a table of earlier kernels, 8 % slower throughout, in which
 // the same shapes led, row by row. A split costs a join of 5 to 6 us, less what it saves: dx of 575, 264, 712 took
 // 17.2 us whole and 13.6 in pieces, of 3000, 768, 2048 50.4 and 37.5, down of 1500, 1024, 2816 27.9 and 24.6.
 struct Plan {

@@ -3,6 +3,7 @@ the backward forms it again. ``nn.Dropout`` draws from torch's generator and kee
 """
 from __future__ import annotations
 
+import ctypes
 import operator
 
 import torch
@@ -44,7 +45,7 @@ def torch_counter_dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> t
         k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
     words = torch.stack((c0, c1, c2, c3), -1)
     keep = (torch.stack((words & 0xFFFF, words >> 16), -1).reshape(-1)[:n] < threshold).view(x.shape)
-    scale = torch.tensor(65536 / threshold if threshold else 0.0, dtype=torch.float32).item()  # as the kernels hold it
+    scale = ctypes.c_float(65536 / threshold if threshold else 0.0).value  # in fp32, as the kernels hold it
     return torch.where(keep, x.float() * scale, 0.0).to(x.dtype)
 
 

@@ -99,8 +99,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     bf16 or fp16, all of one dtype; under a 16-bit autocast fp32 tensors are cast to its dtype
     first, on every call (autocast's cache of weights is that of torch's own linears). d, e and f
-    multiples of 8. Row strides and any number of rows, none included, are
-    taken. Differentiable in every tensor; functorch's transforms, forward-mode differentiation,
+    multiples of 8. Row strides and any number of rows, none included, are taken.
+    Differentiable in every tensor; functorch's transforms, forward-mode differentiation,
     tracing and tensor subclasses take torch's ops instead. Other operands raise ``DsaltError``."""
     if activation not in _hip.ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(_hip.ACTIVATIONS)}, got {activation!r}")

@@ -228,7 +228,7 @@ class DSALTTransformerBlock(nn.Module):
             x = x.to(wide)
 
         def taken(w):
-            return w if w is None or w.dtype is wide or w.dtype is torch.float32 else w.to(wide)
+            return w if w is None or w.dtype is wide else w.float()
 
         n = norm if inside(norm) else None
         x, h = branch_norm(x, o, None if n is None else taken(n.weight),

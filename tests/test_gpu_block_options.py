@@ -375,3 +375,19 @@ def test_feed_forward_sees_the_stream_type(how):
         with torch.set_grad_enabled(grad), torch.autocast("cuda", dtype=BF):
             b(x, cu_seqlens=cu, max_seqlen=256)
     assert seen == [FP, FP]
+
+
+def test_norms_and_gates_of_another_type():
+    """Post norms and gates in the other 16-bit type than the stream's are read at their own value."""
+    b = block(BF, dropout=0.0)
+    with torch.no_grad():
+        for n in ("attn_post_norm", "ffn_post_norm"):
+            getattr(b, n).weight.data = getattr(b, n).weight.data.to(HF)
+        b.ffn_gate.data = b.ffn_gate.data.to(HF)
+        cu = torch.tensor(CU, dtype=torch.int32, device=DEV)
+        x = torch.randn(CU[-1], 128, device=DEV).to(BF)
+        got, _ = b(x, cu_seqlens=cu, max_seqlen=256)
+        for n in ("attn_post_norm", "ffn_post_norm"):
+            getattr(b, n).weight.data = getattr(b, n).weight.data.float()
+        b.ffn_gate.data = b.ffn_gate.data.float()
+        assert got.dtype == BF and torch.equal(got, b(x, cu_seqlens=cu, max_seqlen=256)[0])
