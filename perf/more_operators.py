@@ -183,19 +183,19 @@ def run(s):
 
 # ---- the package's calls ----------------------------------------------------------------
 def _call_own(s):
-    from dsalt.kernels import add_layer_norm, distill_loss, fp8_linear, fp8_matmul, layer_norm
+    from dsalt import kernels
 
     c = s["case"]
     if c["kind"].startswith("norm"):
         out = DTYPES[c["out"]]
         if c["add"]:
-            return add_layer_norm(s["x"], s["h"], s["w"], s["b"], eps=EPS, out_dtype=out)
-        return (layer_norm(s["x"], s["w"], s["b"], eps=EPS, out_dtype=out),)
+            return kernels.add_layer_norm(s["x"], s["h"], s["w"], s["b"], eps=EPS, out_dtype=out)
+        return (kernels.layer_norm(s["x"], s["w"], s["b"], eps=EPS, out_dtype=out),)
     if c["kind"].startswith("distill"):
-        return (distill_loss(s["logits"], s["zt"], s["ids"], s["labels"], temperature=c["tau"], label_weight=c["lam"]),)
+        return (kernels.distill_loss(s["logits"], s["zt"], s["ids"], s["labels"], temperature=c["tau"], label_weight=c["lam"]),)
     if c["kind"] == "linear":
-        return (fp8_linear(s["x"], s["w"], s["ws"]),)
-    return (fp8_matmul(s["a"], s["as"], s["w"], s["ws"], out_dtype=DTYPES[c["dtype"]]),)
+        return (kernels.fp8_linear(s["x"], s["w"], s["ws"]),)
+    return (kernels.fp8_matmul(s["a"], s["as"], s["w"], s["ws"], out_dtype=DTYPES[c["dtype"]]),)
 
 
 def _run_own(s):
