@@ -795,6 +795,65 @@ int64_t dsalt_branch_norm_workspace_size(int64_t rows, int32_t d) {
 }
 size_t dsalt_branch_norm_args_size(void) { return sizeof(dsalt_branch_norm_args); }
 
+int dsalt_layer_norm_check(const dsalt_layer_norm_args *a, int32_t backward) {
+    if (!a) return fail(DSALT_ERR_INVALID, "args must be non-NULL");
+    if (a->rows < 0 || a->rows > ((int64_t)1 << 31))
+        return fail(DSALT_ERR_INVALID, "rows must be in [0, 2^31] (got %lld)", (long long)a->rows);
+    if (a->d < 1 || a->d > dsalt::layer_norm_max_dim())
+        return fail(DSALT_ERR_UNSUPPORTED, "d must be in [1, %d] (got %d)", dsalt::layer_norm_max_dim(), a->d);
+    if (!float_dtype(a->x_dtype)) return fail(DSALT_ERR_INVALID, "x_dtype %d is not a float dtype", a->x_dtype);
+    const bool x32 = a->x_dtype == DSALT_DTYPE_F32;
+    const auto branch = [&](int dt) { return x32 ? float_dtype(dt) : dt == a->x_dtype; };
+    if ((a->h || (backward && a->dh)) && !branch(a->h_dtype))
+        return fail(DSALT_ERR_UNSUPPORTED, "h dtype %d with x dtype %d", a->h_dtype, a->x_dtype);
+    if (!branch(a->y_dtype)) return fail(DSALT_ERR_UNSUPPORTED, "y dtype %d with x dtype %d", a->y_dtype, a->x_dtype);
+    const struct { bool used; int dt; } ws[] = {{a->weight || (backward && a->d_weight), a->w_dtype},
+                                                {a->bias || (backward && a->d_bias), a->b_dtype}};
+    for (const auto &w : ws)
+        if (w.used && w.dt != DSALT_DTYPE_F32 && w.dt != a->x_dtype)
+            return fail(DSALT_ERR_UNSUPPORTED, "weight or bias dtype %d with x dtype %d", w.dt, a->x_dtype);
+    const auto size = [](int dt) { return dt == DSALT_DTYPE_F32 ? 4 : 2; };
+    const struct { const void *p; size_t align; } ps[] = {
+        {a->x, (size_t)size(a->x_dtype)}, {a->h, (size_t)size(a->h_dtype)}, {a->weight, (size_t)size(a->w_dtype)},
+        {a->bias, (size_t)size(a->b_dtype)}, {a->x_out, (size_t)size(a->x_dtype)}, {a->y, (size_t)size(a->y_dtype)},
+        {a->stats, 4}, {a->dx_out, (size_t)size(a->x_dtype)}, {a->dy, (size_t)size(a->y_dtype)},
+        {a->dx, (size_t)size(a->x_dtype)}, {a->dh, (size_t)size(a->h_dtype)}, {a->d_weight, (size_t)size(a->w_dtype)},
+        {a->d_bias, (size_t)size(a->b_dtype)}, {a->workspace, 4}};
+    for (const auto &q : ps)
+        if (!aligned(q.p, q.align)) return fail(DSALT_ERR_INVALID, "pointers must be aligned to their elements");
+    if (!(a->eps >= 0.f)) return fail(DSALT_ERR_INVALID, "eps must be >= 0 (got %g)", (double)a->eps);
+    if (a->rows == 0) return DSALT_OK;
+    if (!a->x) return fail(DSALT_ERR_INVALID, "x must be non-NULL");
+    if (!backward) {
+        if (!a->y || (a->h && !a->x_out)) return fail(DSALT_ERR_INVALID, "y, and x_out with h, must be non-NULL");
+    } else {
+        if (!a->dy || !a->stats) return fail(DSALT_ERR_INVALID, "dy and stats must be non-NULL");
+        if ((a->d_weight || a->d_bias) &&
+            (!a->workspace || a->workspace_bytes < dsalt::layer_norm_workspace_bytes(a->rows, a->d)))
+            return fail(DSALT_ERR_INVALID, "the column sums need workspace of dsalt_layer_norm_workspace_size bytes");
+    }
+    return DSALT_OK;
+}
+
+int dsalt_layer_norm(const dsalt_layer_norm_args *args, void *stream) {
+    if (int rc = dsalt_layer_norm_check(args, 0)) return rc;
+    hipError_t e = dsalt::launch_layer_norm(*args, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_layer_norm launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+
+int dsalt_layer_norm_bwd(const dsalt_layer_norm_args *args, void *stream) {
+    if (int rc = dsalt_layer_norm_check(args, 1)) return rc;
+    hipError_t e = dsalt::launch_layer_norm_bwd(*args, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_layer_norm_bwd launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+
+int64_t dsalt_layer_norm_workspace_size(int64_t rows, int32_t d) {
+    return rows < 0 || d <= 0 ? 0 : dsalt::layer_norm_workspace_bytes(rows, d);
+}
+size_t dsalt_layer_norm_args_size(void) { return sizeof(dsalt_layer_norm_args); }
+
 int dsalt_rope_check(const dsalt_rope_args *a) {
     if (!a) return fail(DSALT_ERR_INVALID, "args is NULL");
     if (a->total_len < 0 || a->n_q_heads < 0 || a->n_k_heads < 0)

@@ -10,7 +10,9 @@ consumers ``DSALTTransformerBlock`` / ``DSALTLMHeadModel``. ``DSALTConfig`` and
 from ._hip import DsaltError
 from .kernels import (
     HybridEnergyLandmarkSelector,
+    LayerNorm,
     RMSENorm,
+    add_layer_norm,
     apply_rotary_emb,
     branch_norm,
     build_local_window_mask,
@@ -23,6 +25,7 @@ from .kernels import (
     dsalt_triton_backward,
     gated_ffn,
     hybrid_scores_per_head,
+    layer_norm,
     select_landmarks,
     soft_landmark_weights,
     sparse_attention_forward,
@@ -45,6 +48,9 @@ __all__ = [
     "gated_ffn",
     "counter_dropout",
     "branch_norm",
+    "layer_norm",
+    "add_layer_norm",
+    "LayerNorm",
     "RMSENorm",
     "compute_window_sizes",
     "build_local_window_mask",

@@ -228,6 +228,19 @@ class BranchNormArgs(ctypes.Structure):
     ]
 
 
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("d", c_int32),
+        ("x_dtype", c_int32), ("h_dtype", c_int32), ("y_dtype", c_int32), ("w_dtype", c_int32), ("b_dtype", c_int32),
+        ("eps", c_float),
+        ("x", c_void_p), ("h", c_void_p), ("weight", c_void_p), ("bias", c_void_p),
+        ("x_out", c_void_p), ("y", c_void_p), ("stats", c_void_p),
+        ("dx_out", c_void_p), ("dy", c_void_p),
+        ("dx", c_void_p), ("dh", c_void_p), ("d_weight", c_void_p), ("d_bias", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "dsalt_fwd", "dsalt_fwd_check", "dsalt_bwd", "dsalt_bwd_check", "dsalt_bwd_workspace_size",
     "dsalt_select_landmarks", "dsalt_select_check", "dsalt_quantize_windows",
@@ -243,6 +256,8 @@ EXPORTED_SYMBOLS = (
     "dsalt_gated_ffn", "dsalt_gated_ffn_bwd", "dsalt_gated_ffn_check", "dsalt_gated_ffn_workspace_size", "dsalt_gated_ffn_kept_size",
     "dsalt_gated_ffn_args_size", "dsalt_dropout", "dsalt_dropout_args_size", "dsalt_branch_norm",
     "dsalt_branch_norm_bwd", "dsalt_branch_norm_check", "dsalt_branch_norm_workspace_size", "dsalt_branch_norm_args_size",
+    "dsalt_layer_norm", "dsalt_layer_norm_bwd", "dsalt_layer_norm_check", "dsalt_layer_norm_workspace_size",
+    "dsalt_layer_norm_args_size",
 )
 NOALLOC_SCRATCH_BYTES = 76 << 20  # DSALT_NOALLOC_SCRATCH_BYTES
 SELECT_SPLIT_MIN = 4096  # longer sequences can be selected chunk-wise
@@ -298,6 +313,9 @@ def lib() -> ctypes.CDLL:
         ("dsalt_branch_norm", [ctypes.POINTER(BranchNormArgs), c_void_p]),
         ("dsalt_branch_norm_bwd", [ctypes.POINTER(BranchNormArgs), c_void_p]),
         ("dsalt_branch_norm_check", [ctypes.POINTER(BranchNormArgs), c_int32]),
+        ("dsalt_layer_norm", [ctypes.POINTER(LayerNormArgs), c_void_p]),
+        ("dsalt_layer_norm_bwd", [ctypes.POINTER(LayerNormArgs), c_void_p]),
+        ("dsalt_layer_norm_check", [ctypes.POINTER(LayerNormArgs), c_int32]),
         ("dsalt_add_rms_norm", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int32,
                                 c_void_p]),
     ):
@@ -320,6 +338,8 @@ def lib() -> ctypes.CDLL:
     h.dsalt_gated_ffn_kept_size.restype = c_int64
     h.dsalt_branch_norm_workspace_size.argtypes = [c_int64, c_int32]
     h.dsalt_branch_norm_workspace_size.restype = c_int64
+    h.dsalt_layer_norm_workspace_size.argtypes = [c_int64, c_int32]
+    h.dsalt_layer_norm_workspace_size.restype = c_int64
     h.dsalt_lmk_weights_workspace_size.argtypes = [c_int32] * 2
     h.dsalt_lmk_weights_workspace_size.restype = c_int64
     h.dsalt_abi_version.restype = ctypes.c_int
@@ -327,7 +347,7 @@ def lib() -> ctypes.CDLL:
     for n in ("dsalt_fwd_args_size", "dsalt_bwd_args_size", "dsalt_select_args_size", "dsalt_scores_args_size",
               "dsalt_rope_args_size", "dsalt_lmk_weights_args_size", "dsalt_rope_tables_size", "dsalt_qkv_args_size",
               "dsalt_module_grads_args_size", "dsalt_norm_train_args_size", "dsalt_gated_ffn_args_size",
-              "dsalt_dropout_args_size", "dsalt_branch_norm_args_size"):
+              "dsalt_dropout_args_size", "dsalt_branch_norm_args_size", "dsalt_layer_norm_args_size"):
         getattr(h, n).restype = c_size_t
     _lib = h
     check_abi()
@@ -344,10 +364,12 @@ def check_abi() -> None:
                        (RopeTables, h.dsalt_rope_tables_size), (QkvArgs, h.dsalt_qkv_args_size),
                        (ModuleGradsArgs, h.dsalt_module_grads_args_size),
                        (NormTrainArgs, h.dsalt_norm_train_args_size), (GatedFfnArgs, h.dsalt_gated_ffn_args_size),
-                       (DropoutArgs, h.dsalt_dropout_args_size), (BranchNormArgs, h.dsalt_branch_norm_args_size)):
+                       (DropoutArgs, h.dsalt_dropout_args_size), (BranchNormArgs, h.dsalt_branch_norm_args_size),
+                       (LayerNormArgs, h.dsalt_layer_norm_args_size)):
         if ctypes.sizeof(args) != fn():
             raise DsaltError(f"{args.__name__} layout mismatch: {ctypes.sizeof(args)} vs {fn()} bytes")
-    for pack, args in ((_FFN_PACK, GatedFfnArgs), (_DROPOUT_PACK, DropoutArgs), (_BRANCH_PACK, BranchNormArgs)):
+    for pack, args in ((_FFN_PACK, GatedFfnArgs), (_DROPOUT_PACK, DropoutArgs), (_BRANCH_PACK, BranchNormArgs),
+                       (_LAYER_PACK, LayerNormArgs)):
         if pack.size != ctypes.sizeof(args):
             raise DsaltError(f"{args.__name__} packs to {pack.size} of {ctypes.sizeof(args)} bytes")
 
@@ -1479,6 +1501,11 @@ def aligned_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+def contiguous_rows(t: torch.Tensor) -> torch.Tensor:
+    """t itself when it is contiguous, otherwise a copy that is."""
+    return t if t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
+
+
 def norm_train_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
     """Whether dsalt_norm_train takes rows of x [..., d] with this weight [d]: GPU tensors,
     contiguous and 16-byte aligned, d a multiple of 8 up to 4096, x bf16, fp16 or fp32, the
@@ -1565,6 +1592,7 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}  # DSALT_ACT_*
 _FFN_PACK = struct.Struct("@q6iPq3P3q3PPq5PPq")
 _DROPOUT_PACK = struct.Struct("@q2iPP2qP")
 _BRANCH_PACK = struct.Struct("@q9i3f2qP5P2P2P2P5PPq")
+_LAYER_PACK = struct.Struct("@q6if4P3P2P4PPq")
 _packed_calls: dict = {}
 
 
@@ -1746,3 +1774,45 @@ def branch_norm_bwd(x, h, weight, post_weight, gate, opts, seed, stats, dx_out, 
           _branch_pack(x, h, weight, post_weight, gate, opts, seed, rstd=at, rstd_post=at + 4 * rows, dx_out=_addr(dx_out),
                        dy=_addr(dy), grads=[_addr(t) for t in out], ws=ws), dev)
     return out
+
+
+LAYER_NORM_MAX_DIM = 8192  # largest row length of dsalt_layer_norm
+
+
+def _layer_pack(x, h, weight, bias, eps, y_dtype, stats, *, h_dtype=None, x_out=0, y=0, dx_out=0, dy=0, grads=(0, 0, 0, 0),
+                ws=(0, 0), b_dtype=None) -> bytes:
+    d = x.shape[-1]
+    return _LAYER_PACK.pack(
+        x.numel() // d, d, _SCORE_DTYPES[x.dtype], _SCORE_DTYPES[h.dtype if h is not None else h_dtype or x.dtype],
+        _SCORE_DTYPES[y_dtype], _code(weight), _code(bias) if b_dtype is None else _SCORE_DTYPES[b_dtype], eps, x.data_ptr(),
+        _addr(h), _addr(weight), _addr(bias), x_out, y, _addr(stats), dx_out, dy, *grads, *ws)
+
+
+def layer_norm(x, h, weight, bias, eps: float, out_dtype: torch.dtype, keep: bool):
+    """``(x_out, y, stats)`` of contiguous operands: see dsalt_layer_norm; x_out None without h, stats
+    ([3, rows], for the backward) None without `keep`."""
+    dev = x.device
+    x_out = torch.empty_like(x) if h is not None else None
+    y = torch.empty_like(x, dtype=out_dtype)
+    stats = torch.empty((3, x.numel() // x.shape[-1]), device=dev, dtype=torch.float32) if keep else None
+    _call("dsalt_layer_norm", _layer_pack(x, h, weight, bias, eps, out_dtype, stats, x_out=_addr(x_out), y=y.data_ptr()), dev)
+    return x_out, y, stats
+
+
+def layer_norm_bwd(x, h, weight, b_dtype: torch.dtype | None, stats, dx_out, dy, h_dtype: torch.dtype | None, need):
+    """``(dx, dh, d_weight, d_bias)``, None where not in `need`: see dsalt_layer_norm_bwd. dh in h_dtype
+    (None: not formed), d_bias in b_dtype."""
+    dev, d = x.device, x.shape[-1]
+    dx = torch.empty_like(x) if need[0] else None
+    dh = torch.empty_like(x, dtype=h_dtype) if need[1] else None
+    dw = torch.empty_like(weight) if need[2] else None
+    db = torch.empty(d, device=dev, dtype=b_dtype) if need[3] else None
+    ws = (0, 0)
+    if need[2] or need[3]:
+        size = lib().dsalt_layer_norm_workspace_size(x.numel() // d, d)
+        scratch = torch.empty(size, device=dev, dtype=torch.uint8)
+        ws = (scratch.data_ptr(), size)
+    _call("dsalt_layer_norm_bwd",
+          _layer_pack(x, h, weight, None, 0.0, dy.dtype, stats, h_dtype=h_dtype, dx_out=_addr(dx_out), dy=dy.data_ptr(),
+                      grads=(_addr(dx), _addr(dh), _addr(dw), _addr(db)), ws=ws, b_dtype=b_dtype), dev)
+    return dx, dh, dw, db

@@ -14,6 +14,7 @@ attention path never calls. ``LigerFusedLinearCrossEntropyFunction`` (the Triton
 is not part of this package.
 """
 from .. import _hip
+from .LayerNorm import LayerNorm, add_layer_norm, layer_norm
 from .RMSENorm import RMSENorm
 from .branch_norm import branch_norm
 from .dropout import counter_dropout
@@ -60,6 +61,9 @@ __all__ = [
     "gated_ffn",
     "counter_dropout",
     "branch_norm",
+    "layer_norm",
+    "add_layer_norm",
+    "LayerNorm",
     "RMSENorm",
     "compute_window_sizes",
     "build_local_window_mask",

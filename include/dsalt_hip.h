@@ -716,6 +716,40 @@ int dsalt_branch_norm_check(const dsalt_branch_norm_args *args, int32_t backward
 int64_t dsalt_branch_norm_workspace_size(int64_t rows, int32_t d);
 size_t dsalt_branch_norm_args_size(void);
 
+/*
+ * Layer norm of rows [rows, d], contiguous, and of the sum of a residual stream and a branch:
+ *   z = x + h (h NULL: z = x), x_out = z in x's dtype (written with h)
+ *   y = (z - mean) * r * weight + bias, r = rsqrt(mean((z - mean)^2) + eps)
+ * weight NULL: 1, bias NULL: 0. y (y_dtype) is formed from the fp32 z. stats [3, rows] fp32 (the
+ * means, what their rounding left, r) may be NULL in the forward and is what the backward reads, with x and h as the
+ * forward had them (or x = an fp32 x_out and h = NULL). Backward: from dy (y_dtype) and dx_out
+ * (x's dtype; NULL: none) dx (x's dtype), dh (h_dtype; the same values), d_weight and d_bias in
+ * their tensors' dtypes, each of which may be NULL (a d_bias is formed whether bias is given or not);
+ * the column sums need workspace of dsalt_layer_norm_workspace_size(rows, d) bytes, dead when the
+ * launches end. rows = 0 gives zero sums. fp32 arithmetic, sums in a fixed order.
+ * dtypes: x BF16 or F16 with h and y of the same, or x F32 with h and y of any; weight and bias of
+ * x's dtype or F32. d in [1, 8192]; pointers aligned to their elements (16-byte alignment of all of
+ * them, and d a multiple of 8, is the fast form); outputs alias no input and no other output.
+ */
+typedef struct dsalt_layer_norm_args {
+    int64_t rows;
+    int32_t d;
+    int32_t x_dtype, h_dtype, y_dtype, w_dtype, b_dtype;
+    float eps;
+    const void *x, *h, *weight, *bias;
+    void *x_out, *y;
+    float *stats;
+    const void *dx_out, *dy;
+    void *dx, *dh, *d_weight, *d_bias;
+    void *workspace;
+    int64_t workspace_bytes;
+} dsalt_layer_norm_args;
+int dsalt_layer_norm(const dsalt_layer_norm_args *args, void *stream);
+int dsalt_layer_norm_bwd(const dsalt_layer_norm_args *args, void *stream);
+int dsalt_layer_norm_check(const dsalt_layer_norm_args *args, int32_t backward);
+int64_t dsalt_layer_norm_workspace_size(int64_t rows, int32_t d);
+size_t dsalt_layer_norm_args_size(void);
+
 int dsalt_abi_version(void);
 const char *dsalt_last_error(void);
 /* sizeof of the argument structs as compiled into the library (ABI layout check). */
