@@ -854,6 +854,62 @@ int64_t dsalt_layer_norm_workspace_size(int64_t rows, int32_t d) {
 }
 size_t dsalt_layer_norm_args_size(void) { return sizeof(dsalt_layer_norm_args); }
 
+int dsalt_distill_check(const dsalt_distill_args *a, int32_t backward) {
+    if (!a) return fail(DSALT_ERR_INVALID, "args must be non-NULL");
+    if (a->rows < 0 || a->rows >= (1 << 24))  // a launch's threads
+        return fail(DSALT_ERR_INVALID, "rows must be in [0, 2^24) (got %lld)", (long long)a->rows);
+    if (a->vocab < 1 || a->vocab > (1 << 30)) return fail(DSALT_ERR_UNSUPPORTED, "vocab must be in [1, 2^30] (got %d)", a->vocab);
+    if (a->k < 1 || a->k > 1024) return fail(DSALT_ERR_UNSUPPORTED, "k must be in [1, 1024] (got %d)", a->k);
+    if (!float_dtype(a->logits_dtype) || !float_dtype(a->teacher_dtype))
+        return fail(DSALT_ERR_INVALID, "logits dtype %d or teacher dtype %d is not a float dtype", a->logits_dtype, a->teacher_dtype);
+    if (a->reduction < DSALT_REDUCE_NONE || a->reduction > DSALT_REDUCE_SUM)
+        return fail(DSALT_ERR_INVALID, "reduction must be DSALT_REDUCE_* (got %d)", a->reduction);
+    if (!(a->temperature > 0.f) || !(a->temperature < INFINITY))
+        return fail(DSALT_ERR_INVALID, "temperature must be positive and finite (got %g)", (double)a->temperature);
+    if (!(a->label_weight >= 0.f && a->label_weight <= 1.f))
+        return fail(DSALT_ERR_INVALID, "label_weight must be in [0, 1] (got %g)", (double)a->label_weight);
+    if (a->label_weight > 0.f && !a->labels && a->rows > 0) return fail(DSALT_ERR_INVALID, "label_weight needs labels");
+    if (a->logits_stride < a->vocab || a->teacher_stride < a->k || a->ids_stride < a->k)
+        return fail(DSALT_ERR_INVALID, "row strides must cover their rows");
+    const size_t ls = a->logits_dtype == DSALT_DTYPE_F32 ? 4 : 2, ts = a->teacher_dtype == DSALT_DTYPE_F32 ? 4 : 2;
+    if (!aligned(a->logits, ls) || !aligned(a->teacher, ts) || !aligned(a->ids, a->ids_int64 ? 8 : 4) ||
+        !aligned(a->labels, a->labels_int64 ? 8 : 4) || !aligned(a->loss, 4) || !aligned(a->stats, 4) ||
+        !aligned(a->d_loss, 4) || !aligned(a->d_logits, ls) || !aligned(a->workspace, 4))
+        return fail(DSALT_ERR_INVALID, "pointers must be aligned to their elements");
+    if (a->rows > 0 && (!a->logits || !a->teacher || !a->ids))
+        return fail(DSALT_ERR_INVALID, "logits, teacher and ids must be non-NULL");
+    if (backward) {
+        if (a->rows > 0 && (!a->stats || !a->d_loss || !a->d_logits))
+            return fail(DSALT_ERR_INVALID, "stats, d_loss and d_logits must be non-NULL");
+        return DSALT_OK;
+    }
+    if (!a->loss && (a->rows > 0 || a->reduction != DSALT_REDUCE_NONE)) return fail(DSALT_ERR_INVALID, "loss must be non-NULL");
+    const int64_t need = dsalt::distill_workspace_bytes(a->rows, a->vocab);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need))
+        return fail(DSALT_ERR_INVALID, "workspace of dsalt_distill_workspace_size (%lld) bytes needed", (long long)need);
+    return DSALT_OK;
+}
+
+int dsalt_distill(const dsalt_distill_args *args, void *stream) {
+    if (int rc = dsalt_distill_check(args, 0)) return rc;
+    hipError_t e = dsalt::launch_distill(*args, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_distill launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+
+int dsalt_distill_bwd(const dsalt_distill_args *args, void *stream) {
+    if (int rc = dsalt_distill_check(args, 1)) return rc;
+    hipError_t e = dsalt::launch_distill_bwd(*args, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_distill_bwd launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+
+int64_t dsalt_distill_workspace_size(int64_t rows, int32_t vocab) {
+    return rows < 0 || vocab <= 0 ? 0 : dsalt::distill_workspace_bytes(rows, vocab);
+}
+int64_t dsalt_distill_stats_count(int64_t rows) { return rows < 0 ? 0 : dsalt::distill_stats_count(rows); }
+size_t dsalt_distill_args_size(void) { return sizeof(dsalt_distill_args); }
+
 int dsalt_rope_check(const dsalt_rope_args *a) {
     if (!a) return fail(DSALT_ERR_INVALID, "args is NULL");
     if (a->total_len < 0 || a->n_q_heads < 0 || a->n_k_heads < 0)

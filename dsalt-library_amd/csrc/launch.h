@@ -88,6 +88,10 @@ hipError_t launch_layer_norm(const dsalt_layer_norm_args &a, hipStream_t stream)
 hipError_t launch_layer_norm_bwd(const dsalt_layer_norm_args &a, hipStream_t stream);
 int64_t layer_norm_workspace_bytes(int64_t rows, int d);
 int layer_norm_max_dim();
+hipError_t launch_distill(const dsalt_distill_args &a, hipStream_t stream);
+hipError_t launch_distill_bwd(const dsalt_distill_args &a, hipStream_t stream);
+int64_t distill_workspace_bytes(int64_t rows, int vocab);
+int64_t distill_stats_count(int64_t rows);
 
 // Number of query blocks of `bm` tokens over a packed batch, as an upper bound that is
 // computable without reading cu_seqlens: sum_s ceil(L_s/bm) <= ceil(T/bm) + S.

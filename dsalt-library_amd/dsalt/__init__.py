@@ -21,6 +21,7 @@ from .kernels import (
     compute_hybrid_scores,
     compute_window_sizes,
     counter_dropout,
+    distill_loss,
     dsalt_triton_attention,
     dsalt_triton_backward,
     gated_ffn,
@@ -48,6 +49,7 @@ __all__ = [
     "gated_ffn",
     "counter_dropout",
     "branch_norm",
+    "distill_loss",
     "layer_norm",
     "add_layer_norm",
     "LayerNorm",

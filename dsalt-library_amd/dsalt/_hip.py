@@ -241,6 +241,20 @@ class LayerNormArgs(ctypes.Structure):
     ]
 
 
+class DistillArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64),
+        ("logits_stride", c_int64), ("teacher_stride", c_int64), ("ids_stride", c_int64), ("ignore_index", c_int64),
+        ("vocab", c_int32), ("k", c_int32),
+        ("logits_dtype", c_int32), ("teacher_dtype", c_int32), ("ids_int64", c_int32), ("labels_int64", c_int32),
+        ("reduction", c_int32),
+        ("temperature", c_float), ("label_weight", c_float),
+        ("logits", c_void_p), ("teacher", c_void_p), ("ids", c_void_p), ("labels", c_void_p),
+        ("loss", c_void_p), ("stats", c_void_p), ("d_loss", c_void_p), ("d_logits", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "dsalt_fwd", "dsalt_fwd_check", "dsalt_bwd", "dsalt_bwd_check", "dsalt_bwd_workspace_size",
     "dsalt_select_landmarks", "dsalt_select_check", "dsalt_quantize_windows",
@@ -257,7 +271,8 @@ EXPORTED_SYMBOLS = (
     "dsalt_gated_ffn_args_size", "dsalt_dropout", "dsalt_dropout_args_size", "dsalt_branch_norm",
     "dsalt_branch_norm_bwd", "dsalt_branch_norm_check", "dsalt_branch_norm_workspace_size", "dsalt_branch_norm_args_size",
     "dsalt_layer_norm", "dsalt_layer_norm_bwd", "dsalt_layer_norm_check", "dsalt_layer_norm_workspace_size",
-    "dsalt_layer_norm_args_size",
+    "dsalt_layer_norm_args_size", "dsalt_distill", "dsalt_distill_bwd", "dsalt_distill_check", "dsalt_distill_workspace_size",
+    "dsalt_distill_stats_count", "dsalt_distill_args_size",
 )
 NOALLOC_SCRATCH_BYTES = 76 << 20  # DSALT_NOALLOC_SCRATCH_BYTES
 SELECT_SPLIT_MIN = 4096  # longer sequences can be selected chunk-wise
@@ -316,6 +331,9 @@ def lib() -> ctypes.CDLL:
         ("dsalt_layer_norm", [ctypes.POINTER(LayerNormArgs), c_void_p]),
         ("dsalt_layer_norm_bwd", [ctypes.POINTER(LayerNormArgs), c_void_p]),
         ("dsalt_layer_norm_check", [ctypes.POINTER(LayerNormArgs), c_int32]),
+        ("dsalt_distill", [ctypes.POINTER(DistillArgs), c_void_p]),
+        ("dsalt_distill_bwd", [ctypes.POINTER(DistillArgs), c_void_p]),
+        ("dsalt_distill_check", [ctypes.POINTER(DistillArgs), c_int32]),
         ("dsalt_add_rms_norm", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int32,
                                 c_void_p]),
     ):
@@ -340,6 +358,10 @@ def lib() -> ctypes.CDLL:
     h.dsalt_branch_norm_workspace_size.restype = c_int64
     h.dsalt_layer_norm_workspace_size.argtypes = [c_int64, c_int32]
     h.dsalt_layer_norm_workspace_size.restype = c_int64
+    h.dsalt_distill_workspace_size.argtypes = [c_int64, c_int32]
+    h.dsalt_distill_workspace_size.restype = c_int64
+    h.dsalt_distill_stats_count.argtypes = [c_int64]
+    h.dsalt_distill_stats_count.restype = c_int64
     h.dsalt_lmk_weights_workspace_size.argtypes = [c_int32] * 2
     h.dsalt_lmk_weights_workspace_size.restype = c_int64
     h.dsalt_abi_version.restype = ctypes.c_int
@@ -347,7 +369,8 @@ def lib() -> ctypes.CDLL:
     for n in ("dsalt_fwd_args_size", "dsalt_bwd_args_size", "dsalt_select_args_size", "dsalt_scores_args_size",
               "dsalt_rope_args_size", "dsalt_lmk_weights_args_size", "dsalt_rope_tables_size", "dsalt_qkv_args_size",
               "dsalt_module_grads_args_size", "dsalt_norm_train_args_size", "dsalt_gated_ffn_args_size",
-              "dsalt_dropout_args_size", "dsalt_branch_norm_args_size", "dsalt_layer_norm_args_size"):
+              "dsalt_dropout_args_size", "dsalt_branch_norm_args_size", "dsalt_layer_norm_args_size",
+              "dsalt_distill_args_size"):
         getattr(h, n).restype = c_size_t
     _lib = h
     check_abi()
@@ -365,11 +388,11 @@ def check_abi() -> None:
                        (ModuleGradsArgs, h.dsalt_module_grads_args_size),
                        (NormTrainArgs, h.dsalt_norm_train_args_size), (GatedFfnArgs, h.dsalt_gated_ffn_args_size),
                        (DropoutArgs, h.dsalt_dropout_args_size), (BranchNormArgs, h.dsalt_branch_norm_args_size),
-                       (LayerNormArgs, h.dsalt_layer_norm_args_size)):
+                       (LayerNormArgs, h.dsalt_layer_norm_args_size), (DistillArgs, h.dsalt_distill_args_size)):
         if ctypes.sizeof(args) != fn():
             raise DsaltError(f"{args.__name__} layout mismatch: {ctypes.sizeof(args)} vs {fn()} bytes")
     for pack, args in ((_FFN_PACK, GatedFfnArgs), (_DROPOUT_PACK, DropoutArgs), (_BRANCH_PACK, BranchNormArgs),
-                       (_LAYER_PACK, LayerNormArgs)):
+                       (_LAYER_PACK, LayerNormArgs), (_DISTILL_PACK, DistillArgs)):
         if pack.size != ctypes.sizeof(args):
             raise DsaltError(f"{args.__name__} packs to {pack.size} of {ctypes.sizeof(args)} bytes")
 
@@ -1593,6 +1616,7 @@ _FFN_PACK = struct.Struct("@q6iPq3P3q3PPq5PPq")
 _DROPOUT_PACK = struct.Struct("@q2iPP2qP")
 _BRANCH_PACK = struct.Struct("@q9i3f2qP5P2P2P2P5PPq")
 _LAYER_PACK = struct.Struct("@q6if4P3P2P4PPq")
+_DISTILL_PACK = struct.Struct("@5q7i2f4P2PPPPq")
 _packed_calls: dict = {}
 
 
@@ -1816,3 +1840,44 @@ def layer_norm_bwd(x, h, weight, b_dtype: torch.dtype | None, stats, dx_out, dy,
           _layer_pack(x, h, weight, None, 0.0, dy.dtype, stats, h_dtype=h_dtype, dx_out=_addr(dx_out), dy=dy.data_ptr(),
                       grads=(_addr(dx), _addr(dh), _addr(dw), _addr(db)), ws=ws, b_dtype=b_dtype), dev)
     return dx, dh, dw, db
+
+
+DISTILL_MAX_K = 1024  # most slots of a teacher's row
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}  # DSALT_REDUCE_*
+
+
+def _distill_pack(logits, teacher, ids, labels, opts, *, loss=0, stats=0, d_loss=0, d_logits=0, ws=(0, 0)) -> bytes:
+    temperature, label_weight, ignore_index, reduction = opts
+    return _DISTILL_PACK.pack(
+        logits.shape[0], logits.stride(0), teacher.stride(0), ids.stride(0), ignore_index, logits.shape[1], ids.shape[1],
+        _SCORE_DTYPES[logits.dtype], _SCORE_DTYPES[teacher.dtype], ids.dtype is torch.int64,
+        labels is not None and labels.dtype is torch.int64, REDUCTIONS[reduction], temperature, label_weight,
+        logits.data_ptr(), teacher.data_ptr(), ids.data_ptr(), _addr(labels), loss, stats, d_loss, d_logits, *ws)
+
+
+def distill(logits, teacher, ids, labels, opts, keep: bool):
+    """``(loss, stats)`` of `unit_rows` logits [T, V], teacher and ids [T, K] and contiguous labels [T] or
+    None: see dsalt_distill; opts = (temperature, label_weight, ignore_index, reduction). loss [T] or
+    scalar; stats, for the backward, None without `keep`."""
+    dev, rows = logits.device, logits.shape[0]
+    loss = torch.empty((rows,) if opts[3] == "none" else (), device=dev, dtype=torch.float32)
+    stats = torch.empty(lib().dsalt_distill_stats_count(rows), device=dev, dtype=torch.float32) if keep else None
+    size = lib().dsalt_distill_workspace_size(rows, logits.shape[1])
+    ws = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
+    _call("dsalt_distill", _distill_pack(logits, teacher, ids, labels, opts, loss=loss.data_ptr(), stats=_addr(stats),
+                                         ws=(_addr(ws), size)), dev)
+    return loss, stats
+
+
+def distill_bwd(logits, teacher, ids, labels, opts, stats, d_loss):
+    """d_logits [T, V], contiguous, of the operands that `distill` had: see dsalt_distill_bwd."""
+    out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    _call("dsalt_distill_bwd", _distill_pack(logits, teacher, ids, labels, opts, stats=stats.data_ptr(), d_loss=d_loss.data_ptr(),
+                                             d_logits=out.data_ptr()), logits.device)
+    return out
+
+
+def unit_rows(t: torch.Tensor) -> torch.Tensor:
+    """t [n, m] with unit stride along the rows and row strides that cover them (a copy only where not so)."""
+    rs, cs = t.stride()
+    return t if (cs == 1 or t.shape[1] == 1) and rs >= t.shape[1] else t.clone(memory_format=torch.contiguous_format)

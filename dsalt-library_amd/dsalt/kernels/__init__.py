@@ -17,6 +17,7 @@ from .. import _hip
 from .LayerNorm import LayerNorm, add_layer_norm, layer_norm
 from .RMSENorm import RMSENorm
 from .branch_norm import branch_norm
+from .distill import distill_loss
 from .dropout import counter_dropout
 from .dsalt_triton_train import dsalt_triton_train_attention
 from .gated_ffn import gated_ffn
@@ -61,6 +62,7 @@ __all__ = [
     "gated_ffn",
     "counter_dropout",
     "branch_norm",
+    "distill_loss",
     "layer_norm",
     "add_layer_norm",
     "LayerNorm",

@@ -750,6 +750,46 @@ int dsalt_layer_norm_check(const dsalt_layer_norm_args *args, int32_t backward);
 int64_t dsalt_layer_norm_workspace_size(int64_t rows, int32_t d);
 size_t dsalt_layer_norm_args_size(void);
 
+/*
+ * Loss of a student's logits s [rows, vocab] against a teacher's top logits z [rows, k] at the tokens
+ * ids [rows, k], and against labels [rows] (NULL: none). With p = softmax(z / temperature) over a
+ * row's slots, q = softmax(s / temperature), q1 = softmax(s):
+ *   loss = (1 - label_weight) temperature^2 sum_k p_k (ln p_k - ln q[ids_k]) - label_weight ln q1[label]
+ * A slot counts where 0 <= id < vocab and its logit is not -inf (an id may repeat); rows without
+ * slots have no first term. Rows whose label is ignore_index or outside [0, vocab) have loss and
+ * gradient zero whatever they hold; without labels every row counts. `loss`: the rows' losses
+ * [rows] (DSALT_REDUCE_NONE), or [1], their sum, or their mean over the rows that count (0 of none).
+ * stats (dsalt_distill_stats_count(rows) floats) may be NULL in the forward and is what the backward
+ * reads, with the other operands as the forward had them. Backward: d_loss ([rows] or [1], like
+ * loss) to d_logits [rows, vocab], contiguous, in the logits' dtype. fp32 arithmetic, sums in a fixed
+ * order, one rounding per gradient.
+ * logits and teacher BF16, F16 or F32, unit strides along their rows, row strides (in elements) of at
+ * least the row length; ids and labels int32, or int64 where ids_int64 / labels_int64. vocab in
+ * [1, 2^30], k in [1, 1024]; temperature > 0; label_weight in [0, 1], 0 without labels. Pointers
+ * aligned to their elements. workspace (forward only): dsalt_distill_workspace_size bytes, dead when
+ * the launches end. d_logits aliases no input.
+ */
+enum { DSALT_REDUCE_NONE = 0, DSALT_REDUCE_MEAN = 1, DSALT_REDUCE_SUM = 2 };
+typedef struct dsalt_distill_args {
+    int64_t rows;
+    int64_t logits_stride, teacher_stride, ids_stride, ignore_index;
+    int32_t vocab, k;
+    int32_t logits_dtype, teacher_dtype, ids_int64, labels_int64, reduction;
+    float temperature, label_weight;
+    const void *logits, *teacher, *ids, *labels;
+    float *loss, *stats;
+    const float *d_loss;
+    void *d_logits;
+    void *workspace;
+    int64_t workspace_bytes;
+} dsalt_distill_args;
+int dsalt_distill(const dsalt_distill_args *args, void *stream);
+int dsalt_distill_bwd(const dsalt_distill_args *args, void *stream);
+int dsalt_distill_check(const dsalt_distill_args *args, int32_t backward);
+int64_t dsalt_distill_workspace_size(int64_t rows, int32_t vocab);
+int64_t dsalt_distill_stats_count(int64_t rows);
+size_t dsalt_distill_args_size(void);
+
 int dsalt_abi_version(void);
 const char *dsalt_last_error(void);
 /* sizeof of the argument structs as compiled into the library (ABI layout check). */

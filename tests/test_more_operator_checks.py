@@ -1,11 +1,13 @@
-"""Host-side refusals of the layer norm's entry points (no GPU), and the modules' forms on the CPU."""
+"""Host-side refusals of the layer norm's and the distillation loss's entry points (no GPU), and their
+plain forms on the CPU."""
 import ctypes
 
 import pytest
 import torch
 
 import dsalt._hip as hip
-from dsalt.kernels import LayerNorm, add_layer_norm, layer_norm
+from dsalt.kernels import LayerNorm, add_layer_norm, distill_loss, layer_norm
+from dsalt.kernels.distill import torch_distill_loss
 
 
 def test_layer_norm_refuses_cpu_tensors():
@@ -56,3 +58,68 @@ def test_layer_norm_module_on_the_cpu(bias):
     torch.testing.assert_close(y, want)
     assert torch.equal(s, x + h) and m(x.bfloat16()).dtype == torch.bfloat16
     assert set(dict(m.named_parameters())) == ({"weight", "bias"} if bias else {"weight"})
+
+
+def test_distill_refuses_cpu_tensors_and_bad_values():
+    s, z, ids = torch.zeros(2, 9), torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.long)
+    with pytest.raises(hip.DsaltError, match="ROCm GPU"):
+        distill_loss(s, z, ids)
+    for kw in (dict(temperature=0.0), dict(label_weight=2.0), dict(label_weight=0.5), dict(reduction="batchmean")):
+        with pytest.raises(ValueError):
+            distill_loss(s, z, ids, **kw)
+
+
+def distill_args(**kw):
+    a = hip.DistillArgs(rows=4, logits_stride=100, teacher_stride=8, ids_stride=8, ignore_index=-100, vocab=100, k=8, logits_dtype=0,
+                        teacher_dtype=2, ids_int64=1, labels_int64=1, reduction=1, temperature=2.0, label_weight=0.5,
+                        workspace_bytes=1 << 30)
+    for i, n in enumerate(("logits", "teacher", "ids", "labels", "loss", "stats", "d_loss", "d_logits", "workspace")):
+        setattr(a, n, 0x10000000 + i * 0x100000)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,backward,code", [
+    ({}, 0, 0), ({}, 1, 0), ({"rows": -1}, 0, 1), ({"rows": 1 << 24}, 0, 1), ({"vocab": 0}, 0, 2), ({"vocab": (1 << 30) + 1}, 0, 2),
+    ({"k": 0}, 0, 2), ({"k": 1025, "teacher_stride": 1025, "ids_stride": 1025}, 0, 2), ({"logits_dtype": 3}, 0, 1), ({"teacher_dtype": -1}, 0, 1),
+    ({"reduction": 3}, 0, 1), ({"temperature": 0.0}, 0, 1), ({"temperature": float("inf")}, 0, 1), ({"temperature": float("nan")}, 0, 1),
+    ({"label_weight": 1.01}, 0, 1), ({"label_weight": float("nan")}, 0, 1), ({"labels": None}, 0, 1), ({"labels": None, "label_weight": 0.0}, 0, 0),
+    ({"logits_stride": 99}, 0, 1), ({"ids_stride": 7}, 0, 1), ({"teacher_stride": -8}, 0, 1), ({"logits": 0x10000001}, 0, 1),
+    ({"logits": 0x10000002}, 0, 0), ({"ids": 0x10000004}, 0, 1), ({"ids": 0x10000004, "ids_int64": 0}, 0, 0), ({"teacher": None}, 0, 1),
+    ({"loss": None}, 0, 1), ({"stats": None}, 0, 0), ({"stats": None}, 1, 1), ({"d_loss": None}, 1, 1), ({"d_logits": None}, 1, 1),
+    ({"workspace": None}, 0, 1), ({"workspace_bytes": 15}, 0, 1), ({"workspace": None}, 1, 0),
+    ({"rows": 0, "logits": None, "teacher": None, "ids": None, "labels": None, "workspace": None}, 0, 0)])
+def test_distill_check(kw, backward, code):
+    assert hip.lib().dsalt_distill_check(ctypes.byref(distill_args(**kw)), backward) == code, hip.lib().dsalt_last_error()
+
+
+def test_distill_workspace():
+    lib = hip.lib()
+    assert lib.dsalt_distill(None, None) == 1 and lib.dsalt_distill_workspace_size(-1, 9) == 0
+    need = lib.dsalt_distill_workspace_size(3, 50000)  # few long rows are cut into slices
+    assert need > 12 and lib.dsalt_distill_workspace_size(3, 500) == 12
+    args = distill_args(rows=3, vocab=50000, logits_stride=50000, workspace_bytes=need - 1)
+    assert lib.dsalt_distill_check(ctypes.byref(args), 0) == 1
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_distill_in_torch_ops(reduction):
+    """The plain form against the definition, rows without slots or label among them."""
+    g = torch.Generator().manual_seed(1)
+    s, z = torch.randn(5, 11, generator=g, dtype=torch.float64), torch.randn(5, 3, generator=g)
+    ids = torch.tensor([[1, 4, 9], [0, 0, -1], [-1, 11, -5], [2, 3, 4], [7, 8, 9]])
+    z[4, 0] = float("-inf")
+    y = torch.tensor([4, 2, 3, -100, 10])
+    want = []
+    for r in range(5):
+        if y[r] < 0:
+            want.append(torch.zeros((), dtype=torch.float64))
+            continue
+        on = (ids[r] >= 0) & (ids[r] < 11) & (z[r] > float("-inf"))
+        p = torch.softmax(z[r][on].double() / 2, 0)
+        kl = (p * (p.log() - torch.log_softmax(s[r] / 2, 0)[ids[r][on]])).sum()
+        want.append(0.7 * 4 * kl - 0.3 * torch.log_softmax(s[r], 0)[y[r]])
+    want = torch.stack(want)
+    got = torch_distill_loss(s, z, ids, y, (2.0, 0.3, -100, reduction))
+    torch.testing.assert_close(got, {"mean": want.sum() / 4, "sum": want.sum(), "none": want}[reduction])
