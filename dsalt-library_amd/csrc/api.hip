@@ -910,6 +910,73 @@ int64_t dsalt_distill_workspace_size(int64_t rows, int32_t vocab) {
 int64_t dsalt_distill_stats_count(int64_t rows) { return rows < 0 ? 0 : dsalt::distill_stats_count(rows); }
 size_t dsalt_distill_args_size(void) { return sizeof(dsalt_distill_args); }
 
+int dsalt_fp8_quantize(const dsalt_fp8_quantize_args *a, void *stream) {
+    if (!a) return fail(DSALT_ERR_INVALID, "args must be non-NULL");
+    if (a->rows < 0 || a->rows > (1 << 30)) return fail(DSALT_ERR_INVALID, "rows must be in [0, 2^30] (got %lld)", (long long)a->rows);
+    if (a->k < 1 || a->k > (1 << 20)) return fail(DSALT_ERR_UNSUPPORTED, "k must be in [1, 2^20] (got %d)", a->k);
+    const int blocks = (a->k + 127) / 128;
+    if (a->tile && (a->rows + 127) / 128 * blocks > (1 << 23))  // a launch's threads
+        return fail(DSALT_ERR_UNSUPPORTED, "more than 2^23 tiles (rows %lld, k %d)", (long long)a->rows, a->k);
+    if (!float_dtype(a->x_dtype)) return fail(DSALT_ERR_INVALID, "x_dtype %d is not a float dtype", a->x_dtype);
+    if (a->x_stride < a->k || a->x_stride > ((int64_t)1 << 40) || a->scale_stride < blocks)
+        return fail(DSALT_ERR_INVALID, "row strides must cover their rows");
+    if (!aligned(a->x, a->x_dtype == DSALT_DTYPE_F32 ? 4 : 2) || !aligned(a->q, 8) || !aligned(a->scale, a->scale_f32 ? 4 : 1))
+        return fail(DSALT_ERR_INVALID, "x and scale must be aligned to their elements, q to 8 bytes");
+    if (a->rows > 0 && (!a->x || !a->q || !a->scale)) return fail(DSALT_ERR_INVALID, "x, q and scale must be non-NULL");
+    hipError_t e = dsalt::launch_fp8_quantize(*a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_fp8_quantize launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+size_t dsalt_fp8_quantize_args_size(void) { return sizeof(dsalt_fp8_quantize_args); }
+
+int dsalt_fp8_matmul_check(const dsalt_fp8_matmul_args *a) {
+    if (!a) return fail(DSALT_ERR_INVALID, "args must be non-NULL");
+    if (a->m < 0 || a->m > (1 << 24)) return fail(DSALT_ERR_INVALID, "m must be in [0, 2^24] (got %lld)", (long long)a->m);
+    if (a->n < 1 || a->n > (1 << 20) || a->k < 16 || a->k % 16 || a->k > (1 << 20))
+        return fail(DSALT_ERR_UNSUPPORTED, "n must be in [1, 2^20], k a multiple of 16 up to 2^20 (got %d, %d)", a->n, a->k);
+    if (a->m * a->n > ((int64_t)1 << 38)) return fail(DSALT_ERR_UNSUPPORTED, "m * n is more than 2^38 (%lld x %d)", (long long)a->m, a->n);
+    const bool quant = a->a_dtype != DSALT_DTYPE_E4M3;
+    if (quant && !float_dtype(a->a_dtype)) return fail(DSALT_ERR_INVALID, "a_dtype %d is no type of rows", a->a_dtype);
+    if (quant && a->m > dsalt::fp8_few_rows())
+        return fail(DSALT_ERR_UNSUPPORTED, "rows of dtype %d are quantised on the way up to m = %d (got %lld)", a->a_dtype,
+                    dsalt::fp8_few_rows(), (long long)a->m);
+    if (!float_dtype(a->out_dtype) || (a->bias && !float_dtype(a->bias_dtype)))
+        return fail(DSALT_ERR_INVALID, "out_dtype %d or bias_dtype %d is not a float dtype", a->out_dtype, a->bias_dtype);
+    const int64_t size = !quant ? 1 : a->a_dtype == DSALT_DTYPE_F32 ? 4 : 2;
+    const struct { const char *name; int64_t stride, bytes; } rows[] = {{"a", a->a_stride, a->a_stride * size},
+                                                                        {"b", a->b_stride, a->b_stride}};
+    for (const auto &r : rows)
+        if (r.stride < a->k || r.stride > (1 << 22) || r.bytes % 16 || r.bytes > (1 << 22))
+            return fail(DSALT_ERR_UNSUPPORTED, "%s row stride must cover k, its bytes a multiple of 16 up to 2^22 (got %lld elements)",
+                        r.name, (long long)r.stride);
+    const int64_t strides[] = {a->b_scale_stride_n, a->b_scale_stride_k, quant ? 1 : a->a_scale_stride_m, quant ? 1 : a->a_scale_stride_k};
+    for (int64_t s : strides)
+        if (s < 1 || s > (1 << 21)) return fail(DSALT_ERR_UNSUPPORTED, "scale strides must be in [1, 2^21] (got %lld)", (long long)s);
+    if (!aligned(a->a, 16) || !aligned(a->b, 16) || !aligned(a->out, 16) || !aligned(a->workspace, 16) ||
+        (!quant && !aligned(a->a_scale, a->a_scale_e8m0 ? 1 : 4)) || !aligned(a->b_scale, a->b_scale_e8m0 ? 1 : 4) ||
+        !aligned(a->bias, a->bias_dtype == DSALT_DTYPE_F32 ? 4 : 2))
+        return fail(DSALT_ERR_INVALID, "a, b, out and workspace must be 16-byte aligned, scales and bias to their elements");
+    if (a->m > 0 && (!a->a || !a->b || !a->b_scale || !a->out || (!quant && !a->a_scale)))
+        return fail(DSALT_ERR_INVALID, "operands, scales and out must be non-NULL");
+    const int64_t need = dsalt::fp8_workspace_bytes(a->m, a->n, a->k);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need))
+        return fail(DSALT_ERR_INVALID, "workspace of dsalt_fp8_matmul_workspace_size (%lld) bytes needed", (long long)need);
+    return DSALT_OK;
+}
+
+int dsalt_fp8_matmul(const dsalt_fp8_matmul_args *args, void *stream) {
+    if (int rc = dsalt_fp8_matmul_check(args)) return rc;
+    hipError_t e = dsalt::launch_fp8_matmul(*args, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(DSALT_ERR_LAUNCH, "dsalt_fp8_matmul launch failed: %s", hipGetErrorString(e));
+    return DSALT_OK;
+}
+
+int64_t dsalt_fp8_matmul_workspace_size(int64_t m, int32_t n, int32_t k) {
+    return m < 0 || n < 1 || k < 1 ? 0 : dsalt::fp8_workspace_bytes(m, n, k);
+}
+int dsalt_fp8_few_rows(void) { return dsalt::fp8_few_rows(); }
+size_t dsalt_fp8_matmul_args_size(void) { return sizeof(dsalt_fp8_matmul_args); }
+
 int dsalt_rope_check(const dsalt_rope_args *a) {
     if (!a) return fail(DSALT_ERR_INVALID, "args is NULL");
     if (a->total_len < 0 || a->n_q_heads < 0 || a->n_k_heads < 0)

@@ -92,6 +92,10 @@ hipError_t launch_distill(const dsalt_distill_args &a, hipStream_t stream);
 hipError_t launch_distill_bwd(const dsalt_distill_args &a, hipStream_t stream);
 int64_t distill_workspace_bytes(int64_t rows, int vocab);
 int64_t distill_stats_count(int64_t rows);
+hipError_t launch_fp8_quantize(const dsalt_fp8_quantize_args &a, hipStream_t stream);
+hipError_t launch_fp8_matmul(const dsalt_fp8_matmul_args &a, hipStream_t stream);
+int64_t fp8_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int fp8_few_rows();
 
 // Number of query blocks of `bm` tokens over a packed batch, as an upper bound that is
 // computable without reading cu_seqlens: sum_s ceil(L_s/bm) <= ceil(T/bm) + S.

@@ -9,6 +9,7 @@ consumers ``DSALTTransformerBlock`` / ``DSALTLMHeadModel``. ``DSALTConfig`` and
 """
 from ._hip import DsaltError
 from .kernels import (
+    FP8Linear,
     HybridEnergyLandmarkSelector,
     LayerNorm,
     RMSENorm,
@@ -24,6 +25,9 @@ from .kernels import (
     distill_loss,
     dsalt_triton_attention,
     dsalt_triton_backward,
+    fp8_linear,
+    fp8_matmul,
+    fp8_quantize,
     gated_ffn,
     hybrid_scores_per_head,
     layer_norm,
@@ -49,6 +53,10 @@ __all__ = [
     "gated_ffn",
     "counter_dropout",
     "branch_norm",
+    "fp8_quantize",
+    "fp8_matmul",
+    "fp8_linear",
+    "FP8Linear",
     "distill_loss",
     "layer_norm",
     "add_layer_norm",

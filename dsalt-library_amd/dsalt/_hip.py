@@ -255,6 +255,27 @@ class DistillArgs(ctypes.Structure):
     ]
 
 
+class Fp8QuantizeArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64), ("x_stride", c_int64), ("scale_stride", c_int64),
+        ("k", c_int32), ("x_dtype", c_int32), ("tile", c_int32), ("scale_f32", c_int32),
+        ("x", c_void_p), ("q", c_void_p), ("scale", c_void_p),
+    ]
+
+
+class Fp8MatmulArgs(ctypes.Structure):
+    _fields_ = [
+        ("m", c_int64), ("n", c_int32), ("k", c_int32),
+        ("a_dtype", c_int32), ("a_scale_e8m0", c_int32), ("b_scale_e8m0", c_int32), ("bias_dtype", c_int32),
+        ("out_dtype", c_int32), ("reserved", c_int32),
+        ("a", c_void_p), ("a_scale", c_void_p),
+        ("a_stride", c_int64), ("a_scale_stride_m", c_int64), ("a_scale_stride_k", c_int64),
+        ("b", c_void_p), ("b_scale", c_void_p),
+        ("b_stride", c_int64), ("b_scale_stride_n", c_int64), ("b_scale_stride_k", c_int64),
+        ("bias", c_void_p), ("out", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "dsalt_fwd", "dsalt_fwd_check", "dsalt_bwd", "dsalt_bwd_check", "dsalt_bwd_workspace_size",
     "dsalt_select_landmarks", "dsalt_select_check", "dsalt_quantize_windows",
@@ -272,7 +293,9 @@ EXPORTED_SYMBOLS = (
     "dsalt_branch_norm_bwd", "dsalt_branch_norm_check", "dsalt_branch_norm_workspace_size", "dsalt_branch_norm_args_size",
     "dsalt_layer_norm", "dsalt_layer_norm_bwd", "dsalt_layer_norm_check", "dsalt_layer_norm_workspace_size",
     "dsalt_layer_norm_args_size", "dsalt_distill", "dsalt_distill_bwd", "dsalt_distill_check", "dsalt_distill_workspace_size",
-    "dsalt_distill_stats_count", "dsalt_distill_args_size",
+    "dsalt_distill_stats_count", "dsalt_distill_args_size", "dsalt_fp8_quantize", "dsalt_fp8_quantize_args_size",
+    "dsalt_fp8_matmul", "dsalt_fp8_matmul_check", "dsalt_fp8_matmul_workspace_size", "dsalt_fp8_few_rows",
+    "dsalt_fp8_matmul_args_size",
 )
 NOALLOC_SCRATCH_BYTES = 76 << 20  # DSALT_NOALLOC_SCRATCH_BYTES
 SELECT_SPLIT_MIN = 4096  # longer sequences can be selected chunk-wise
@@ -334,6 +357,10 @@ def lib() -> ctypes.CDLL:
         ("dsalt_distill", [ctypes.POINTER(DistillArgs), c_void_p]),
         ("dsalt_distill_bwd", [ctypes.POINTER(DistillArgs), c_void_p]),
         ("dsalt_distill_check", [ctypes.POINTER(DistillArgs), c_int32]),
+        ("dsalt_fp8_quantize", [ctypes.POINTER(Fp8QuantizeArgs), c_void_p]),
+        ("dsalt_fp8_matmul", [ctypes.POINTER(Fp8MatmulArgs), c_void_p]),
+        ("dsalt_fp8_matmul_check", [ctypes.POINTER(Fp8MatmulArgs)]),
+        ("dsalt_fp8_few_rows", []),
         ("dsalt_add_rms_norm", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int32,
                                 c_void_p]),
     ):
@@ -362,6 +389,8 @@ def lib() -> ctypes.CDLL:
     h.dsalt_distill_workspace_size.restype = c_int64
     h.dsalt_distill_stats_count.argtypes = [c_int64]
     h.dsalt_distill_stats_count.restype = c_int64
+    h.dsalt_fp8_matmul_workspace_size.argtypes = [c_int64, c_int32, c_int32]
+    h.dsalt_fp8_matmul_workspace_size.restype = c_int64
     h.dsalt_lmk_weights_workspace_size.argtypes = [c_int32] * 2
     h.dsalt_lmk_weights_workspace_size.restype = c_int64
     h.dsalt_abi_version.restype = ctypes.c_int
@@ -370,7 +399,7 @@ def lib() -> ctypes.CDLL:
               "dsalt_rope_args_size", "dsalt_lmk_weights_args_size", "dsalt_rope_tables_size", "dsalt_qkv_args_size",
               "dsalt_module_grads_args_size", "dsalt_norm_train_args_size", "dsalt_gated_ffn_args_size",
               "dsalt_dropout_args_size", "dsalt_branch_norm_args_size", "dsalt_layer_norm_args_size",
-              "dsalt_distill_args_size"):
+              "dsalt_distill_args_size", "dsalt_fp8_quantize_args_size", "dsalt_fp8_matmul_args_size"):
         getattr(h, n).restype = c_size_t
     _lib = h
     check_abi()
@@ -388,11 +417,14 @@ def check_abi() -> None:
                        (ModuleGradsArgs, h.dsalt_module_grads_args_size),
                        (NormTrainArgs, h.dsalt_norm_train_args_size), (GatedFfnArgs, h.dsalt_gated_ffn_args_size),
                        (DropoutArgs, h.dsalt_dropout_args_size), (BranchNormArgs, h.dsalt_branch_norm_args_size),
-                       (LayerNormArgs, h.dsalt_layer_norm_args_size), (DistillArgs, h.dsalt_distill_args_size)):
+                       (LayerNormArgs, h.dsalt_layer_norm_args_size), (DistillArgs, h.dsalt_distill_args_size),
+                       (Fp8QuantizeArgs, h.dsalt_fp8_quantize_args_size),
+                       (Fp8MatmulArgs, h.dsalt_fp8_matmul_args_size)):
         if ctypes.sizeof(args) != fn():
             raise DsaltError(f"{args.__name__} layout mismatch: {ctypes.sizeof(args)} vs {fn()} bytes")
     for pack, args in ((_FFN_PACK, GatedFfnArgs), (_DROPOUT_PACK, DropoutArgs), (_BRANCH_PACK, BranchNormArgs),
-                       (_LAYER_PACK, LayerNormArgs), (_DISTILL_PACK, DistillArgs)):
+                       (_LAYER_PACK, LayerNormArgs), (_DISTILL_PACK, DistillArgs),
+                       (_FP8_QUANT_PACK, Fp8QuantizeArgs), (_FP8_PACK, Fp8MatmulArgs)):
         if pack.size != ctypes.sizeof(args):
             raise DsaltError(f"{args.__name__} packs to {pack.size} of {ctypes.sizeof(args)} bytes")
 
@@ -1617,6 +1649,8 @@ _DROPOUT_PACK = struct.Struct("@q2iPP2qP")
 _BRANCH_PACK = struct.Struct("@q9i3f2qP5P2P2P2P5PPq")
 _LAYER_PACK = struct.Struct("@q6if4P3P2P4PPq")
 _DISTILL_PACK = struct.Struct("@5q7i2f4P2PPPPq")
+_FP8_QUANT_PACK = struct.Struct("@3q4i3P")
+_FP8_PACK = struct.Struct("@q8i2P3q2P3q3Pq")
 _packed_calls: dict = {}
 
 
@@ -1881,3 +1915,46 @@ def unit_rows(t: torch.Tensor) -> torch.Tensor:
     """t [n, m] with unit stride along the rows and row strides that cover them (a copy only where not so)."""
     rs, cs = t.stride()
     return t if (cs == 1 or t.shape[1] == 1) and rs >= t.shape[1] else t.clone(memory_format=torch.contiguous_format)
+
+
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+FP8_BLOCK = 128  # elements of a row, or rows and columns of a tile, that share a scale
+FP8_FEW_ROWS = 32  # dsalt_fp8_few_rows(): rows that dsalt_fp8_matmul quantises on the way
+
+
+def fp8_quantize(x: torch.Tensor, tile: bool, scale_f32: bool):
+    """``(q, scale)`` of `unit_rows` x [n, k]: see dsalt_fp8_quantize."""
+    n, k = x.shape
+    blocks = -(-k // FP8_BLOCK)
+    q = torch.empty((n, k), device=x.device, dtype=E4M3)
+    scale = torch.empty((-(-n // FP8_BLOCK) if tile else n, blocks), device=x.device, dtype=torch.float32 if scale_f32 else E8M0)
+    _call("dsalt_fp8_quantize", _FP8_QUANT_PACK.pack(n, x.stride(0), blocks, k, _SCORE_DTYPES[x.dtype], tile, scale_f32,
+                                                     x.data_ptr(), q.data_ptr(), scale.data_ptr()), x.device)
+    return q, scale
+
+
+def fp8_operand(t: torch.Tensor) -> torch.Tensor:
+    """t [n, k] as dsalt_fp8_matmul reads it: unit stride along k, 16-byte aligned rows (a copy only where
+    it is not so)."""
+    rs, cs = t.stride()
+    size = t.element_size()
+    if (cs == 1 or t.shape[1] == 1) and rs >= t.shape[1] and rs * size % 16 == 0 and rs * size <= 1 << 22 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def fp8_matmul(a, a_scale, b, b_scale, bias, lead, out_dtype: torch.dtype) -> torch.Tensor:
+    """[*lead, n] of `fp8_operand` a [m, k] and b [n, k] with their scales, or of up to FP8_FEW_ROWS rows a of
+    a wider type (a_scale None): see dsalt_fp8_matmul."""
+    m, k = a.shape
+    n, dev = b.shape[0], a.device
+    out = torch.empty((*lead, n), device=dev, dtype=out_dtype)
+    need = lib().dsalt_fp8_matmul_workspace_size(m, n, k) if m > FP8_FEW_ROWS else 0
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    sa = (0, 1, 1) if a_scale is None else (a_scale.data_ptr(), *a_scale.stride())
+    _call("dsalt_fp8_matmul",
+          _FP8_PACK.pack(m, n, k, 3 if a_scale is not None else _SCORE_DTYPES[a.dtype], a_scale is not None and a_scale.dtype is E8M0,
+                         b_scale.dtype is E8M0, _code(bias), _SCORE_DTYPES[out_dtype], 0, a.data_ptr(), sa[0], a.stride(0), sa[1], sa[2],
+                         b.data_ptr(), b_scale.data_ptr(), b.stride(0), *b_scale.stride(), _addr(bias), out.data_ptr(), _addr(ws),
+                         need), dev)
+    return out

@@ -20,6 +20,7 @@ from .branch_norm import branch_norm
 from .distill import distill_loss
 from .dropout import counter_dropout
 from .dsalt_triton_train import dsalt_triton_train_attention
+from .fp8 import FP8Linear, fp8_linear, fp8_matmul, fp8_quantize
 from .gated_ffn import gated_ffn
 from .landmark_tokens_ker import (
     HybridEnergyLandmarkSelector,
@@ -62,6 +63,10 @@ __all__ = [
     "gated_ffn",
     "counter_dropout",
     "branch_norm",
+    "fp8_quantize",
+    "fp8_matmul",
+    "fp8_linear",
+    "FP8Linear",
     "distill_loss",
     "layer_norm",
     "add_layer_norm",

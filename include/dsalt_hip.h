@@ -790,6 +790,58 @@ int64_t dsalt_distill_workspace_size(int64_t rows, int32_t vocab);
 int64_t dsalt_distill_stats_count(int64_t rows);
 size_t dsalt_distill_args_size(void);
 
+/*
+ * Quantisation of rows x [rows, k] to 8-bit floats (e4m3: 4 significant bits, up to 448) with a scale for
+ * each block: 128 consecutive elements of a row (tile = 0; scale [rows, ceil(k / 128)]), or a tile of 128 x
+ * 128 (tile = 1; scale [ceil(rows / 128), ceil(k / 128)]), blocks at the ends smaller. A block's scale s is
+ * the smallest power of two with max |x| <= 448 s, not below 2^-127 (1 for a block of zeros), and q = x / s
+ * rounded to nearest even. A block that holds infinities or NaN has scale and elements NaN. q [rows, k]
+ * contiguous; scale as fp32 (scale_f32) or as its exponent's byte (e8m0: 2^(b - 127), 255 NaN), with row
+ * stride scale_stride (elements). x BF16, F16 or F32, unit stride along k, aligned to its elements
+ * (16-byte aligned rows are the fast form).
+ */
+enum { DSALT_DTYPE_E4M3 = 3 };
+typedef struct dsalt_fp8_quantize_args {
+    int64_t rows, x_stride, scale_stride;
+    int32_t k, x_dtype, tile, scale_f32;
+    const void *x;
+    void *q, *scale;
+} dsalt_fp8_quantize_args;
+int dsalt_fp8_quantize(const dsalt_fp8_quantize_args *args, void *stream);
+size_t dsalt_fp8_quantize_args_size(void);
+
+/*
+ * Product of e4m3 matrices with block scales, a [m, k] and b [n, k]:
+ *   out[i, j] = sum over blocks t of 128 along k of
+ *               a_scale[i, t] * b_scale[j / 128, t] * (sum over k in t of a[i, k] b[j, k])  + bias[j]
+ * in fp32 with one rounding to out_dtype (BF16, F16, F32); out [m, n] contiguous. Scales are fp32, or e8m0
+ * bytes where *_e8m0, of any positive strides; with both e8m0 the matrix instruction applies them. With
+ * a_dtype BF16, F16 or F32 and m up to dsalt_fp8_few_rows(), a holds rows that are quantised on the way as
+ * dsalt_fp8_quantize (tile = 0) does, and a_scale is not read. bias [n] in bias_dtype, or NULL.
+ * k a multiple of 16 up to 2^20, n up to 2^20, m up to 2^24 with m * n up to 2^38; row strides (elements)
+ * at least k, their bytes multiples of 16 up to 2^22; a, b and out 16-byte aligned, scales and bias to their
+ * elements, scale strides in [1, 2^21]. workspace: dsalt_fp8_matmul_workspace_size bytes, 16-byte aligned,
+ * dead when the launches end (NULL where that is 0). out aliases no input. Sums run in a fixed order.
+ */
+typedef struct dsalt_fp8_matmul_args {
+    int64_t m;
+    int32_t n, k;
+    int32_t a_dtype, a_scale_e8m0, b_scale_e8m0, bias_dtype, out_dtype, reserved;
+    const void *a, *a_scale;
+    int64_t a_stride, a_scale_stride_m, a_scale_stride_k;
+    const void *b, *b_scale;
+    int64_t b_stride, b_scale_stride_n, b_scale_stride_k;
+    const void *bias;
+    void *out;
+    void *workspace;
+    int64_t workspace_bytes;
+} dsalt_fp8_matmul_args;
+int dsalt_fp8_matmul(const dsalt_fp8_matmul_args *args, void *stream);
+int dsalt_fp8_matmul_check(const dsalt_fp8_matmul_args *args);
+int64_t dsalt_fp8_matmul_workspace_size(int64_t m, int32_t n, int32_t k);
+int dsalt_fp8_few_rows(void);
+size_t dsalt_fp8_matmul_args_size(void);
+
 int dsalt_abi_version(void);
 const char *dsalt_last_error(void);
 /* sizeof of the argument structs as compiled into the library (ABI layout check). */

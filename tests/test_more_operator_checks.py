@@ -1,13 +1,14 @@
-"""Host-side refusals of the layer norm's and the distillation loss's entry points (no GPU), and their
-plain forms on the CPU."""
+"""Host-side refusals of the layer norm's, the distillation loss's and the 8-bit products' entry points
+(no GPU), and their plain forms on the CPU."""
 import ctypes
 
 import pytest
 import torch
 
 import dsalt._hip as hip
-from dsalt.kernels import LayerNorm, add_layer_norm, distill_loss, layer_norm
+from dsalt.kernels import FP8Linear, LayerNorm, add_layer_norm, distill_loss, fp8_linear, fp8_matmul, fp8_quantize, layer_norm
 from dsalt.kernels.distill import torch_distill_loss
+from dsalt.kernels.fp8 import torch_fp8_matmul, torch_fp8_quantize
 
 
 def test_layer_norm_refuses_cpu_tensors():
@@ -123,3 +124,88 @@ def test_distill_in_torch_ops(reduction):
     want = torch.stack(want)
     got = torch_distill_loss(s, z, ids, y, (2.0, 0.3, -100, reduction))
     torch.testing.assert_close(got, {"mean": want.sum() / 4, "sum": want.sum(), "none": want}[reduction])
+
+
+E4, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def test_fp8_refuses_cpu_tensors():
+    x, q, s = torch.zeros(4, 64), torch.zeros(4, 64).to(E4), torch.ones(4, 1)
+    for call in (lambda: fp8_quantize(x), lambda: fp8_matmul(q, s, q, s[:1]), lambda: fp8_linear(x, q, s[:1])):
+        with pytest.raises(hip.DsaltError, match="ROCm GPU"):
+            call()
+    with pytest.raises(ValueError, match="multiple of 16"):
+        FP8Linear(40, 8)
+
+
+def fp8_args(**kw):
+    a = hip.Fp8MatmulArgs(m=100, n=96, k=256, a_dtype=3, a_scale_e8m0=1, b_scale_e8m0=1, bias_dtype=2, out_dtype=0, a_stride=256,
+                          a_scale_stride_m=2, a_scale_stride_k=1, b_stride=256, b_scale_stride_n=2, b_scale_stride_k=1,
+                          workspace_bytes=1 << 40)
+    for i, n in enumerate(("a", "a_scale", "b", "b_scale", "bias", "out", "workspace")):
+        setattr(a, n, 0x10000000 + i * 0x100000)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({}, 0), ({"m": -1}, 1), ({"m": (1 << 24) + 1}, 1), ({"n": 0}, 2), ({"n": (1 << 20) + 1}, 2), ({"k": 0}, 2), ({"k": 120, "a_stride": 128}, 2),
+    ({"k": (1 << 20) + 16, "a_stride": 1 << 21, "b_stride": 1 << 21}, 2), ({"m": 1 << 24, "n": 1 << 15}, 2), ({"a_dtype": 4}, 1), ({"a_dtype": 0}, 2),
+    ({"a_dtype": 0, "m": 32}, 0), ({"a_dtype": 0, "m": 32, "a_scale": None}, 0), ({"a_scale": None}, 1), ({"out_dtype": 3}, 1),
+    ({"bias_dtype": 5}, 1), ({"bias_dtype": 5, "bias": None}, 0), ({"a_stride": 240}, 2), ({"b_stride": 264}, 2), ({"a_stride": (1 << 22) + 16}, 2),
+    ({"a_dtype": 2, "m": 3, "a_stride": 1 << 21}, 2), ({"a_scale_stride_m": 0}, 2), ({"b_scale_stride_k": (1 << 21) + 1}, 2), ({"a": 0x10000008}, 1),
+    ({"out": 0x10000004}, 1), ({"a_scale": 0x10000003}, 0), ({"a_scale": 0x10000003, "a_scale_e8m0": 0}, 1), ({"bias": 0x10000002}, 1),
+    ({"bias": 0x10000002, "bias_dtype": 0}, 0), ({"b": None}, 1), ({"out": None}, 1),
+    ({"m": 0, "a": None, "a_scale": None, "out": None}, 0)])
+def test_fp8_matmul_check(kw, code):
+    assert hip.lib().dsalt_fp8_matmul_check(ctypes.byref(fp8_args(**kw))) == code, hip.lib().dsalt_last_error()
+
+
+def test_fp8_workspace():
+    """A product of few tiles and many blocks of k is split along k and needs room for its parts."""
+    lib = hip.lib()
+    need = lib.dsalt_fp8_matmul_workspace_size(40, 64, 1 << 14)
+    assert need >= 2 * 40 * 64 * 4 and lib.dsalt_fp8_matmul_workspace_size(32, 64, 1 << 14) == 0
+    size = dict(m=40, n=64, k=1 << 14, a_stride=1 << 14, b_stride=1 << 14)
+    for more, code in (({"workspace_bytes": need}, 0), ({"workspace_bytes": need - 1}, 1), ({"workspace": None}, 1), ({"workspace": 0x10000004}, 1)):
+        assert lib.dsalt_fp8_matmul_check(ctypes.byref(fp8_args(**size, **more))) == code
+    assert lib.dsalt_fp8_matmul_check(None) == 1 and lib.dsalt_fp8_matmul(None, None) == 1
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({"rows": -1}, 1), ({"k": 0}, 2), ({"k": (1 << 20) + 1}, 2), ({"x_dtype": 3}, 1), ({"x_stride": 299}, 1), ({"scale_stride": 2}, 1),
+    ({"x": 0x10000001}, 1), ({"q": 0x10000004}, 1), ({"scale": 0x10000002, "scale_f32": 1}, 1), ({"x": None}, 1), ({"q": None}, 1),
+    ({"scale": None}, 1), ({"rows": 1 << 30, "tile": 1}, 2), ({"rows": 0, "x": None}, 0)])
+def test_fp8_quantize_check(kw, code):
+    a = hip.Fp8QuantizeArgs(rows=4, x_stride=300, scale_stride=3, k=300, x_dtype=0, x=0x10000000, q=0x10100000, scale=0x10200000)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    assert hip.lib().dsalt_fp8_quantize(ctypes.byref(a), None) == code, hip.lib().dsalt_last_error()
+
+
+def test_fp8_in_torch_ops():
+    """The plain forms on values whose scales and roundings can be named."""
+    x = torch.zeros(2, 200)
+    x[0, 0], x[0, 1], x[0, 150] = 448.0, 17.0, -449.0  # scales 1 and 2; 17 lies between 16 and 18, to even: 16
+    x[1, 3] = 3.0
+    q, s = torch_fp8_quantize(x, False, E8)
+    assert s.float().tolist() == [[1.0, 2.0], [2.0 ** -7, 1.0]]
+    assert q.float()[0, :2].tolist() == [448.0, 16.0] and q.float()[0, 150] == -224.0 and q.float()[1, 3] == 384.0
+    tq, ts = torch_fp8_quantize(x, True, torch.float32)
+    assert ts.tolist() == [[1.0, 2.0]] and tq.shape == x.shape
+    w, ws = torch_fp8_quantize(torch.eye(200), True, E8)
+    torch.testing.assert_close(torch_fp8_matmul(q, s, w, ws, torch.ones(200), torch.float32),
+                               q.float() * s.float().repeat_interleave(128, 1)[:, :200] + 1)
+
+
+def test_fp8_module_keeps_its_bytes():
+    m = FP8Linear(32, 130, bias=True)
+    assert m.weight_q.dtype is E4 and m.weight_scale.dtype is E8 and m.weight_scale.shape == (2, 1)
+    m.weight_bits.random_(0, 120)
+    kept = m.weight_bits.clone()
+    m.to(torch.bfloat16)
+    assert torch.equal(m.weight_bits, kept) and m.bias.dtype is torch.bfloat16
+    other = FP8Linear(32, 130, bias=True)
+    other.load_state_dict(m.state_dict())
+    assert torch.equal(other.weight_bits, kept)
