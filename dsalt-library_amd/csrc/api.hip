@@ -940,6 +940,8 @@ int dsalt_fp8_matmul_check(const dsalt_fp8_matmul_args *a) {
     if (quant && a->m > dsalt::fp8_few_rows())
         return fail(DSALT_ERR_UNSUPPORTED, "rows of dtype %d are quantised on the way up to m = %d (got %lld)", a->a_dtype,
                     dsalt::fp8_few_rows(), (long long)a->m);
+    if (!quant && !a->a_scale_e8m0 != !a->b_scale_e8m0)
+        return fail(DSALT_ERR_UNSUPPORTED, "scales must be of one type");
     if (!float_dtype(a->out_dtype) || (a->bias && !float_dtype(a->bias_dtype)))
         return fail(DSALT_ERR_INVALID, "out_dtype %d or bias_dtype %d is not a float dtype", a->out_dtype, a->bias_dtype);
     const int64_t size = !quant ? 1 : a->a_dtype == DSALT_DTYPE_F32 ? 4 : 2;

@@ -171,10 +171,16 @@ __device__ __forceinline__ void store_out(const Fp8Params &p, int64_t row, int64
     }
 }
 
-// A workgroup's tile: WM x WN waves over BM x BN, RING stages of one block of k in LDS. MX: both scales
-// are e8m0 and the matrix instruction applies them; otherwise a block's product is formed from zero and
-// added to the sums times the product of the scales, four multiply-adds an instruction.
-template <bool MX, int BM, int BN, int RING, int WM, int WN>
+// A workgroup's tile: WM x WN waves over BM x BN, two stages of one block of k in LDS. MX: both scales
+// are e8m0 and the matrix instruction applies them; otherwise both are fp32, and a block's product is formed
+// from zero and added to the sums times the product of the scales, four multiply-adds an instruction.
+//
+// A wave holds one set of B's operands and a ring of four of A's, each read two groups of products (a
+// group: one of A's with all of B's) before its own. The barrier that frees a stage stands before the last
+// two groups of a step: what they need is in registers by then and the next stage has landed. Under them
+// the next step's first two of A's are read, and each of B's as soon as its last product has been issued: it
+// is needed a group later.
+template <bool MX, int BM, int BN, int WM, int WN>
 struct Fp8Core {
     static constexpr int NW = WM * WN, THREADS = NW * 64, M16 = BM / WM / 16, N16 = BN / WN / 16;
     typedef GemmTile<kKContig, BM, 64, NW> TA;  // 64 pairs of bytes: a block
@@ -182,8 +188,9 @@ struct Fp8Core {
     static constexpr int LA = TA::LPW, LB = TB::LPW, LT = LA + LB + 1;
     // a stage: A's tile, B's tile, and 64 scales a wave: A's rows, then B's blocks
     static constexpr int ASTAGE = BM * 128, BSTAGE = BN * 128, SSTAGE = NW * 256, STAGE = ASTAGE + BSTAGE + SSTAGE;
-    static constexpr int LDS_BYTES = RING * STAGE;
-    static_assert(BM % 64 == 0 && BM / 64 < NW && BN / WN <= kFp8Block && RING >= 2, "a wave for B's scales beside A's");
+    static constexpr int LDS_BYTES = 2 * STAGE;
+    static_assert(BM % 64 == 0 && BM / 64 < NW && BN / WN <= kFp8Block, "a wave for B's scales beside A's");
+    static_assert(M16 % 4 == 0 && N16 % 2 == 0, "the ring of A's operands, and the pairs of the epilogue");
 
     f32x4 acc[M16][N16];
     int lane, wave, wm, wn;
@@ -207,102 +214,138 @@ struct Fp8Core {
         const Fp8Scales &sc = is_a ? p.sa : p.sb;
         const int64_t srow = is_a ? m0 + wave * 64 : n0 / kFp8Block;
         const int64_t sleft = wave > BM / 64 ? 0 : sc.rows - srow;
-        const uint32_t ssize = sc.size();
-        const bool sbyte = sc.e8m0;
+        constexpr uint32_t ssize = MX ? 1 : 4;
         const int slots = is_a ? 64 : (BN + kFp8Block - 1) / kFp8Block;
         const uint32_t soff = lane < sleft && lane < slots ? (uint32_t)(lane * sc.row_stride) * ssize : kOutOfRange;
-        auto issue = [&](int step, int stage, const typename TA::Step &sa, const typename TB::Step &sb, int u) {
+        typename TA::Step da;
+        typename TB::Step db;
+        i32x4 ds;
+        // past `last` the loads read nothing, so that every step counts the same number of loads
+        auto prepare = [&](int step) {
+            const bool on = step < last;
+            da = ta.step(p.a, m0, on ? (int64_t)step * 64 : k2, k2);
+            db = tb.step(p.b, n0, on ? (int64_t)step * 64 : k2, k2);
+            const char *q = sc.base + (srow * sc.row_stride + (on ? step : 0) * sc.k_stride) * ssize;
+            ds = uniform_rsrc(buffer_rsrc(q, on && sleft > 0 ? kOutOfRange - 1 : 0));
+        };
+        auto issue = [&](int stage, int u) {
             const uint32_t at = base + stage * STAGE;
-            if (u < LA) TA::issue(sa, u, at, wave);
-            else if (u < LA + LB) TB::issue(sb, u - LA, at + ASTAGE, wave);
+            if (u < LA) TA::issue(da, u, at, wave);
+            else if (u < LA + LB) TB::issue(db, u - LA, at + ASTAGE, wave);
             else {
-                const bool on = step < last && sleft > 0;
-                const char *q = sc.base + (srow * sc.row_stride + (on ? step : 0) * sc.k_stride) * ssize;
-                const i32x4 rsrc = uniform_rsrc(buffer_rsrc(q, on ? kOutOfRange - 1 : 0));
                 const uint32_t to = __builtin_amdgcn_readfirstlane(at + ASTAGE + BSTAGE + wave * 256);
-                if (sbyte) dma1(soff, rsrc, to);
-                else dma4(soff, rsrc, to);
+                if constexpr (MX) dma1(soff, ds, to);
+                else dma4(soff, ds, to);
             }
         };
-        // past `last` the loads read nothing, so that every step counts the same number of loads
-        auto prepare_a = [&](int step) { return ta.step(p.a, m0, step < last ? (int64_t)step * 64 : k2, k2); };
-        auto prepare_b = [&](int step) { return tb.step(p.b, n0, step < last ? (int64_t)step * 64 : k2, k2); };
 #pragma unroll
         for (int i = 0; i < M16; ++i)
 #pragma unroll
             for (int j = 0; j < N16; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (first >= last) return;
+        Fp8Frag ra[4], rb[N16];
+        uint32_t sa[4], sb, sb_next;
+        auto read_a = [&](const char *at, int i) {
+            ra[i % 4] = fp8_frag(fa.read(at, wm * M16 + i, 0), fa.read(at, wm * M16 + i, 1));
+            sa[i % 4] = reinterpret_cast<const uint32_t *>(at + ASTAGE + BSTAGE)[(wm * M16 + i) * 16 + (lane & 15)];
+        };
+        auto read_b = [&](const char *at, int j) {
+            rb[j] = fp8_frag(fb.read(at + ASTAGE, wn * N16 + j, 0), fb.read(at + ASTAGE, wn * N16 + j, 1));
+        };
+        auto read_sb = [&](const char *at) {
+            return reinterpret_cast<const uint32_t *>(at + ASTAGE + BSTAGE)[BM + wn * (N16 * 16) / kFp8Block];
+        };
+        prepare(first);
 #pragma unroll
-        for (int t = 0; t < RING - 1; ++t) {
-            const auto sa = prepare_a(first + t);
-            const auto sb = prepare_b(first + t);
+        for (int u = 0; u < LT; ++u) issue(0, u);
+        prepare(first + 1);
 #pragma unroll
-            for (int u = 0; u < LT; ++u) issue(first + t, t, sa, sb, u);
+        for (int u = 0; u < LT; ++u) issue(1, u);
+        tile_barrier<LT>();
+        // in the loop's order: its first waits then count the same reads behind theirs on every step
+        sb = read_sb(lds);
+        read_a(lds, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        read_a(lds, 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < N16; ++j) {
+            read_b(lds, j);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        int stage = 0, next = RING - 1;
+        int stage = 0;
         for (int t = first; t < last; ++t) {
-            // the step's tiles have landed, and every wave is done reading the stage that is loaded next
-            tile_barrier<(RING - 2) * LT>();
-            const char *at = lds + stage * STAGE, *bt = at + ASTAGE, *st = bt + BSTAGE;
-            const auto sa = prepare_a(t + RING - 1);
-            const auto sb = prepare_b(t + RING - 1);
-            Fp8Frag fbr[N16];
-#pragma unroll
-            for (int j = 0; j < N16; ++j) fbr[j] = fp8_frag(fb.read(bt, wn * N16 + j, 0), fb.read(bt, wn * N16 + j, 1));
-            const uint32_t *ss = reinterpret_cast<const uint32_t *>(st);
-            const uint32_t sbv = ss[BM + wn * (N16 * 16) / kFp8Block];
-            const float sbf = p.sb.e8m0 ? e8m0_f32(sbv) : __uint_as_float(sbv);
-            constexpr int NM = M16 * N16;
+            const char *at = lds + stage * STAGE, *next = lds + (stage ^ 1) * STAGE;
+            float sbf = 0.f;
+            if constexpr (!MX) sbf = __uint_as_float(sb);
 #pragma unroll
             for (int i = 0; i < M16; ++i) {
-                const Fp8Frag far = fp8_frag(fa.read(at, wm * M16 + i, 0), fa.read(at, wm * M16 + i, 1));
-                const uint32_t sav = ss[(wm * M16 + i) * 16 + (lane & 15)];
-                const float s = MX ? 0.f : (p.sa.e8m0 ? e8m0_f32(sav) : __uint_as_float(sav)) * sbf;
+                if (i == M16 - 2) {
+                    prepare(t + 2);
+                    __builtin_amdgcn_sched_barrier(0);
+                    tile_barrier<0>();
+                    sb_next = read_sb(next);
+                }
+                if (i < M16 - 2) read_a(at, i + 2);
+                else read_a(next, i - M16 + 2);
+                float s = 0.f;
+                if constexpr (!MX) s = __uint_as_float(sa[i % 4]) * sbf;
 #pragma unroll
                 for (int j = 0; j < N16; ++j) {
                     if constexpr (MX) {
-                        acc[i][j] = mfma_fp8(fbr[j], far, acc[i][j], (int)sbv, (int)sav);
+                        acc[i][j] = mfma_fp8(rb[j], ra[i % 4], acc[i][j], (int)sb, (int)sa[i % 4]);
+                        // held here: a product has no side effect that would keep it from drifting behind the
+                        // loads and the barrier, with copies of all that it needs
+                        asm volatile("" : "+v"(acc[i][j]));
                     } else {
-                        const f32x4 d = mfma_fp8(fbr[j], far);
+                        const f32x4 d = mfma_fp8(rb[j], ra[i % 4]);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s, acc[i][j][e]);
                     }
+                    if (i == M16 - 1) {
+                        __builtin_amdgcn_sched_barrier(0);  // not before the product that still needs the old one
+                        read_b(next, j);
+                    }
+                    // the loads of step t + 2, spread over the groups behind the barrier
+                    if (i >= M16 - 2) {
+                        constexpr int NM = 2 * N16;
 #pragma unroll
-                    for (int u = 0; u < LT; ++u)
-                        if (u * NM / LT == i * N16 + j) issue(t + RING - 1, next, sa, sb, u);
+                        for (int u = 0; u < LT; ++u)
+                            if (u * NM / LT == (i - M16 + 2) * N16 + j) issue(stage, u);
+                    }
                 }
+                if constexpr (!MX)
+#pragma unroll
+                    for (int j = 0; j < N16; ++j)
+                        if (i > 0) asm volatile("" : "+v"(acc[i - 1][j]));
+                __builtin_amdgcn_sched_barrier(0);
             }
-            next = stage;
-            stage = stage + 1 == RING ? 0 : stage + 1;
+            sb = sb_next;
+            stage ^= 1;
         }
         tile_barrier<0>();  // no load may land in LDS that another workgroup has by then
     }
 
-    // The accumulators hold four consecutive n of one m a lane. Each wave turns 16 rows at a time in its own
-    // part of LDS, free after run(), and takes them back as pieces of eight columns of whole rows.
-    static constexpr int COLS = N16 * 16, CHUNKS = COLS / 4, PIECES = COLS / 8;
-    static_assert(NW * 16 * COLS * 4 <= LDS_BYTES && 64 % PIECES == 0, "the waves' parts");
+    // Calls f(row, column, v) for eight consecutive columns of the tile a lane. The accumulators hold four
+    // consecutive n of one m; of two neighbouring blocks of 16 columns a lane takes eight of one, in exchange
+    // with the lanes 16 further on.
     template <class F>
-    __device__ __forceinline__ void each_piece(char *lds, F f) const {
-        char *part = lds + wave * (16 * COLS * 4);
+    __device__ __forceinline__ void each_piece(F f) const {
+        const int g = lane >> 4;
 #pragma unroll
-        for (int i = 0; i < M16; ++i) {
+        for (int i = 0; i < M16; ++i)
 #pragma unroll
-            for (int j = 0; j < N16; ++j)
-                *reinterpret_cast<f32x4 *>(part + (lane & 15) * (COLS * 4) +
-                                           (((j * 4 + (lane >> 4)) ^ (lane & 15 & (CHUNKS - 1))) << 4)) = acc[i][j];
-            __builtin_amdgcn_wave_barrier();
+            for (int j = 0; j < N16; j += 2) {
+                float v[8];
 #pragma unroll
-            for (int t = 0; t < 16 * PIECES / 64; ++t) {
-                const int piece = t * 64 + lane, r = piece / PIECES, c = piece % PIECES * 2;
-                const char *q = part + r * (COLS * 4);
-                const float4 lo = *reinterpret_cast<const float4 *>(q + ((c ^ (r & (CHUNKS - 1))) << 4));
-                const float4 hi = *reinterpret_cast<const float4 *>(q + (((c + 1) ^ (r & (CHUNKS - 1))) << 4));
-                float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                f((wm * M16 + i) * 16 + r, wn * COLS + c * 4, v);
+                for (int e = 0; e < 4; ++e) {
+                    // lane groups (0, 1, 2, 3) of the pair: (j, j + 1, j, j + 1) at columns (0, 0, 8, 8)
+                    auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][j][e]), __float_as_uint(acc[i][j + 1][e]), false, false);
+                    v[e] = __uint_as_float(x[0]);
+                    v[4 + e] = __uint_as_float(x[1]);
+                }
+                f((wm * M16 + i) * 16 + (lane & 15), (wn * N16 + j + (g & 1)) * 16 + (g >> 1) * 8, v);
             }
-            __builtin_amdgcn_wave_barrier();
-        }
     }
 };
 
@@ -320,9 +363,9 @@ __device__ __forceinline__ bool fp8_tile(const Fp8Params &p, int &tm, int &tn, i
     return true;
 }
 
-template <bool MX, int BM, int BN, int RING, int WM, int WN>
+template <bool MX, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM *WN * 64) fp8_tile_kernel(const Fp8Params p) {
-    typedef Fp8Core<MX, BM, BN, RING, WM, WN> Core;
+    typedef Fp8Core<MX, BM, BN, WM, WN> Core;
     extern __shared__ char lds[];
     int tm, tn, split;
     if (!fp8_tile(p, tm, tn, split)) return;
@@ -331,7 +374,7 @@ __global__ void __launch_bounds__(WM *WN * 64) fp8_tile_kernel(const Fp8Params p
     const int per = (p.kb + p.splits - 1) / p.splits, first = split * per;
     core.run(lds, p, m0, n0, first, min(first + per, p.kb));
     float *part = p.splits > 1 ? p.part + split * p.m * p.n : nullptr;
-    core.each_piece(lds, [&](int r, int c, float (&v)[8]) {
+    core.each_piece([&](int r, int c, float (&v)[8]) {
         const int64_t row = m0 + r, col = n0 + c;
         if (row >= p.m || col >= p.n) return;
         if (!part) return store_out<8>(p, row, col, v);
@@ -474,13 +517,13 @@ __global__ void __launch_bounds__(64 * kRowWaves) fp8_rows_kernel(const Fp8Param
 constexpr int kFewRows = 32;
 
 // ---- launches -------------------------------------------------------------------------------
-template <bool MX, int BM, int BN, int RING, int WM, int WN>
+template <bool MX, int BM, int BN, int WM, int WN>
 hipError_t launch_tile(Fp8Params p, hipStream_t stream) {
-    typedef Fp8Core<MX, BM, BN, RING, WM, WN> Core;
+    typedef Fp8Core<MX, BM, BN, WM, WN> Core;
     p.tiles_m = (int)((p.m + BM - 1) / BM);
     p.tiles_n = (int)((p.n + BN - 1) / BN);
     const int64_t groups = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    const auto kernel = fp8_tile_kernel<MX, BM, BN, RING, WM, WN>;
+    const auto kernel = fp8_tile_kernel<MX, BM, BN, WM, WN>;
     if (Core::LDS_BYTES > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                  Core::LDS_BYTES);
@@ -490,16 +533,16 @@ hipError_t launch_tile(Fp8Params p, hipStream_t stream) {
     return hipGetLastError();
 }
 
-enum { kTile256, kTile128, kTile64 };
+enum { kTile256, kTile128, kTile64 };  // 256 x 256 (x 128 without MX), 128 x 128, 64 x 128
 struct Plan {
     int tile, splits;
 };
-constexpr int kTileSize[] = {256, 128, 64};
 
 Plan plan(int64_t m, int64_t n, int64_t k) {
     const int kb = (int)((k + kFp8Block - 1) / kFp8Block);
     for (int t : {kTile256, kTile128, kTile64}) {
-        const int64_t s = kTileSize[t], tiles = ((m + s - 1) / s) * ((n + s - 1) / s);
+        const int64_t bm = t == kTile256 ? 256 : t == kTile128 ? 128 : 64, bn = t == kTile256 ? 256 : 128;
+        const int64_t tiles = ((m + bm - 1) / bm) * ((n + bn - 1) / bn);
         if (tiles >= 256 || t == kTile64) {
             int splits = 1;
             while (t == kTile64 && tiles * splits * 2 <= 512 && kb / (splits * 2) >= 4) splits *= 2;
@@ -513,10 +556,10 @@ template <bool MX>
 hipError_t launch_tiles(const Fp8Params &p, int tile, hipStream_t stream) {
     switch (tile) {
         case kTile256:  // without MX a wave's 128 x 64 would need more registers than two waves a SIMD have
-            if constexpr (MX) return launch_tile<true, 256, 256, 2, 2, 4>(p, stream);
-            else return launch_tile<false, 256, 128, 3, 4, 2>(p, stream);
-        case kTile128: return launch_tile<MX, 128, 128, 2, 2, 2>(p, stream);
-        default: return launch_tile<MX, 64, 64, 3, 2, 2>(p, stream);
+            if constexpr (MX) return launch_tile<true, 256, 256, 2, 4>(p, stream);
+            else return launch_tile<false, 256, 128, 4, 2>(p, stream);
+        case kTile128: return launch_tile<MX, 128, 128, 2, 2>(p, stream);
+        default: return launch_tile<MX, 64, 128, 1, 4>(p, stream);
     }
 }
 

@@ -108,6 +108,8 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     _no_grad(bias)
     if not eager(*(t for t in (a, a_scale, b, b_scale, bias) if t is not None)):
         return torch_fp8_matmul(a, a_scale, b, b_scale, bias, out_dtype)
+    if a_scale.dtype is not b_scale.dtype:  # the kernel takes both alike
+        a_scale, b_scale = a_scale.float(), b_scale.float()
     flat, s = (a, a_scale) if a.dim() == 2 else (a.reshape(-1, k), a_scale.reshape(-1, a_scale.shape[-1]))
     return _hip.fp8_matmul(_hip.fp8_operand(flat), _scale(s), _hip.fp8_operand(b), _scale(b_scale),
                            None if bias is None else _hip.contiguous_rows(bias), a.shape[:-1], out_dtype)

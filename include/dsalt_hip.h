@@ -814,8 +814,8 @@ size_t dsalt_fp8_quantize_args_size(void);
  * Product of e4m3 matrices with block scales, a [m, k] and b [n, k]:
  *   out[i, j] = sum over blocks t of 128 along k of
  *               a_scale[i, t] * b_scale[j / 128, t] * (sum over k in t of a[i, k] b[j, k])  + bias[j]
- * in fp32 with one rounding to out_dtype (BF16, F16, F32); out [m, n] contiguous. Scales are fp32, or e8m0
- * bytes where *_e8m0, of any positive strides; with both e8m0 the matrix instruction applies them. With
+ * in fp32 with one rounding to out_dtype (BF16, F16, F32); out [m, n] contiguous. Scales are both fp32, or both
+ * e8m0 bytes (*_e8m0), which the matrix instruction applies, of any positive strides. With
  * a_dtype BF16, F16 or F32 and m up to dsalt_fp8_few_rows(), a holds rows that are quantised on the way as
  * dsalt_fp8_quantize (tile = 0) does, and a_scale is not read. bias [n] in bias_dtype, or NULL.
  * k a multiple of 16 up to 2^20, n up to 2^20, m up to 2^24 with m * n up to 2^38; row strides (elements)

@@ -155,7 +155,8 @@ def fp8_args(**kw):
     ({"a_dtype": 0, "m": 32}, 0), ({"a_dtype": 0, "m": 32, "a_scale": None}, 0), ({"a_scale": None}, 1), ({"out_dtype": 3}, 1),
     ({"bias_dtype": 5}, 1), ({"bias_dtype": 5, "bias": None}, 0), ({"a_stride": 240}, 2), ({"b_stride": 264}, 2), ({"a_stride": (1 << 22) + 16}, 2),
     ({"a_dtype": 2, "m": 3, "a_stride": 1 << 21}, 2), ({"a_scale_stride_m": 0}, 2), ({"b_scale_stride_k": (1 << 21) + 1}, 2), ({"a": 0x10000008}, 1),
-    ({"out": 0x10000004}, 1), ({"a_scale": 0x10000003}, 0), ({"a_scale": 0x10000003, "a_scale_e8m0": 0}, 1), ({"bias": 0x10000002}, 1),
+    ({"out": 0x10000004}, 1), ({"a_scale": 0x10000003}, 0), ({"a_scale": 0x10000003, "a_scale_e8m0": 0, "b_scale_e8m0": 0}, 1), ({"a_scale_e8m0": 0}, 2),
+    ({"a_scale_e8m0": 0, "a_dtype": 0, "m": 8}, 0), ({"bias": 0x10000002}, 1),
     ({"bias": 0x10000002, "bias_dtype": 0}, 0), ({"b": None}, 1), ({"out": None}, 1),
     ({"m": 0, "a": None, "a_scale": None, "out": None}, 0)])
 def test_fp8_matmul_check(kw, code):
