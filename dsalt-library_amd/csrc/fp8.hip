@@ -128,8 +128,9 @@ struct Fp8Params {
     int bias_dtype;
     void *out;
     int out_dtype;
-    float *part;  // [splits][m][n], where k is split
-    int splits;
+    float *part;  // [splits][m][part_ld], where k is split
+    int splits, per_split;
+    int64_t part_ld;  // n rounded up to a multiple of eight
     int tiles_m, tiles_n;
     int a_dtype;  // few rows: of x, which is quantised on the way
 };
@@ -171,7 +172,72 @@ __device__ __forceinline__ void store_out(const Fp8Params &p, int64_t row, int64
     }
 }
 
-// A workgroup's tile: WM x WN waves over BM x BN, two stages of one block of k in LDS. MX: both scales
+// The kernel's arguments, read where they are needed: held in scalar registers over the loop over the
+// blocks, they would not fit beside its own.
+typedef const __attribute__((address_space(4))) Fp8Params *Fp8Args;
+__device__ __forceinline__ Fp8Args fp8_args(bool first = false) {
+    Fp8Args a = (Fp8Args)__builtin_amdgcn_kernarg_segment_ptr();
+    if (!first) asm volatile("" : "+s"(a));
+    return a;
+}
+
+// Tile number `w` of a launch: its corner and its blocks of k. Consecutive numbers go down groups of eight
+// tile rows, so that tiles that run beside each other share their operands' rows in an XCD's L2.
+struct Fp8Item {
+    int m0, n0, first, steps;  // steps = 0: no such tile
+    int split;
+};
+template <int BM, int BN>
+__device__ __forceinline__ Fp8Item fp8_item(const Fp8Args p, int w) {
+    const int tiles_m = p->tiles_m, tiles_n = p->tiles_n, per = tiles_m * tiles_n;
+    Fp8Item it = {};
+    if (w >= per * p->splits) return it;
+    const auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // quotients come from vector units
+    it.split = p->splits == 1 ? 0 : uniform(w / per);
+    const int t = w - it.split * per;
+    constexpr int G = 8;
+    const int group = uniform(t / (G * tiles_n)), in = t - group * G * tiles_n, rows = min(G, tiles_m - group * G);
+    const int column = uniform(in / rows);
+    it.m0 = (group * G + in - column * rows) * BM;
+    it.n0 = column * BN;
+    it.first = it.split * p->per_split;
+    it.steps = min(p->per_split, p->kb - it.first);
+    return it;
+}
+
+// A stream of an operand's tiles: ROWS rows, a block of k a step, to LDS as GemmTile lays it out.
+template <int ROWS, int NW>
+struct Fp8Stream {
+    typedef GemmTile<kKContig, ROWS, 64, NW> Tile;  // 64 pairs of bytes: a block
+    static constexpr int LOADS = Tile::LPW, OFFS = Tile::OFFS;
+    Tile tile;
+    const char *at;  // the tile's first row at the step's block
+    int bytes;       // from there to the end of its last row; 0: nothing to load
+    uint32_t ld;
+    i32x4 rsrc;
+    uint32_t v[OFFS];
+    __device__ __forceinline__ Fp8Stream(int wave, int lane, uint32_t ld_) : tile(wave, lane, ld_), at(nullptr), bytes(0), ld(ld_) {}
+    __device__ __forceinline__ void start(const char *base, int64_t r0, int64_t rows, int kb, int k) {
+        at = base + r0 * (int64_t)ld + (int64_t)kb * kFp8Block;
+        const int n = (int)min(rows - r0, (int64_t)ROWS);
+        bytes = n > 0 ? (n - 1) * (int)ld + k - kb * kFp8Block : 0;
+    }
+    // The loads of the step whose first byte of k has `left` bytes behind it, and on to the next. A chunk past k
+    // would read the next row's first bytes.
+    __device__ __forceinline__ void prepare(int left) {
+        rsrc = uniform_rsrc(buffer_rsrc(at, (uint32_t)bytes));
+#pragma unroll
+        for (int u = 0; u < OFFS; ++u) v[u] = tile.kchunk[u] * 16 >= left ? kOutOfRange : tile.off[u];
+        at += kFp8Block;
+        bytes = max(bytes - kFp8Block, 0);
+    }
+    __device__ __forceinline__ void issue(int u, uint32_t lds, int wave) const {
+        dma16(v[u % OFFS] + (uint32_t)(u / OFFS * OFFS * Tile::RPL) * ld, rsrc,
+              __builtin_amdgcn_readfirstlane(lds + (wave * LOADS + u) * 1024));
+    }
+};
+
+// A workgroup goes through tiles of BM x BN with WM x WN waves, over two stages of one block of k in LDS. MX: both scales
 // are e8m0 and the matrix instruction applies them; otherwise both are fp32, and a block's product is formed
 // from zero and added to the sums times the product of the scales, four multiply-adds an instruction.
 //
@@ -180,12 +246,13 @@ __device__ __forceinline__ void store_out(const Fp8Params &p, int64_t row, int64
 // two groups of a step: what they need is in registers by then and the next stage has landed. Under them
 // the next step's first two of A's are read, and each of B's as soon as its last product has been issued: it
 // is needed a group later.
+//
+// The loads run two steps ahead of the products and from one tile straight into the next, so that a tile's
+// results are stored while the next one's operands arrive.
 template <bool MX, int BM, int BN, int WM, int WN>
 struct Fp8Core {
     static constexpr int NW = WM * WN, THREADS = NW * 64, M16 = BM / WM / 16, N16 = BN / WN / 16;
-    typedef GemmTile<kKContig, BM, 64, NW> TA;  // 64 pairs of bytes: a block
-    typedef GemmTile<kKContig, BN, 64, NW> TB;
-    static constexpr int LA = TA::LPW, LB = TB::LPW, LT = LA + LB + 1;
+    static constexpr int LA = Fp8Stream<BM, NW>::LOADS, LB = Fp8Stream<BN, NW>::LOADS, LT = LA + LB + 1;
     // a stage: A's tile, B's tile, and 64 scales a wave: A's rows, then B's blocks
     static constexpr int ASTAGE = BM * 128, BSTAGE = BN * 128, SSTAGE = NW * 256, STAGE = ASTAGE + BSTAGE + SSTAGE;
     static constexpr int LDS_BYTES = 2 * STAGE;
@@ -202,47 +269,64 @@ struct Fp8Core {
         wn = wave / WM;
     }
 
-    __device__ __forceinline__ void run(char *lds, const Fp8Params &p, int64_t m0, int64_t n0, int first, int last) {
+    // Tiles w, w + stride, ..
+    __device__ __forceinline__ void run(char *lds, int w, int stride) {
         const uint32_t base = lds_addr(lds);
-        const int64_t k2 = p.k / 2;
-        const TA ta(wave, lane, (uint32_t)p.a.ld);
-        const TB tb(wave, lane, (uint32_t)p.b.ld);
+        Fp8Item cur = fp8_item<BM, BN>(fp8_args(true), w);
+        if (!cur.steps) return;
         const GemmFrag<kKContig, BM, 64> fa(lane);
         const GemmFrag<kKContig, BN, 64> fb(lane);
-        // the wave's 64 scales of a step
+        // the loads' streams, up to two steps ahead of the products: A, B and the wave's 64 scales of a step (rows
+        // of A, or one wave B's blocks)
+        Fp8Stream<BM, NW> da(wave, lane, (uint32_t)fp8_args(true)->a.ld);
+        Fp8Stream<BN, NW> db(wave, lane, (uint32_t)fp8_args(true)->b.ld);
         const bool is_a = wave < BM / 64;
-        const Fp8Scales &sc = is_a ? p.sa : p.sb;
-        const int64_t srow = is_a ? m0 + wave * 64 : n0 / kFp8Block;
-        const int64_t sleft = wave > BM / 64 ? 0 : sc.rows - srow;
-        constexpr uint32_t ssize = MX ? 1 : 4;
-        const int slots = is_a ? 64 : (BN + kFp8Block - 1) / kFp8Block;
-        const uint32_t soff = lane < sleft && lane < slots ? (uint32_t)(lane * sc.row_stride) * ssize : kOutOfRange;
-        typename TA::Step da;
-        typename TB::Step db;
+        constexpr int ssize = MX ? 1 : 4;
+        const char *sat = nullptr;
+        int sstep, ahead_w = w, ahead = 0, left = 0;
+        uint32_t soff = kOutOfRange;
         i32x4 ds;
-        // past `last` the loads read nothing, so that every step counts the same number of loads
-        auto prepare = [&](int step) {
-            const bool on = step < last;
-            da = ta.step(p.a, m0, on ? (int64_t)step * 64 : k2, k2);
-            db = tb.step(p.b, n0, on ? (int64_t)step * 64 : k2, k2);
-            const char *q = sc.base + (srow * sc.row_stride + (on ? step : 0) * sc.k_stride) * ssize;
-            ds = uniform_rsrc(buffer_rsrc(q, on && sleft > 0 ? kOutOfRange - 1 : 0));
+        auto start = [&](const Fp8Args p, const Fp8Item &it) {  // the streams go on to tile `it`
+            ahead = it.steps;
+            if (!ahead) {  // behind the last tile they read nothing, so that every step counts the same number of loads
+                da.bytes = db.bytes = 0;
+                soff = kOutOfRange;
+                return;
+            }
+            da.start(p->a.base, it.m0, p->a.rows, it.first, (int)p->k);
+            db.start(p->b.base, it.n0, p->b.rows, it.first, (int)p->k);
+            left = (int)p->k - it.first * kFp8Block;
+            const int64_t rs = is_a ? p->sa.row_stride : p->sb.row_stride, ks = is_a ? p->sa.k_stride : p->sb.k_stride;
+            const int64_t row = is_a ? it.m0 + wave * 64 : it.n0 / kFp8Block;
+            const int64_t rows = (is_a ? p->sa.rows : p->sb.rows) - row;
+            const int slots = is_a ? 64 : wave == BM / 64 ? (BN + kFp8Block - 1) / kFp8Block : 0;
+            sat = (is_a ? p->sa.base : p->sb.base) + (row * rs + it.first * ks) * ssize;
+            sstep = (int)ks * ssize;
+            soff = lane < slots && lane < rows ? (uint32_t)(lane * rs) * ssize : kOutOfRange;
+        };
+        auto prepare = [&] {
+            da.prepare(left);
+            db.prepare(left);
+            ds = uniform_rsrc(buffer_rsrc(sat, kOutOfRange - 1));
+            left -= kFp8Block;
+            sat += sstep;
         };
         auto issue = [&](int stage, int u) {
             const uint32_t at = base + stage * STAGE;
-            if (u < LA) TA::issue(da, u, at, wave);
-            else if (u < LA + LB) TB::issue(db, u - LA, at + ASTAGE, wave);
+            if (u < LA) da.issue(u, at, wave);
+            else if (u < LA + LB) db.issue(u - LA, at + ASTAGE, wave);
             else {
                 const uint32_t to = __builtin_amdgcn_readfirstlane(at + ASTAGE + BSTAGE + wave * 256);
                 if constexpr (MX) dma1(soff, ds, to);
                 else dma4(soff, ds, to);
             }
         };
-#pragma unroll
-        for (int i = 0; i < M16; ++i)
-#pragma unroll
-            for (int j = 0; j < N16; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (first >= last) return;
+        auto next_tile = [&] {  // behind a step's loads: on to the next tile where this one has no step left
+            if (ahead && --ahead == 0) {
+                const Fp8Args p = fp8_args();
+                start(p, fp8_item<BM, BN>(p, ahead_w += stride));
+            }
+        };
         Fp8Frag ra[4], rb[N16];
         uint32_t sa[4], sb, sb_next;
         auto read_a = [&](const char *at, int i) {
@@ -255,12 +339,14 @@ struct Fp8Core {
         auto read_sb = [&](const char *at) {
             return reinterpret_cast<const uint32_t *>(at + ASTAGE + BSTAGE)[BM + wn * (N16 * 16) / kFp8Block];
         };
-        prepare(first);
+        start(fp8_args(true), cur);
 #pragma unroll
-        for (int u = 0; u < LT; ++u) issue(0, u);
-        prepare(first + 1);
+        for (int t = 0; t < 2; ++t) {
+            prepare();
 #pragma unroll
-        for (int u = 0; u < LT; ++u) issue(1, u);
+            for (int u = 0; u < LT; ++u) issue(t, u);
+            next_tile();
+        }
         tile_barrier<LT>();
         // in the loop's order: its first waits then count the same reads behind theirs on every step
         sb = read_sb(lds);
@@ -274,138 +360,172 @@ struct Fp8Core {
             __builtin_amdgcn_sched_barrier(0);
         }
         int stage = 0;
-        for (int t = first; t < last; ++t) {
-            const char *at = lds + stage * STAGE, *next = lds + (stage ^ 1) * STAGE;
-            float sbf = 0.f;
-            if constexpr (!MX) sbf = __uint_as_float(sb);
+        for (;;) {
 #pragma unroll
-            for (int i = 0; i < M16; ++i) {
-                if (i == M16 - 2) {
-                    prepare(t + 2);
+            for (int i = 0; i < M16; ++i)
+#pragma unroll
+                for (int j = 0; j < N16; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < cur.steps; ++t) {
+                const char *at = lds + stage * STAGE, *next = lds + (stage ^ 1) * STAGE;
+                float sbf = 0.f, s[2];  // without MX: B's scale, and its product with A's of two groups
+                f32x4 d[3];
+                if constexpr (!MX) sbf = __uint_as_float(sb);
+                auto add = [&](int q, f32x4 v) {
+                    asm volatile("" : "+v"(v));  // no sooner: it would wait for the product
+                    f32x4 &c = acc[q / N16][q % N16];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[e] = fmaf(v[e], s[q / N16 % 2], c[e]);
+                    asm volatile("" : "+v"(c));
+                };
+#pragma unroll
+                for (int i = 0; i < M16; ++i) {
+                    if (i == M16 - 2) {
+                        prepare();
+                        __builtin_amdgcn_sched_barrier(0);
+                        tile_barrier<0>();
+                        sb_next = read_sb(next);
+                    }
+                    if (i < M16 - 2) read_a(at, i + 2);
+                    else read_a(next, i - M16 + 2);
+                    if constexpr (!MX) s[i % 2] = __uint_as_float(sa[i % 4]) * sbf;
+#pragma unroll
+                    for (int j = 0; j < N16; ++j) {
+                        if constexpr (MX) {
+                            acc[i][j] = mfma_fp8(rb[j], ra[i % 4], acc[i][j], (int)sb, (int)sa[i % 4]);
+                            // held here: a product has no side effect that would keep it from drifting behind the
+                            // loads and the barrier, with copies of all that it needs
+                            asm volatile("" : "+v"(acc[i][j]));
+                        } else {
+                            constexpr int D = 2;  // products between one and its sum: its latency
+                            const int q = i * N16 + j;
+                            d[q % (D + 1)] = mfma_fp8(rb[j], ra[i % 4]);
+                            asm volatile("" : "+v"(d[q % (D + 1)]));
+                            if (q >= D) add(q - D, d[(q - D) % (D + 1)]);
+                            if (q == M16 * N16 - 1)
+#pragma unroll
+                                for (int r = q - D + 1; r <= q; ++r) add(r, d[r % (D + 1)]);
+                        }
+                        if (i == M16 - 1) {
+                            __builtin_amdgcn_sched_barrier(0);  // not before the product that still needs the old one
+                            read_b(next, j);
+                        }
+                        // the loads of step t + 2, spread over the groups behind the barrier
+                        if (i >= M16 - 2) {
+                            constexpr int NM = 2 * N16;
+#pragma unroll
+                            for (int u = 0; u < LT; ++u)
+                                if (u * NM / LT == (i - M16 + 2) * N16 + j) issue(stage, u);
+                        }
+                    }
                     __builtin_amdgcn_sched_barrier(0);
-                    tile_barrier<0>();
-                    sb_next = read_sb(next);
                 }
-                if (i < M16 - 2) read_a(at, i + 2);
-                else read_a(next, i - M16 + 2);
-                float s = 0.f;
-                if constexpr (!MX) s = __uint_as_float(sa[i % 4]) * sbf;
-#pragma unroll
-                for (int j = 0; j < N16; ++j) {
-                    if constexpr (MX) {
-                        acc[i][j] = mfma_fp8(rb[j], ra[i % 4], acc[i][j], (int)sb, (int)sa[i % 4]);
-                        // held here: a product has no side effect that would keep it from drifting behind the
-                        // loads and the barrier, with copies of all that it needs
-                        asm volatile("" : "+v"(acc[i][j]));
-                    } else {
-                        const f32x4 d = mfma_fp8(rb[j], ra[i % 4]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s, acc[i][j][e]);
-                    }
-                    if (i == M16 - 1) {
-                        __builtin_amdgcn_sched_barrier(0);  // not before the product that still needs the old one
-                        read_b(next, j);
-                    }
-                    // the loads of step t + 2, spread over the groups behind the barrier
-                    if (i >= M16 - 2) {
-                        constexpr int NM = 2 * N16;
-#pragma unroll
-                        for (int u = 0; u < LT; ++u)
-                            if (u * NM / LT == (i - M16 + 2) * N16 + j) issue(stage, u);
-                    }
-                }
-                if constexpr (!MX)
-#pragma unroll
-                    for (int j = 0; j < N16; ++j)
-                        if (i > 0) asm volatile("" : "+v"(acc[i - 1][j]));
-                __builtin_amdgcn_sched_barrier(0);
+                next_tile();
+                sb = sb_next;
+                stage ^= 1;
             }
-            sb = sb_next;
-            stage ^= 1;
+            store(cur);
+            cur = fp8_item<BM, BN>(fp8_args(), w += stride);
+            if (!cur.steps) break;
         }
         tile_barrier<0>();  // no load may land in LDS that another workgroup has by then
     }
 
-    // Calls f(row, column, v) for eight consecutive columns of the tile a lane. The accumulators hold four
-    // consecutive n of one m; of two neighbouring blocks of 16 columns a lane takes eight of one, in exchange
-    // with the lanes 16 further on.
-    template <class F>
-    __device__ __forceinline__ void each_piece(F f) const {
-        const int g = lane >> 4;
+    // The tile's results. The accumulators hold four consecutive n of one m; of two neighbouring blocks of 16
+    // columns a lane takes eight of one, in exchange with the lanes 16 further on, and writes 16 bytes. Rows
+    // past the operand's fall out of the descriptors, columns take an offset that does.
+    __device__ __forceinline__ void store(const Fp8Item &it) {
+        const Fp8Args p = fp8_args();
+        const int g = lane >> 4, row = wm * M16 * 16 + (lane & 15);
+        const bool part = p->splits > 1;
+        const void *bias = p->bias;
+        if (bias && !part)
 #pragma unroll
-        for (int i = 0; i < M16; ++i)
-#pragma unroll
-            for (int j = 0; j < N16; j += 2) {
-                float v[8];
+            for (int j = 0; j < N16; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    // lane groups (0, 1, 2, 3) of the pair: (j, j + 1, j, j + 1) at columns (0, 0, 8, 8)
-                    auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][j][e]), __float_as_uint(acc[i][j + 1][e]), false, false);
-                    v[e] = __uint_as_float(x[0]);
-                    v[4 + e] = __uint_as_float(x[1]);
+                    const int64_t col = it.n0 + (wn * N16 + j) * 16 + g * 4 + e;
+                    const float b = col < p->n ? load_dt(bias, col, p->bias_dtype) : 0.f;
+#pragma unroll
+                    for (int i = 0; i < M16; ++i) acc[i][j][e] += b;
                 }
-                f((wm * M16 + i) * 16 + (lane & 15), (wn * N16 + j + (g & 1)) * 16 + (g >> 1) * 8, v);
+        const int64_t ld = part ? p->part_ld : p->n, m = p->m;
+        char *out = part ? reinterpret_cast<char *>(p->part + it.split * m * ld) : static_cast<char *>(p->out);
+        const int dtype = part ? DSALT_DTYPE_F32 : p->out_dtype;
+        if (ld % 8) return store_ragged(out, dtype, ld, it, m);
+        const int64_t col = it.n0 + wn * N16 * 16 + (g & 1) * 16 + (g >> 1) * 8;
+        if (dtype == DSALT_DTYPE_F32) store_rows<F32>(out, ld, it, m, row, col);
+        else if (dtype == DSALT_DTYPE_BF16) store_rows<BF16>(out, ld, it, m, row, col);
+        else store_rows<F16>(out, ld, it, m, row, col);
+    }
+    template <typename DT>
+    __device__ __forceinline__ void store_rows(char *out, int64_t ld, const Fp8Item &it, int64_t m, int row, int64_t col) const {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        constexpr int SZ = std::is_same<DT, F32>::value ? 4 : 2;
+        const int64_t total = (min(m - it.m0, (int64_t)BM) * ld - it.n0) * SZ;
+        char *base = out + ((int64_t)it.m0 * ld + it.n0) * SZ;
+        const uint32_t lane_off = (uint32_t)((row * ld + (col - it.n0)) * SZ);
+#pragma unroll
+        for (int i = 0; i < M16; ++i) {
+            const int64_t skip = i * 16 * ld * SZ;
+            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(base + skip, (short)0, (int)max(total - skip, (int64_t)0), 0x00020000);
+#pragma unroll
+            for (int j = 0; j < N16; j += 2) {
+                const uint32_t off = col + j * 16 < ld ? lane_off + j * 16 * SZ : kOutOfRange;
+                if constexpr (SZ == 4) {
+                    u32x4 lo, hi;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][j][e]),
+                                                                        __float_as_uint(acc[i][j + 1][e]), false, false);
+                        lo[e] = x[0];
+                        hi[e] = x[1];
+                    }
+                    __builtin_amdgcn_raw_buffer_store_b128(lo, rsrc, off, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(hi, rsrc, off + 16, 0, 0);
+                } else {
+                    const f32x4 c = acc[i][j], d = acc[i][j + 1];
+                    const auto x = __builtin_amdgcn_permlane16_swap(DT::pack2(c[0], c[1]), DT::pack2(d[0], d[1]), false, false);
+                    const auto y = __builtin_amdgcn_permlane16_swap(DT::pack2(c[2], c[3]), DT::pack2(d[2], d[3]), false, false);
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], y[0], x[1], y[1]}, rsrc, off, 0, 0);
+                }
             }
+        }
+    }
+    // Rows that do not start on 16 bytes: an element at a time.
+    __device__ __forceinline__ void store_ragged(char *out, int dtype, int64_t ld, const Fp8Item &it, int64_t m) const {
+#pragma unroll
+        for (int i = 0; i < M16; ++i) {
+            const int64_t row = it.m0 + (wm * M16 + i) * 16 + (lane & 15);
+            if (row >= m) continue;
+#pragma unroll
+            for (int j = 0; j < N16; ++j) {
+                const int64_t col = it.n0 + (wn * N16 + j) * 16 + (lane >> 4) * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < ld) store_dt(out, row * ld + col + e, dtype, acc[i][j][e]);
+            }
+        }
     }
 };
 
-// Tile of a workgroup: consecutive ids of one XCD take groups of eight tile rows, so that the tiles that run
-// beside each other share their operands' rows in that XCD's L2.
-__device__ __forceinline__ bool fp8_tile(const Fp8Params &p, int &tm, int &tn, int &split) {
-    const int per = p.tiles_m * p.tiles_n, id = xcd_remap(blockIdx.x, gridDim.x);
-    if (id >= per * p.splits) return false;
-    split = id / per;
-    const int t = id - split * per;
-    constexpr int G = 8;
-    const int group = t / (G * p.tiles_n), in = t - group * G * p.tiles_n, rows = min(G, p.tiles_m - group * G);
-    tm = group * G + in % rows;
-    tn = in / rows;
-    return true;
-}
-
 template <bool MX, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(WM *WN * 64) fp8_tile_kernel(const Fp8Params p) {
+__global__ void __launch_bounds__(WM *WN * 64) fp8_tile_kernel(const Fp8Params) {
     typedef Fp8Core<MX, BM, BN, WM, WN> Core;
     extern __shared__ char lds[];
-    int tm, tn, split;
-    if (!fp8_tile(p, tm, tn, split)) return;
     Core core;
-    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-    const int per = (p.kb + p.splits - 1) / p.splits, first = split * per;
-    core.run(lds, p, m0, n0, first, min(first + per, p.kb));
-    float *part = p.splits > 1 ? p.part + split * p.m * p.n : nullptr;
-    core.each_piece([&](int r, int c, float (&v)[8]) {
-        const int64_t row = m0 + r, col = n0 + c;
-        if (row >= p.m || col >= p.n) return;
-        if (!part) return store_out<8>(p, row, col, v);
-        float *o = part + row * p.n + col;
-        if (p.n % 4 == 0 && col + 8 <= p.n) {
-            reinterpret_cast<float4 *>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (col + e < p.n) o[e] = v[e];
-        }
-    });
+    core.run(lds, xcd_remap(blockIdx.x, gridDim.x), gridDim.x);
 }
 
 // Sum of the splits' parts in their order.
 __global__ void __launch_bounds__(256) fp8_join_kernel(const Fp8Params p) {
-    const int64_t total = p.m * p.n, per = (p.n + 3) / 4;
+    const int64_t total = p.m * p.part_ld, per = (p.n + 3) / 4;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.m * per; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / per, col = (i - row * per) * 4;
-        const float *in = p.part + row * p.n + col;
+        const float *in = p.part + row * p.part_ld + col;
         float v[4] = {};
         for (int s = 0; s < p.splits; ++s, in += total) {
-            if (p.n % 4 == 0) {
-                const float4 f = *reinterpret_cast<const float4 *>(in);
-                v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < p.n) v[e] += in[e];
-            }
+            const float4 f = *reinterpret_cast<const float4 *>(in);
+            v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
         }
         store_out<4>(p, row, col, v);
     }
@@ -522,7 +642,8 @@ hipError_t launch_tile(Fp8Params p, hipStream_t stream) {
     typedef Fp8Core<MX, BM, BN, WM, WN> Core;
     p.tiles_m = (int)((p.m + BM - 1) / BM);
     p.tiles_n = (int)((p.n + BN - 1) / BN);
-    const int64_t groups = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    // as many workgroups as the card holds at once (LDS): they go through the tiles
+    const int64_t groups = std::min<int64_t>((int64_t)p.tiles_m * p.tiles_n * p.splits, 256 * (163840 / Core::LDS_BYTES));
     const auto kernel = fp8_tile_kernel<MX, BM, BN, WM, WN>;
     if (Core::LDS_BYTES > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -546,7 +667,8 @@ Plan plan(int64_t m, int64_t n, int64_t k) {
         if (tiles >= 256 || t == kTile64) {
             int splits = 1;
             while (t == kTile64 && tiles * splits * 2 <= 512 && kb / (splits * 2) >= 4) splits *= 2;
-            return {t, splits};
+            const int per = (kb + splits - 1) / splits;
+            return {t, (kb + per - 1) / per};  // none of them empty
         }
     }
     return {kTile64, 1};
@@ -601,7 +723,7 @@ int fp8_few_rows() { return kFewRows; }
 int64_t fp8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
     if (m <= kFewRows) return 0;
     const Plan pl = plan(m, n, k);
-    return pl.splits > 1 ? pl.splits * m * n * 4 : 0;
+    return pl.splits > 1 ? pl.splits * m * ((n + 7) / 8 * 8) * 4 : 0;
 }
 
 hipError_t launch_fp8_quantize(const dsalt_fp8_quantize_args &a, hipStream_t stream) {
@@ -651,6 +773,8 @@ hipError_t launch_fp8_matmul(const dsalt_fp8_matmul_args &a, hipStream_t stream)
     }
     const Plan pl = plan(a.m, a.n, a.k);
     p.splits = pl.splits;
+    p.per_split = (p.kb + pl.splits - 1) / pl.splits;
+    p.part_ld = (p.n + 7) / 8 * 8;
     p.part = static_cast<float *>(a.workspace);
     const hipError_t e = p.sa.e8m0 && p.sb.e8m0 ? launch_tiles<true>(p, pl.tile, stream) : launch_tiles<false>(p, pl.tile, stream);
     if (e != hipSuccess || p.splits == 1) return e;
