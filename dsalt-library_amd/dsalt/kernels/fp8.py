@@ -10,7 +10,7 @@ import torch.nn.functional as F
 
 from .. import _hip
 from .._hip import E4M3, E8M0, FP8_BLOCK
-from ._block_train import eager
+from ._block_train import autocast_dtype, eager
 from .dsalt_triton_attn import _dynamo_opaque
 
 
@@ -154,7 +154,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
 class FP8Linear(nn.Module):
     """A frozen linear layer in 8 bits (``fp8_linear``): ``FP8Linear.from_linear`` quantises an nn.Linear's
     weight by tiles of 128 x 128. The weight and its scales are kept as bytes, which ``.to(dtype)`` leaves as they are.
-    GPU tensors only, for inference."""
+    The result has x's dtype, or autocast's. GPU tensors only, for inference."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = False, device=None, dtype=None):
         super().__init__()
@@ -187,7 +187,7 @@ class FP8Linear(nn.Module):
         return self.scale_bits.view(E8M0)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return fp8_linear(x, self.weight_q, self.weight_scale, self.bias)
+        return fp8_linear(x, self.weight_q, self.weight_scale, self.bias, autocast_dtype(x))
 
     def extra_repr(self) -> str:
         return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}"

@@ -22,9 +22,13 @@ block's norm, the last one to the final norm); the FFN's gated product and the w
 gate run as HIP passes too (SwiGLUFFN, DSALTAttention).
 
 The options of DSALTTransformerBlock beyond the reference (post_norm, layer_scale,
-residual_scale, fused_ffn, activation, counter_dropout) apply to every layer; with
+residual_scale, fused_ffn, activation, counter_dropout, norm) apply to every layer; with
 counter_dropout the embedding's dropout is a CounterDropout too, and one seed drawn a forward
-serves all places, told apart by their offsets.
+serves all places, told apart by their offsets; norm="layer" makes the final norm a LayerNorm too.
+
+Distillation: with ``teacher_logits`` and ``teacher_ids`` [..., K] the loss is ``distill_loss`` against a
+teacher's top logits, over the same chunks. ``quantize_fp8`` makes the feed-forwards and the head frozen
+8-bit layers, for a model that answers or teaches.
 """
 from __future__ import annotations
 
@@ -36,22 +40,41 @@ import torch.nn.functional as F
 
 from .. import _hip
 from ..kernels import _block_train
-from ..kernels.RMSENorm import RMSENorm
+from ..kernels.LayerNorm import LayerNorm
+from ..kernels.distill import distill_loss, torch_distill_loss
 from ..kernels.dropout import draw_seed
-from ..modules.dsalt_transformer import CounterDropout, DSALTTransformerBlock
+from ..kernels.fp8 import FP8Linear
+from ..modules.dsalt_transformer import CounterDropout, DSALTTransformerBlock, SwiGLUFFN, norm_class
 
 _LOSS_FNS = ("auto", "liger", "chunked")
 
 
-def _chunked_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
-                           chunk_size: int = 512) -> torch.Tensor:
-    """Sum of token cross-entropies over chunks of rows of ``x @ weight.T``, divided by
+def _chunked_cross_entropy(x: torch.Tensor, head, labels: torch.Tensor, chunk_size: int = 512) -> torch.Tensor:
+    """Sum of token cross-entropies over chunks of rows of ``head(x)``, divided by
     the number of labels other than -100 (at least 1)."""
     total = torch.zeros((), device=x.device, dtype=torch.float32)
     for a in range(0, x.shape[0], chunk_size):
-        logits = F.linear(x[a:a + chunk_size], weight)
+        logits = head(x[a:a + chunk_size])
         total = total + F.cross_entropy(logits, labels[a:a + chunk_size], ignore_index=-100, reduction="sum")
     n = (labels != -100).sum().clamp(min=1).to(torch.float32)
+    return total / n
+
+
+def _chunked_distillation(x: torch.Tensor, head, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                          labels: torch.Tensor | None, temperature: float, label_weight: float,
+                          chunk_size: int = 512) -> torch.Tensor:
+    """``distill_loss`` of ``head(x)`` over chunks of rows: its mean over the labels other than -100 (or all
+    rows, without labels)."""
+    total = torch.zeros((), device=x.device, dtype=torch.float32)
+    for a in range(0, x.shape[0], chunk_size):
+        part = slice(a, a + chunk_size)
+        y = None if labels is None else labels[part]
+        args = head(x[part]), teacher_logits[part], teacher_ids[part], y
+        if x.is_cuda:
+            total = total + distill_loss(*args, temperature=temperature, label_weight=label_weight, reduction="sum")
+        else:
+            total = total + torch_distill_loss(*args, (temperature, label_weight, -100, "sum"))
+    n = max(x.shape[0], 1) if labels is None else (labels != -100).sum().clamp(min=1).to(torch.float32)
     return total / n
 
 
@@ -62,7 +85,7 @@ class DSALTLMHeadModel(nn.Module):
                  lm_head_chunk_size: int = 2048, loss_fn: str = "chunked", aux_loss_weight: float = 0.0,
                  n_kv_heads: int | None = None, qkv_bias: bool = False, rope_base: float = 10000.0,
                  post_norm: bool = False, layer_scale: float | None = None, residual_scale: float = 1.0,
-                 fused_ffn: bool = False, activation: str = "silu", counter_dropout: bool = False):
+                 fused_ffn: bool = False, activation: str = "silu", counter_dropout: bool = False, norm: str = "rms"):
         super().__init__()
         if loss_fn not in _LOSS_FNS:
             raise ValueError(f"loss_fn must be one of {list(_LOSS_FNS)}, got {loss_fn!r}")
@@ -85,9 +108,9 @@ class DSALTLMHeadModel(nn.Module):
                                   max_seq_len=max_seq_len, d_ff=d_ff, dropout=dropout, yarn_scale=yarn_scale,
                                   layer_idx=i, n_kv_heads=n_kv_heads, qkv_bias=qkv_bias, rope_base=rope_base,
                                   post_norm=post_norm, layer_scale=layer_scale, residual_scale=residual_scale,
-                                  fused_ffn=fused_ffn, activation=activation, counter_dropout=counter_dropout)
+                                  fused_ffn=fused_ffn, activation=activation, counter_dropout=counter_dropout, norm=norm)
             for i in range(n_layers))
-        self.final_norm = RMSENorm(d_model)
+        self.final_norm = norm_class(norm)(d_model)
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)
         if tie_weights:
             self.lm_head.weight = self.embed_tokens.weight
@@ -108,6 +131,21 @@ class DSALTLMHeadModel(nn.Module):
             if mod.bias is not None:
                 nn.init.zeros_(mod.bias)
 
+    def quantize_fp8(self, lm_head: bool = True) -> "DSALTLMHeadModel":
+        """The feed-forwards' projections and (``lm_head``) the head as frozen 8-bit layers, in place, for
+        inference; the embedding, the attention and the norms stay as they are. On the GPU, widths that are
+        multiples of 16."""
+        for layer in self.layers:
+            if type(layer.ffn) is SwiGLUFFN:
+                layer.ffn.quantize_fp8()
+        if lm_head and type(self.lm_head) is nn.Linear:
+            self.lm_head = FP8Linear.from_linear(self.lm_head)
+        return self
+
+    def _head(self, x: torch.Tensor) -> torch.Tensor:
+        """The head's logits within a loss."""
+        return self.lm_head(x) if type(self.lm_head) is FP8Linear else F.linear(x, self.lm_head.weight)
+
     def set_collect_last_P(self, on: bool) -> None:
         """Turn the attention modules' ``_last_P`` diagnostic on or off."""
         for layer in self.layers:
@@ -124,7 +162,14 @@ class DSALTLMHeadModel(nn.Module):
 
     def forward(self, input_ids: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
                 max_seqlen: int | None = None, labels: torch.Tensor | None = None,
-                gradient_checkpointing: bool = False, padding_mask: torch.Tensor | None = None) -> dict:
+                gradient_checkpointing: bool = False, padding_mask: torch.Tensor | None = None,
+                teacher_logits: torch.Tensor | None = None, teacher_ids: torch.Tensor | None = None,
+                temperature: float = 1.0, label_weight: float = 0.0) -> dict:
+        """``teacher_logits`` and ``teacher_ids`` (input_ids' shape and K slots): the loss is the distillation
+        loss of ``distill_loss`` with ``temperature`` and ``label_weight``; ``labels`` are then optional."""
+        if (teacher_logits is None) != (teacher_ids is None):
+            raise ValueError("teacher_logits and teacher_ids are given together")
+        with_loss = labels is not None or teacher_ids is not None
         if max_seqlen is None:
             max_seqlen = input_ids.shape[-1]
         seed = None
@@ -136,13 +181,13 @@ class DSALTLMHeadModel(nn.Module):
         cu_list = None
         if cu_seqlens is not None and not self._device_packing(cu_seqlens, x):
             cu_list = cu_seqlens.detach().cpu().tolist()
-        if labels is None and self._norms_fusable(x):
+        if not with_loss and self._norms_fusable(x):
             # inference: each residual add runs in the pass of the norm that follows it
             delta = None
             for layer in self.layers:
                 x, delta, _ = layer._forward_fused(x, delta, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
                                                    cu_list=cu_list)
-            _, x = _hip.add_rms_norm(x, delta, self.final_norm.weight, self.final_norm.eps)
+            _, x = DSALTTransformerBlock._add_norm(x, delta, self.final_norm)
             return {"loss": None, "logits": self.lm_head(x), "aux_loss": None}
         aux = torch.zeros((), device=input_ids.device, dtype=x.dtype)
         joins = bool(self.layers) and all(type(layer) is DSALTTransformerBlock and layer.joins_branches
@@ -156,13 +201,17 @@ class DSALTLMHeadModel(nn.Module):
             else:
                 x, a = layer(x, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
                              gradient_checkpointing=gradient_checkpointing, cu_list=cu_list)
-            if labels is not None:  # the layers' auxiliary losses are only returned with a loss
+            if with_loss:  # the layers' auxiliary losses are only returned with a loss
                 aux = aux + a
         x = h if joins else self.final_norm(x)
-        if labels is None:
+        if not with_loss:
             return {"loss": None, "logits": self.lm_head(x), "aux_loss": None}
-        loss = _chunked_cross_entropy(x.reshape(-1, self.d_model), self.lm_head.weight,
-                                      labels.reshape(-1).long(), self.lm_head_chunk_size)
+        x, y = x.reshape(-1, self.d_model), None if labels is None else labels.reshape(-1).long()
+        if teacher_ids is None:
+            loss = _chunked_cross_entropy(x, self._head, y, self.lm_head_chunk_size)
+        else:
+            loss = _chunked_distillation(x, self._head, *(t.reshape(-1, t.shape[-1]) for t in (teacher_logits, teacher_ids)), y,
+                                         temperature, label_weight, self.lm_head_chunk_size)
         return {"loss": loss + self.aux_loss_weight * aux, "logits": None, "aux_loss": aux.detach()}
 
     def _device_packing(self, cu_seqlens: torch.Tensor, x: torch.Tensor) -> bool:
@@ -174,8 +223,13 @@ class DSALTLMHeadModel(nn.Module):
 
     def _norms_fusable(self, x: torch.Tensor) -> bool:
         """Whether every residual add and norm of the forward can run as dsalt_add_rms_norm
-        passes (inference without autograd, 16-bit rows, norm weights of x's dtype)."""
-        if not self.layers or not _hip.add_rms_norm_supported(x, self.final_norm.weight):
+        passes (inference without autograd, 16-bit rows, norm weights of x's dtype), or, of LayerNorms,
+        as dsalt_layer_norm passes (inference without autograd)."""
+        if not self.layers:
+            return False
+        final = self.final_norm
+        if not (DSALTTransformerBlock._layer_joins(x, x, final) if isinstance(final, LayerNorm)
+                else _hip.add_rms_norm_supported(x, final.weight)):
             return False
         if any(getattr(layer, "joins_branches", False) for layer in self.layers):
             return False

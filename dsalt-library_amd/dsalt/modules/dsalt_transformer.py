@@ -11,7 +11,8 @@ those do not take run torch's ops).
 Options beyond the reference, off by default: a feed-forward whose projections, activation and
 product are one kernel (``gated_ffn``) and other activations; dropout whose mask is never
 stored (``CounterDropout``); a norm after each branch, a learned layer scale and a residual
-scale, joined to the residual stream in one pass (``branch_norm``).
+scale, joined to the residual stream in one pass (``branch_norm``); layer norms instead of RMS norms
+(``LayerNorm``); a feed-forward whose projections are frozen 8-bit ones (``quantize_fp8``).
 """
 from __future__ import annotations
 
@@ -22,11 +23,23 @@ import torch.utils.checkpoint
 
 from .. import _hip
 from ..kernels import _block_train
+from ..kernels.LayerNorm import LayerNorm
 from ..kernels.RMSENorm import RMSENorm
 from ..kernels.branch_norm import branch_norm
 from ..kernels.dropout import counter_dropout, draw_seed
+from ..kernels.fp8 import FP8Linear, fp8_matmul, fp8_quantize
 from ..kernels.gated_ffn import _TORCH_ACT, gated_ffn, gated_ffn_supported
 from .dsalt_attention import DSALTAttention
+
+
+_NORMS = {"rms": RMSENorm, "layer": LayerNorm}
+
+
+def norm_class(norm: str):
+    """The module of a ``norm`` option."""
+    if norm not in _NORMS:
+        raise ValueError(f"norm must be one of {list(_NORMS)}, got {norm!r}")
+    return _NORMS[norm]
 
 
 class CounterDropout(nn.Module):
@@ -75,20 +88,39 @@ class SwiGLUFFN(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.drop(self.project(x))
 
+    def quantize_fp8(self) -> "SwiGLUFFN":
+        """The projections as frozen 8-bit ones (``FP8Linear``), in place, for inference: widths that are
+        multiples of 16, weights on the GPU. gate and up then share one quantisation of x."""
+        for name in ("gate_proj", "up_proj", "down_proj"):
+            if type(getattr(self, name)) is nn.Linear:
+                setattr(self, name, FP8Linear.from_linear(getattr(self, name)))
+        return self
+
     def project(self, x: torch.Tensor) -> torch.Tensor:
         """The feed-forward without its dropout."""
         if self.fused and self._one_kernel(x):
             return gated_ffn(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, self.activation)
-        if self.activation != "silu":
-            return self.down_proj(_TORCH_ACT[self.activation](self.gate_proj(x)) * self.up_proj(x))
-        if torch.is_grad_enabled() and _block_train.swiglu_supported(self, x):
+        if self._shared_rows(x):
+            rows, dt = fp8_quantize(x), _block_train.autocast_dtype(x)
+            g, u = (fp8_matmul(*rows, m.weight_q, m.weight_scale, m.bias, dt) for m in (self.gate_proj, self.up_proj))
+        elif self.activation == "silu" and torch.is_grad_enabled() and _block_train.swiglu_supported(self, x):
             return _block_train.swiglu_ffn(self, x)
-        g, u = self.gate_proj(x), self.up_proj(x)
+        else:
+            g, u = self.gate_proj(x), self.up_proj(x)
+        if self.activation != "silu":
+            return self.down_proj(_TORCH_ACT[self.activation](g) * u)
         if not torch.is_grad_enabled() and _hip.swiglu_supported(g, u):
             h = _hip.swiglu(g, u)  # one pass, the same bits as the two torch ops below
         else:
             h = F.silu(g) * u
         return self.down_proj(h)
+
+    def _shared_rows(self, x: torch.Tensor) -> bool:
+        """Whether gate and up are 8-bit layers that quantise the same rows before their products."""
+        lin = (self.gate_proj, self.up_proj)
+        return (all(type(m) is FP8Linear for m in lin) and _block_train.plain(*lin)
+                and not (torch.is_grad_enabled() and x.requires_grad)
+                and x.shape[-1] > 0 and x.numel() // x.shape[-1] > _hip.FP8_FEW_ROWS)
 
     def _one_kernel(self, x: torch.Tensor) -> bool:
         lin = (self.gate_proj, self.up_proj, self.down_proj)
@@ -110,7 +142,10 @@ class DSALTTransformerBlock(nn.Module):
     ``layer_scale`` (a learned gate of each branch per channel, attn_gate and ffn_gate, that starts
     at this value), ``residual_scale`` and ``counter_dropout`` make a branch
     ``residual_scale * x + gate * post_norm(branch)`` on ``branch_norm``, which takes the
-    feed-forward's dropout and the next norm along. ``fused_ffn``, ``activation``: see SwiGLUFFN."""
+    feed-forward's dropout and the next norm along. ``fused_ffn``, ``activation``: see SwiGLUFFN.
+
+    ``norm``: "rms", or "layer" for LayerNorm modules in the place of every RMSENorm; a residual add and the
+    layer norm after it are one pass too, forward and backward (``add_layer_norm``)."""
 
     _fuse_norms = True
     joins_branches = False
@@ -119,11 +154,12 @@ class DSALTTransformerBlock(nn.Module):
                  d_ff: int, dropout: float = 0.0, yarn_scale: float = 1.0, layer_idx: int = 0,
                  n_kv_heads: int | None = None, qkv_bias: bool = False, rope_base: float = 10000.0,
                  post_norm: bool = False, layer_scale: float | None = None, residual_scale: float = 1.0,
-                 fused_ffn: bool = False, activation: str = "silu", counter_dropout: bool = False):
+                 fused_ffn: bool = False, activation: str = "silu", counter_dropout: bool = False, norm: str = "rms"):
         super().__init__()
+        Norm = norm_class(norm)
         self.layer_idx = layer_idx
-        self.attn_norm = RMSENorm(d_model)
-        self.ffn_norm = RMSENorm(d_model)
+        self.attn_norm = Norm(d_model)
+        self.ffn_norm = Norm(d_model)
         self.attn = DSALTAttention(d_model=d_model, n_heads=n_heads, n_min=n_min, n_max=n_max, k_lmk=k_lmk,
                                    max_seq_len=max_seq_len, dropout=dropout, yarn_scale=yarn_scale,
                                    layer_idx=layer_idx, n_kv_heads=n_kv_heads, qkv_bias=qkv_bias,
@@ -131,8 +167,8 @@ class DSALTTransformerBlock(nn.Module):
         self.ffn = SwiGLUFFN(d_model=d_model, d_ff=d_ff, dropout=dropout, activation=activation, fused=fused_ffn,
                              counter_dropout=counter_dropout)
         self.residual_scale = residual_scale
-        self.attn_post_norm = RMSENorm(d_model) if post_norm else None
-        self.ffn_post_norm = RMSENorm(d_model) if post_norm else None
+        self.attn_post_norm = Norm(d_model) if post_norm else None
+        self.ffn_post_norm = Norm(d_model) if post_norm else None
         self.attn_gate = nn.Parameter(torch.full((d_model,), float(layer_scale))) if layer_scale is not None else None
         self.ffn_gate = nn.Parameter(torch.full((d_model,), float(layer_scale))) if layer_scale is not None else None
         self.joins_branches = post_norm or layer_scale is not None or residual_scale != 1.0 or counter_dropout
@@ -169,7 +205,9 @@ class DSALTTransformerBlock(nn.Module):
                   else attend(h, h_cast))
         if self._norms_fusable(x, x_attn, self.ffn_norm):
             # the residual add and the FFN's norm in one HIP pass (inference)
-            x, h = _hip.add_rms_norm(x, x_attn, self.ffn_norm.weight, self.ffn_norm.eps)
+            x, h = self._add_norm(x, x_attn, self.ffn_norm)
+        elif train_norms and self._layer_joins(x, x_attn, self.ffn_norm):
+            x, h = self.ffn_norm(x, x_attn, cast if self._plain_ffn() else None)
         elif train_norms and self._train_norm(x, x_attn, self.ffn_norm):
             low = (cast is not None and type(self.ffn) is SwiGLUFFN and _block_train.plain(self.ffn)
                    and _block_train.swiglu_supported(self.ffn, x))
@@ -245,11 +283,28 @@ class DSALTTransformerBlock(nn.Module):
                 and norm.normalized_shape == (x.shape[-1],)
                 and (h is None or _hip.norm_train_branch_supported(x, h)))
 
+    @staticmethod
+    def _layer_joins(x: torch.Tensor, h: torch.Tensor, norm: nn.Module) -> bool:
+        """Whether x + h and the LayerNorm `norm` can run as one add_layer_norm pass."""
+        return (type(norm) is LayerNorm and _block_train.plain(norm) and x.is_cuda and h.device == x.device and h.shape == x.shape
+                and 1 <= x.shape[-1] <= _hip.LAYER_NORM_MAX_DIM and x.dtype in _hip._SCORE_DTYPES
+                and (h.dtype is x.dtype or (x.dtype is torch.float32 and h.dtype in _hip._SCORE_DTYPES)))
+
+    @staticmethod
+    def _add_norm(x: torch.Tensor, h: torch.Tensor | None, norm: nn.Module):
+        """``(x + h, norm(x + h))`` (without h: ``(None, norm(x))``) of norms that `_norms_fusable` takes."""
+        if type(norm) is LayerNorm:
+            return (None, norm(x)) if h is None else norm(x, h)
+        return _hip.add_rms_norm(x, h, norm.weight, norm.eps)
+
     def _norms_fusable(self, x: torch.Tensor, h: torch.Tensor | None, norm: nn.Module) -> bool:
         """Whether x (+ h) and the RMSENorm `norm` can run as one dsalt_add_rms_norm pass:
-        inference without autograd, 16-bit rows on the GPU, a weight of x's dtype."""
+        inference without autograd, 16-bit rows on the GPU, a weight of x's dtype; or the LayerNorm
+        `norm` as one dsalt_layer_norm pass, without autograd."""
         if self.training or torch.is_grad_enabled() or not self._fuse_norms:
             return False
+        if isinstance(norm, LayerNorm):
+            return self._layer_joins(x, x if h is None else h, norm)
         if h is not None and (h.shape != x.shape or h.dtype != x.dtype or not h.is_contiguous()
                               or h.data_ptr() % 16):
             return False
@@ -262,13 +317,13 @@ class DSALTTransformerBlock(nn.Module):
         makes no zero aux tensor), so that the next block's norm (or the final norm) takes
         that add in its own pass. `delta` is the previous block's pending FFN
         output (None for the first block). The caller checks `_norms_fusable` first."""
-        x_sum, h = _hip.add_rms_norm(x, delta, self.attn_norm.weight, self.attn_norm.eps)
+        x_sum, h = self._add_norm(x, delta, self.attn_norm)
         if x_sum is not None:
             x = x_sum
         x_attn, aux = self.attn(h, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, rope_cs=rope_cs, cu_list=cu_list,
                                 _need_aux=False)
         if self._norms_fusable(x, x_attn, self.ffn_norm):
-            x, h = _hip.add_rms_norm(x, x_attn, self.ffn_norm.weight, self.ffn_norm.eps)
+            x, h = self._add_norm(x, x_attn, self.ffn_norm)
         else:
             x = x + x_attn
             h = self.ffn_norm(x)
