@@ -915,8 +915,8 @@ int dsalt_fp8_quantize(const dsalt_fp8_quantize_args *a, void *stream) {
     if (a->rows < 0 || a->rows > (1 << 30)) return fail(DSALT_ERR_INVALID, "rows must be in [0, 2^30] (got %lld)", (long long)a->rows);
     if (a->k < 1 || a->k > (1 << 20)) return fail(DSALT_ERR_UNSUPPORTED, "k must be in [1, 2^20] (got %d)", a->k);
     const int blocks = (a->k + 127) / 128;
-    if (a->tile && (a->rows + 127) / 128 * blocks > (1 << 23))  // a launch's threads
-        return fail(DSALT_ERR_UNSUPPORTED, "more than 2^23 tiles (rows %lld, k %d)", (long long)a->rows, a->k);
+    if ((a->tile ? (a->rows + 127) / 128 : (a->rows + 63) / 64) * blocks > (1 << 23))  // a launch's threads
+        return fail(DSALT_ERR_UNSUPPORTED, "more than 2^23 tiles, or 2^29 blocks (rows %lld, k %d)", (long long)a->rows, a->k);
     if (!float_dtype(a->x_dtype)) return fail(DSALT_ERR_INVALID, "x_dtype %d is not a float dtype", a->x_dtype);
     if (a->x_stride < a->k || a->x_stride > ((int64_t)1 << 40) || a->scale_stride < blocks)
         return fail(DSALT_ERR_INVALID, "row strides must cover their rows");

@@ -7,9 +7,11 @@
 // term. Rows whose label is ignore_index (or lies outside [0, V)) count for nothing; the mean is over
 // the others.
 //
-// The forward reads the logits once with running maxima and sums of exp2((s - m) c), c = log2(e) / tau:
-// the difference first, since s c overflows where a mask holds the type's lowest value. It keeps m
-// and the sums' inverses of each row, and the backward reads the logits
+// The forward reads the logits once with running maxima and sums: exponents are fma(s, c, -m c), c =
+// log2(e) / tau, in the forward and in the backward, so that whatever m c was rounded to drops out of
+// every quotient; where m c overflows (a mask of the type's lowest value that leaves nothing) they are
+// (s - m) c. At tau = 2 the exponential at 1 is the square of that at tau. It keeps m and the sums'
+// inverses of each row, and the backward reads the logits
 // once more and writes the gradient, each rounded once from fp32 under the upstream gradient that
 // it is given (formed in the forward it would be rounded before a loss scale is known, which in fp16
 // loses most of a vocabulary's small probabilities). Both are bound by HBM bytes.
@@ -72,47 +74,83 @@ __device__ __forceinline__ float wave_maxf(float x) {
     for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
     return x;
 }
-// A maximum as a reference for exp2: of nothing but -inf any finite one will do.
-__device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ float wave_maximum(float x) {  // NaN stays
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = __builtin_elementwise_maximum(x, __shfl_xor(x, o));
+    return x;
+}
+// Which exponentials a logit has: at tau, also at 1, or at 1 as the square of that at tau = 2.
+enum { kOne = 0, kTwo = 1, kSquare = 2 };
 
-// Running maximum and sums of exp2(c v - c m), and of exp2(c1 v - c1 m) where TWO.
-template <bool TWO>
+// A maximum as a reference for exp2 (of nothing but -inf any finite one will do), and exponents against it.
+struct Reference {
+    float m, mc, mc1;
+    bool far;  // m c overflows
+    __device__ __forceinline__ Reference(float max, float c) : m(max == -INFINITY ? 0.f : max), mc(m * c), mc1(m * kLog2e) {
+        far = !(fmaxf(fabsf(mc), fabsf(mc1)) < INFINITY);
+    }
+    __device__ __forceinline__ float at(float v, float c) const { return far ? (v - m) * c : fmaf(v, c, -mc); }
+    __device__ __forceinline__ float at1(float v) const { return far ? (v - m) * kLog2e : fmaf(v, kLog2e, -mc1); }
+    // the exponent at temperature 1
+    template <int KIND>
+    __device__ __forceinline__ float label(float v, float c) const {
+        return KIND == kTwo ? at1(v) : KIND == kSquare ? 2.f * at(v, c) : at(v, c);
+    }
+};
+
+// Running maximum and sums of the exponentials.
+template <int KIND>
 struct Running {
     float m = -INFINITY, s = 0.f, s1 = 0.f;
     __device__ __forceinline__ void rescale(float mn, float c) {
-        const float d = m - reference(mn);
-        s *= fast_exp2(d * c);
-        if (TWO) s1 *= fast_exp2(d * kLog2e);
+        const Reference r(mn, c);
+        const float t = fast_exp2(r.at(m, c));
+        s *= t;
+        if (KIND == kTwo) s1 *= fast_exp2(r.at1(m));
+        if (KIND == kSquare) s1 *= t * t;
         m = mn;
     }
     template <int N>
     __device__ __forceinline__ void add(const float (&v)[N], float c) {
-        float mn = v[0];
+        float mn = m;  // NaN stays: the row is NaN then
 #pragma unroll
-        for (int i = 1; i < N; ++i) mn = fmaxf(mn, v[i]);
-        mn = fmaxf(m, mn);
+        for (int i = 0; i + 1 < N; i += 2) mn = max3f(mn, v[i], v[i + 1]);
+        if (N % 2) mn = __builtin_elementwise_maximum(mn, v[N - 1]);
         if (mn != m) rescale(mn, c);
-        const float r = reference(m);
+        const Reference r(m, c);
         float t = 0.f, t1 = 0.f;
+        if (!r.far) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float d = v[i] - r;
-            t += fast_exp2(d * c);
-            if (TWO) t1 += fast_exp2(d * kLog2e);
+            for (int i = 0; i < N; ++i) {
+                const float x = fast_exp2(fmaf(v[i], c, -r.mc));
+                t += x;
+                if (KIND == kTwo) t1 += fast_exp2(fmaf(v[i], kLog2e, -r.mc1));
+                if (KIND == kSquare) t1 = fmaf(x, x, t1);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float x = fast_exp2(r.at(v[i], c));
+                t += x;
+                if (KIND == kTwo) t1 += fast_exp2(r.at1(v[i]));
+                if (KIND == kSquare) t1 = fmaf(x, x, t1);
+            }
         }
         s += t;
-        if (TWO) s1 += t1;
+        if (KIND != kOne) s1 += t1;
     }
     __device__ __forceinline__ void join(float m2, float t, float t1, float c) {
-        const float mn = fmaxf(m, m2), d = m2 - reference(mn);
-        rescale(mn, c);
-        s += t * fast_exp2(d * c);
-        if (TWO) s1 += t1 * fast_exp2(d * kLog2e);
+        rescale(__builtin_elementwise_maximum(m, m2), c);
+        const Reference r(m, c);
+        const float x = fast_exp2(r.at(m2, c));
+        s += t * x;
+        if (KIND == kTwo) s1 += t1 * fast_exp2(r.at1(m2));
+        if (KIND == kSquare) s1 += t1 * (x * x);
     }
     __device__ __forceinline__ void join_wave(float c) {
-        rescale(wave_maxf(m), c);
+        rescale(wave_maximum(m), c);
         s = group_sum_lanes(s, 64);
-        if (TWO) s1 = group_sum_lanes(s1, 64);
+        if (KIND != kOne) s1 = group_sum_lanes(s1, 64);
     }
 };
 
@@ -139,16 +177,18 @@ __device__ __forceinline__ float slot(const DistillParams &p, int64_t row, int k
 }
 
 // A row's loss and statistics from its maximum and sums, by one wave.
-template <typename DT, bool TWO>
-__device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, const Running<TWO> &run, int lane) {
+template <typename DT, int KIND>
+__device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, const Running<KIND> &run, int lane) {
     const int label = row_label(p, row);
-    const float m = reference(run.m), s1 = TWO ? run.s1 : run.s, c1 = TWO ? kLog2e : p.c;
+    const Reference ref(run.m, p.c);
+    const float s1 = KIND == kOne ? run.s : run.s1;
     const char *logits = static_cast<const char *>(p.logits) + row * p.logits_stride * elem_size<DT>();
     float tm = -INFINITY, ts = 0.f, kl = 0.f;
     if (p.kl_w != 0.f && label >= 0) {
         int id;
         for (int k = lane; k < p.k; k += 64) tm = fmaxf(tm, slot(p, row, k, id));
-        tm = reference(wave_maxf(tm));
+        tm = wave_maxf(tm);
+        if (tm == -INFINITY) tm = 0.f;
         bool any = false;
         for (int k = lane; k < p.k; k += 64) {
             const float t = slot(p, row, k, id);
@@ -162,7 +202,7 @@ __device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, 
                 const float t = slot(p, row, k, id);
                 if (id < 0) continue;
                 const float lp = (t - tm) - lt, w = expf(t - tm) / ts;
-                const float lq = ((Elem<DT>::ld(logits, id) - m) * p.c - ls) * kLn2;
+                const float lq = (ref.at(Elem<DT>::ld(logits, id), p.c) - ls) * kLn2;
                 if (w != 0.f) kl += w * (lp - lq);
             }
             kl = group_sum_lanes(kl, 64);
@@ -171,11 +211,11 @@ __device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, 
     if (lane) return;
     float loss = p.kl_w * kl;
     if (p.lam != 0.f && label >= 0)
-        loss += p.lam * (log2f(s1) - (Elem<DT>::ld(logits, label) - m) * c1) * kLn2;
+        loss += p.lam * (log2f(s1) - ref.template label<KIND>(Elem<DT>::ld(logits, label), p.c)) * kLn2;
     p.row_loss[row] = label < 0 ? 0.f : loss;
     if (p.stats) {
         float *st = p.stats + row * kStats;
-        st[0] = m;
+        st[0] = ref.m;
         st[1] = 1.f / run.s;
         st[2] = 1.f / s1;
         st[3] = tm;
@@ -206,7 +246,7 @@ __device__ __forceinline__ void slice_of(const DistillParams &p, int split, int 
 }
 
 // NW waves a row (or slice), 256 threads a workgroup.
-template <typename DT, bool TWO, int NW>
+template <typename DT, int KIND, int NW>
 __global__ void __launch_bounds__(256) distill_rows_kernel(const DistillParams p) {
     constexpr int VE = Vec<DT>::N, NT = NW * 64, U = 32 / VE;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -219,7 +259,7 @@ __global__ void __launch_bounds__(256) distill_rows_kernel(const DistillParams p
     int first, last;
     slice_of(p, split, first, last);
     const Span sp = Span::of<DT>(base, first, last);
-    Running<TWO> run;
+    Running<KIND> run;
     if (t < sp.head + sp.tail) {
         const float v[1] = {Elem<DT>::ld(base, t < sp.head ? first + t : sp.tail_at + t - sp.head)};
         run.add(v, p.c);
@@ -250,11 +290,11 @@ __global__ void __launch_bounds__(256) distill_rows_kernel(const DistillParams p
         }
         __syncthreads();
         if (wave) return;
-        run = Running<TWO>();
+        run = Running<KIND>();
 #pragma unroll
         for (int w = 0; w < NW; ++w) run.join(lds[w][0], lds[w][1], lds[w][2], p.c);
     }
-    if (p.splits == 1) return finish_row<DT, TWO>(p, row, run, lane);
+    if (p.splits == 1) return finish_row<DT, KIND>(p, row, run, lane);
     if (lane == 0) {
         float *out = p.part + item * 3;
         out[0] = run.m;
@@ -291,17 +331,17 @@ __device__ __forceinline__ void reduce_rows(const DistillParams &p, float *lds) 
 }
 
 // Rows joined from their slices, a wave each; a lone workgroup also forms their sum.
-template <typename DT, bool TWO>
+template <typename DT, int KIND>
 __global__ void __launch_bounds__(1024) distill_join_kernel(const DistillParams p) {
     __shared__ float lds[32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = (int64_t)blockIdx.x * 16 + wave;
     if (row < p.rows) {
-        Running<TWO> run;
+        Running<KIND> run;
         const float *in = p.part + row * p.splits * 3;
         for (int i = lane; i < p.splits; i += 64) run.join(in[i * 3], in[i * 3 + 1], in[i * 3 + 2], p.c);
         run.join_wave(p.c);
-        finish_row<DT, TWO>(p, row, run, lane);
+        finish_row<DT, KIND>(p, row, run, lane);
     }
     if (gridDim.x == 1 && p.reduce) {
         __syncthreads();
@@ -316,7 +356,7 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const DistillParam
 
 // The gradient of a row (or slice): over the vocabulary first, then again at the teacher's ids and the
 // label, whose values are formed whole (ids that repeat take the sum of their slots).
-template <typename DT, bool TWO, int NW>
+template <typename DT, int KIND, int NW>
 __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p) {
     constexpr int VE = Vec<DT>::N, NT = NW * 64, U = 4;
     extern __shared__ char dyn[];
@@ -340,7 +380,7 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p)
         up = p.reduce ? *p.d_loss * p.stats[p.rows * kStats] : p.d_loss[row];
         kl = st[4] != 0.f ? up * p.grad_w : 0.f;
         k0 = kl * st[1];
-        if (TWO) k1 = up * p.lam * st[2];
+        if (KIND != kOne) k1 = up * p.lam * st[2];
         else k0 += up * p.lam * st[2];
         if (kl != 0.f)  // the teacher's probabilities
             for (int k = t; k < p.k; k += NT) {
@@ -350,10 +390,12 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p)
                 w[k] = i >= 0 ? expf(z - st[3]) * st[4] : 0.f;
             }
     }
+    const Reference ref(m, p.c);
     const auto value = [&](float v) {
-        const float d = v - m;
-        float g = k0 * fast_exp2(d * p.c);
-        if (TWO) g = fmaf(k1, fast_exp2(d * kLog2e), g);
+        const float x = fast_exp2(ref.at(v, p.c));
+        float g = k0 * x;
+        if (KIND == kTwo) g = fmaf(k1, fast_exp2(ref.at1(v)), g);
+        if (KIND == kSquare) g = fmaf(k1 * x, x, g);
         return g;
     };
     const Span sp = Span::of<DT>(base, first, last);
@@ -453,20 +495,20 @@ DistillParams params(const dsalt_distill_args &a) {
     return p;
 }
 
-template <typename DT, bool TWO>
+template <typename DT, int KIND>
 void launch_types(const DistillParams &p, bool bwd, hipStream_t stream) {
     const bool one_wave = p.vocab <= kRowMax;
     const dim3 grid((unsigned)(one_wave ? (p.rows + 3) / 4 : p.rows * p.splits)), block(256);
     const size_t lds = (size_t)(one_wave ? 4 : 1) * p.k * 8;
     if (bwd) {
-        if (one_wave) hipLaunchKernelGGL((distill_bwd_kernel<DT, TWO, 1>), grid, block, lds, stream, p);
-        else hipLaunchKernelGGL((distill_bwd_kernel<DT, TWO, 4>), grid, block, lds, stream, p);
+        if (one_wave) hipLaunchKernelGGL((distill_bwd_kernel<DT, KIND, 1>), grid, block, lds, stream, p);
+        else hipLaunchKernelGGL((distill_bwd_kernel<DT, KIND, 4>), grid, block, lds, stream, p);
         return;
     }
-    if (one_wave) hipLaunchKernelGGL((distill_rows_kernel<DT, TWO, 1>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((distill_rows_kernel<DT, TWO, 4>), grid, block, 0, stream, p);
+    if (one_wave) hipLaunchKernelGGL((distill_rows_kernel<DT, KIND, 1>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((distill_rows_kernel<DT, KIND, 4>), grid, block, 0, stream, p);
     const unsigned joins = (unsigned)((p.rows + 15) / 16);
-    if (p.splits > 1) hipLaunchKernelGGL((distill_join_kernel<DT, TWO>), dim3(joins), dim3(1024), 0, stream, p);
+    if (p.splits > 1) hipLaunchKernelGGL((distill_join_kernel<DT, KIND>), dim3(joins), dim3(1024), 0, stream, p);
     if (p.reduce && !(p.splits > 1 && joins == 1))
         hipLaunchKernelGGL(distill_reduce_kernel, dim3(1), dim3(1024), 0, stream, p);
 }
@@ -479,8 +521,9 @@ hipError_t launch(const dsalt_distill_args &a, bool bwd, hipStream_t stream) {
     }
     const bool two = a.label_weight != 0.f && a.label_weight != 1.f && a.temperature != 1.f;
     const auto go = [&](auto dt) {
-        if (two) launch_types<decltype(dt), true>(p, bwd, stream);
-        else launch_types<decltype(dt), false>(p, bwd, stream);
+        if (!two) launch_types<decltype(dt), kOne>(p, bwd, stream);
+        else if (a.temperature == 2.f) launch_types<decltype(dt), kSquare>(p, bwd, stream);
+        else launch_types<decltype(dt), kTwo>(p, bwd, stream);
     };
     if (a.logits_dtype == DSALT_DTYPE_BF16) go(BF16());
     else if (a.logits_dtype == DSALT_DTYPE_F16) go(F16());

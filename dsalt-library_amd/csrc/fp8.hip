@@ -72,19 +72,29 @@ __device__ __forceinline__ void store_scale(const QuantParams &p, int64_t row, i
     else static_cast<uint8_t *>(p.scale)[at] = (uint8_t)e8;
 }
 
-// Sixteen lanes a block of 128 of a row.
+// Sixteen lanes a block of 128 of a row, kQuantRun blocks a lane in flight.
+constexpr int kQuantRun = 4;
 template <typename DT>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantParams p) {
-    const int64_t items = p.rows * p.blocks;
+    const int64_t items = p.rows * p.blocks, first = (int64_t)blockIdx.x * (16 * kQuantRun) + (threadIdx.x >> 4);
     const int l = threadIdx.x & 15;
-    for (int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); item < items; item += (int64_t)gridDim.x * 16) {
-        const int64_t row = item / p.blocks;
-        const int block = (int)(item - row * p.blocks), c = block * kFp8Block + l * 8;
-        float v[8];
-        load8<DT>(p, row, c, v);
-        const uint32_t e8 = e8m0_of_amax(row16_max(amax8(v)));
-        if (c < p.k) store_q(p, row, c, quantised(v, e8));
-        if (l == 0) store_scale(p, row, block, e8);
+    float v[kQuantRun][8];
+    int64_t row[kQuantRun];
+    int block[kQuantRun];
+#pragma unroll
+    for (int u = 0; u < kQuantRun; ++u) {
+        const int64_t item = min(first + u * 16, items - 1);  // past the end: the last one again
+        row[u] = item / p.blocks;
+        block[u] = (int)(item - row[u] * p.blocks);
+        load8<DT>(p, row[u], block[u] * kFp8Block + l * 8, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kQuantRun; ++u) {
+        const int c = block[u] * kFp8Block + l * 8;
+        const uint32_t e8 = e8m0_of_amax(row16_max(amax8(v[u])));
+        if (first + u * 16 >= items) break;
+        if (c < p.k) store_q(p, row[u], c, quantised(v[u], e8));
+        if (l == 0) store_scale(p, row[u], block[u], e8);
     }
 }
 
@@ -451,7 +461,11 @@ struct Fp8Core {
         const int64_t ld = part ? p->part_ld : p->n, m = p->m;
         char *out = part ? reinterpret_cast<char *>(p->part + it.split * m * ld) : static_cast<char *>(p->out);
         const int dtype = part ? DSALT_DTYPE_F32 : p->out_dtype;
-        if (ld % 8) return store_ragged(out, dtype, ld, it, m);
+        if (ld % 8) {
+            if (dtype == DSALT_DTYPE_F32) return store_ragged<F32>(out, ld, it, m);
+            if (dtype == DSALT_DTYPE_BF16) return store_ragged<BF16>(out, ld, it, m);
+            return store_ragged<F16>(out, ld, it, m);
+        }
         const int64_t col = it.n0 + wn * N16 * 16 + (g & 1) * 16 + (g >> 1) * 8;
         if (dtype == DSALT_DTYPE_F32) store_rows<F32>(out, ld, it, m, row, col);
         else if (dtype == DSALT_DTYPE_BF16) store_rows<BF16>(out, ld, it, m, row, col);
@@ -491,18 +505,42 @@ struct Fp8Core {
             }
         }
     }
-    // Rows that do not start on 16 bytes: an element at a time.
-    __device__ __forceinline__ void store_ragged(char *out, int dtype, int64_t ld, const Fp8Item &it, int64_t m) const {
+    // Rows that do not start on 16 bytes: the same pieces, written to wherever they lie.
+    template <typename DT>
+    __device__ __forceinline__ void store_ragged(char *out, int64_t ld, const Fp8Item &it, int64_t m) const {
+        constexpr int SZ = std::is_same<DT, F32>::value ? 4 : 2;
+        struct __attribute__((packed)) Piece {
+            uint32_t w[2 * SZ];
+        };
+        const int g = lane >> 4;
 #pragma unroll
         for (int i = 0; i < M16; ++i) {
             const int64_t row = it.m0 + (wm * M16 + i) * 16 + (lane & 15);
-            if (row >= m) continue;
 #pragma unroll
-            for (int j = 0; j < N16; ++j) {
-                const int64_t col = it.n0 + (wn * N16 + j) * 16 + (lane >> 4) * 4;
+            for (int j = 0; j < N16; j += 2) {
+                float v[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < ld) store_dt(out, row * ld + col + e, dtype, acc[i][j][e]);
+                for (int e = 0; e < 4; ++e) {
+                    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][j][e]), __float_as_uint(acc[i][j + 1][e]),
+                                                                    false, false);
+                    v[e] = __uint_as_float(x[0]);
+                    v[4 + e] = __uint_as_float(x[1]);
+                }
+                const int64_t col = it.n0 + (wn * N16 + j + (g & 1)) * 16 + (g >> 1) * 8;
+                char *to = out + (row * ld + col) * SZ;
+                if (row < m && col + 8 <= ld) {
+                    Piece q;
+#pragma unroll
+                    for (int e = 0; e < 2 * SZ; ++e) {
+                        if constexpr (SZ == 4) q.w[e] = __float_as_uint(v[e]);
+                        else q.w[e] = DT::pack2(v[2 * e], v[2 * e + 1]);
+                    }
+                    *reinterpret_cast<Piece *>(to) = q;
+                } else if (row < m) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (col + e < ld) Elem<DT>::st(to, e, v[e]);
+                }
             }
         }
     }
@@ -531,105 +569,111 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const Fp8Params p) {
     }
 }
 
-// Up to 16 MF rows against 16 rows of weights a wave: the weights come straight from memory, eight blocks of k
-// in flight, and KW waves of the workgroup share out k and join their sums in LDS. TX: the rows are x's
-// element type and each wave quantises what it reads of them; void: they are e4m3 with scales.
+// Up to 16 MF rows against 16 NT rows of weights: the eight waves of a workgroup share out the blocks of k, read
+// the weights straight from memory and join their sums in LDS. TX: the rows are x's element type and a wave
+// quantises what it reads of them, once for all its NT; void: they are e4m3 with scales. Bound by the
+// weights' bytes, and by latency where they are few: all loads of a wave's blocks go out before the first
+// product (U blocks at a time).
 constexpr int kRowWaves = 8;
-template <typename TX, int MF, int KW>
+template <typename TX, int MF, int NT>
 __global__ void __launch_bounds__(64 * kRowWaves) fp8_rows_kernel(const Fp8Params p) {
     constexpr bool QUANT = !std::is_void<TX>::value;
-    constexpr int U = 4;
-    __shared__ f32x4 lds[KW > 1 ? kRowWaves : 1][MF][64];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int kw = wave % KW, group = lane >> 4;
-    const int64_t n0 = ((int64_t)blockIdx.x * (kRowWaves / KW) + wave / KW) * 16;
-    const int64_t brow = n0 + (lane & 15);
-    const bool b_in = brow < p.n;
-    const char *bp = p.b.base + (b_in ? brow : 0) * p.b.ld;
-    const int64_t nb = min(n0, p.n - 1) / kFp8Block;
-    f32x4 acc[MF] = {};
-    const int per = (p.kb + KW - 1) / KW, first = kw * per, last = n0 < p.n ? min(first + per, p.kb) : 0;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    // one block of k: the weights w against the rows
-    const auto block = [&](int kb, Fp8Frag w) {
-        const int64_t k0 = (int64_t)kb * kFp8Block + group * 16;
-        const float sb = p.sb.at(nb, kb);
+    constexpr int U = NT > 2 ? 1 : 4 / NT;
+    __shared__ f32x4 lds[kRowWaves][NT * MF][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, group = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
+    const char *bp[NT];
+    bool b_in[NT];
 #pragma unroll
-        for (int i = 0; i < MF; ++i) {
-            const int64_t row = i * 16 + (lane & 15);
-            const bool in = row < p.m;
-            Fp8Frag fa = fp8_frag(zero, zero);
-            float s = 0.f;
-            if constexpr (QUANT) {
-                const char *ap = p.a.base + (in ? row : 0) * p.a.ld;
-                Raw8<TX> r0 = {}, r1 = {}, r2 = {}, r3 = {};
-                if (in && k0 < p.k) {
-                    r0.load(ap, k0 / 8);
-                    r1.load(ap, k0 / 8 + 1);
-                }
-                if (in && k0 + 64 < p.k) {
-                    r2.load(ap, k0 / 8 + 8);
-                    r3.load(ap, k0 / 8 + 9);
-                }
-                float v0[8], v1[8], v2[8], v3[8];
-                r0.get(v0);
-                r1.get(v1);
-                r2.get(v2);
-                r3.get(v3);
-                uint32_t m = max(max(amax8(v0), amax8(v1)), max(amax8(v2), amax8(v3)));
-                m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-                m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-                const uint32_t e8 = e8m0_of_amax(m);
-                const uint2 q0 = quantised(v0, e8), q1 = quantised(v1, e8), q2 = quantised(v2, e8), q3 = quantised(v3, e8);
-                fa = fp8_frag(make_uint4(q0.x, q0.y, q1.x, q1.y), make_uint4(q2.x, q2.y, q3.x, q3.y));
-                s = e8m0_f32(e8);
-            } else if (in) {
-                const char *ap = p.a.base + row * p.a.ld;
-                uint4 lo = zero, hi = zero;
-                if (k0 < p.k) lo = *reinterpret_cast<const uint4 *>(ap + k0);
-                if (k0 + 64 < p.k) hi = *reinterpret_cast<const uint4 *>(ap + k0 + 64);
-                fa = fp8_frag(lo, hi);
-                s = p.sa.at(row, kb);
-            }
-            const f32x4 d = mfma_fp8(w, fa);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(d[e], s * sb, acc[i][e]);
-        }
-    };
-    for (int t = first; t < last; t += U) {
-        Fp8Frag fb[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t k0 = (int64_t)(t + u) * kFp8Block + group * 16;
-            uint4 lo = zero, hi = zero;
-            if (t + u < last && b_in && k0 < p.k) lo = *reinterpret_cast<const uint4 *>(bp + k0);
-            if (t + u < last && b_in && k0 + 64 < p.k) hi = *reinterpret_cast<const uint4 *>(bp + k0 + 64);
-            fb[u] = fp8_frag(lo, hi);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (t + u < last) block(t + u, fb[u]);
-        }
+    for (int j = 0; j < NT; ++j) {
+        const int64_t row = n0 + j * 16 + (lane & 15);
+        b_in[j] = row < p.n;
+        bp[j] = p.b.base + (b_in[j] ? row : 0) * p.b.ld + group * 16;
     }
-    if constexpr (KW > 1) {
+    f32x4 acc[NT][MF] = {};
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int t = wave; t < p.kb; t += kRowWaves * U) {
+        Fp8Frag fb[U][NT];
+        float sb[U][NT];
 #pragma unroll
-        for (int i = 0; i < MF; ++i) lds[wave][i][lane] = acc[i];
-        __syncthreads();
-        if (kw) return;
+        for (int u = 0; u < U; ++u) {
+            const int kb = t + u * kRowWaves;
+            const int64_t k0 = (int64_t)kb * kFp8Block, k = k0 + group * 16;
 #pragma unroll
-        for (int w = 1; w < KW; ++w)
+            for (int j = 0; j < NT; ++j) {
+                uint4 lo = zero, hi = zero;
+                if (kb < p.kb && b_in[j] && k < p.k) lo = *reinterpret_cast<const uint4 *>(bp[j] + k0);
+                if (kb < p.kb && b_in[j] && k + 64 < p.k) hi = *reinterpret_cast<const uint4 *>(bp[j] + k0 + 64);
+                fb[u][j] = fp8_frag(lo, hi);
+                sb[u][j] = kb < p.kb ? p.sb.at(min(n0 + j * 16, p.n - 1) / kFp8Block, kb) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int kb = t + u * kRowWaves;
+            if (kb >= p.kb) continue;
+            const int64_t k = (int64_t)kb * kFp8Block + group * 16;
 #pragma unroll
             for (int i = 0; i < MF; ++i) {
-                const f32x4 o = lds[wave + w][i][lane];
+                const int64_t row = i * 16 + (lane & 15);
+                const bool in = row < p.m;
+                Fp8Frag fa = fp8_frag(zero, zero);
+                float s = 0.f;
+                if constexpr (QUANT) {
+                    const char *ap = p.a.base + (in ? row : 0) * p.a.ld;
+                    Raw8<TX> r0 = {}, r1 = {}, r2 = {}, r3 = {};
+                    if (in && k < p.k) {
+                        r0.load(ap, k / 8);
+                        r1.load(ap, k / 8 + 1);
+                    }
+                    if (in && k + 64 < p.k) {
+                        r2.load(ap, k / 8 + 8);
+                        r3.load(ap, k / 8 + 9);
+                    }
+                    float v0[8], v1[8], v2[8], v3[8];
+                    r0.get(v0);
+                    r1.get(v1);
+                    r2.get(v2);
+                    r3.get(v3);
+                    uint32_t m = max(max(amax8(v0), amax8(v1)), max(amax8(v2), amax8(v3)));
+                    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+                    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+                    const uint32_t e8 = e8m0_of_amax(m);
+                    const uint2 q0 = quantised(v0, e8), q1 = quantised(v1, e8), q2 = quantised(v2, e8), q3 = quantised(v3, e8);
+                    fa = fp8_frag(make_uint4(q0.x, q0.y, q1.x, q1.y), make_uint4(q2.x, q2.y, q3.x, q3.y));
+                    s = e8m0_f32(e8);
+                } else if (in) {
+                    const char *ap = p.a.base + row * p.a.ld;
+                    uint4 lo = zero, hi = zero;
+                    if (k < p.k) lo = *reinterpret_cast<const uint4 *>(ap + k);
+                    if (k + 64 < p.k) hi = *reinterpret_cast<const uint4 *>(ap + k + 64);
+                    fa = fp8_frag(lo, hi);
+                    s = p.sa.at(row, kb);
+                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][e] += o[e];
+                for (int j = 0; j < NT; ++j) {
+                    const f32x4 d = mfma_fp8(fb[u][j], fa);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(d[e], s * sb[u][j], acc[j][i][e]);
+                }
             }
+        }
     }
-    const int64_t col = n0 + group * 4;
 #pragma unroll
-    for (int i = 0; i < MF; ++i) {
-        const int64_t row = i * 16 + (lane & 15);
-        float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MF; ++i) lds[wave][j * MF + i][lane] = acc[j][i];
+    __syncthreads();
+    for (int q = wave; q < NT * MF; q += kRowWaves) {
+        f32x4 sum = lds[0][q][lane];
+#pragma unroll
+        for (int w = 1; w < kRowWaves; ++w) {
+            const f32x4 o = lds[w][q][lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += o[e];
+        }
+        const int64_t row = q % MF * 16 + (lane & 15), col = n0 + q / MF * 16 + group * 4;
+        float v[4] = {sum[0], sum[1], sum[2], sum[3]};
         if (row < p.m && col < p.n) store_out<4>(p, row, col, v);
     }
 }
@@ -687,17 +731,15 @@ hipError_t launch_tiles(const Fp8Params &p, int tile, hipStream_t stream) {
 
 template <typename TX, int MF>
 void launch_few(const Fp8Params &p, hipStream_t stream) {
-    // waves along k until the card has two a SIMD, each with two blocks of k at least
-    const int64_t tiles = (p.n + 15) / 16;
-    int kw = 1;
-    while (kw < kRowWaves && tiles * kw < 2048 && p.kb >= kw * 4) kw *= 2;
-    const dim3 block(64 * kRowWaves), grid((unsigned)((tiles * kw + kRowWaves - 1) / kRowWaves));
-    switch (kw) {
-        case 1: hipLaunchKernelGGL((fp8_rows_kernel<TX, MF, 1>), grid, block, 0, stream, p); break;
-        case 2: hipLaunchKernelGGL((fp8_rows_kernel<TX, MF, 2>), grid, block, 0, stream, p); break;
-        case 4: hipLaunchKernelGGL((fp8_rows_kernel<TX, MF, 4>), grid, block, 0, stream, p); break;
-        default: hipLaunchKernelGGL((fp8_rows_kernel<TX, MF, 8>), grid, block, 0, stream, p); break;
-    }
+    // wider workgroups quantise and read the rows less often; narrower ones where there would be fewer than two a CU
+    const auto go = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
+        hipLaunchKernelGGL((fp8_rows_kernel<TX, MF, NT>), dim3((unsigned)((p.n + 16 * NT - 1) / (16 * NT))), dim3(64 * kRowWaves), 0,
+                           stream, p);
+    };
+    if (p.n >= 4 * 16 * 480) go(std::integral_constant<int, 4>());
+    else if (p.n >= 2 * 16 * 480) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 1>());
 }
 template <typename TX>
 void launch_few_rows(const Fp8Params &p, hipStream_t stream) {
@@ -711,8 +753,8 @@ void launch_quant(const QuantParams &p, bool tile, hipStream_t stream) {
         const int64_t groups = (p.rows + kFp8Block - 1) / kFp8Block * p.blocks;
         hipLaunchKernelGGL(quant_tile_kernel<DT>, dim3((unsigned)groups), dim3(256), 0, stream, p);
     } else {
-        const int64_t groups = (p.rows * p.blocks + 15) / 16;
-        hipLaunchKernelGGL(quant_rows_kernel<DT>, dim3((unsigned)std::min<int64_t>(groups, 1 << 20)), dim3(256), 0, stream, p);
+        const int64_t groups = (p.rows * p.blocks + 16 * kQuantRun - 1) / (16 * kQuantRun);
+        hipLaunchKernelGGL(quant_rows_kernel<DT>, dim3((unsigned)groups), dim3(256), 0, stream, p);
     }
 }
 

@@ -71,7 +71,7 @@ def fp8_quantize(x: torch.Tensor, tile: bool = False, scale_dtype: torch.dtype =
     k = x.shape[-1] if x.dim() else 0
     ok = (x.device.type == "cuda" and x.dtype in _hip._SCORE_DTYPES and 1 <= k <= 1 << 20 and scale_dtype in (torch.float32, E8M0)
           and (not tile or x.dim() == 2) and x.numel() // k <= 1 << 30
-          and (not tile or _blocks(x.shape[0]) * _blocks(k) <= 1 << 23))
+          and (_blocks(x.shape[0]) if tile else -(-(x.numel() // k) // 64)) * _blocks(k) <= 1 << 23)
     if not ok:
         _hip.require_gpu(x)
         raise _hip.DsaltError(f"fp8_quantize needs bf16, fp16 or fp32 x [..., k], [n, k] for tiles, and fp32 or e8m0 scales "
