@@ -76,16 +76,16 @@ __device__ __forceinline__ void store_scale(const QuantParams &p, int64_t row, i
 constexpr int kQuantRun = 4;
 template <typename DT>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantParams p) {
-    const int64_t items = p.rows * p.blocks, first = (int64_t)blockIdx.x * (16 * kQuantRun) + (threadIdx.x >> 4);
+    const uint32_t items = (uint32_t)(p.rows * p.blocks);  // below 2^30
+    const uint32_t first = blockIdx.x * (16 * kQuantRun) + (threadIdx.x >> 4);
     const int l = threadIdx.x & 15;
     float v[kQuantRun][8];
-    int64_t row[kQuantRun];
-    int block[kQuantRun];
+    uint32_t row[kQuantRun], block[kQuantRun];
 #pragma unroll
     for (int u = 0; u < kQuantRun; ++u) {
-        const int64_t item = min(first + u * 16, items - 1);  // past the end: the last one again
-        row[u] = item / p.blocks;
-        block[u] = (int)(item - row[u] * p.blocks);
+        const uint32_t item = min(first + u * 16, items - 1);  // past the end: the last one again
+        row[u] = item / (uint32_t)p.blocks;
+        block[u] = item - row[u] * p.blocks;
         load8<DT>(p, row[u], block[u] * kFp8Block + l * 8, v[u]);
     }
 #pragma unroll
@@ -509,8 +509,11 @@ struct Fp8Core {
     template <typename DT>
     __device__ __forceinline__ void store_ragged(char *out, int64_t ld, const Fp8Item &it, int64_t m) const {
         constexpr int SZ = std::is_same<DT, F32>::value ? 4 : 2;
-        struct __attribute__((packed)) Piece {
+        struct __attribute__((packed, aligned(4))) Piece {
             uint32_t w[2 * SZ];
+        };
+        struct __attribute__((packed, aligned(4))) Inner {
+            uint32_t w[3];
         };
         const int g = lane >> 4;
 #pragma unroll
@@ -535,7 +538,17 @@ struct Fp8Core {
                         if constexpr (SZ == 4) q.w[e] = __float_as_uint(v[e]);
                         else q.w[e] = DT::pack2(v[2 * e], v[2 * e + 1]);
                     }
-                    *reinterpret_cast<Piece *>(to) = q;
+                    if (SZ == 4 || ((uintptr_t)to & 3) == 0) {
+                        *reinterpret_cast<Piece *>(to) = q;
+                    } else {  // rows of odd length: an element, six on dwords, an element
+                        uint16_t *o = reinterpret_cast<uint16_t *>(to);
+                        o[0] = (uint16_t)q.w[0];
+                        Inner in;
+#pragma unroll
+                        for (int e = 0; e < 3; ++e) in.w[e] = q.w[e] >> 16 | q.w[e + 1] << 16;
+                        *reinterpret_cast<Inner *>(o + 1) = in;
+                        o[7] = (uint16_t)(q.w[3] >> 16);
+                    }
                 } else if (row < m) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
@@ -703,19 +716,35 @@ struct Plan {
     int tile, splits;
 };
 
+// The tile and the number of splits of k with the least time by a model of what they measured, in us: a
+// workgroup's `start` (launch, first loads, results) and the steps over its blocks of k, which take longer the
+// more workgroups share a CU, once for each round of the card. 512 x 2816 x 1024: 64 x 128 tiles 11.5, 128 x 128
+// 14.8, 256 x 256 33.5; 8192 x 1024 x 5632: 73, 61, 55; 1000 x 4096 x 4096: 24.7, 28, 48. Splits cost a second
+// launch and the traffic of their parts: 64 x 4096 x 4096 14.9, 12.7, 11.7 and 14.2 with 1, 2, 4 and 8.
 Plan plan(int64_t m, int64_t n, int64_t k) {
+    struct Tile {
+        int bm, bn, per_cu;
+        double start, step[3];
+    };
+    static const Tile tiles[] = {{256, 256, 1, 6.0, {1.4}}, {128, 128, 2, 4.5, {0.7, 0.95}}, {64, 128, 3, 4.0, {0.39, 0.6, 0.8}}};
     const int kb = (int)((k + kFp8Block - 1) / kFp8Block);
-    for (int t : {kTile256, kTile128, kTile64}) {
-        const int64_t bm = t == kTile256 ? 256 : t == kTile128 ? 128 : 64, bn = t == kTile256 ? 256 : 128;
-        const int64_t tiles = ((m + bm - 1) / bm) * ((n + bn - 1) / bn);
-        if (tiles >= 256 || t == kTile64) {
-            int splits = 1;
-            while (t == kTile64 && tiles * splits * 2 <= 512 && kb / (splits * 2) >= 4) splits *= 2;
-            const int per = (kb + splits - 1) / splits;
-            return {t, (kb + per - 1) / per};  // none of them empty
+    Plan best = {kTile64, 1};
+    double least = 1e30;
+    for (int t : {kTile256, kTile128, kTile64})
+        for (int splits = 1; splits <= (t == kTile64 ? 16 : 1) && splits <= kb; splits *= 2) {
+            const Tile &tile = tiles[t];
+            const int per = (kb + splits - 1) / splits, used = (kb + per - 1) / per;  // none of them empty
+            const int64_t groups = ((m + tile.bm - 1) / tile.bm) * ((n + tile.bn - 1) / tile.bn) * used;
+            const int64_t rounds = (groups + 256 * tile.per_cu - 1) / (256 * tile.per_cu);
+            const int shared = rounds > 1 ? tile.per_cu : (int)((groups + 255) / 256);
+            double time = (double)rounds * (tile.start + per * tile.step[shared - 1]);
+            if (used > 1) time += 3.0 + (double)used * (double)m * (double)n * 8.0 / 3e6;
+            if (time < least) {
+                least = time;
+                best = {t, used};
+            }
         }
-    }
-    return {kTile64, 1};
+    return best;
 }
 
 template <bool MX>
