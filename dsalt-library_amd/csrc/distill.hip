@@ -16,7 +16,7 @@
 // it is given (formed in the forward it would be rounded before a loss scale is known, which in fp16
 // loses most of a vocabulary's small probabilities). Both are bound by HBM bytes.
 //
-// Rows of up to 2048 logits take one wave, longer ones four; few long rows are cut into slices whose
+// Rows of up to 4096 logits take one wave, longer ones four; few long rows are cut into slices whose
 // sums a second kernel joins.
 #include "launch.h"
 #include "lanes.h"
@@ -28,7 +28,7 @@ namespace dsalt {
 namespace {
 
 constexpr int kStats = 5;         // of a row: m, 1 / sum at tau, 1 / sum at 1, the teacher's m, 1 / the teacher's sum
-constexpr int kRowMax = 2048;     // logits of a row that one wave takes
+constexpr int kRowMax = 4096;     // logits of a row that one wave takes
 constexpr int kSlice = 2048;      // least logits of a slice
 constexpr int kSliceGroups = 1024;  // workgroups that slices are made for
 
@@ -176,21 +176,38 @@ __device__ __forceinline__ float slot(const DistillParams &p, int64_t row, int k
     return z * p.inv_tau;
 }
 
+// What a row's end needs of memory, read before the row itself: its label, and the lane's first slot.
+template <typename DT>
+struct RowEnd {
+    int label, id = -1;
+    float t = -INFINITY, at_id = 0.f, at_label = 0.f;  // the slot's logit over tau; the student's at the id and at the label
+    __device__ __forceinline__ RowEnd(const DistillParams &p, int64_t row, int lane, bool ends = true) : label(ends ? row_label(p, row) : -1) {
+        const char *logits = static_cast<const char *>(p.logits) + row * p.logits_stride * elem_size<DT>();
+        if (label < 0) return;
+        if (p.kl_w != 0.f && lane < p.k) t = slot(p, row, lane, id);
+        if (id >= 0) at_id = Elem<DT>::ld(logits, id);
+        if (p.lam != 0.f) at_label = Elem<DT>::ld(logits, label);
+    }
+};
+
 // A row's loss and statistics from its maximum and sums, by one wave.
 template <typename DT, int KIND>
-__device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, const Running<KIND> &run, int lane) {
-    const int label = row_label(p, row);
+__device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, const Running<KIND> &run, const RowEnd<DT> &end,
+                                           int lane) {
+    const int label = end.label;
     const Reference ref(run.m, p.c);
     const float s1 = KIND == kOne ? run.s : run.s1;
     const char *logits = static_cast<const char *>(p.logits) + row * p.logits_stride * elem_size<DT>();
     float tm = -INFINITY, ts = 0.f, kl = 0.f;
     if (p.kl_w != 0.f && label >= 0) {
         int id;
-        for (int k = lane; k < p.k; k += 64) tm = fmaxf(tm, slot(p, row, k, id));
+        tm = end.t;
+        for (int k = 64 + lane; k < p.k; k += 64) tm = fmaxf(tm, slot(p, row, k, id));
         tm = wave_maxf(tm);
         if (tm == -INFINITY) tm = 0.f;
-        bool any = false;
-        for (int k = lane; k < p.k; k += 64) {
+        bool any = end.id >= 0;
+        ts = end.id >= 0 ? expf(end.t - tm) : 0.f;
+        for (int k = 64 + lane; k < p.k; k += 64) {
             const float t = slot(p, row, k, id);
             any |= id >= 0;
             ts += id >= 0 ? expf(t - tm) : 0.f;
@@ -198,12 +215,15 @@ __device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, 
         ts = group_sum_lanes(ts, 64);
         if (__ballot(any)) {
             const float lt = logf(ts), ls = log2f(run.s);
-            for (int k = lane; k < p.k; k += 64) {
-                const float t = slot(p, row, k, id);
-                if (id < 0) continue;
+            const auto term = [&](float t, float v) {
                 const float lp = (t - tm) - lt, w = expf(t - tm) / ts;
-                const float lq = (ref.at(Elem<DT>::ld(logits, id), p.c) - ls) * kLn2;
-                if (w != 0.f) kl += w * (lp - lq);
+                const float lq = (ref.at(v, p.c) - ls) * kLn2;
+                return w != 0.f ? w * (lp - lq) : 0.f;
+            };
+            if (end.id >= 0) kl = term(end.t, end.at_id);
+            for (int k = 64 + lane; k < p.k; k += 64) {
+                const float t = slot(p, row, k, id);
+                if (id >= 0) kl += term(t, Elem<DT>::ld(logits, id));
             }
             kl = group_sum_lanes(kl, 64);
         }
@@ -211,7 +231,7 @@ __device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, 
     if (lane) return;
     float loss = p.kl_w * kl;
     if (p.lam != 0.f && label >= 0)
-        loss += p.lam * (log2f(s1) - ref.template label<KIND>(Elem<DT>::ld(logits, label), p.c)) * kLn2;
+        loss += p.lam * (log2f(s1) - ref.template label<KIND>(end.at_label, p.c)) * kLn2;
     p.row_loss[row] = label < 0 ? 0.f : loss;
     if (p.stats) {
         float *st = p.stats + row * kStats;
@@ -259,27 +279,44 @@ __global__ void __launch_bounds__(256) distill_rows_kernel(const DistillParams p
     int first, last;
     slice_of(p, split, first, last);
     const Span sp = Span::of<DT>(base, first, last);
+    const uint4 *body = reinterpret_cast<const uint4 *>(base + (int64_t)(first + sp.head) * elem_size<DT>());
+    // whole runs of U vectors a lane, the next one's loads before this one's sums; what is left is loaded ahead
+    const int runs = sp.vecs / (NT * U);
+    uint4 u[U], rest[U];
+    const uint4 *at = body + t;
+    if (runs)
+#pragma unroll
+        for (int j = 0; j < U; ++j) u[j] = at[j * NT];
+    const RowEnd<DT> end(p, row, lane, p.splits == 1);  // a split's row is ended by the join
     Running<KIND> run;
     if (t < sp.head + sp.tail) {
         const float v[1] = {Elem<DT>::ld(base, t < sp.head ? first + t : sp.tail_at + t - sp.head)};
         run.add(v, p.c);
     }
-    const uint4 *body = reinterpret_cast<const uint4 *>(base + (int64_t)(first + sp.head) * elem_size<DT>());
-    for (int i = t; i < sp.vecs; i += NT * U) {
-        uint4 u[U];
+    const int behind = sp.vecs - runs * NT * U;
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+        if (j * NT + t < behind) rest[j] = body[runs * NT * U + j * NT + t];
+    for (int i = 0; i < runs; ++i) {
+        at += NT * U;
+        uint4 next[U];
+        if (i + 1 < runs)
+#pragma unroll
+            for (int j = 0; j < U; ++j) next[j] = at[j * NT];
         float v[U * VE];
 #pragma unroll
-        for (int j = 0; j < U; ++j)
-            if (i + j * NT < sp.vecs) u[j] = body[i + j * NT];
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            if (i + j * NT < sp.vecs) Vec<DT>::get(u[j], v + j * VE);
-            else
-#pragma unroll
-                for (int e = 0; e < VE; ++e) v[j * VE + e] = -INFINITY;
-        }
+        for (int j = 0; j < U; ++j) Vec<DT>::get(u[j], v + j * VE);
         run.add(v, p.c);
+#pragma unroll
+        for (int j = 0; j < U; ++j) u[j] = next[j];
     }
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+        if (j * NT + t < behind) {
+            float v[VE];
+            Vec<DT>::get(rest[j], v);
+            run.add(v, p.c);
+        }
     run.join_wave(p.c);
     if constexpr (NW > 1) {
         __shared__ float lds[NW][3];
@@ -294,7 +331,7 @@ __global__ void __launch_bounds__(256) distill_rows_kernel(const DistillParams p
 #pragma unroll
         for (int w = 0; w < NW; ++w) run.join(lds[w][0], lds[w][1], lds[w][2], p.c);
     }
-    if (p.splits == 1) return finish_row<DT, KIND>(p, row, run, lane);
+    if (p.splits == 1) return finish_row<DT, KIND>(p, row, run, end, lane);
     if (lane == 0) {
         float *out = p.part + item * 3;
         out[0] = run.m;
@@ -337,11 +374,12 @@ __global__ void __launch_bounds__(1024) distill_join_kernel(const DistillParams 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = (int64_t)blockIdx.x * 16 + wave;
     if (row < p.rows) {
+        const RowEnd<DT> end(p, row, lane);
         Running<KIND> run;
         const float *in = p.part + row * p.splits * 3;
         for (int i = lane; i < p.splits; i += 64) run.join(in[i * 3], in[i * 3 + 1], in[i * 3 + 2], p.c);
         run.join_wave(p.c);
-        finish_row<DT, KIND>(p, row, run, lane);
+        finish_row<DT, KIND>(p, row, run, end, lane);
     }
     if (gridDim.x == 1 && p.reduce) {
         __syncthreads();
@@ -373,6 +411,16 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p)
     char *out = static_cast<char *>(p.d_logits) + row * p.vocab * elem_size<DT>();
     int first = 0, last = 0;
     if (live) slice_of(p, split, first, last);
+    const Span sp = Span::of<DT>(base, first, last);
+    const uint4 *body = reinterpret_cast<const uint4 *>(base + (int64_t)(first + sp.head) * elem_size<DT>());
+    uint4 u[U];  // the first run's loads, ahead of what the row's statistics take
+    if (label >= 0)
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (t + j * NT < sp.vecs) u[j] = body[t + j * NT];
+    int id0 = -1;
+    float z0 = 0.f;
+    if (label >= 0 && p.grad_w != 0.f && t < p.k) z0 = slot(p, row, t, id0);
     float m = 0.f, k0 = 0.f, k1 = 0.f, up = 0.f, kl = 0.f;
     if (label >= 0) {
         const float *st = p.stats + row * kStats;
@@ -384,8 +432,8 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p)
         else k0 += up * p.lam * st[2];
         if (kl != 0.f)  // the teacher's probabilities
             for (int k = t; k < p.k; k += NT) {
-                int i;
-                const float z = slot(p, row, k, i);
+                int i = id0;
+                const float z = k == t ? z0 : slot(p, row, k, i);
                 id[k] = i;
                 w[k] = i >= 0 ? expf(z - st[3]) * st[4] : 0.f;
             }
@@ -398,7 +446,6 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p)
         if (KIND == kSquare) g = fmaf(k1 * x, x, g);
         return g;
     };
-    const Span sp = Span::of<DT>(base, first, last);
     if (live && (label < 0 || (k0 == 0.f && k1 == 0.f))) {  // nothing of the row counts: zeros, whatever it holds
         for (int i = first + t; i < last; i += NT) Elem<DT>::st(out, i, 0.f);
     } else if (live) {
@@ -407,14 +454,13 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p)
             Elem<DT>::st(out, i, value(Elem<DT>::ld(base, i)));
         }
         const int at = first + sp.head;
-        const uint4 *body = reinterpret_cast<const uint4 *>(base + (int64_t)at * elem_size<DT>());
         char *dst = out + (int64_t)at * elem_size<DT>();
         const bool whole = ((uintptr_t)dst & 15) == 0;  // else the gradient's rows lie otherwise than the logits'
         for (int i = t; i < sp.vecs; i += NT * U) {
-            uint4 u[U];
+            uint4 next[U];
 #pragma unroll
             for (int j = 0; j < U; ++j)
-                if (i + j * NT < sp.vecs) u[j] = body[i + j * NT];
+                if (i + (U + j) * NT < sp.vecs) next[j] = body[i + (U + j) * NT];
 #pragma unroll
             for (int j = 0; j < U; ++j) {
                 const int at_vec = i + j * NT;
@@ -428,6 +474,8 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p)
 #pragma unroll
                     for (int e = 0; e < VE; ++e) Elem<DT>::st(dst, at_vec * VE + e, v[e]);
             }
+#pragma unroll
+            for (int j = 0; j < U; ++j) u[j] = next[j];
         }
     }
     __syncthreads();  // the slots are in LDS, and the row's stores precede those that follow
