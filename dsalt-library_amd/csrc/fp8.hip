@@ -142,7 +142,6 @@ struct Fp8Params {
     int splits, per_split;
     int64_t part_ld;  // n rounded up to a multiple of eight
     int tiles_m, tiles_n;
-    int a_dtype;  // few rows: of x, which is quantised on the way
 };
 
 __device__ __forceinline__ float load_dt(const void *p, int64_t i, int dtype) {
@@ -153,31 +152,25 @@ __device__ __forceinline__ void store_dt(void *p, int64_t i, int dtype, float v)
     else if (dtype == DSALT_DTYPE_BF16) Elem<BF16>::st(p, i, v);
     else Elem<F16>::st(p, i, v);
 }
-// N (4 or 8) results of columns col .. of a row, with the bias; whole: all lie inside and vectors may be written.
-template <int N>
-__device__ __forceinline__ void store_out(const Fp8Params &p, int64_t row, int64_t col, float (&v)[N]) {
+// Four results of columns col .. of a row, with the bias.
+__device__ __forceinline__ void store_out(const Fp8Params &p, int64_t row, int64_t col, float (&v)[4]) {
     const int64_t at = row * p.n + col;
     if (p.bias)
 #pragma unroll
-        for (int e = 0; e < N; ++e)
+        for (int e = 0; e < 4; ++e)
             if (col + e < p.n) v[e] += load_dt(p.bias, col + e, p.bias_dtype);
-    if (p.n % N == 0) {  // rows start on the vectors' boundaries; col < n then means col + N <= n
+    if (p.n % 4 == 0) {  // rows start on the vectors' boundaries; col < n then means col + 4 <= n
         if (p.out_dtype == DSALT_DTYPE_F32) {
-#pragma unroll
-            for (int e = 0; e < N; e += 4)
-                reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at)[e / 4] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
-            uint32_t w[N / 2];
-#pragma unroll
-            for (int e = 0; e < N; e += 2)
-                w[e / 2] = p.out_dtype == DSALT_DTYPE_BF16 ? BF16::pack2(v[e], v[e + 1]) : F16::pack2(v[e], v[e + 1]);
-            uint16_t *o = static_cast<uint16_t *>(p.out) + at;
-            if constexpr (N == 8) *reinterpret_cast<uint4 *>(o) = make_uint4(w[0], w[1], w[2], w[3]);
-            else *reinterpret_cast<uint2 *>(o) = make_uint2(w[0], w[1]);
+            const bool bf16 = p.out_dtype == DSALT_DTYPE_BF16;
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) =
+                make_uint2(bf16 ? BF16::pack2(v[0], v[1]) : F16::pack2(v[0], v[1]),
+                           bf16 ? BF16::pack2(v[2], v[3]) : F16::pack2(v[2], v[3]));
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < N; ++e)
+        for (int e = 0; e < 4; ++e)
             if (col + e < p.n) store_dt(p.out, at + e, p.out_dtype, v[e]);
     }
 }
@@ -578,7 +571,7 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const Fp8Params p) {
             const float4 f = *reinterpret_cast<const float4 *>(in);
             v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
         }
-        store_out<4>(p, row, col, v);
+        store_out(p, row, col, v);
     }
 }
 
@@ -687,7 +680,7 @@ __global__ void __launch_bounds__(64 * kRowWaves) fp8_rows_kernel(const Fp8Param
         }
         const int64_t row = q % MF * 16 + (lane & 15), col = n0 + q / MF * 16 + group * 4;
         float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-        if (row < p.m && col < p.n) store_out<4>(p, row, col, v);
+        if (row < p.m && col < p.n) store_out(p, row, col, v);
     }
 }
 
@@ -711,7 +704,7 @@ hipError_t launch_tile(Fp8Params p, hipStream_t stream) {
     return hipGetLastError();
 }
 
-enum { kTile256, kTile128, kTile64 };  // 256 x 256 (x 128 without MX), 128 x 128, 64 x 128
+enum { kTile256, kTile128, kTile64 };  // 256 x 256, 128 x 128, 64 x 128
 struct Plan {
     int tile, splits;
 };
@@ -721,7 +714,10 @@ struct Plan {
 // more workgroups share a CU, once for each round of the card. 512 x 2816 x 1024: 64 x 128 tiles 11.5, 128 x 128
 // 14.8, 256 x 256 33.5; 8192 x 1024 x 5632: 73, 61, 55; 1000 x 4096 x 4096: 24.7, 28, 48. Splits cost a second
 // launch and the traffic of their parts: 64 x 4096 x 4096 14.9, 12.7, 11.7 and 14.2 with 1, 2, 4 and 8.
-Plan plan(int64_t m, int64_t n, int64_t k) {
+// The largest tile is for e8m0 scales only: with fp32 ones a wave's 128 x 64 would need more registers than
+// two waves a SIMD have, and 256 x 128, which fits, was no faster than 128 x 128 anywhere (8192^3: 601
+// against 581; 6473 x 1360 x 1001: 23.3 against 22.3).
+Plan plan(int64_t m, int64_t n, int64_t k, bool mx) {
     struct Tile {
         int bm, bn, per_cu;
         double start, step[3];
@@ -730,7 +726,8 @@ Plan plan(int64_t m, int64_t n, int64_t k) {
     const int kb = (int)((k + kFp8Block - 1) / kFp8Block);
     Plan best = {kTile64, 1};
     double least = 1e30;
-    for (int t : {kTile256, kTile128, kTile64})
+    for (int t : {kTile256, kTile128, kTile64}) {
+        if (t == kTile256 && !mx) continue;
         for (int splits = 1; splits <= (t == kTile64 ? 16 : 1) && splits <= kb; splits *= 2) {
             const Tile &tile = tiles[t];
             const int per = (kb + splits - 1) / splits, used = (kb + per - 1) / per;  // none of them empty
@@ -744,18 +741,15 @@ Plan plan(int64_t m, int64_t n, int64_t k) {
                 best = {t, used};
             }
         }
+    }
     return best;
 }
 
 template <bool MX>
 hipError_t launch_tiles(const Fp8Params &p, int tile, hipStream_t stream) {
-    switch (tile) {
-        case kTile256:  // without MX a wave's 128 x 64 would need more registers than two waves a SIMD have
-            if constexpr (MX) return launch_tile<true, 256, 256, 2, 4>(p, stream);
-            else return launch_tile<false, 256, 128, 4, 2>(p, stream);
-        case kTile128: return launch_tile<MX, 128, 128, 2, 2>(p, stream);
-        default: return launch_tile<MX, 64, 128, 1, 4>(p, stream);
-    }
+    if constexpr (MX)
+        if (tile == kTile256) return launch_tile<true, 256, 256, 2, 4>(p, stream);
+    return tile == kTile128 ? launch_tile<MX, 128, 128, 2, 2>(p, stream) : launch_tile<MX, 64, 128, 1, 4>(p, stream);
 }
 
 template <typename TX, int MF>
@@ -793,8 +787,8 @@ int fp8_few_rows() { return kFewRows; }
 
 int64_t fp8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
     if (m <= kFewRows) return 0;
-    const Plan pl = plan(m, n, k);
-    return pl.splits > 1 ? pl.splits * m * ((n + 7) / 8 * 8) * 4 : 0;
+    const int64_t splits = std::max(plan(m, n, k, true).splits, plan(m, n, k, false).splits);
+    return splits > 1 ? splits * m * ((n + 7) / 8 * 8) * 4 : 0;
 }
 
 hipError_t launch_fp8_quantize(const dsalt_fp8_quantize_args &a, hipStream_t stream) {
@@ -834,7 +828,6 @@ hipError_t launch_fp8_matmul(const dsalt_fp8_matmul_args &a, hipStream_t stream)
     p.bias_dtype = a.bias_dtype;
     p.out = a.out;
     p.out_dtype = a.out_dtype;
-    p.a_dtype = a.a_dtype;
     if (a.m <= kFewRows) {
         if (a.a_dtype == DSALT_DTYPE_E4M3) launch_few_rows<void>(p, stream);
         else if (a.a_dtype == DSALT_DTYPE_BF16) launch_few_rows<BF16>(p, stream);
@@ -842,12 +835,13 @@ hipError_t launch_fp8_matmul(const dsalt_fp8_matmul_args &a, hipStream_t stream)
         else launch_few_rows<F32>(p, stream);
         return hipGetLastError();
     }
-    const Plan pl = plan(a.m, a.n, a.k);
+    const bool mx = p.sa.e8m0 && p.sb.e8m0;
+    const Plan pl = plan(a.m, a.n, a.k, mx);
     p.splits = pl.splits;
     p.per_split = (p.kb + pl.splits - 1) / pl.splits;
     p.part_ld = (p.n + 7) / 8 * 8;
     p.part = static_cast<float *>(a.workspace);
-    const hipError_t e = p.sa.e8m0 && p.sb.e8m0 ? launch_tiles<true>(p, pl.tile, stream) : launch_tiles<false>(p, pl.tile, stream);
+    const hipError_t e = mx ? launch_tiles<true>(p, pl.tile, stream) : launch_tiles<false>(p, pl.tile, stream);
     if (e != hipSuccess || p.splits == 1) return e;
     const int64_t items = p.m * ((p.n + 3) / 4);
     hipLaunchKernelGGL(fp8_join_kernel, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 4096)), dim3(256), 0, stream, p);
