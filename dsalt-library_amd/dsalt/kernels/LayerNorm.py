@@ -9,7 +9,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import _hip
-from ._block_train import eager, graph_grads, without_autocast
+from ._block_train import eager, graph_grads, keep, kept, without_autocast
 from .dsalt_triton_attn import _dynamo_opaque
 
 
@@ -32,14 +32,14 @@ class _LayerNorm(torch.autograd.Function):
         x_out, y, stats = _hip.layer_norm(*_operands(x, h, weight, bias), eps, out_dtype, True)
         # an fp32 sum is what the backward normalises; a 16-bit one has lost bits of it
         whole = h is not None and x.dtype is torch.float32
-        ctx.save_for_backward(x_out if whole else x, None if whole else h, weight, bias, stats)
+        keep(ctx, x_out if whole else x, None if whole else h, weight, bias, stats)
         ctx.dsalt = h is not None, whole, None if h is None else h.dtype, eps, out_dtype
         return y if h is None else (x_out, y)
 
     @staticmethod
     @without_autocast
     def backward(ctx, *grads):
-        x, h, weight, bias, stats = ctx.saved_tensors
+        x, h, weight, bias, stats = kept(ctx)
         add, whole, h_dtype, eps, out_dtype = ctx.dsalt
         dx_out, dy = grads if add else (None, *grads)
         need_x, need_h, need_w, need_b = ctx.needs_input_grad[:4]

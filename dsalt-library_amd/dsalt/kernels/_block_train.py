@@ -61,6 +61,18 @@ def without_autocast(backward):
     return call
 
 
+def keep(ctx, *ts) -> None:
+    """``ctx.save_for_backward``, which refuses inference tensors (a teacher's answers, frozen weights):
+    those count no versions that it could check, and stay on ctx as they are."""
+    ctx.dsalt_frozen = frozen = tuple(t if t is not None and t.is_inference() else None for t in ts)
+    ctx.save_for_backward(*(t if f is None else None for t, f in zip(ts, frozen)))
+
+
+def kept(ctx) -> tuple:
+    """The tensors of ``keep``."""
+    return tuple(t if f is None else f for t, f in zip(ctx.saved_tensors, ctx.dsalt_frozen))
+
+
 def graph_grads(fn, inputs, dys):
     """Differentiable gradients of fn(*inputs), with the upstream gradients dys of its outputs (None:
     none), with respect to the inputs that require one (else None). fn sees aliases of the

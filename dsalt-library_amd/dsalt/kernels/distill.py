@@ -7,7 +7,7 @@ from __future__ import annotations
 import torch
 
 from .. import _hip
-from ._block_train import eager, graph_grads, without_autocast
+from ._block_train import eager, graph_grads, keep, kept, without_autocast
 from .dsalt_triton_attn import _dynamo_opaque
 
 
@@ -40,14 +40,14 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher, ids, labels, opts):
         loss, stats = _hip.distill(logits, teacher, ids, labels, opts, True)
-        ctx.save_for_backward(logits, teacher, ids, labels, stats)
+        keep(ctx, logits, teacher, ids, labels, stats)
         ctx.dsalt = opts
         return loss
 
     @staticmethod
     @without_autocast
     def backward(ctx, d_loss):
-        logits, teacher, ids, labels, stats = ctx.saved_tensors
+        logits, teacher, ids, labels, stats = kept(ctx)
         if torch.is_grad_enabled():  # a graph of the backward is wanted: torch's own ops
             d, = graph_grads(lambda s: (torch_distill_loss(s, teacher, ids, labels, ctx.dsalt),), (logits,), (d_loss,))
             return d, None, None, None, None

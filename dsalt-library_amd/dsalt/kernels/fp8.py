@@ -126,7 +126,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``fp8_matmul(*fp8_quantize(x), weight, weight_scale, bias)`` of x [..., k] in bf16, fp16 or fp32, in
     ``out_dtype`` (by default x's); up to 32 rows are quantised by the product's kernel as it reads
-    them, to the same bits. weight [n, k] and its scales as ``fp8_matmul`` takes b. For inference: x or a bias that
+    them, to the same 8-bit values. weight [n, k] and its scales as ``fp8_matmul`` takes b. For inference: x or a bias that
     requires a gradient is refused where gradients are recorded."""
     dev, k = x.device, x.shape[-1] if x.dim() else 0
     out_dtype = x.dtype if out_dtype is None else out_dtype
