@@ -64,13 +64,17 @@ def without_autocast(backward):
 def keep(ctx, *ts) -> None:
     """``ctx.save_for_backward``, which refuses inference tensors (a teacher's answers, frozen weights):
     those count no versions that it could check, and stay on ctx as they are."""
-    ctx.dsalt_frozen = frozen = tuple(t if t is not None and t.is_inference() else None for t in ts)
-    ctx.save_for_backward(*(t if f is None else None for t, f in zip(ts, frozen)))
+    ctx.dsalt_frozen = None
+    if any(t is not None and t.is_inference() for t in ts):
+        ctx.dsalt_frozen = frozen = tuple(t if t is not None and t.is_inference() else None for t in ts)
+        ts = (t if f is None else None for t, f in zip(ts, frozen))
+    ctx.save_for_backward(*ts)
 
 
 def kept(ctx) -> tuple:
     """The tensors of ``keep``."""
-    return tuple(t if f is None else f for t, f in zip(ctx.saved_tensors, ctx.dsalt_frozen))
+    ts = ctx.saved_tensors
+    return ts if ctx.dsalt_frozen is None else tuple(t if f is None else f for t, f in zip(ts, ctx.dsalt_frozen))
 
 
 def graph_grads(fn, inputs, dys):
