@@ -16,7 +16,7 @@
 // before a loss scale is known, which in fp16 loses most of a vocabulary's small probabilities).
 //
 // Rows of up to 4096 logits take one wave, longer ones four; few long rows are cut into slices whose
-// sums a second kernel joins. Long rows are bound by HBM bytes: 6473 x 32000 bf16 at tau = 2 with labels,
+// sums a second kernel joins, but for a lone one, which sixteen waves take. Long rows are bound by HBM bytes: 6473 x 32000 bf16 at tau = 2 with labels,
 // 85 us forward (4.9 TB/s; 126 right behind a backward, whose gradients still drain) and 155-199 us
 // backward (5.3-4.2 TB/s: what the forward left in the last-level cache counts); fp32 144 and 377 us. A
 // loop that loaded a run only behind the last one's sums took 124 us. Short rows are bound by what a row
@@ -34,6 +34,9 @@ constexpr int kStats = 5;         // of a row: m, 1 / sum at tau, 1 / sum at 1, 
 // Logits of a row that one wave takes. One wave and four, in us: 16384 x 2100 bf16 36 and 56 forward, 50 and 61
 // backward; 16384 x 4000 47 and 62, 77 and 77; 8000 x 8000 39 and 39, 69 and 61.
 constexpr int kRowMax = 4096;
+// Logits of a lone row that one workgroup of 16 waves takes and ends by itself, with its reduction; beyond, slices and
+// their join. us of each: 5000 bf16 4.2 and 6.5, 32000 5.8 and 6.7, 50257 6.2 and 6.6, 100003 8.2 and 6.9.
+constexpr int kLoneMax = 65536;
 constexpr int kSlice = 2048;      // least logits of a slice
 constexpr int kSliceGroups = 1024;  // workgroups that slices are made for
 
@@ -46,6 +49,7 @@ struct DistillParams {
     float *row_loss, *stats;
     float *loss;                  // of a reduction
     int mean, reduce;
+    int lone;  // the reduction of one row, which is its loss
     const float *d_loss;
     void *d_logits;
     float grad_w;  // (1 - lam) tau
@@ -239,6 +243,7 @@ __device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, 
         loss += p.lam * (log2f(s1) - ref.template label<KIND>(end.at_label, p.c)) * kLn2;
     p.row_loss[row] = label < 0 ? 0.f : loss;
     if (p.stats) {
+        if (p.lone) p.stats[kStats] = 1.f;
         float *st = p.stats + row * kStats;
         st[0] = ref.m;
         st[1] = 1.f / run.s;
@@ -270,15 +275,15 @@ __device__ __forceinline__ void slice_of(const DistillParams &p, int split, int 
     last = min(first + per, p.vocab);
 }
 
-// NW waves a row (or slice), 256 threads a workgroup.
+// NW waves a row (or slice), of a workgroup of at least four.
 template <typename DT, int KIND, int NW>
-__global__ void __launch_bounds__(256) distill_rows_kernel(const DistillParams p) {
-    constexpr int VE = Vec<DT>::N, NT = NW * 64, U = 32 / VE;
+__global__ void __launch_bounds__(NW > 4 ? NW * 64 : 256) distill_rows_kernel(const DistillParams p) {
+    constexpr int VE = Vec<DT>::N, NT = NW * 64, U = NW > 4 ? 4 : 32 / VE;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * (4 / NW) + (NW == 1 ? wave : 0);
+    const int64_t item = NW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
     const int64_t row = item / p.splits;
     const int split = (int)(item - row * p.splits);
-    if (row >= p.rows) return;  // a whole wave (NW = 1); never with NW = 4
+    if (row >= p.rows) return;  // a whole wave (NW = 1); never with more
     const int t = NW == 1 ? lane : threadIdx.x;
     const char *base = static_cast<const char *>(p.logits) + row * p.logits_stride * elem_size<DT>();
     int first, last;
@@ -333,8 +338,12 @@ __global__ void __launch_bounds__(256) distill_rows_kernel(const DistillParams p
         __syncthreads();
         if (wave) return;
         run = Running<KIND>();
-#pragma unroll
-        for (int w = 0; w < NW; ++w) run.join(lds[w][0], lds[w][1], lds[w][2], p.c);
+        if (lane < NW) {
+            run.m = lds[lane][0];
+            run.s = lds[lane][1];
+            run.s1 = lds[lane][2];
+        }
+        run.join_wave(p.c);
     }
     if (p.splits == 1) return finish_row<DT, KIND>(p, row, run, end, lane);
     if (lane == 0) {
@@ -508,13 +517,13 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p)
     }
 }
 
-int distill_splits(int64_t rows, int vocab) {
-    if (vocab <= kRowMax || rows <= 0) return 1;
+int distill_splits(int64_t rows, int vocab, bool bwd) {
+    if (vocab <= kRowMax || rows <= 0 || (rows == 1 && !bwd && vocab <= kLoneMax)) return 1;
     const int64_t most = (vocab + kSlice - 1) / kSlice;
     return (int)std::max<int64_t>(1, std::min<int64_t>(most, kSliceGroups / rows));
 }
 
-DistillParams params(const dsalt_distill_args &a) {
+DistillParams params(const dsalt_distill_args &a, bool bwd) {
     DistillParams p = {};
     p.logits = a.logits;
     p.teacher = a.teacher;
@@ -530,7 +539,7 @@ DistillParams params(const dsalt_distill_args &a) {
     p.teacher_dtype = a.teacher_dtype;
     p.ids64 = a.ids_int64;
     p.labels64 = a.labels_int64;
-    p.splits = distill_splits(a.rows, a.vocab);
+    p.splits = distill_splits(a.rows, a.vocab, bwd);
     const bool only_labels = a.label_weight == 1.f;  // then everything is at temperature 1
     p.inv_tau = only_labels ? 1.f : (float)(1.0 / (double)a.temperature);
     p.c = only_labels ? kLog2e : (float)(1.4426950408889634 / (double)a.temperature);
@@ -541,7 +550,8 @@ DistillParams params(const dsalt_distill_args &a) {
     p.loss = a.loss;
     p.reduce = a.reduction != DSALT_REDUCE_NONE;
     p.mean = a.reduction == DSALT_REDUCE_MEAN;
-    p.row_loss = p.reduce ? static_cast<float *>(a.workspace) : a.loss;
+    p.lone = a.rows == 1 && p.splits == 1 && p.reduce;
+    p.row_loss = p.reduce && !p.lone ? static_cast<float *>(a.workspace) : a.loss;
     p.part = static_cast<float *>(a.workspace) + (p.reduce ? a.rows : 0);
     p.d_loss = a.d_loss;
     p.d_logits = a.d_logits;
@@ -559,15 +569,16 @@ void launch_types(const DistillParams &p, bool bwd, hipStream_t stream) {
         return;
     }
     if (one_wave) hipLaunchKernelGGL((distill_rows_kernel<DT, KIND, 1>), grid, block, 0, stream, p);
+    else if (p.rows == 1 && p.splits == 1) hipLaunchKernelGGL((distill_rows_kernel<DT, KIND, 16>), grid, dim3(1024), 0, stream, p);
     else hipLaunchKernelGGL((distill_rows_kernel<DT, KIND, 4>), grid, block, 0, stream, p);
     const unsigned joins = (unsigned)((p.rows + 15) / 16);
     if (p.splits > 1) hipLaunchKernelGGL((distill_join_kernel<DT, KIND>), dim3(joins), dim3(1024), 0, stream, p);
-    if (p.reduce && !(p.splits > 1 && joins == 1))
+    if (p.reduce && !p.lone && !(p.splits > 1 && joins == 1))
         hipLaunchKernelGGL(distill_reduce_kernel, dim3(1), dim3(1024), 0, stream, p);
 }
 
 hipError_t launch(const dsalt_distill_args &a, bool bwd, hipStream_t stream) {
-    const DistillParams p = params(a);
+    const DistillParams p = params(a, bwd);
     if (a.rows == 0) {
         if (!bwd && p.reduce) hipLaunchKernelGGL(distill_reduce_kernel, dim3(1), dim3(1024), 0, stream, p);
         return hipGetLastError();
@@ -587,8 +598,8 @@ hipError_t launch(const dsalt_distill_args &a, bool bwd, hipStream_t stream) {
 }  // namespace
 
 int64_t distill_workspace_bytes(int64_t rows, int vocab) {
-    const int splits = distill_splits(rows, vocab);
-    return rows * 4 * (1 + (splits > 1 ? 3 * splits : 0));
+    const int splits = distill_splits(rows, vocab, false);
+    return rows == 1 && splits == 1 ? 0 : rows * 4 * (1 + (splits > 1 ? 3 * splits : 0));
 }
 int64_t distill_stats_count(int64_t rows) { return rows * kStats + 1; }
 hipError_t launch_distill(const dsalt_distill_args &a, hipStream_t stream) { return launch(a, false, stream); }

@@ -323,3 +323,35 @@ def test_rows_of_the_lowest_value(V):
     s, z, ids, y = inputs((4,), V, 4, FP, holes=False)
     s[:] = torch.finfo(FP).min
     compare(s, z, ids, y, tau=2.0, lam=0.5)
+
+
+@pytest.mark.parametrize("V", [1, 100, 4096, 4097, 8200, 32000, 65536, 65537, 70001])
+@pytest.mark.parametrize("tau,lam", [(1.0, 0.0), (2.0, 0.5), (3.0, 0.5), (1.0, 1.0)])
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_lone_row(V, tau, lam, dtype):
+    """One row, which one workgroup ends, or slices do: every reduction, a row that starts off 16 bytes."""
+    s, z, ids, y = inputs((1,), V, 66, dtype)
+    for reduction in ("mean", "sum", "none"):
+        up = torch.tensor([1.7] if reduction == "none" else 1.7, device=DEV)
+        compare(s, z, ids, y, tau=tau, lam=lam, reduction=reduction, up=up)
+    wide = torch.zeros(1, V + 3, device=DEV, dtype=dtype)
+    wide[:, 3:] = s
+    want = distill_loss(s, z, ids, y, temperature=tau, label_weight=lam)
+    got = distill_loss(wide[:, 3:], z, ids, y, temperature=tau, label_weight=lam)
+    # the same terms in another order: 2^-16 of a log of up to 60, as above
+    assert abs(got - want) <= 2.0 ** -16 * 60 * max(tau * tau, 1.0)
+
+
+@pytest.mark.parametrize("V", [100, 32000, 70001])
+def test_lone_row_that_does_not_count(V):
+    s, z, ids, y = inputs((1,), V, 5)
+    for labels in (torch.full_like(y, -100), torch.full_like(y, V)):
+        loss, g = compare(s, z, ids, labels, tau=2.0, lam=0.5)
+        assert loss == 0 and not g.any()
+    loss, g = compare(s, z, torch.full_like(ids, -1), None)
+    assert loss == 0 and not g.any()
+    s[0, 3] = float("nan")
+    leaf = s.detach().requires_grad_()
+    loss = distill_loss(leaf, z, ids, y, label_weight=0.5)
+    g, = torch.autograd.grad(loss, leaf)
+    assert loss.isnan() and g.isnan().all()
