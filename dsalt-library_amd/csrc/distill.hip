@@ -8,9 +8,10 @@
 // the others.
 //
 // The forward reads the logits once with running maxima and sums: exponents are fma(s, c, -m c), c =
-// log2(e) / tau, in the forward and in the backward, so that whatever m c was rounded to drops out of
-// every quotient; where m c overflows (a mask of the type's lowest value that leaves nothing) they are
-// (s - m) c. At tau = 2 the exponential at 1 is the square of that at tau. It keeps m and the sums'
+// log2(e) / tau, in the forward and in the backward. What the rounding of m c left is the exponent at s = m; sums that
+// go on to another maximum leave theirs behind, and it drops out of every quotient. From |m c| = 2^16 on (a
+// mask that leaves nothing: the residue is 2^-24 of m c, and of a mask of -1e10 its power is no longer finite)
+// exponents are (s - m) c. At tau = 2 the exponential at 1 is the square of that at tau. It keeps m and the sums'
 // inverses of each row, and the backward reads the logits once more and writes the gradient, each rounded
 // once from fp32 under the upstream gradient that it is given (formed in the forward it would be rounded
 // before a loss scale is known, which in fp16 loses most of a vocabulary's small probabilities).
@@ -94,12 +95,21 @@ enum { kOne = 0, kTwo = 1, kSquare = 2 };
 // A maximum as a reference for exp2 (of nothing but -inf any finite one will do), and exponents against it.
 struct Reference {
     float m, mc, mc1;
-    bool far;  // m c overflows
+    bool far;  // m c is too large for its residue
     __device__ __forceinline__ Reference(float max, float c) : m(max == -INFINITY ? 0.f : max), mc(m * c), mc1(m * kLog2e) {
-        far = !(fmaxf(fabsf(mc), fabsf(mc1)) < INFINITY);
+        far = !(fmaxf(fabsf(mc), fabsf(mc1)) < 65536.f);
     }
     __device__ __forceinline__ float at(float v, float c) const { return far ? (v - m) * c : fmaf(v, c, -mc); }
     __device__ __forceinline__ float at1(float v) const { return far ? (v - m) * kLog2e : fmaf(v, kLog2e, -mc1); }
+    // the exponents that take sums against the maximum `max` to this reference
+    __device__ __forceinline__ float from(float max, float c) const {
+        const Reference o(max, c);
+        return at(max, c) - o.at(o.m, c);
+    }
+    __device__ __forceinline__ float from1(float max, float c) const {
+        const Reference o(max, c);
+        return at1(max) - o.at1(o.m);
+    }
     // the exponent at temperature 1
     template <int KIND>
     __device__ __forceinline__ float label(float v, float c) const {
@@ -113,9 +123,9 @@ struct Running {
     float m = -INFINITY, s = 0.f, s1 = 0.f;
     __device__ __forceinline__ void rescale(float mn, float c) {
         const Reference r(mn, c);
-        const float t = fast_exp2(r.at(m, c));
+        const float t = fast_exp2(r.from(m, c));
         s *= t;
-        if (KIND == kTwo) s1 *= fast_exp2(r.at1(m));
+        if (KIND == kTwo) s1 *= fast_exp2(r.from1(m, c));
         if (KIND == kSquare) s1 *= t * t;
         m = mn;
     }
@@ -151,9 +161,9 @@ struct Running {
     __device__ __forceinline__ void join(float m2, float t, float t1, float c) {
         rescale(__builtin_elementwise_maximum(m, m2), c);
         const Reference r(m, c);
-        const float x = fast_exp2(r.at(m2, c));
+        const float x = fast_exp2(r.from(m2, c));
         s += t * x;
-        if (KIND == kTwo) s1 += t1 * fast_exp2(r.at1(m2));
+        if (KIND == kTwo) s1 += t1 * fast_exp2(r.from1(m2, c));
         if (KIND == kSquare) s1 += t1 * (x * x);
     }
     __device__ __forceinline__ void join_wave(float c) {
