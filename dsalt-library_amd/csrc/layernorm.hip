@@ -125,7 +125,8 @@ __global__ void __launch_bounds__(RowShape<WPR>::THREADS) layer_fwd_kernel(const
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[0] += z[e];
         row_sum(s, 1);
-        const float mean = s[0] * p.inv_d;
+        float mean = s[0] * p.inv_d;
+        asm volatile("" : "+v"(mean));  // the rounded one, as the backward has it: not z - s inv_d in one step
         s[0] = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
