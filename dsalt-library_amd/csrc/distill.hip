@@ -182,7 +182,7 @@ __device__ __forceinline__ int row_label(const DistillParams &p, int64_t row) {
     const int64_t l = load_int(p.labels, row, p.labels64);
     return l == p.ignore_index || l < 0 || l >= p.vocab ? -1 : (int)l;
 }
-// Slot k's logit over tau, -inf where the slot does not count, and its id.
+// Slot k's logit, -inf where the slot does not count, and its id.
 __device__ __forceinline__ float slot(const DistillParams &p, int64_t row, int k, int &id) {
     const int64_t i = load_int(p.ids, row * p.ids_stride + k, p.ids64);
     id = i >= 0 && i < p.vocab ? (int)i : -1;
@@ -192,14 +192,14 @@ __device__ __forceinline__ float slot(const DistillParams &p, int64_t row, int k
                     : p.teacher_dtype == DSALT_DTYPE_BF16 ? Elem<BF16>::ld(p.teacher, at)
                                                           : Elem<F16>::ld(p.teacher, at);
     if (z == -INFINITY) id = -1;
-    return z * p.inv_tau;
+    return z;
 }
 
 // What a row's end needs of memory, read before the row itself: its label, and the lane's first slot.
 template <typename DT>
 struct RowEnd {
     int label, id = -1;
-    float t = -INFINITY, at_id = 0.f, at_label = 0.f;  // the slot's logit over tau; the student's at the id and at the label
+    float t = -INFINITY, at_id = 0.f, at_label = 0.f;  // the slot's logit; the student's at the id and at the label
     __device__ __forceinline__ RowEnd(const DistillParams &p, int64_t row, int lane, bool ends = true) : label(ends ? row_label(p, row) : -1) {
         const char *logits = static_cast<const char *>(p.logits) + row * p.logits_stride * elem_size<DT>();
         if (label < 0) return;
@@ -224,18 +224,20 @@ __device__ __forceinline__ void finish_row(const DistillParams &p, int64_t row, 
         for (int k = 64 + lane; k < p.k; k += 64) tm = fmaxf(tm, slot(p, row, k, id));
         tm = wave_maxf(tm);
         if (tm == -INFINITY) tm = 0.f;
+        // over tau behind the difference: over a tau below 1 the type's lowest value has no finite quotient
+        const auto exponent = [&](float t) { return (t - tm) * p.inv_tau; };
         bool any = end.id >= 0;
-        ts = end.id >= 0 ? expf(end.t - tm) : 0.f;
+        ts = end.id >= 0 ? expf(exponent(end.t)) : 0.f;
         for (int k = 64 + lane; k < p.k; k += 64) {
             const float t = slot(p, row, k, id);
             any |= id >= 0;
-            ts += id >= 0 ? expf(t - tm) : 0.f;
+            ts += id >= 0 ? expf(exponent(t)) : 0.f;
         }
         ts = group_sum_lanes(ts, 64);
         if (__ballot(any)) {
             const float lt = logf(ts), ls = log2f(run.s);
             const auto term = [&](float t, float v) {
-                const float lp = (t - tm) - lt, w = expf(t - tm) / ts;
+                const float lp = exponent(t) - lt, w = expf(exponent(t)) / ts;
                 const float lq = (ref.at(v, p.c) - ls) * kLn2;
                 return w != 0.f ? w * (lp - lq) : 0.f;
             };
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const DistillParams p)
                 int i = id0;
                 const float z = k == t ? z0 : slot(p, row, k, i);
                 id[k] = i;
-                w[k] = i >= 0 ? expf(z - st[3]) * st[4] : 0.f;
+                w[k] = i >= 0 ? expf((z - st[3]) * p.inv_tau) * st[4] : 0.f;
             }
     }
     const Reference ref(m, p.c);

@@ -20,6 +20,7 @@ def torch_distill_loss(logits, teacher, ids, labels, opts):
     on = (ids >= 0) & (ids < vocab) & (z != float("-inf"))
     at = torch.where(on, ids, 0).long()
     low = torch.finfo(s.dtype).min
+    z = z - torch.where(on, z, low).amax(-1, keepdim=True)  # first: the lowest value has no finite quotient by less than 1
     log_p = torch.log_softmax(torch.where(on, z / temperature, low), -1)
     p = torch.where(on, log_p.exp(), 0.0)  # of a row without slots, too
     log_q = torch.log_softmax(s / temperature, -1).gather(-1, at)
