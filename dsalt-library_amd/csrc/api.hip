@@ -864,8 +864,8 @@ int dsalt_distill_check(const dsalt_distill_args *a, int32_t backward) {
         return fail(DSALT_ERR_INVALID, "logits dtype %d or teacher dtype %d is not a float dtype", a->logits_dtype, a->teacher_dtype);
     if (a->reduction < DSALT_REDUCE_NONE || a->reduction > DSALT_REDUCE_SUM)
         return fail(DSALT_ERR_INVALID, "reduction must be DSALT_REDUCE_* (got %d)", a->reduction);
-    if (!(a->temperature > 0.f) || !(a->temperature < INFINITY))
-        return fail(DSALT_ERR_INVALID, "temperature must be positive and finite (got %g)", (double)a->temperature);
+    if (!(a->temperature >= 0x1p-63f) || !(a->temperature < 0x1p63f))  // its inverse and its square in fp32
+        return fail(DSALT_ERR_INVALID, "temperature must be in [2^-63, 2^63) (got %g)", (double)a->temperature);
     if (!(a->label_weight >= 0.f && a->label_weight <= 1.f))
         return fail(DSALT_ERR_INVALID, "label_weight must be in [0, 1] (got %g)", (double)a->label_weight);
     if (a->label_weight > 0.f && !a->labels && a->rows > 0) return fail(DSALT_ERR_INVALID, "label_weight needs labels");

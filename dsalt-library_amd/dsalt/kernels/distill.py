@@ -73,15 +73,15 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids
     repeats takes the sum of its slots.
 
     logits and teacher_logits bf16, fp16 or fp32; teacher_ids and labels int32 or int64; V up to 2^30, K up
-    to 1024; rows of any stride. Sums are fp32, the gradient is rounded once, and its sums have a fixed
+    to 1024; rows of any stride; temperature in [2^-63, 2^63). Sums are fp32, the gradient is rounded once, and its sums have a fixed
     order. Differentiable in logits alone: no gradient goes to the teacher. Functorch's transforms,
     forward-mode differentiation, tracing and tensor subclasses take torch's ops instead. Other operands
     raise ``DsaltError``."""
     if reduction not in _hip.REDUCTIONS:
         raise ValueError(f"reduction must be one of {list(_hip.REDUCTIONS)}, got {reduction!r}")
     temperature, label_weight = float(temperature), float(label_weight)
-    if not 0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive and finite (got {temperature})")
+    if not 2.0 ** -63 <= temperature < 2.0 ** 63:  # its inverse and its square in fp32
+        raise ValueError(f"temperature must be in [2^-63, 2^63) (got {temperature})")
     if not 0 <= label_weight <= 1:
         raise ValueError(f"label_weight must be in [0, 1] (got {label_weight})")
     if label_weight > 0 and labels is None:

@@ -765,7 +765,7 @@ size_t dsalt_layer_norm_args_size(void);
  * order, one rounding per gradient.
  * logits and teacher BF16, F16 or F32, unit strides along their rows, row strides (in elements) of at
  * least the row length; ids and labels int32, or int64 where ids_int64 / labels_int64. vocab in
- * [1, 2^30], k in [1, 1024]; temperature > 0; label_weight in [0, 1], 0 without labels. Pointers
+ * [1, 2^30], k in [1, 1024]; temperature in [2^-63, 2^63); label_weight in [0, 1], 0 without labels. Pointers
  * aligned to their elements. workspace (forward only): dsalt_distill_workspace_size bytes, dead when
  * the launches end. d_logits aliases no input.
  */

@@ -1,8 +1,11 @@
 """The distillation loss on the CPU: its torch form at the edges, and the LM's use of it."""
+import ctypes
+
 import pytest
 import torch
 
-from dsalt import DsaltError
+import dsalt._hip as hip
+from dsalt.kernels import distill_loss
 from dsalt.kernels.distill import torch_distill_loss
 
 
@@ -21,3 +24,18 @@ def test_teacher_of_lowest_values(tau):
     got = torch_distill_loss(s, z, ids, None, (tau, 0.0, -100, "none"))
     want = torch_distill_loss(s.double(), z.double(), ids, None, (tau, 0.0, -100, "none"))
     torch.testing.assert_close(got.double(), want, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("tau", [1e-39, 2.0 ** -64, 2.0 ** 63, 1e20, 1e39])
+def test_temperatures_past_fp32(tau):
+    """A temperature whose inverse or square fp32 does not hold is refused (the first term would be NaN)."""
+    s, z, ids, _ = operands()
+    with pytest.raises(ValueError, match="temperature"):
+        distill_loss(s, z, ids, temperature=tau)
+    args = hip.DistillArgs(rows=4, logits_stride=100, teacher_stride=8, ids_stride=8, ignore_index=-100, vocab=100, k=8, teacher_dtype=2,
+                           reduction=1, temperature=2.0, workspace_bytes=1 << 30)
+    for i, n in enumerate(("logits", "teacher", "ids", "loss", "workspace")):
+        setattr(args, n, 0x10000000 + i * 0x100000)
+    for t, code in ((tau, 1), (2.0 ** -63, 0), (2.0 ** 62, 0)):
+        args.temperature = t
+        assert hip.lib().dsalt_distill_check(ctypes.byref(args), 0) == code
