@@ -17,6 +17,10 @@ def torch_distill_loss(logits, teacher, ids, labels, opts):
     s = logits.float() if logits.dtype in (torch.bfloat16, torch.float16) else logits
     vocab = s.shape[-1]
     z = teacher.to(s.dtype)
+    counted = None
+    if labels is not None:
+        counted = (labels != ignore_index) & (labels >= 0) & (labels < vocab)
+        s, z = (torch.where(counted.unsqueeze(-1), t, 0.0) for t in (s, z))  # no gradient through what such rows hold
     on = (ids >= 0) & (ids < vocab) & (z != float("-inf"))
     at = torch.where(on, ids, 0).long()
     low = torch.finfo(s.dtype).min
@@ -26,14 +30,13 @@ def torch_distill_loss(logits, teacher, ids, labels, opts):
     log_q = torch.log_softmax(s / temperature, -1).gather(-1, at)
     rows = (1 - label_weight) * temperature ** 2 * torch.where(p > 0, p * (log_p - log_q), torch.where(on, p, 0.0)).sum(-1)
     if labels is not None:
-        on = (labels != ignore_index) & (labels >= 0) & (labels < vocab)
         if label_weight:
-            at = torch.where(on, labels, 0).long().unsqueeze(-1)
+            at = torch.where(counted, labels, 0).long().unsqueeze(-1)
             rows = rows - label_weight * torch.log_softmax(s, -1).gather(-1, at).squeeze(-1)
-        rows = torch.where(on, rows, 0.0)
+        rows = torch.where(counted, rows, 0.0)
     if reduction == "none":
         return rows
-    n = 1 if reduction == "sum" else max(rows.numel(), 1) if labels is None else on.sum().clamp(min=1)
+    n = 1 if reduction == "sum" else max(rows.numel(), 1) if labels is None else counted.sum().clamp(min=1)
     return rows.sum() / n
 
 

@@ -39,3 +39,20 @@ def test_temperatures_past_fp32(tau):
     for t, code in ((tau, 1), (2.0 ** -63, 0), (2.0 ** 62, 0)):
         args.temperature = t
         assert hip.lib().dsalt_distill_check(ctypes.byref(args), 0) == code
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_rows_that_do_not_count_have_no_gradient(bad):
+    """Whatever they hold, in the loss, its gradient and a graph of the gradient."""
+    s, z, ids, y = operands()
+    y[1], y[3] = -100, 11
+    want, = torch.autograd.grad(torch_distill_loss(s, z, ids, y, (2.0, 0.5, -100, "mean")), s)
+    rows = s.detach().clone()
+    rows[1, 4], rows[3] = bad, bad
+    z[3, 0] = bad
+    leaf = rows.requires_grad_()
+    loss = torch_distill_loss(leaf, z, ids, y, (2.0, 0.5, -100, "mean"))
+    got, = torch.autograd.grad(loss, leaf, create_graph=True)
+    assert bool(torch.isfinite(loss)) and torch.equal(got, want) and not got[1].any() and not got[3].any()
+    second, = torch.autograd.grad(got.square().sum(), leaf)
+    assert bool(torch.isfinite(second).all())
