@@ -56,3 +56,16 @@ def test_rows_that_do_not_count_have_no_gradient(bad):
     assert bool(torch.isfinite(loss)) and torch.equal(got, want) and not got[1].any() and not got[3].any()
     second, = torch.autograd.grad(got.square().sum(), leaf)
     assert bool(torch.isfinite(second).all())
+
+
+def test_labels_alone():
+    """label_weight 1: the cross-entropy, also where the student cannot say what the teacher does."""
+    s, z, ids, y = operands()
+    ids[:, 0] = (y + 1) % 11
+    rows = s.detach().clone()
+    rows[torch.arange(5), ids[:, 0]] = float("-inf")
+    leaf = rows.requires_grad_()
+    got = torch_distill_loss(leaf, z, ids, y, (2.0, 1.0, -100, "mean"))
+    want = torch.nn.functional.cross_entropy(leaf, y)
+    torch.testing.assert_close(got, want)
+    torch.testing.assert_close(*(torch.autograd.grad(t, leaf)[0] for t in (got, want)))
