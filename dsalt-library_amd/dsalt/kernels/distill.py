@@ -27,7 +27,7 @@ def torch_distill_loss(logits, teacher, ids, labels, opts):
     z = z - torch.where(on, z, low).amax(-1, keepdim=True)  # first: the lowest value has no finite quotient by less than 1
     log_p = torch.log_softmax(torch.where(on, z / temperature, low), -1)
     p = torch.where(on, log_p.exp(), 0.0)  # of a row without slots, too
-    log_q = torch.log_softmax(s / temperature, -1).gather(-1, at)
+    log_q = torch.log_softmax((s - s.detach().amax(-1, keepdim=True)) / temperature, -1).gather(-1, at)
     rows = torch.where(p > 0, p * (log_p - log_q), torch.where(on, p, 0.0)).sum(-1) * ((1 - label_weight) * temperature ** 2)
     if label_weight == 1:  # the teacher's term, which may be infinite, is not there
         rows = torch.zeros_like(rows)

@@ -69,3 +69,17 @@ def test_labels_alone():
     want = torch.nn.functional.cross_entropy(leaf, y)
     torch.testing.assert_close(got, want)
     torch.testing.assert_close(*(torch.autograd.grad(t, leaf)[0] for t in (got, want)))
+
+
+@pytest.mark.parametrize("mask", [-1e30, torch.finfo(torch.float32).min])
+def test_student_masks(mask):
+    """A mask that leaves nothing of a row is a uniform softmax, and beside other logits has no share."""
+    s, z, ids, y = operands()
+    rows = s.detach().clone()
+    rows[1], rows[2, 5:] = mask, mask
+    ids, y = ids % 5, y % 5
+    leaf = rows.requires_grad_()
+    opts = (0.25, 0.5, -100, "sum")
+    got, want = (torch_distill_loss(t, z, ids, y, opts) for t in (leaf, leaf.double()))
+    torch.testing.assert_close(got.double(), want)
+    torch.testing.assert_close(*(torch.autograd.grad(t, leaf)[0] for t in (got, want)))
