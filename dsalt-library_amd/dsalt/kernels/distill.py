@@ -42,6 +42,47 @@ def torch_distill_loss(logits, teacher, ids, labels, opts):
     return rows.sum() / n
 
 
+def _options(labels, temperature, label_weight, ignore_index, reduction):
+    """The options as the kernels take them; values outside their ranges are refused."""
+    if reduction not in _hip.REDUCTIONS:
+        raise ValueError(f"reduction must be one of {list(_hip.REDUCTIONS)}, got {reduction!r}")
+    temperature, label_weight = float(temperature), float(label_weight)
+    if not 2.0 ** -63 <= temperature < 2.0 ** 63:  # its inverse and its square in fp32
+        raise ValueError(f"temperature must be in [2^-63, 2^63) (got {temperature})")
+    if not 0 <= label_weight <= 1:
+        raise ValueError(f"label_weight must be in [0, 1] (got {label_weight})")
+    if label_weight > 0 and labels is None:
+        raise ValueError("label_weight needs labels")
+    return temperature, label_weight, int(ignore_index), reduction
+
+
+def _fit(logits, teacher_logits, teacher_ids, labels, dtypes) -> bool:
+    """Whether the operands' shapes, types (of `dtypes`) and devices go together."""
+    dev, lead, ints = logits.device, logits.shape[:-1], (torch.int32, torch.int64)
+    return (logits.dtype in dtypes and teacher_logits.dtype in dtypes
+            and teacher_ids.dtype in ints and logits.dim() >= 1 and 1 <= logits.shape[-1] <= 1 << 30
+            and teacher_logits.shape == teacher_ids.shape and teacher_ids.shape[:-1] == lead and teacher_ids.dim() == logits.dim()
+            and 1 <= teacher_ids.shape[-1] <= _hip.DISTILL_MAX_K and teacher_logits.device == dev and teacher_ids.device == dev
+            and (labels is None or (labels.shape == lead and labels.dtype in ints and labels.device == dev))
+            and lead.numel() < 1 << 24)
+
+
+def _refuse(*operands):
+    raise _hip.DsaltError(
+        f"distill_loss needs bf16, fp16 or fp32 logits [..., V] and teacher_logits [..., K], int32 or int64 teacher_ids "
+        f"[..., K] and labels [...], K up to {_hip.DISTILL_MAX_K} (got "
+        f"{[None if t is None else (tuple(t.shape), t.dtype) for t in operands]})")
+
+
+def cpu_distill_loss(logits, teacher_logits, teacher_ids, labels=None, *, temperature=1.0, label_weight=0.0, ignore_index=-100,
+                     reduction="mean"):
+    """``distill_loss`` of CPU tensors (of float64 too) in torch's ops, with its checks: for the models."""
+    opts = _options(labels, temperature, label_weight, ignore_index, reduction)
+    if not _fit(logits, teacher_logits, teacher_ids, labels, (*_hip._SCORE_DTYPES, torch.float64)):
+        _refuse(logits, teacher_logits, teacher_ids, labels)
+    return torch_distill_loss(logits, teacher_logits.detach(), teacher_ids, labels, opts)
+
+
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher, ids, labels, opts):
@@ -82,29 +123,11 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids
     order. Differentiable in logits alone: no gradient goes to the teacher. Functorch's transforms,
     forward-mode differentiation, tracing and tensor subclasses take torch's ops instead. Other operands
     raise ``DsaltError``."""
-    if reduction not in _hip.REDUCTIONS:
-        raise ValueError(f"reduction must be one of {list(_hip.REDUCTIONS)}, got {reduction!r}")
-    temperature, label_weight = float(temperature), float(label_weight)
-    if not 2.0 ** -63 <= temperature < 2.0 ** 63:  # its inverse and its square in fp32
-        raise ValueError(f"temperature must be in [2^-63, 2^63) (got {temperature})")
-    if not 0 <= label_weight <= 1:
-        raise ValueError(f"label_weight must be in [0, 1] (got {label_weight})")
-    if label_weight > 0 and labels is None:
-        raise ValueError("label_weight needs labels")
-    dev, lead, ints = logits.device, logits.shape[:-1], (torch.int32, torch.int64)
-    ok = (dev.type == "cuda" and logits.dtype in _hip._SCORE_DTYPES and teacher_logits.dtype in _hip._SCORE_DTYPES
-          and teacher_ids.dtype in ints and logits.dim() >= 1 and 1 <= logits.shape[-1] <= 1 << 30
-          and teacher_logits.shape == teacher_ids.shape and teacher_ids.shape[:-1] == lead and teacher_ids.dim() == logits.dim()
-          and 1 <= teacher_ids.shape[-1] <= _hip.DISTILL_MAX_K and teacher_logits.device == dev and teacher_ids.device == dev
-          and (labels is None or (labels.shape == lead and labels.dtype in ints and labels.device == dev))
-          and lead.numel() < 1 << 24)
-    if not ok:
+    opts = _options(labels, temperature, label_weight, ignore_index, reduction)
+    lead = logits.shape[:-1]
+    if not (logits.device.type == "cuda" and _fit(logits, teacher_logits, teacher_ids, labels, _hip._SCORE_DTYPES)):
         _hip.require_gpu(logits, teacher_logits, teacher_ids, labels)
-        raise _hip.DsaltError(
-            f"distill_loss needs bf16, fp16 or fp32 logits [..., V] and teacher_logits [..., K], int32 or int64 teacher_ids "
-            f"[..., K] and labels [...], K up to {_hip.DISTILL_MAX_K} (got "
-            f"{[None if t is None else (tuple(t.shape), t.dtype) for t in (logits, teacher_logits, teacher_ids, labels)]})")
-    opts = (temperature, label_weight, int(ignore_index), reduction)
+        _refuse(logits, teacher_logits, teacher_ids, labels)
     if not eager(*(t for t in (logits, teacher_logits, teacher_ids, labels) if t is not None)):
         return torch_distill_loss(logits, teacher_logits.detach(), teacher_ids, labels, opts)
     rows = _hip.unit_rows

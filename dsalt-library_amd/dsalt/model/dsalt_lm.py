@@ -41,7 +41,7 @@ import torch.nn.functional as F
 from .. import _hip
 from ..kernels import _block_train
 from ..kernels.LayerNorm import LayerNorm
-from ..kernels.distill import distill_loss, torch_distill_loss
+from ..kernels.distill import cpu_distill_loss, distill_loss
 from ..kernels.dropout import draw_seed
 from ..kernels.fp8 import FP8Linear
 from ..modules.dsalt_transformer import CounterDropout, DSALTTransformerBlock, SwiGLUFFN, norm_class
@@ -69,11 +69,9 @@ def _chunked_distillation(x: torch.Tensor, head, teacher_logits: torch.Tensor, t
     for a in range(0, x.shape[0], chunk_size):
         part = slice(a, a + chunk_size)
         y = None if labels is None else labels[part]
-        args = head(x[part]), teacher_logits[part], teacher_ids[part], y
-        if x.is_cuda:
-            total = total + distill_loss(*args, temperature=temperature, label_weight=label_weight, reduction="sum")
-        else:
-            total = total + torch_distill_loss(*args, (temperature, label_weight, -100, "sum"))
+        loss = distill_loss if x.is_cuda else cpu_distill_loss
+        total = total + loss(head(x[part]), teacher_logits[part], teacher_ids[part], y, temperature=temperature,
+                             label_weight=label_weight, reduction="sum")
     n = max(x.shape[0], 1) if labels is None else (labels != -100).sum().clamp(min=1).to(torch.float32)
     return total / n
 

@@ -7,6 +7,7 @@ import torch
 import dsalt._hip as hip
 from dsalt.kernels import distill_loss
 from dsalt.kernels.distill import torch_distill_loss
+from dsalt.model import DSALTLMHeadModel
 
 
 def operands(rows=5, V=11, K=3, seed=1):
@@ -83,3 +84,31 @@ def test_student_masks(mask):
     got, want = (torch_distill_loss(t, z, ids, y, opts) for t in (leaf, leaf.double()))
     torch.testing.assert_close(got.double(), want)
     torch.testing.assert_close(*(torch.autograd.grad(t, leaf)[0] for t in (got, want)))
+
+
+def lm():
+    """The LM without blocks, whose attention the CPU does not have: embedding, norm, head and loss."""
+    torch.manual_seed(3)
+    model = DSALTLMHeadModel(vocab_size=11, d_model=32, n_layers=1, n_heads=2, n_min=2, n_max=8, k_lmk=2, max_seq_len=64,
+                             lm_head_chunk_size=3)
+    model.layers = torch.nn.ModuleList()
+    return model
+
+
+def test_model_checks_as_the_loss_does():
+    """On the CPU too: values and operands are refused, no gradient goes to the teacher."""
+    _, z, ids, y = operands()
+    model, tokens = lm(), torch.arange(5)
+    kw = dict(teacher_logits=z.requires_grad_(), teacher_ids=ids)
+    for bad in (dict(label_weight=0.5), dict(labels=y, label_weight=1.5), dict(temperature=0.0), dict(temperature=float("nan"))):
+        with pytest.raises(ValueError):
+            model(tokens, **kw, **bad)
+    for bad in (dict(teacher_ids=ids.float()), dict(teacher_ids=ids[:, :2]), dict(labels=y[:, None].expand(5, 2))):
+        with pytest.raises(hip.DsaltError):
+            model(tokens, **{**kw, **bad})
+    out = model(tokens, labels=y, temperature=2.0, label_weight=0.5, **kw)
+    out["loss"].backward()
+    assert z.grad is None and bool(model.final_norm.weight.grad.any())
+    logits = model(tokens)["logits"]
+    want = torch_distill_loss(logits, z.detach(), ids, y, (2.0, 0.5, -100, "mean"))
+    torch.testing.assert_close(out["loss"], want)
