@@ -167,6 +167,12 @@ class DSALTLMHeadModel(nn.Module):
         loss of ``distill_loss`` with ``temperature`` and ``label_weight``; ``labels`` are then optional."""
         if (teacher_logits is None) != (teacher_ids is None):
             raise ValueError("teacher_logits and teacher_ids are given together")
+        if teacher_ids is not None:  # the loss goes over chunks of all of them
+            n = input_ids.numel()
+            if (any(t.dim() < 1 or t.shape[:-1].numel() != n for t in (teacher_logits, teacher_ids))
+                    or (labels is not None and labels.numel() != n)):
+                got = [None if t is None else tuple(t.shape) for t in (teacher_logits, teacher_ids, labels)]
+                raise _hip.DsaltError(f"teacher_logits, teacher_ids and labels must cover the {n} tokens (got {got})")
         with_loss = labels is not None or teacher_ids is not None
         if max_seqlen is None:
             max_seqlen = input_ids.shape[-1]

@@ -112,3 +112,16 @@ def test_model_checks_as_the_loss_does():
     logits = model(tokens)["logits"]
     want = torch_distill_loss(logits, z.detach(), ids, y, (2.0, 0.5, -100, "mean"))
     torch.testing.assert_close(out["loss"], want)
+
+
+def test_model_refuses_teachers_of_other_lengths():
+    """Rows of a teacher or labels beyond the tokens, also where they end on a chunk of the head."""
+    _, z, ids, y = operands(rows=6)
+    model, tokens = lm(), torch.arange(3)
+    for n in (2, 4, 6):
+        with pytest.raises(hip.DsaltError, match="tokens"):
+            model(tokens, teacher_logits=z[:n], teacher_ids=ids[:n])
+        with pytest.raises(hip.DsaltError, match="tokens"):
+            model(tokens, teacher_logits=z[:3], teacher_ids=ids[:3], labels=y[:n])
+    assert bool(torch.isfinite(model(tokens, teacher_logits=z[:3], teacher_ids=ids[:3], labels=y[:3])["loss"]))
+    assert bool(torch.isfinite(model(tokens[None], teacher_logits=z[None, :3], teacher_ids=ids[None, :3])["loss"]))
