@@ -63,17 +63,22 @@ def _chunked_cross_entropy(x: torch.Tensor, head, labels: torch.Tensor, chunk_si
 def _chunked_distillation(x: torch.Tensor, head, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
                           labels: torch.Tensor | None, temperature: float, label_weight: float,
                           chunk_size: int = 512) -> torch.Tensor:
-    """``distill_loss`` of ``head(x)`` over chunks of rows: its mean over the labels other than -100 (or all
-    rows, without labels)."""
+    """``distill_loss`` of ``head(x)`` over chunks of rows: its mean over the rows that count (all of them,
+    without labels)."""
     total = torch.zeros((), device=x.device, dtype=torch.float32)
     for a in range(0, x.shape[0], chunk_size):
         part = slice(a, a + chunk_size)
         y = None if labels is None else labels[part]
         loss = distill_loss if x.is_cuda else cpu_distill_loss
-        total = total + loss(head(x[part]), teacher_logits[part], teacher_ids[part], y, temperature=temperature,
+        logits = head(x[part])
+        total = total + loss(logits, teacher_logits[part], teacher_ids[part], y, temperature=temperature,
                              label_weight=label_weight, reduction="sum")
-    n = max(x.shape[0], 1) if labels is None else (labels != -100).sum().clamp(min=1).to(torch.float32)
-    return total / n
+        vocab = logits.shape[-1]
+        del logits  # not held while the next chunk's are formed
+    if labels is None or not x.shape[0]:
+        return total / max(x.shape[0], 1)
+    counted = (labels != -100) & (labels >= 0) & (labels < vocab)
+    return total / counted.sum().clamp(min=1).to(torch.float32)
 
 
 class DSALTLMHeadModel(nn.Module):

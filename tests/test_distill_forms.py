@@ -125,3 +125,13 @@ def test_model_refuses_teachers_of_other_lengths():
             model(tokens, teacher_logits=z[:3], teacher_ids=ids[:3], labels=y[:n])
     assert bool(torch.isfinite(model(tokens, teacher_logits=z[:3], teacher_ids=ids[:3], labels=y[:3])["loss"]))
     assert bool(torch.isfinite(model(tokens[None], teacher_logits=z[None, :3], teacher_ids=ids[None, :3])["loss"]))
+
+
+def test_model_averages_over_the_rows_that_count():
+    """Labels that are no token count for nothing in the model's mean, as in the loss of its logits."""
+    _, z, ids, y = operands(rows=7)
+    y[1], y[3], y[4] = -100, 11, -3
+    model, tokens = lm(), torch.arange(7)
+    got = model(tokens, teacher_logits=z, teacher_ids=ids, labels=y, temperature=2.0, label_weight=0.5)["loss"]
+    want = torch_distill_loss(model(tokens)["logits"], z, ids, y, (2.0, 0.5, -100, "mean"))
+    torch.testing.assert_close(got, want)
