@@ -57,6 +57,12 @@ def _scale(s: torch.Tensor) -> torch.Tensor:
     return s if all(1 <= t <= 1 << 21 for t in s.stride()) else s.clone(memory_format=torch.contiguous_format)
 
 
+def _no_grad(*ts) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise _hip.DsaltError("8-bit products and quantisation are for inference: call them under torch.no_grad(), or on tensors "
+                              "that require no gradient")
+
+
 @_dynamo_opaque
 def fp8_quantize(x: torch.Tensor, tile: bool = False, scale_dtype: torch.dtype = E8M0) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q, scale)`` of x [..., k]: 8-bit floats (``torch.float8_e4m3fn``) of x's shape, contiguous, and the
@@ -66,8 +72,8 @@ def fp8_quantize(x: torch.Tensor, tile: bool = False, scale_dtype: torch.dtype =
 
     A scale is the smallest power of two that brings its block's largest magnitude to at most 448 (1 for a
     block of zeros), as ``torch.float8_e8m0fnu`` or ``torch.float32``; x over it is rounded to nearest even. A
-    block that holds an infinity or NaN becomes NaN. x bf16, fp16 or fp32, k up to 2^20, any strides. Not
-    differentiable. Other operands raise ``DsaltError``."""
+    block that holds an infinity or NaN becomes NaN. x bf16, fp16 or fp32, k up to 2^20, any strides. For
+    inference: x that requires a gradient is refused where gradients are recorded. Other operands raise ``DsaltError``."""
     k = x.shape[-1] if x.dim() else 0
     ok = (x.device.type == "cuda" and x.dtype in _hip._SCORE_DTYPES and 1 <= k <= 1 << 20 and scale_dtype in (torch.float32, E8M0)
           and (not tile or x.dim() == 2) and x.numel() // k <= 1 << 30
@@ -76,7 +82,7 @@ def fp8_quantize(x: torch.Tensor, tile: bool = False, scale_dtype: torch.dtype =
         _hip.require_gpu(x)
         raise _hip.DsaltError(f"fp8_quantize needs bf16, fp16 or fp32 x [..., k], [n, k] for tiles, and fp32 or e8m0 scales "
                               f"(got {tuple(x.shape)} {x.dtype}, {scale_dtype})")
-    x = x.detach()
+    _no_grad(x)
     if not eager(x):
         return torch_fp8_quantize(x, tile, scale_dtype)
     if x.dim() == 2:
@@ -94,7 +100,8 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     to ``out_dtype`` (bf16, fp16 or fp32); bias [n] in any of those.
 
     k a multiple of 16; k and n up to 2^20; any strides (rows that are not 16-byte aligned are copied). For
-    inference: not differentiable. Other operands raise ``DsaltError``."""
+    inference: operands that require a gradient are refused where gradients are recorded. Other operands raise
+    ``DsaltError``."""
     dev, k = a.device, a.shape[-1] if a.dim() else 0
     ok = (dev.type == "cuda" and a.dtype is E4M3 and _weight_ok(b, b_scale, bias, dev) and k == b.shape[1]
           and a_scale.shape == (*a.shape[:-1], _blocks(k)) and a_scale.dtype in (torch.float32, E8M0) and a_scale.device == dev
@@ -105,7 +112,7 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
             f"fp8_matmul needs e4m3 a [..., k] and b [n, k], k a multiple of 16, fp32 or e8m0 scales [..., ceil(k / 128)] and "
             f"[ceil(n / 128), ceil(k / 128)], a bias [n] (got "
             f"{[None if t is None else (tuple(t.shape), t.dtype) for t in (a, a_scale, b, b_scale, bias)]}, {out_dtype})")
-    _no_grad(bias)
+    _no_grad(a, a_scale, b, b_scale, bias)
     if not eager(*(t for t in (a, a_scale, b, b_scale, bias) if t is not None)):
         return torch_fp8_matmul(a, a_scale, b, b_scale, bias, out_dtype)
     if a_scale.dtype is not b_scale.dtype:  # the kernel takes both alike
@@ -115,19 +122,13 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
                            None if bias is None else _hip.contiguous_rows(bias), a.shape[:-1], out_dtype)
 
 
-def _no_grad(*ts) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise _hip.DsaltError("8-bit products are for inference: call them under torch.no_grad(), or on tensors that require "
-                              "no gradient")
-
-
 @_dynamo_opaque
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``fp8_matmul(*fp8_quantize(x), weight, weight_scale, bias)`` of x [..., k] in bf16, fp16 or fp32, in
     ``out_dtype`` (by default x's); up to 32 rows are quantised by the product's kernel as it reads
-    them, to the same 8-bit values. weight [n, k] and its scales as ``fp8_matmul`` takes b. For inference: x or a bias that
-    requires a gradient is refused where gradients are recorded."""
+    them, to the same 8-bit values. weight [n, k] and its scales as ``fp8_matmul`` takes b. For inference: operands
+    that require a gradient are refused where gradients are recorded."""
     dev, k = x.device, x.shape[-1] if x.dim() else 0
     out_dtype = x.dtype if out_dtype is None else out_dtype
     ok = (dev.type == "cuda" and x.dtype in _hip._SCORE_DTYPES and out_dtype in _hip._SCORE_DTYPES
@@ -139,7 +140,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
             f"fp8_linear needs bf16, fp16 or fp32 x [..., k], e4m3 weight [n, k], k a multiple of 16, fp32 or e8m0 scales "
             f"[ceil(n / 128), ceil(k / 128)], a bias [n] (got "
             f"{[None if t is None else (tuple(t.shape), t.dtype) for t in (x, weight, weight_scale, bias)]}, {out_dtype})")
-    _no_grad(x, bias)
+    _no_grad(x, weight, weight_scale, bias)
     if not eager(*(t for t in (x, weight, weight_scale, bias) if t is not None)):
         return torch_fp8_matmul(*torch_fp8_quantize(x, False, torch.float32), weight, weight_scale, bias, out_dtype)
     flat = x if x.dim() == 2 else x.reshape(-1, k)
