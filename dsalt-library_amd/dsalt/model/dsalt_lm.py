@@ -137,12 +137,12 @@ class DSALTLMHeadModel(nn.Module):
     def quantize_fp8(self, lm_head: bool = True) -> "DSALTLMHeadModel":
         """The feed-forwards' projections and (``lm_head``) the head as frozen 8-bit layers, in place, for
         inference; the embedding, the attention and the norms stay as they are. On the GPU, widths that are
-        multiples of 16."""
-        for layer in self.layers:
-            if type(layer.ffn) is SwiGLUFFN:
-                layer.ffn.quantize_fp8()
+        multiples of 16 (else it raises and changes nothing)."""
+        new = [(layer.ffn, *item) for layer in self.layers if type(layer.ffn) is SwiGLUFFN for item in layer.ffn._fp8_layers()]
         if lm_head and type(self.lm_head) is nn.Linear:
-            self.lm_head = FP8Linear.from_linear(self.lm_head)
+            new.append((self, "lm_head", FP8Linear.from_linear(self.lm_head)))
+        for owner, name, layer in new:
+            setattr(owner, name, layer)
         return self
 
     def _head(self, x: torch.Tensor) -> torch.Tensor:

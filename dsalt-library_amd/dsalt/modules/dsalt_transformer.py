@@ -90,11 +90,16 @@ class SwiGLUFFN(nn.Module):
 
     def quantize_fp8(self) -> "SwiGLUFFN":
         """The projections as frozen 8-bit ones (``FP8Linear``), in place, for inference: widths that are
-        multiples of 16, weights on the GPU. gate and up then share one quantisation of x."""
-        for name in ("gate_proj", "up_proj", "down_proj"):
-            if type(getattr(self, name)) is nn.Linear:
-                setattr(self, name, FP8Linear.from_linear(getattr(self, name)))
+        multiples of 16, weights on the GPU (else it raises and changes nothing). gate and up then share one
+        quantisation of x."""
+        for name, layer in self._fp8_layers():
+            setattr(self, name, layer)
         return self
+
+    def _fp8_layers(self) -> list:
+        """The names of the plain projections, each with its 8-bit layer."""
+        names = ("gate_proj", "up_proj", "down_proj")
+        return [(n, FP8Linear.from_linear(getattr(self, n))) for n in names if type(getattr(self, n)) is nn.Linear]
 
     def project(self, x: torch.Tensor) -> torch.Tensor:
         """The feed-forward without its dropout."""
