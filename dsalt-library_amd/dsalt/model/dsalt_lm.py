@@ -196,7 +196,7 @@ class DSALTLMHeadModel(nn.Module):
             for layer in self.layers:
                 x, delta, _ = layer._forward_fused(x, delta, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
                                                    cu_list=cu_list)
-            _, x = DSALTTransformerBlock._add_norm(x, delta, self.final_norm)
+            _, x = self.layers[-1]._sum_norm(x, delta, self.final_norm)
             return {"loss": None, "logits": self.lm_head(x), "aux_loss": None}
         aux = torch.zeros((), device=input_ids.device, dtype=x.dtype)
         joins = bool(self.layers) and all(type(layer) is DSALTTransformerBlock and layer.joins_branches

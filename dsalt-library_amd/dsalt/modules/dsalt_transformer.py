@@ -322,14 +322,17 @@ class DSALTTransformerBlock(nn.Module):
         makes no zero aux tensor), so that the next block's norm (or the final norm) takes
         that add in its own pass. `delta` is the previous block's pending FFN
         output (None for the first block). The caller checks `_norms_fusable` first."""
-        x_sum, h = self._add_norm(x, delta, self.attn_norm)
-        if x_sum is not None:
-            x = x_sum
+        x, h = self._sum_norm(x, delta, self.attn_norm)
         x_attn, aux = self.attn(h, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, rope_cs=rope_cs, cu_list=cu_list,
                                 _need_aux=False)
-        if self._norms_fusable(x, x_attn, self.ffn_norm):
-            x, h = self._add_norm(x, x_attn, self.ffn_norm)
-        else:
-            x = x + x_attn
-            h = self.ffn_norm(x)
+        x, h = self._sum_norm(x, x_attn, self.ffn_norm)
         return x, self.ffn(h), aux
+
+    def _sum_norm(self, x: torch.Tensor, h: torch.Tensor | None, norm: nn.Module):
+        """``(x + h, norm(x + h))``, in one pass where the two go together: a replaced feed-forward's output may be
+        of a wider type than the stream."""
+        if self._norms_fusable(x, h, norm):
+            x_sum, y = self._add_norm(x, h, norm)
+            return x if x_sum is None else x_sum, y
+        x = x if h is None else x + h
+        return x, norm(x)
