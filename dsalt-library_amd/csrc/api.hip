@@ -976,6 +976,15 @@ int dsalt_fp8_matmul(const dsalt_fp8_matmul_args *args, void *stream) {
 int64_t dsalt_fp8_matmul_workspace_size(int64_t m, int32_t n, int32_t k) {
     return m < 0 || n < 1 || k < 1 ? 0 : dsalt::fp8_workspace_bytes(m, n, k);
 }
+int dsalt_fp8_matmul_plan(int64_t m, int32_t n, int32_t k, int32_t e8m0, int32_t *plan) {
+    if (m < 1 || m > (1 << 24) || n < 1 || n > (1 << 20) || k < 16 || k > (1 << 20) || !plan)
+        return fail(DSALT_ERR_INVALID, "sizes of a product and a plan to write to needed (m %lld, n %d, k %d)", (long long)m, n, k);
+    const dsalt::Fp8Plan p = dsalt::fp8_plan(m, n, k, e8m0 != 0);
+    plan[0] = p.rows;
+    plan[1] = p.columns;
+    plan[2] = p.splits;
+    return DSALT_OK;
+}
 int dsalt_fp8_few_rows(void) { return dsalt::fp8_few_rows(); }
 size_t dsalt_fp8_matmul_args_size(void) { return sizeof(dsalt_fp8_matmul_args); }
 

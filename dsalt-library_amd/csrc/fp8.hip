@@ -760,17 +760,22 @@ hipError_t launch_tiles(const Fp8Params &p, int tile, hipStream_t stream) {
     return tile == kTile128 ? launch_tile<MX, 128, 128, 2, 2>(p, stream) : launch_tile<MX, 64, 128, 1, 4>(p, stream);
 }
 
+// Columns of a few-row workgroup, in 16s: wider ones quantise and read the rows less often; narrower ones where
+// there would be fewer than two a CU.
+int few_columns(int64_t n) { return n >= 4 * 16 * 480 ? 4 : n >= 2 * 16 * 480 ? 2 : 1; }
+
 template <typename TX, int MF>
 void launch_few(const Fp8Params &p, hipStream_t stream) {
-    // wider workgroups quantise and read the rows less often; narrower ones where there would be fewer than two a CU
     const auto go = [&](auto nt) {
         constexpr int NT = decltype(nt)::value;
         hipLaunchKernelGGL((fp8_rows_kernel<TX, MF, NT>), dim3((unsigned)((p.n + 16 * NT - 1) / (16 * NT))), dim3(64 * kRowWaves), 0,
                            stream, p);
     };
-    if (p.n >= 4 * 16 * 480) go(std::integral_constant<int, 4>());
-    else if (p.n >= 2 * 16 * 480) go(std::integral_constant<int, 2>());
-    else go(std::integral_constant<int, 1>());
+    switch (few_columns(p.n)) {
+        case 4: return go(std::integral_constant<int, 4>());
+        case 2: return go(std::integral_constant<int, 2>());
+        default: return go(std::integral_constant<int, 1>());
+    }
 }
 template <typename TX>
 void launch_few_rows(const Fp8Params &p, hipStream_t stream) {
@@ -792,6 +797,12 @@ void launch_quant(const QuantParams &p, bool tile, hipStream_t stream) {
 }  // namespace
 
 int fp8_few_rows() { return kFewRows; }
+
+Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, bool e8m0) {
+    if (m <= kFewRows) return {m <= 16 ? 16 : 32, few_columns(n) * 16, 1};
+    const Plan pl = plan(m, n, k, e8m0);
+    return {pl.tile == kTile256 ? 256 : pl.tile == kTile128 ? 128 : 64, pl.tile == kTile256 ? 256 : 128, pl.splits};
+}
 
 int64_t fp8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
     if (m <= kFewRows) return 0;

@@ -96,6 +96,10 @@ hipError_t launch_fp8_quantize(const dsalt_fp8_quantize_args &a, hipStream_t str
 hipError_t launch_fp8_matmul(const dsalt_fp8_matmul_args &a, hipStream_t stream);
 int64_t fp8_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int fp8_few_rows();
+struct Fp8Plan {
+    int rows, columns, splits;  // of a workgroup's tile, and of k
+};
+Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, bool e8m0);
 
 // Number of query blocks of `bm` tokens over a packed batch, as an upper bound that is
 // computable without reading cu_seqlens: sum_s ceil(L_s/bm) <= ceil(T/bm) + S.

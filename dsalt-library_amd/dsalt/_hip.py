@@ -294,7 +294,7 @@ EXPORTED_SYMBOLS = (
     "dsalt_layer_norm", "dsalt_layer_norm_bwd", "dsalt_layer_norm_check", "dsalt_layer_norm_workspace_size",
     "dsalt_layer_norm_args_size", "dsalt_distill", "dsalt_distill_bwd", "dsalt_distill_check", "dsalt_distill_workspace_size",
     "dsalt_distill_stats_count", "dsalt_distill_args_size", "dsalt_fp8_quantize", "dsalt_fp8_quantize_args_size",
-    "dsalt_fp8_matmul", "dsalt_fp8_matmul_check", "dsalt_fp8_matmul_workspace_size", "dsalt_fp8_few_rows",
+    "dsalt_fp8_matmul", "dsalt_fp8_matmul_check", "dsalt_fp8_matmul_workspace_size", "dsalt_fp8_matmul_plan", "dsalt_fp8_few_rows",
     "dsalt_fp8_matmul_args_size",
 )
 NOALLOC_SCRATCH_BYTES = 76 << 20  # DSALT_NOALLOC_SCRATCH_BYTES
@@ -361,6 +361,7 @@ def lib() -> ctypes.CDLL:
         ("dsalt_fp8_matmul", [ctypes.POINTER(Fp8MatmulArgs), c_void_p]),
         ("dsalt_fp8_matmul_check", [ctypes.POINTER(Fp8MatmulArgs)]),
         ("dsalt_fp8_few_rows", []),
+        ("dsalt_fp8_matmul_plan", [c_int64, c_int32, c_int32, c_int32, ctypes.POINTER(c_int32)]),
         ("dsalt_add_rms_norm", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int32,
                                 c_void_p]),
     ):
@@ -1941,6 +1942,13 @@ def fp8_operand(t: torch.Tensor) -> torch.Tensor:
     if (cs == 1 or t.shape[1] == 1) and rs >= t.shape[1] and rs * size % 16 == 0 and rs * size <= 1 << 22 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def fp8_plan(m: int, n: int, k: int, e8m0: bool) -> tuple[int, int, int]:
+    """Rows and columns of a workgroup's tile and splits of k that a product takes: see dsalt_fp8_matmul_plan."""
+    plan = (c_int32 * 3)()
+    _raise(lib().dsalt_fp8_matmul_plan(m, n, k, e8m0, plan), "dsalt_fp8_matmul_plan")
+    return tuple(plan)
 
 
 def fp8_matmul(a, a_scale, b, b_scale, bias, lead, out_dtype: torch.dtype) -> torch.Tensor:

@@ -840,6 +840,9 @@ int dsalt_fp8_matmul(const dsalt_fp8_matmul_args *args, void *stream);
 int dsalt_fp8_matmul_check(const dsalt_fp8_matmul_args *args);
 int64_t dsalt_fp8_matmul_workspace_size(int64_t m, int32_t n, int32_t k);
 int dsalt_fp8_few_rows(void);
+/* What dsalt_fp8_matmul takes for a size (e8m0: with scales of that type): plan[3] = rows and columns of a
+ * workgroup's tile, splits of k. */
+int dsalt_fp8_matmul_plan(int64_t m, int32_t n, int32_t k, int32_t e8m0, int32_t *plan);
 size_t dsalt_fp8_matmul_args_size(void);
 
 int dsalt_abi_version(void);
