@@ -41,6 +41,7 @@ import torch.nn.functional as F
 from .. import _hip
 from ..kernels import _block_train
 from ..kernels.LayerNorm import LayerNorm
+from ..kernels.RMSENorm import RMSENorm
 from ..kernels.distill import cpu_distill_loss, distill_loss
 from ..kernels.dropout import draw_seed
 from ..kernels.fp8 import FP8Linear
@@ -238,7 +239,7 @@ class DSALTLMHeadModel(nn.Module):
             return False
         final = self.final_norm
         if not (DSALTTransformerBlock._layer_joins(x, x, final) if isinstance(final, LayerNorm)
-                else _hip.add_rms_norm_supported(x, final.weight)):
+                else type(final) is RMSENorm and _block_train.plain(final) and _hip.add_rms_norm_supported(x, final.weight)):
             return False
         if any(getattr(layer, "joins_branches", False) for layer in self.layers):
             return False

@@ -310,6 +310,8 @@ class DSALTTransformerBlock(nn.Module):
             return False
         if isinstance(norm, LayerNorm):
             return self._layer_joins(x, x if h is None else h, norm)
+        if type(norm) is not RMSENorm or not _block_train.plain(norm):  # replaced or hooked: called as it is
+            return False
         if h is not None and (h.shape != x.shape or h.dtype != x.dtype or not h.is_contiguous()
                               or h.data_ptr() % 16):
             return False
