@@ -17,11 +17,12 @@
 // before a loss scale is known, which in fp16 loses most of a vocabulary's small probabilities).
 //
 // Rows of up to 4096 logits take one wave, longer ones four; few long rows are cut into slices whose
-// sums a second kernel joins, but for a lone one, which sixteen waves take. Long rows are bound by HBM bytes: 6473 x 32000 bf16 at tau = 2 with labels,
-// 85 us forward (4.9 TB/s; 126 right behind a backward, whose gradients still drain) and 155-199 us
-// backward (5.3-4.2 TB/s: what the forward left in the last-level cache counts); fp32 144 and 377 us. A
+// sums a second kernel joins, but for a lone one, which sixteen waves take. Long rows are bound by HBM bytes:
+// 6473 x 32000 bf16 at tau = 2 with labels, 88 us forward (4.7 TB/s; 126 right behind a backward, whose gradients
+// still drain) and 155-201 us backward (5.3-4.1 TB/s: what the forward left in the last-level cache counts); at
+// tau = 1.5, with two exponentials a logit, 98 and 201 us; fp32 146 and 378 us. A
 // loop that loaded a run only behind the last one's sums took 124 us. Short rows are bound by what a row
-// costs beside its logits, the label, the slots and a wave's joins: 60000 x 1500 85 and 135 us.
+// costs beside its logits, the label, the slots and a wave's joins: 60000 x 1500 88 and 133 us.
 #include "launch.h"
 #include "lanes.h"
 #include "rotary.h"

@@ -17,7 +17,9 @@
 // each operand is read once and each result written once. 16384 x 4096 bf16 with a branch: 96 us forward
 // (5.6 TB/s), 142 us backward (4.7 TB/s) and 5 for the sums over its workgroups; 6473 x 1024, fp32 stream
 // and bf16 branch: 17.4 us (4.6 TB/s), 21.9 (4.8) and 3.9; a copy of 1 GiB reaches 5.1 TB/s. One row takes
-// 2.8 us: a launch and two exchanges.
+// 2.8 us: a launch and two exchanges. Widths that are no multiple of 8 and unaligned rows go element by element, two to
+// four times as slow: bf16 with a branch, one call after another on the same rows, 6473 x 1023 24 us forward and 47
+// backward with its sums (1024: 11 and 17), 16384 x 4097 258 and 520 (4096: 98 and 118).
 #include "launch.h"
 #include "rowsums.h"
 

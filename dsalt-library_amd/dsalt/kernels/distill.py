@@ -119,10 +119,10 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids
     repeats takes the sum of its slots.
 
     logits and teacher_logits bf16, fp16 or fp32; teacher_ids and labels int32 or int64; V up to 2^30, K up
-    to 1024; rows of any stride; temperature in [2^-63, 2^63). Sums are fp32, the gradient is rounded once, and its sums have a fixed
-    order. Differentiable in logits alone: no gradient goes to the teacher. Functorch's transforms,
-    forward-mode differentiation, tracing and tensor subclasses take torch's ops instead. Other operands
-    raise ``DsaltError``."""
+    to 1024; rows of any stride; temperature in [2^-63, 2^63). Masks of any finite value are what the formula makes of
+    them. Sums are fp32, the gradient is rounded once, and its sums have a fixed order. Differentiable in logits
+    alone: no gradient goes to the teacher. Functorch's transforms, forward-mode differentiation, tracing and tensor
+    subclasses take torch's ops instead. Other operands raise ``DsaltError``."""
     opts = _options(labels, temperature, label_weight, ignore_index, reduction)
     lead = logits.shape[:-1]
     if not (logits.device.type == "cuda" and _fit(logits, teacher_logits, teacher_ids, labels, _hip._SCORE_DTYPES)):

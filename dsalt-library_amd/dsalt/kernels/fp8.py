@@ -96,8 +96,10 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``a @ b.T + bias`` [..., n] of 8-bit floats (``torch.float8_e4m3fn``) a [..., k] and b [n, k] with the
     scales that ``fp8_quantize`` gives: a_scale [..., ceil(k / 128)] and b_scale [ceil(n / 128),
-    ceil(k / 128)], ``torch.float8_e8m0fnu`` or any values in fp32, each its own. Products and sums in fp32, one rounding
-    to ``out_dtype`` (bf16, fp16 or fp32); bias [n] in any of those.
+    ceil(k / 128)], ``torch.float8_e8m0fnu`` or any values in fp32 whose products fp32 holds, each its own. One rounding to
+    ``out_dtype`` (bf16, fp16 or fp32); bias [n] in any of those. Sums are fp32, but for those of each eight consecutive k, which
+    the matrix instruction adds to 13 bits below their largest product: an error of at most 7 * 2^-13 of it, 1.5e-5 of a
+    result of normal values (2-norm), more than fp32's where ``out_dtype`` is that.
 
     k a multiple of 16; k and n up to 2^20; any strides (rows that are not 16-byte aligned are copied). For
     inference: operands that require a gradient are refused where gradients are recorded. Other operands raise
@@ -126,7 +128,7 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``fp8_matmul(*fp8_quantize(x), weight, weight_scale, bias)`` of x [..., k] in bf16, fp16 or fp32, in
-    ``out_dtype`` (by default x's); up to 32 rows are quantised by the product's kernel as it reads
+    ``out_dtype`` (by default x's), with its precision; up to 32 rows are quantised by the product's kernel as it reads
     them, to the same 8-bit values. weight [n, k] and its scales as ``fp8_matmul`` takes b. For inference: operands
     that require a gradient are refused where gradients are recorded."""
     dev, k = x.device, x.shape[-1] if x.dim() else 0

@@ -149,8 +149,10 @@ class DSALTTransformerBlock(nn.Module):
     ``residual_scale * x + gate * post_norm(branch)`` on ``branch_norm``, which takes the
     feed-forward's dropout and the next norm along. ``fused_ffn``, ``activation``: see SwiGLUFFN.
 
-    ``norm``: "rms", or "layer" for LayerNorm modules in the place of every RMSENorm; a residual add and the
-    layer norm after it are one pass too, forward and backward (``add_layer_norm``)."""
+    ``norm``: "rms", or "layer" for LayerNorm modules in the place of every RMSENorm. The attention's residual add and
+    the layer norm after it are one pass forward and one backward (``add_layer_norm``); without autograd in the LM
+    the feed-forward's add and the next block's norm too. With the options of ``branch_norm`` above, layer norms are
+    passes of their own. Norms that are replaced or hooked are called as they are."""
 
     _fuse_norms = True
     joins_branches = False
